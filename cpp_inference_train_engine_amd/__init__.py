@@ -25,6 +25,8 @@ STEP_NO_READ_AHEAD = 4
 DECODE_STATUS_XCD, DECODE_STATUS_UNPLACED = 1, 2
 DECODE_WORKSPACE_HEAD, DECODE_STATUS_OFFSET = 1280, 1024
 PLACE_MAX_SESSIONS = 256
+CACHE_16BIT, CACHE_Q8 = 0, 1
+PLAN_INFO_INTS = 8
 
 
 class MlaError(RuntimeError):
@@ -69,6 +71,19 @@ _SIGNATURES = {
     "mla_prefill_attention": (C.c_int, [C.c_void_p] + [C.c_int] * 6 + [C.c_float] +
                               [C.c_void_p] * 3 + [C.c_int] * 2 + [C.c_void_p] * 4 +
                               [C.c_int, C.c_void_p, C.c_void_p, C.c_int]),
+    "mla_q8_page_bytes": (C.c_size_t, [C.c_int] * 3),
+    "mla_append_latent_q8": (C.c_int, [C.c_void_p] + [C.c_int] * 5 + [C.c_void_p] * 3 +
+                             [C.c_int, C.c_void_p]),
+    "mla_read_latent_q8": (C.c_int, [C.c_void_p] + [C.c_int] * 5 + [C.c_void_p, C.c_int] +
+                           [C.c_void_p] * 3),
+    "mla_attention_plan_bytes": (C.c_size_t, [C.c_int] * 6),
+    "mla_attention_workspace_bytes": (C.c_size_t, [C.c_int] * 6),
+    "mla_plan_attention": (C.c_int, [C.c_void_p] + [C.c_int] * 6 + [C.c_void_p] * 3 + [C.c_int] +
+                           [C.c_void_p] * 4 + [C.c_int, C.c_int, C.c_void_p, C.c_size_t]),
+    "mla_read_plan_info": (C.c_int, [C.c_void_p] * 3),
+    "mla_latent_attention": (C.c_int, [C.c_void_p] + [C.c_int] * 9 + [C.c_float, C.c_void_p] +
+                             [C.c_int] * 2 + [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 3 +
+                             [C.c_size_t] + [C.c_void_p] * 3 + [C.c_size_t]),
     "mla_config_validate": (C.c_int, [C.c_void_p]),
     "mla_config_parameter_count": (C.c_size_t, [C.c_void_p]),
     "mla_model_create": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int,
@@ -180,9 +195,11 @@ def stream_handle(stream=None) -> int | None:
 
 
 from .ops import (  # noqa: E402  (re-exported operator interface)
-    PagedLatentCache, RaggedBatch, append_latent, build_metadata, decode_attention,
+    AttentionPlan, PagedLatentCache, QuantizedLatentCache, RaggedBatch, SharedPrefixes,
+    append_latent, append_latent_q8, attention_workspace, build_metadata, decode_attention,
     decode_merge, decode_partials, decode_status, decode_workspace, decode_workspace_bytes,
-    placed_work_slots, prefill_attention, xcd_count)
+    latent_attention, placed_work_slots, plan_attention, prefill_attention, read_latent_q8,
+    xcd_count)
 from . import ops  # noqa: E402
 
 from .model import (HipModel, ModelConfig, config_hash, config_parameter_count,  # noqa: E402
@@ -200,4 +217,6 @@ __all__ = ["MlaError", "lib", "check", "build_metadata", "append_latent", "decod
            "clean_utf8", "generate", "generate_ids", "GenerationConfig", "sample_token",
            "banned_tokens", "Scheduler",
            "decode_workspace_bytes", "RaggedBatch", "PagedLatentCache", "DTYPE_F16",
-           "DTYPE_BF16"]
+           "DTYPE_BF16", "QuantizedLatentCache", "append_latent_q8", "read_latent_q8",
+           "SharedPrefixes", "AttentionPlan", "plan_attention", "attention_workspace",
+           "latent_attention"]

@@ -1,0 +1,538 @@
+// Attention of a batch's query rows over the paged latent cache by a plan's jobs, gfx950: the
+// kernel of both lists and both cache formats (the units latent_attend_*.hip instantiate it).
+//
+// For a (query, head) row with query (q, qr) and keys i = (latent c_i, rope key k_i) that it sees
+//     s_i = (q . c_i + qr . k_i) scale,   o = sum_i softmax(s)_i c_i,   lse = ln sum_i exp(s_i)
+// as the framework's other attention kernels (src/infer/inference.cpp:116-153 in the reference,
+// causal rows src/model/ops.cpp:109-142).
+//
+// latent_attend_kernel -- a workgroup of 4 waves takes a job: up to 16 QT rows (list K) or 128 rows
+//   (list R) of a segment over a range of its keys, 32 keys (a unit: two 16-token tiles, which may
+//   lie on different pages) at a time.  List K: every wave holds all rows and takes every 4th
+//   unit through a slot of its own; the waves' states meet in LDS at the end.  List R: every wave
+//   holds 32 rows, the four stage a unit together into one of two buffers (one barrier a unit), and
+//   no state is exchanged: each key is read once for 128 rows, which is what makes a shared prefix
+//   cheap.  A unit goes from memory to registers while the unit before it is computed, and from
+//   there to LDS as 16-bit words in MFMA-operand order (8-bit latents: v_cvt_scalef32_pk_*, exact,
+//   see mla_q8.hpp), so that both formats share everything behind it:
+//     S^T = K . Q^T     v_mfma_f32_16x16x32, Q^T in registers for the whole job
+//     online softmax    log2 domain in 32 bits, the reference maximum raised lazily
+//     O^T += C^T . P^T  C^T by transpose reads (ds_read_b64_tr_b16); P^T rounded to the 16-bit type
+//                       of the cache: the row is a weighted mean whose weights are off by half a
+//                       step of that type each, and is itself rounded to it in the end
+// A key past a row's position adds nothing to the row, whatever it holds: its rope key only enters
+// the score, which is replaced, and a non-finite latent is staged as zero with the key marked, and
+// makes the scores of the rows that see it NaN.  (Without causal rows every row of a job sees all
+// of its keys, and such a latent spreads to them by itself.)
+#pragma once
+
+#include "mla_latent.hpp"
+#include "mla_q8.hpp"
+
+#include <cmath>
+
+namespace mla {
+namespace {
+
+// Rows of odd 256-byte sub-chunks of a latent block sit at slot row ^ kRot in LDS, so that the
+// transpose reads of a sub-chunk pair fall in disjoint banks.
+constexpr int kRot = 12;
+// The reference maximum sits kHead below the row's when it is set, and is raised again when a
+// score passes it by more than kRise: probabilities stay within fp16, and those near the maximum
+// clear of its subnormals.
+constexpr float kHead = 6.0f, kRise = 14.0f;
+
+__device__ __forceinline__ u32x2 read_tr16(const uint16_t* p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    const auto v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (s4 __attribute__((address_space(3)))*)((__attribute__((address_space(3))) char*)p));
+    return __builtin_bit_cast(u32x2, v);
+}
+
+// The 16-bit words of v whose exponent is all ones become 0; true if there was one.
+template <typename T>
+__device__ __forceinline__ bool drop_nonfinite16(u32x4& v) {
+    constexpr uint32_t e = T::exp_mask, both = e | e << 16;
+    constexpr uint32_t step = (e & -e) | (e & -e) << 16;  // the exponent's lowest bit
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        any |= ((v[i] & both) + step) & 0x80008000u;
+    if (!any)
+        return false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((v[i] & e) == e)
+            v[i] &= 0xffff0000u;
+        if ((v[i] >> 16 & e) == e)
+            v[i] &= 0x0000ffffu;
+    }
+    return true;
+}
+// The NaN bytes of v become 0; true if there was one.
+__device__ __forceinline__ bool drop_nan8(u32x4& v) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        any |= q8_nan_bits(v[i]);
+    if (!any)
+        return false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] &= ~((q8_nan_bits(v[i]) >> 7) * 0xffu);
+    return true;
+}
+
+// T: 16-bit type of the queries, rope keys, 16-bit latents and rows; Q8: 8-bit latents; KSM: latent
+// k-steps (kv_rank / 32 <= KSM); QT: 16-row tiles of a wave; ROWS: list R.
+template <typename T, bool Q8, int KSM, int QT, bool ROWS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
+    KSM >= 16 ? 1 : 2, 8))) void latent_attend_kernel(LatentArgs a) {
+    constexpr int RSM = 2;                              // rope k-steps (rope_dim <= 64)
+    constexpr int RTM = 2 * KSM;                        // 16-row tiles of O^T
+    constexpr int SLOT = 32 * 32 * (KSM + RSM);         // words of a unit
+    constexpr int UPT = Q8 ? (KSM + 1) / 2 : KSM;       // 16-byte loads of a lane per tile
+    constexpr int NL = ROWS ? (2 * UPT + 3) / 4 : 2 * UPT;
+    constexpr int NR = ROWS ? 1 : 2 * RSM;              // rope loads: 2 * rope_dim / 8 chunks
+    constexpr int SLOTS = ROWS ? 2 : 4;
+    using V8 = typename T::vec8;
+    __shared__ __attribute__((aligned(16))) uint16_t smem[SLOTS][SLOT];
+    __shared__ uint32_t marks[3];  // list R: keys of a unit with a non-finite latent
+
+    const int32_t* d = a.plan + (ROWS ? a.p.jobs_r_at : a.p.jobs_k_at) + (long long)blockIdx.x * kJobInts;
+    const int n_jobs = a.plan[ROWS ? kPlanJobsR : kPlanJobsK];
+    const int seg = d[0], f0 = d[1], n_rows = d[2], rb = d[3], key0 = d[4], key_end = d[5],
+              ctx = d[6], part = d[7];
+    if ((int)blockIdx.x >= n_jobs || a.plan[kPlanTag] != (int)a.p.tag)
+        return;
+
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int H = a.H, KV = a.kv_rank, RP = a.rope_dim, PS = a.page_size;
+    const int ks = KV >> 5, rs = (RP + 31) >> 5, tpp = PS >> 4;
+    const long long rec = Q8 ? q8_page_bytes(PS, KV, RP) : 2LL * PS * (KV + RP);
+    const int32_t* ptab = seg >= 0 ? a.page_table + (long long)seg * a.max_pages
+                                   : a.prefix_page_ids + a.cu_prefix_pages[~seg];
+    const int n_units = key_end > key0 ? (key_end - key0 + 31) >> 5 : 0;
+    const int row0 = ROWS ? 16 * QT * wave : 0;  // the wave's first row of the block
+
+    // ---- Q^T operands: row 16q + n, latent columns 32j + 8g .., then the rope key's ----
+    V8 qv[QT][KSM + RSM];
+    int lim[QT];  // lane's row n sees keys [0, lim] of the segment
+    int lim_wave = -1;
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int r = row0 + 16 * q + n;
+        const bool ok = r < n_rows;
+        const long long fr = (long long)f0 + r;
+        lim[q] = a.causal && seg >= 0 ? ctx + (rb + r) / H : key_end - 1;
+#pragma unroll
+        for (int j = 0; j < KSM; ++j)
+            qv[q][j] = ok && j < ks
+                           ? *reinterpret_cast<const V8*>(a.q_latent + fr * KV + 32 * j + 8 * g)
+                           : V8{};
+#pragma unroll
+        for (int j = 0; j < RSM; ++j)
+            qv[q][KSM + j] = ok && 32 * j + 8 * g < RP
+                                 ? *reinterpret_cast<const V8*>(a.q_rope + fr * RP + 32 * j + 8 * g)
+                                 : V8{};
+    }
+    {   // the last key that any of the wave's rows sees (-1: it has no rows)
+        const int last = min(n_rows, row0 + 16 * QT) - 1;
+        if (last >= row0)
+            lim_wave = a.causal && seg >= 0 ? ctx + (rb + last) / H : key_end - 1;
+    }
+
+    // ---- a unit's way into LDS ----
+    const int s_lane = g * 128 + (n ^ ((g & 1) * kRot)) * 8;
+    u32x4 st[NL], sr[NR];
+    uint32_t sk[Q8 ? NL : 1];  // scale bytes of a load's one or two k-steps
+    const int upt = Q8 ? (ks + 1) >> 1 : ks;
+    const int rcs = RP >> 3;
+    int rope_tt[NR], rope_ch[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int c = ROWS ? tid >> 4 : 4 * i + g;
+        rope_tt[i] = c >= rcs;
+        rope_ch[i] = c < 2 * rcs ? (c >= rcs ? c - rcs : c) : -1;
+    }
+    // Tile t's page id, -1 past the keys or outside the pool.
+    auto tile_page = [&](int t) {
+        const int id = 16 * t < key_end ? __builtin_amdgcn_readfirstlane(ptab[t / tpp]) : -1;
+        return (unsigned)id < (unsigned)a.num_pool_pages ? id : -1;
+    };
+    auto load_unit = [&](int t0, int pg0, int pg1) {
+        const uint8_t* base0 = a.pages + pg0 * rec;
+        const uint8_t* base1 = a.pages + pg1 * rec;
+        const int in0 = t0 % tpp, in1 = (t0 + 1) % tpp;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int u = ROWS ? wave + 4 * i : i;
+            const int tt = u / UPT, k = u % UPT;
+            st[i] = u32x4{0, 0, 0, 0};
+            if constexpr (Q8)
+                sk[i] = 0;
+            if (u >= 2 * UPT || k >= upt || (tt ? pg1 : pg0) < 0)
+                continue;
+            const uint8_t* base = tt ? base1 : base0;
+            const int in = tt ? in1 : in0;
+            if constexpr (Q8) {
+                const uint8_t* lat = base + in * 16 * KV + k * 1024;
+                const uint8_t* sc = base + (long long)PS * (KV + 2 * RP) + (in * 16 + n) * ks + 2 * k;
+                if (2 * k + 1 < ks) {
+                    st[i] = *reinterpret_cast<const u32x4*>(lat + lane * 16);
+                    sk[i] = ks & 1 ? sc[0] | sc[1] << 8 : *reinterpret_cast<const uint16_t*>(sc);
+                } else {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(lat + lane * 8);
+                    st[i][0] = x[0];
+                    st[i][1] = x[1];
+                    sk[i] = sc[0];
+                }
+            } else {
+                st[i] = *reinterpret_cast<const u32x4*>(base + in * 32 * KV + k * 1024 + lane * 16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            sr[i] = u32x4{0, 0, 0, 0};
+            if (rope_ch[i] >= 0 && (rope_tt[i] ? pg1 : pg0) >= 0)
+                sr[i] = *reinterpret_cast<const u32x4*>(
+                    (rope_tt[i] ? base1 : base0) + (long long)PS * KV * (Q8 ? 1 : 2) +
+                    ((rope_tt[i] ? in1 : in0) * rcs + rope_ch[i]) * 256 + n * 16);
+        }
+    };
+    // Writes the loaded unit to `sp`; keys [valid, 32) become 0.  Returns the wave's marked keys.
+    auto stage_unit = [&](uint16_t* sp, int valid) {
+        uint32_t mark = 0;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int u = ROWS ? wave + 4 * i : i;
+            const int tt = u / UPT, k = u % UPT;
+            if (u >= 2 * UPT || k >= upt)
+                continue;
+            u32x4 v = st[i];
+            uint32_t k8 = Q8 ? sk[i] : 0;
+            if (valid < 32 && 16 * tt + n >= valid) {
+                v = u32x4{0, 0, 0, 0};
+                k8 = 0;  // a free slot's scale may be anything too
+            }
+            if (a.causal) {
+                bool bad;
+                if constexpr (Q8)
+                    bad = drop_nan8(v);
+                else
+                    bad = drop_nonfinite16<T>(v);
+                const uint64_t b = __builtin_amdgcn_ballot_w64(bad);
+                if (b)
+                    mark |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff) << (16 * tt);
+            }
+            uint16_t* dst = sp + tt * 16 * KV + s_lane;
+            if constexpr (Q8) {
+                *reinterpret_cast<u32x4*>(dst + 2 * k * 512) =
+                    q8_decode8<T>(v[0], v[1], q8_scale(k8 & 0xff));
+                if (2 * k + 1 < ks)
+                    *reinterpret_cast<u32x4*>(dst + (2 * k + 1) * 512) =
+                        q8_decode8<T>(v[2], v[3], q8_scale(k8 >> 8));
+            } else {
+                *reinterpret_cast<u32x4*>(dst + k * 512) = v;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (rope_ch[i] >= 0) {
+                u32x4 v = sr[i];
+                if (valid < 32 && 16 * rope_tt[i] + n >= valid)
+                    v = u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4*>(sp + 32 * KV + rope_tt[i] * 16 * RP + rope_ch[i] * 128 +
+                                          n * 8) = v;
+            }
+        return mark;
+    };
+
+    const int tr_par = (n & 3) >> 1;
+    const int tr_lane = tr_par * 128 + ((4 * g + (n >> 2)) ^ (tr_par * kRot)) * 8 + 4 * (n & 1);
+    int rope_off[RSM];  // lanes past the rope columns read a valid chunk (their Q^T is zero)
+#pragma unroll
+    for (int j = 0; j < RSM; ++j)
+        rope_off[j] = (32 * j + 8 * g < RP ? 4 * j + g : 0) * 128 + n * 8;
+
+    float m_run[QT], l_run[QT];
+    floatx4 acc[QT][RTM];
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        m_run[q] = -INFINITY;
+        l_run[q] = 0.0f;
+#pragma unroll
+        for (int rt = 0; rt < RTM; ++rt)
+            acc[q][rt] = floatx4{0, 0, 0, 0};
+    }
+
+    // ---- scores, softmax and product of the unit at `sp`, whose first tile is t0; `ok`: keys of
+    // the unit that exist, `mark`: those with a non-finite latent ----
+    auto compute_unit = [&](const uint16_t* sp, int t0, uint32_t ok, uint32_t mark) {
+        floatx4 sc[2][QT];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+                sc[tt][q] = floatx4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < KSM; ++j)
+            if (j < ks)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    const V8 ka =
+                        *reinterpret_cast<const V8*>(sp + tt * 16 * KV + j * 512 + s_lane);
+#pragma unroll
+                    for (int q = 0; q < QT; ++q)
+                        sc[tt][q] = T::mma32(ka, qv[q][j], sc[tt][q]);
+                }
+#pragma unroll
+        for (int j = 0; j < RSM; ++j)
+            if (j < rs)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    const V8 ka = *reinterpret_cast<const V8*>(sp + 32 * KV + tt * 16 * RP +
+                                                               rope_off[j]);
+#pragma unroll
+                    for (int q = 0; q < QT; ++q)
+                        sc[tt][q] = T::mma32(ka, qv[q][KSM + j], sc[tt][q]);
+                }
+
+        V8 pb[QT];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            bool rise = false;
+            float mp = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = 16 * tt + 4 * g + i;
+                    float x = sc[tt][q][i] * a.scale_log2;
+                    if (mark >> key & 1)
+                        x = NAN;
+                    if (!(ok >> key & 1) || 16 * t0 + key > lim[q])
+                        x = -INFINITY;
+                    sc[tt][q][i] = x;
+                    rise |= x > m_run[q] + kRise;
+                    mp = fmaxf(mp, x);
+                }
+            if (__builtin_amdgcn_ballot_w64(rise)) {
+                const float m_new = fmaxf(m_run[q], rows_max(mp) - kHead);
+                const bool had = m_run[q] != -INFINITY;  // the row has accumulated state
+                if (__builtin_amdgcn_ballot_w64(had && m_new > m_run[q])) {
+                    const float alpha = had ? __builtin_amdgcn_exp2f(m_run[q] - m_new) : 1.0f;
+                    l_run[q] *= alpha;
+#pragma unroll
+                    for (int rt = 0; rt < RTM; ++rt)
+                        acc[q][rt] *= alpha;
+                }
+                m_run[q] = m_new;
+            }
+            const float m_ref = m_run[q] == -INFINITY ? 0.0f : m_run[q];
+            float psum = 0.0f;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(sc[tt][q][i] - m_ref);
+                    psum += e;
+                    pb[q][4 * tt + i] = static_cast<typename T::scalar>(e);
+                }
+            l_run[q] += psum;
+        }
+#pragma unroll
+        for (int rt = 0; rt < RTM; ++rt)
+            if (rt < 2 * ks) {
+                const int blk = ((rt >> 1) * 4 + 2 * (rt & 1)) * 128;  // latent columns 16rt..
+                const u32x2 lo = read_tr16(sp + blk + tr_lane);
+                const u32x2 hi = read_tr16(sp + 16 * KV + blk + tr_lane);
+                const V8 ca = __builtin_bit_cast(V8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+                for (int q = 0; q < QT; ++q)
+                    acc[q][rt] = T::mma32(ca, pb[q], acc[q][rt]);
+            }
+    };
+    // The unit's keys that exist: before key_end, on a page of the pool.
+    auto keys_of = [&](int t0, int pg0, int pg1) {
+        const int valid = min(32, key_end - 16 * t0);
+        uint32_t ok = valid >= 32 ? 0xffffffffu : (1u << valid) - 1u;
+        if (pg0 < 0)
+            ok &= 0xffff0000u;
+        if (pg1 < 0)
+            ok &= 0x0000ffffu;
+        return ok;
+    };
+
+    // ---- the units: loaded one ahead, page ids two ahead ----
+    constexpr int STEP = ROWS ? 1 : 4;
+    const int first = ROWS ? 0 : wave, tile0 = key0 >> 4;
+    if (ROWS && a.causal) {
+        if (tid < 3)
+            marks[tid] = 0;
+        __syncthreads();
+    }
+    int pg0 = -1, pg1 = -1, nx0 = -1, nx1 = -1;
+    if (first < n_units) {
+        pg0 = tile_page(tile0 + 2 * first);
+        pg1 = tile_page(tile0 + 2 * first + 1);
+        load_unit(tile0 + 2 * first, pg0, pg1);
+        if (first + STEP < n_units) {
+            nx0 = tile_page(tile0 + 2 * (first + STEP));
+            nx1 = tile_page(tile0 + 2 * (first + STEP) + 1);
+        }
+    }
+    for (int u = first; u < n_units; u += STEP) {
+        const int t0 = tile0 + 2 * u;
+        uint16_t* sp = smem[ROWS ? u & 1 : wave];
+        const uint32_t ok = keys_of(t0, pg0, pg1);
+        uint32_t mark = stage_unit(sp, min(32, key_end - 16 * t0));
+        if (ROWS && a.causal && mark && lane == 0)
+            atomicOr(&marks[u % 3], mark);
+        if (u + STEP < n_units) {
+            load_unit(t0 + 2 * STEP, nx0, nx1);
+            pg0 = nx0;
+            pg1 = nx1;
+            if (u + 2 * STEP < n_units) {
+                nx0 = tile_page(t0 + 4 * STEP);
+                nx1 = tile_page(t0 + 4 * STEP + 1);
+            }
+        }
+        if constexpr (ROWS) {
+            // The other buffer is free: every wave that passed the barrier before this one has
+            // finished with it.  Likewise marks: unit u + 2's word, last read in unit u - 1, is
+            // cleared behind this barrier and set again behind the next.
+            __syncthreads();
+            if (a.causal) {
+                mark = marks[u % 3];
+                if (tid == 0)
+                    marks[(u + 2) % 3] = 0;
+            }
+        } else {
+            wave_lds_fence();
+        }
+        if (16 * t0 <= lim_wave)
+            compute_unit(sp, t0, ok, mark);
+        if constexpr (!ROWS)
+            wave_lds_fence();  // the slot's reads are done before the next unit's writes
+    }
+
+    // ---- final rows, or partials ----
+    if constexpr (ROWS) {
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            const float l = rows_sum(l_run[q]);
+            const int r = row0 + 16 * q + n;
+            if (r >= n_rows)
+                continue;
+            if (part < 0) {
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                uint16_t* o = a.out + ((long long)f0 + r) * KV;
+#pragma unroll
+                for (int rt = 0; rt < RTM; ++rt)
+                    if (rt < 2 * ks) {
+                        typedef typename T::scalar s4 __attribute__((ext_vector_type(4)));
+                        s4 x;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            x[i] = static_cast<typename T::scalar>(acc[q][rt][i] * inv);
+                        *reinterpret_cast<s4*>(o + 16 * rt + 4 * g) = x;
+                    }
+                if (a.lse && g == 0)
+                    a.lse[(long long)f0 + r] = (m_run[q] + __log2f(l)) * kLn2;
+            } else {
+                float* o = a.part_o + ((long long)part + r) * KV;
+#pragma unroll
+                for (int rt = 0; rt < RTM; ++rt)
+                    if (rt < 2 * ks)
+                        *reinterpret_cast<floatx4*>(o + 16 * rt + 4 * g) = acc[q][rt];
+                if (g == 0) {
+                    a.part_ml[2 * ((long long)part + r)] = m_run[q];
+                    a.part_ml[2 * ((long long)part + r) + 1] = l;
+                }
+            }
+        }
+    } else {
+        // A wave parks a row tile in its own slot: 16 rows of KV + 4 floats, then m and l.
+        const int pitch = KV + 4;
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            const float l = rows_sum(l_run[q]);
+            float* mine = reinterpret_cast<float*>(smem[wave]);
+            if (q > 0)
+                __syncthreads();  // the previous tile's rows have been read
+#pragma unroll
+            for (int rt = 0; rt < RTM; ++rt)
+                if (rt < 2 * ks)
+                    *reinterpret_cast<floatx4*>(mine + n * pitch + 16 * rt + 4 * g) = acc[q][rt];
+            if (g == 0) {
+                mine[16 * pitch + n] = m_run[q];
+                mine[16 * pitch + 16 + n] = l;
+            }
+            __syncthreads();
+            const int per_row = KV / 4;
+            for (int e = tid; e < 16 * per_row; e += 256) {
+                const int r = e / per_row, c = (e % per_row) * 4, row = 16 * q + r;
+                if (row >= n_rows)
+                    break;
+                float M = -INFINITY;
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    M = fmaxf(M, reinterpret_cast<const float*>(smem[v])[16 * pitch + r]);
+                float L = 0.0f;
+                floatx4 o = {0, 0, 0, 0};
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const float* x = reinterpret_cast<const float*>(smem[v]);
+                    const float mv = x[16 * pitch + r];
+                    const float f = mv == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mv - M);
+                    L += x[16 * pitch + 16 + r] * f;
+                    o += *reinterpret_cast<const floatx4*>(x + r * pitch + c) * f;
+                }
+                if (part < 0) {
+                    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+                    typedef typename T::scalar s4 __attribute__((ext_vector_type(4)));
+                    s4 y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        y[i] = static_cast<typename T::scalar>(o[i] * inv);
+                    *reinterpret_cast<s4*>(a.out + ((long long)f0 + row) * KV + c) = y;
+                    if (a.lse && c == 0)
+                        a.lse[(long long)f0 + row] = (M + __log2f(L)) * kLn2;
+                } else {
+                    *reinterpret_cast<floatx4*>(a.part_o + ((long long)part + row) * KV + c) = o;
+                    if (c == 0) {
+                        a.part_ml[2 * ((long long)part + row)] = M;
+                        a.part_ml[2 * ((long long)part + row) + 1] = L;
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <typename T, bool Q8, int KSM, int QT, bool ROWS>
+hipError_t launch_one(const LatentArgs& a, hipStream_t stream) {
+    const int jobs = ROWS ? a.p.max_jobs_r : a.p.max_jobs_k;
+    hipLaunchKernelGGL((latent_attend_kernel<T, Q8, KSM, QT, ROWS>), dim3(jobs), dim3(256), 0,
+                       stream, a);
+    return hipGetLastError();
+}
+
+template <typename T, bool Q8>
+hipError_t launch_list(const LatentArgs& a, bool rows, hipStream_t stream) {
+    const int ks = a.kv_rank / 32;
+    if (rows)
+        return ks <= 4   ? launch_one<T, Q8, 4, 2, true>(a, stream)
+               : ks <= 8 ? launch_one<T, Q8, 8, 2, true>(a, stream)
+                         : launch_one<T, Q8, 16, 2, true>(a, stream);
+    if (a.p.qt == 2)
+        return launch_one<T, Q8, 4, 2, false>(a, stream);
+    return ks <= 4   ? launch_one<T, Q8, 4, 1, false>(a, stream)
+           : ks <= 8 ? launch_one<T, Q8, 8, 1, false>(a, stream)
+                     : launch_one<T, Q8, 16, 1, false>(a, stream);
+}
+
+}  // namespace
+}  // namespace mla

@@ -123,6 +123,17 @@ std::string probe_xcd_placement();
 // words): the status word, plus kStatusXcd when a merge counter was left nonzero (capi.hip).
 int32_t decode_head_status(const int32_t* head);
 hipError_t launch_append(const AppendArgs& a, int dtype, hipStream_t stream);
+
+// Append to, or read back from, the 8-bit latent cache (latent_q8.hip; layout: mla_q8.hpp).
+struct Q8Args {
+    int T, kv_rank, rope_dim, page_size, num_pool_pages;
+    const float *ckv, *krope;  // append: fp32 rows
+    const int32_t* slot_mapping;
+    uint8_t* pages;            // read-back only reads it
+    uint16_t *ckv16, *krope16; // read-back: 16-bit rows
+};
+hipError_t launch_append_q8(const Q8Args& a, int dtype, hipStream_t stream);
+hipError_t launch_read_q8(const Q8Args& a, int dtype, hipStream_t stream);
 // Decode kernel only (MFMA page kernel, or the generic one when force_generic or the
 // shape is outside it): final rows of one-item sessions, partials of the others.
 hipError_t launch_decode_partials(const DecodeArgs& a, int dtype, bool force_generic,

@@ -1,0 +1,64 @@
+// Planned attention over the paged latent cache (latent_attention.hip), its plan
+// (attention_plan.hip) and the sizes both derive from a call's scalars.  Host-visible.
+#pragma once
+
+#include "mla_internal.hpp"
+
+namespace mla {
+
+// A segment is a run of keys that a set of consecutive query rows sees: a session's own pages
+// with its rows, or a group's shared prefix with the rows of all of the group's sessions.  A job
+// is one block of a segment's (query, head) rows over one range of its keys.  Segments of at most
+// kFewRows rows go to list K (a workgroup's four waves split the keys), the others to list R (they
+// split the rows).
+constexpr int kFewRows = 64;
+constexpr int kRowsR = 128;  // rows of a block of list R
+constexpr int kTile = 32;    // keys a wave takes at a time
+constexpr int kJobInts = 8;  // segment (>= 0 session, ~group), first flat row, rows, first row's
+                             // index in the segment, first key, last key + 1, ctx, partial row
+constexpr int kSegInts = 8;
+constexpr int kMergeInts = 8;
+constexpr int kPlanHead = 64;  // words
+enum { kPlanStatus, kPlanBad, kPlanJobsK, kPlanJobsR, kPlanParts, kPlanRows, kPlanTag };
+
+// What a plan and the calls over it derive from the same scalars.
+struct PlanShape {
+    int B, groups, rows, H, kv_rank, max_q_len;
+    int qt;                 // 16-row tiles of a list-K block
+    int target_k, target_r; // workgroups that the lists aim at
+    int least_k, least_r;   // tiles that a job takes at least
+    int max_jobs_k, max_jobs_r;
+    long long max_parts;    // (query, head) rows of partials
+    long long seg_at, merge_at, session_at, jobs_k_at, jobs_r_at, words;  // word offsets
+    uint32_t tag;
+};
+PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_len);
+
+struct PlanArgs {
+    PlanShape p;
+    int page_size, num_pool_pages, n_prefix_pages;
+    const int32_t *cu_q, *cu_k, *info, *cu_groups, *prefix_len, *cu_prefix_pages,
+        *prefix_page_ids;
+    int32_t* plan;
+};
+hipError_t launch_plan(const PlanArgs& a, hipStream_t stream);
+
+struct LatentArgs {
+    PlanShape p;
+    int H, kv_rank, rope_dim, page_size, max_pages, num_pool_pages;
+    int causal;        // the rows of a block may see different keys
+    int q8;
+    float scale_log2;  // softmax scale * log2(e)
+    const int32_t *plan, *page_table, *cu_prefix_pages, *prefix_page_ids;
+    const uint8_t* pages;
+    const uint16_t *q_latent, *q_rope;
+    uint16_t* out;
+    float *lse, *part_o, *part_ml;
+};
+hipError_t launch_latent_attention(const LatentArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_latent_merge(const LatentArgs& a, int dtype, hipStream_t stream);
+// The lists' kernels, one translation unit for each cache format (latent_attend_*.hip).
+hipError_t launch_attend_16(const LatentArgs& a, int dtype, bool rows, hipStream_t stream);
+hipError_t launch_attend_q8(const LatentArgs& a, int dtype, bool rows, hipStream_t stream);
+
+}  // namespace mla

@@ -4,6 +4,10 @@ Mirrors the three subsystems of the path:
   (a) ``build_metadata``   -> ``mla_build_metadata``   (GPU ragged-batch metadata)
   (b) ``append_latent``    -> ``mla_append_latent``    (paged latent/rope append)
   (c) ``decode_attention`` -> ``mla_decode_attention`` (absorbed split-K decode)
+and, beside them,
+  (d) ``append_latent_q8``, ``read_latent_q8`` -> the 8-bit latent cache
+  (e) ``plan_attention``, ``latent_attention`` -> attention of any rows of a batch over a 16-bit or
+      8-bit cache, prefixes that sessions share computed once
 All tensors are torch CUDA (HIP) tensors; calls are stream-ordered on the
 current torch stream unless ``stream`` is given.
 """
@@ -11,8 +15,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass, field
 
-from . import (DECODE_FUSED_MERGE, DTYPE_BF16, DTYPE_F16, INFO_INTS, MAX_WORK,
-               PLACE_MAX_SESSIONS, WORK_DESC_INTS, WORK_PAGES, check, lib, ptr, stream_handle)
+from . import (CACHE_16BIT, CACHE_Q8, DECODE_FUSED_MERGE, DTYPE_BF16, DTYPE_F16, INFO_INTS, MAX_WORK,
+               PLACE_MAX_SESSIONS, PLAN_INFO_INTS, WORK_DESC_INTS, WORK_PAGES, check, lib, ptr, stream_handle)
 
 
 def _torch():
@@ -258,9 +262,215 @@ def prefill_attention(batch: RaggedBatch, pages, q_latent, q_rope, scale: float,
     return out
 
 
+# ------------------------------------------------- 8-bit cache, planned attention ----
+def _dtype_of(code: int):
+    torch = _torch()
+    return torch.float16 if code == DTYPE_F16 else torch.bfloat16
+
+
+def _check(what: str, t, shape, dtype) -> None:
+    """A contiguous tensor of this shape (None: any size) and type on the current GPU, or
+    ValueError: the kernels see addresses only."""
+    torch = _torch()
+    if (t.dtype != dtype or len(t.shape) != len(shape) or not t.is_contiguous() or
+            any(n is not None and n != m for n, m in zip(shape, t.shape))):
+        raise ValueError(f"{what}: wanted a contiguous {dtype} tensor of shape {tuple(shape)}, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: wanted on the current GPU, is on {t.device}")
+
+
+class QuantizedLatentCache:
+    """Device page pool of the 8-bit latent cache: uint8 [layers, pages, record bytes], a record
+    as mla_hip.h lays it out (e4m3 latents with a power-of-two scale for each 32 columns, rope
+    keys in 16 bits of ``dtype``)."""
+
+    def __init__(self, n_layers: int, num_pages: int, page_size: int, kv_rank: int,
+                 rope_dim: int, dtype: int = DTYPE_F16, device="cuda", storage=None):
+        torch = _torch()
+        self.n_layers, self.num_pages, self.page_size = n_layers, num_pages, page_size
+        self.kv_rank, self.rope_dim, self.dtype = kv_rank, rope_dim, dtype
+        rec = int(lib().mla_q8_page_bytes(page_size, kv_rank, rope_dim))
+        if rec == 0:
+            raise ValueError("8-bit latent cache: page_size must be a multiple of 16, kv_rank of "
+                             "32 up to 512, rope_dim of 8 up to 64")
+        if storage is None:
+            storage = torch.zeros((n_layers, num_pages, rec), dtype=torch.uint8, device=device)
+        if (tuple(storage.shape) != (n_layers, num_pages, rec) or storage.dtype != torch.uint8 or
+                not storage.is_contiguous()):
+            raise ValueError(f"8-bit latent cache: storage must be a contiguous uint8 tensor of "
+                             f"shape {(n_layers, num_pages, rec)}")
+        self.pages = storage
+
+    def layer(self, l: int):
+        return self.pages[l]
+
+    @property
+    def record_bytes(self) -> int:
+        return int(self.pages.shape[2])
+
+
+def append_latent_q8(cache: QuantizedLatentCache, layer: int, ckv, krope, slot_mapping,
+                     stream=None) -> None:
+    """(d) Quantise ckv [T x kv_rank] (fp32) to 8 bits, round krope [T x rope_dim] (fp32) to the
+    cache's 16-bit dtype, and write row t to flat slot slot_mapping[t] of ``layer``'s pool.  Slots
+    outside the pool are skipped; the others are distinct."""
+    torch = _torch()
+    T, pages = int(ckv.shape[0]), cache.layer(layer)
+    _check("ckv", ckv, (T, cache.kv_rank), torch.float32)
+    _check("krope", krope, (T, cache.rope_dim), torch.float32)
+    _check("slot_mapping", slot_mapping, (None,), torch.int32)
+    _check("cache", pages, (None, None), torch.uint8)
+    if slot_mapping.shape[0] < T:
+        raise ValueError(f"slot_mapping: {slot_mapping.shape[0]} slots for {T} rows")
+    check(lib().mla_append_latent_q8(stream_handle(stream), T, cache.kv_rank, cache.rope_dim,
+                                     cache.page_size, cache.dtype, ptr(ckv), ptr(krope),
+                                     ptr(slot_mapping), cache.num_pages, ptr(pages)))
+
+
+def read_latent_q8(cache: QuantizedLatentCache, layer: int, slot_mapping, ckv=None, krope=None,
+                   stream=None):
+    """(d) The tokens at flat slots slot_mapping[T] of ``layer``'s pool as 16-bit rows of the
+    cache's dtype: (ckv [T x kv_rank], krope [T x rope_dim]), exact.  Rows whose slot lies outside
+    the pool are left as they were (zero in tensors that this call makes)."""
+    torch = _torch()
+    T, pages, dt = int(slot_mapping.shape[0]), cache.layer(layer), _dtype_of(cache.dtype)
+    if ckv is None:
+        ckv = torch.zeros((T, cache.kv_rank), dtype=dt, device=pages.device)
+    if krope is None:
+        krope = torch.zeros((T, cache.rope_dim), dtype=dt, device=pages.device)
+    _check("slot_mapping", slot_mapping, (T,), torch.int32)
+    _check("ckv", ckv, (T, cache.kv_rank), dt)
+    _check("krope", krope, (T, cache.rope_dim), dt)
+    _check("cache", pages, (None, None), torch.uint8)
+    check(lib().mla_read_latent_q8(stream_handle(stream), T, cache.kv_rank, cache.rope_dim,
+                                   cache.page_size, cache.dtype, ptr(slot_mapping),
+                                   cache.num_pages, ptr(pages), ptr(ckv), ptr(krope)))
+    return ckv, krope
+
+
+@dataclass
+class SharedPrefixes:
+    """Prefixes that groups of consecutive sessions share (device int32 tensors): group g is the
+    sessions [cu_groups[g], cu_groups[g+1]), its prefix prefix_len[g] tokens on the pages
+    page_ids[cu_pages[g]:cu_pages[g+1]]."""
+
+    cu_groups: object
+    prefix_len: object
+    cu_pages: object
+    page_ids: object
+
+    @property
+    def n_groups(self) -> int:
+        return int(self.prefix_len.shape[0])
+
+
+@dataclass
+class AttentionPlan:
+    """What ``plan_attention`` built, for ``latent_attention`` calls over the same batch."""
+
+    batch: RaggedBatch
+    n_heads: int
+    kv_rank: int
+    rows: int
+    max_q_len: int
+    prefixes: SharedPrefixes | None
+    words: object  # the plan itself (device int32)
+
+    @property
+    def n_groups(self) -> int:
+        return self.prefixes.n_groups if self.prefixes is not None else 0
+
+    def read_info(self, stream=None):
+        """Synchronise and return [jobs, 0, jobs of few rows, jobs of many rows, partial rows,
+        query rows, ..]; raises when the batch or the prefixes are invalid."""
+        import numpy as np
+        h = np.zeros(PLAN_INFO_INTS, np.int32)
+        check(lib().mla_read_plan_info(stream_handle(stream), ptr(self.words), h.ctypes.data))
+        return h.tolist()
+
+
+def plan_attention(batch: RaggedBatch, n_heads: int, kv_rank: int, *, rows: int | None = None,
+                   max_q_len: int = 1, prefixes: SharedPrefixes | None = None,
+                   stream=None) -> AttentionPlan:
+    """(e) Plan the attention of a batch (one launch): which workgroup takes which query rows over
+    which keys.  ``rows``: query rows of the calls (default the batch's max_rows); ``max_q_len``:
+    at least every session's q_len.  The plan serves every layer's ``latent_attention``."""
+    torch = _torch()
+    rows = batch.max_rows if rows is None else rows
+    groups = 0
+    if prefixes is not None:
+        groups = prefixes.n_groups
+        _check("cu_groups", prefixes.cu_groups, (groups + 1,), torch.int32)
+        _check("prefix_len", prefixes.prefix_len, (groups,), torch.int32)
+        _check("cu_pages", prefixes.cu_pages, (groups + 1,), torch.int32)
+        _check("page_ids", prefixes.page_ids, (None,), torch.int32)
+    n = int(lib().mla_attention_plan_bytes(batch.B, rows, n_heads, kv_rank, max_q_len, groups))
+    if n == 0:
+        raise ValueError(f"plan_attention: no plan for B={batch.B}, rows={rows}, n_heads={n_heads}, "
+                         f"kv_rank={kv_rank}, max_q_len={max_q_len}, groups={groups}")
+    words = torch.empty(n // 4, dtype=torch.int32, device=batch.info.device)
+    _check("batch", batch.info, (None,), torch.int32)
+    x = prefixes
+    check(lib().mla_plan_attention(
+        stream_handle(stream), batch.B, rows, n_heads, kv_rank, batch.page_size, max_q_len,
+        ptr(batch.cu_seqlens_q), ptr(batch.cu_seqlens_k), ptr(batch.info), groups,
+        ptr(x.cu_groups) if x else None, ptr(x.prefix_len) if x else None,
+        ptr(x.cu_pages) if x else None, ptr(x.page_ids) if x else None,
+        int(x.page_ids.shape[0]) if x else 0, batch.num_pool_pages, ptr(words), n))
+    return AttentionPlan(batch, n_heads, kv_rank, rows, max_q_len, prefixes, words)
+
+
+def attention_workspace(plan: AttentionPlan):
+    """Workspace of ``latent_attention`` calls with this plan (or one of the same sizes).  Calls
+    that share one are ordered on one stream."""
+    torch = _torch()
+    n = int(lib().mla_attention_workspace_bytes(plan.batch.B, plan.rows, plan.n_heads,
+                                                plan.kv_rank, plan.max_q_len, plan.n_groups))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=plan.words.device)
+
+
+def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float, *,
+                     rope_dim: int, dtype: int = DTYPE_F16, q8: bool = False, out=None, lse=None,
+                     workspace=None, stream=None):
+    """(e) Attention of every query row of the plan's batch over its cache and its group's prefix:
+    ``pages`` is a layer of a PagedLatentCache or, with ``q8``, of a QuantizedLatentCache.
+    q_latent [rows, H, kv_rank] and q_rope [rows, H, rope_dim] in ``dtype``; returns out
+    [rows, H, kv_rank] in ``dtype`` (and fills lse [rows, H], fp32, if given).  Rows past the
+    batch's are left as they were."""
+    torch = _torch()
+    b, rows, H, kv, x = plan.batch, plan.rows, plan.n_heads, plan.kv_rank, plan.prefixes
+    dt = _dtype_of(dtype)
+    if out is None:
+        out = torch.zeros((rows, H, kv), dtype=dt, device=q_latent.device)
+    if workspace is None:
+        workspace = attention_workspace(plan)
+    _check("q_latent", q_latent, (rows, H, kv), dt)
+    _check("q_rope", q_rope, (rows, H, rope_dim), dt)
+    _check("out", out, (rows, H, kv), dt)
+    _check("workspace", workspace, (None,), torch.uint8)
+    if lse is not None:
+        _check("lse", lse, (rows, H), torch.float32)
+    if q8:
+        rec = int(lib().mla_q8_page_bytes(b.page_size, kv, rope_dim))
+        _check("pages", pages, (b.num_pool_pages, rec), torch.uint8)
+    else:
+        _check("pages", pages, (b.num_pool_pages, b.page_size * (kv + rope_dim)), dt)
+    check(lib().mla_latent_attention(
+        stream_handle(stream), b.B, rows, H, kv, rope_dim, b.page_size, plan.max_q_len, dtype,
+        CACHE_Q8 if q8 else CACHE_16BIT, float(scale), ptr(b.page_table), b.max_pages,
+        b.num_pool_pages, ptr(pages), ptr(q_latent), ptr(q_rope), plan.n_groups,
+        ptr(x.cu_pages) if x else None, ptr(x.page_ids) if x else None, ptr(plan.words),
+        plan.words.numel() * 4, ptr(out), ptr(lse), ptr(workspace), workspace.numel()))
+    return out
+
+
 __all__ = ["RaggedBatch", "build_metadata", "PagedLatentCache", "append_latent",
            "decode_workspace_bytes", "decode_workspace", "decode_status", "decode_attention",
-           "decode_partials", "decode_merge", "prefill_attention", "DTYPE_F16", "DTYPE_BF16"]
+           "decode_partials", "decode_merge", "prefill_attention", "QuantizedLatentCache",
+           "append_latent_q8", "read_latent_q8", "SharedPrefixes", "AttentionPlan",
+           "plan_attention", "attention_workspace", "latent_attention", "DTYPE_F16",
+           "DTYPE_BF16"]
 
 
 # ---------------------------------------------------------------- page layout ----

@@ -318,6 +318,102 @@ int mla_prefill_attention(void* stream, int B, int n_heads, int kv_rank, int rop
                           const void* q_rope, const int32_t* info, int max_q_len, float* out,
                           float* lse, int flags);
 
+/* ------------------------------------------------------------------ (d)
+ * The 8-bit latent cache: a page pool as above with the latents in 8 bits, 164 bytes a token
+ * instead of 288 at kv_rank 128 and rope_dim 16.  No reference counterpart (its cache is fp16,
+ * src/infer/inference.cpp:15-18).  A token's latent is cut into blocks of 32 columns; a block
+ * holds e4m3 (OCP) values and one scale 2^k, k the smallest with max|x| <= 448 * 2^k over the
+ * block's finite values, held to -15..7 (MLA_DTYPE_F16) or -117..119 (MLA_DTYPE_BF16): every
+ * stored value is then a value of the 16-bit type as well, and rounding to e4m3 (to nearest even)
+ * the only rounding.  Larger finite values saturate (57,344 for F16); an infinity or NaN is stored
+ * as NaN.  Rope keys stay 16-bit words of `dtype`, rounded as mla_append_latent rounds them.
+ * Page p is one record of mla_q8_page_bytes bytes: latents, rope keys, scales.  With t = slot/16,
+ * n = slot%16, j = column/32, g = column%32/8, e = column%8 and J = kv_rank/32
+ *     latent  byte t*16*kv_rank + (j/2)*1024 + (16 g + n)*16 + (j%2)*8 + e
+ *             (J odd, j = J-1: t*16*kv_rank + j*512 + (16 g + n)*8 + e)
+ *     rope    word (t*(rope_dim/8) + c/8)*128 + n*8 + c%8 of the section at byte page_size*kv_rank
+ *     scale   byte page_size*(kv_rank + 2 rope_dim) + slot*J + j, holding k + 127
+ * Shapes: page_size % 16 == 0, kv_rank % 32 == 0 up to 512, rope_dim % 8 == 0 up to 64
+ * (MLA_ERR_UNSUPPORTED otherwise); pages at a multiple of 16 bytes. */
+/* Bytes of a page record, 0 for a shape outside the above. */
+size_t mla_q8_page_bytes(int page_size, int kv_rank, int rope_dim);
+/* mla_append_latent into an 8-bit pool: row t of ckv [T x kv_rank] and krope [T x rope_dim]
+ * (device fp32) goes to flat slot slot_mapping[t]; slots outside the pool are skipped.  The slots
+ * of a call are distinct, as mla_build_metadata makes them: two rows with one slot leave a mix of
+ * the two there. */
+int mla_append_latent_q8(void* stream, int T, int kv_rank, int rope_dim, int page_size, int dtype,
+                         const float* ckv, const float* krope, const int32_t* slot_mapping,
+                         int num_pool_pages, void* pages);
+/* The reverse: row t of ckv [T x kv_rank] and krope [T x rope_dim], 16-bit words of `dtype` at
+ * multiples of 16 bytes, receives the token at flat slot slot_mapping[t], exactly (see above).
+ * Rows whose slot lies outside the pool are left as they were; a slot may be named twice. */
+int mla_read_latent_q8(void* stream, int T, int kv_rank, int rope_dim, int page_size, int dtype,
+                       const int32_t* slot_mapping, int num_pool_pages, const void* pages,
+                       void* ckv, void* krope);
+
+/* ------------------------------------------------------------------ (e)
+ * Planned attention: every query row of a batch -- decode rows, the rows of drafted tokens, prompt
+ * chunks, mixed -- over a 16-bit or an 8-bit pool, with prefixes that groups of sessions share
+ * read and multiplied once for the group.  For query row i of a session with ctx tokens cached
+ * before the call's rows, in a group whose prefix has P tokens (0 without one)
+ *     s_j = (q_latent[h] . c_j + q_rope[h] . k_j) * scale
+ *     over the P keys of the prefix and the session's own keys j <= ctx + i,
+ *     out[h] = sum_j softmax(s)_j c_j,   lse[h] = ln(sum_j exp(s_j)):
+ * mla_decode_attention and mla_prefill_attention of the concatenated cache (the reference's
+ * src/infer/inference.cpp:116-153 and src/model/ops.cpp:109-142).  `out` holds 16-bit words of
+ * `dtype`, as the queries do: sums, maxima and masses are fp32, the softmax weights are rounded to
+ * `dtype` where they enter the product, and the row once at the end.
+ *
+ * The plan says which workgroup takes which rows over which keys, and what is added up in the end.
+ * It is built on the device from one mla_build_metadata call's cu_seqlens_q, cu_seqlens_k and
+ * info, once for a batch, and serves any number of calls (all layers of a step).  Plan and calls
+ * take the same B, rows (the rows of q_latent; at least the batch's, rows past those are left as
+ * they were), n_heads, kv_rank, max_q_len (at least every session's q_len) and n_groups; a call
+ * with a plan made for others writes nothing.
+ *
+ * Shared prefixes: group g is the sessions [cu_groups[g], cu_groups[g+1]) (n_groups <= B; sessions
+ * outside every group have no prefix); its prefix is prefix_len[g] tokens on the pool's pages
+ * prefix_page_ids[cu_prefix_pages[g] ..], from slot 0 of the first; the last page may be partial.
+ * The sessions' ctx_len, page lists and slots count their own tokens only.  All device int32. */
+#define MLA_CACHE_16BIT 0 /* the page records of mla_append_latent */
+#define MLA_CACHE_Q8 1    /* those of mla_append_latent_q8 */
+#define MLA_PLAN_INFO_INTS 8
+/* Sizes of a plan and of a call's workspace, 0 for sizes that no plan takes (a plan takes
+ * rows * n_heads up to 2^30). */
+size_t mla_attention_plan_bytes(int B, int rows, int n_heads, int kv_rank, int max_q_len,
+                                int n_groups);
+size_t mla_attention_workspace_bytes(int B, int rows, int n_heads, int kv_rank, int max_q_len,
+                                     int n_groups);
+/* Builds the plan (one launch).  n_prefix_pages is the length of prefix_page_ids.  What the device
+ * arrays get wrong -- a failed metadata build, more rows than `rows`, a session past max_q_len,
+ * groups that overlap or leave [0, B], a prefix longer than its page list, a page id outside the
+ * pool -- fails the plan: mla_read_plan_info reports it, and calls with a failed plan write
+ * nothing. */
+int mla_plan_attention(void* stream, int B, int rows, int n_heads, int kv_rank, int page_size,
+                       int max_q_len, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                       const int32_t* info, int n_groups, const int32_t* cu_groups,
+                       const int32_t* prefix_len, const int32_t* cu_prefix_pages,
+                       const int32_t* prefix_page_ids, int n_prefix_pages, int num_pool_pages,
+                       void* plan, size_t plan_bytes);
+/* Synchronises `stream` and copies host_info[MLA_PLAN_INFO_INTS]: {jobs, 0, jobs of few rows, jobs
+ * of many rows, partial rows, query rows, 0 or more of no meaning}, or {-1, first bad entry, ..}
+ * with MLA_ERR_INVALID_ARGUMENT and a message. */
+int mla_read_plan_info(void* stream, const void* plan, int32_t* host_info);
+/* The attention.  page_table and max_pages are those of the metadata, cache_format one of
+ * MLA_CACHE_*, q_latent [rows x n_heads x kv_rank], q_rope [rows x n_heads x rope_dim] and out
+ * [rows x n_heads x kv_rank] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.  Shapes
+ * as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace at multiples of 16
+ * bytes.  The workspace needs no initialisation; calls that share one must be ordered on one
+ * stream.  Page ids outside the pool are skipped, with the keys on them.  A non-finite latent
+ * makes the rows that see its key NaN, and no others. */
+int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank, int rope_dim,
+                         int page_size, int max_q_len, int dtype, int cache_format, float scale,
+                         const int32_t* page_table, int max_pages, int num_pool_pages,
+                         const void* pages, const void* q_latent, const void* q_rope, int n_groups,
+                         const int32_t* cu_prefix_pages, const int32_t* prefix_page_ids,
+                         const void* plan, size_t plan_bytes, void* out, float* lse,
+                         void* workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------------ model
  * The batched decode step around the attention: everything of
  * CpuDecoder::decode (src/infer/inference.cpp:76-173) for B sessions at once,
