@@ -84,16 +84,20 @@ __device__ __forceinline__ bool drop_nan8(u32x4& v) {
 }
 
 // T: 16-bit type of the queries, rope keys, 16-bit latents and rows; Q8: 8-bit latents; KSM: latent
-// k-steps (kv_rank / 32 <= KSM); QT: 16-row tiles of a wave; ROWS: list R.
-template <typename T, bool Q8, int KSM, int QT, bool ROWS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
-    KSM >= 16 ? 1 : 2, 8))) void latent_attend_kernel(LatentArgs a) {
-    constexpr int RSM = 2;                              // rope k-steps (rope_dim <= 64)
+// k-steps (kv_rank / 32 <= KSM); QT: 16-row tiles of a wave; ROWS: list R; RP_: the rope columns of
+// an instantiation for one shape (kv_rank = 32 KSM, rope_dim = RP_), -1 for any.
+template <typename T, bool Q8, int KSM, int QT, bool ROWS, int RP_ = -1>
+__global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__((
+    amdgpu_waves_per_eu(KSM >= 16 && !ROWS ? 1 : 2, 8))) void latent_attend_kernel(LatentArgs a) {
+    constexpr int NW = ROWS ? kRowsR / (16 * QT) : 4;   // waves
+    constexpr bool ONE = RP_ >= 0;
+    constexpr int RSM = ONE ? (RP_ + 31) / 32 : 2;      // rope k-steps (rope_dim <= 64)
     constexpr int RTM = 2 * KSM;                        // 16-row tiles of O^T
     constexpr int SLOT = 32 * 32 * (KSM + RSM);         // words of a unit
     constexpr int UPT = Q8 ? (KSM + 1) / 2 : KSM;       // 16-byte loads of a lane per tile
-    constexpr int NL = ROWS ? (2 * UPT + 3) / 4 : 2 * UPT;
-    constexpr int NR = ROWS ? 1 : 2 * RSM;              // rope loads: 2 * rope_dim / 8 chunks
+    constexpr int NL = ROWS ? (2 * UPT + NW - 1) / NW : 2 * UPT;
+    constexpr int RCS = ONE ? RP_ / 8 : 8;              // rope chunks of a tile, at most
+    constexpr int NR = ROWS ? 1 : (2 * RCS + 3) / 4;    // rope loads of a lane per unit
     constexpr int SLOTS = ROWS ? 2 : 4;
     using V8 = typename T::vec8;
     __shared__ __attribute__((aligned(16))) uint16_t smem[SLOTS][SLOT];
@@ -108,12 +112,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int H = a.H, KV = a.kv_rank, RP = a.rope_dim, PS = a.page_size;
+    const int H = a.H, PS = a.page_size;
+    const int KV = ONE ? 32 * KSM : a.kv_rank, RP = ONE ? RP_ : a.rope_dim;
     const int ks = KV >> 5, rs = (RP + 31) >> 5, tpp = PS >> 4;
     const long long rec = Q8 ? q8_page_bytes(PS, KV, RP) : 2LL * PS * (KV + RP);
     const int32_t* ptab = seg >= 0 ? a.page_table + (long long)seg * a.max_pages
                                    : a.prefix_page_ids + a.cu_prefix_pages[~seg];
-    const int n_units = key_end > key0 ? (key_end - key0 + 31) >> 5 : 0;
+    const int n_units = key_end > key0 && a.num_pool_pages > 0 ? (key_end - key0 + 31) >> 5 : 0;
     const int row0 = ROWS ? 16 * QT * wave : 0;  // the wave's first row of the block
 
     // ---- Q^T operands: row 16q + n, latent columns 32j + 8g .., then the rope key's ----
@@ -122,20 +127,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
     int lim_wave = -1;
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-        const int r = row0 + 16 * q + n;
-        const bool ok = r < n_rows;
+        const int r = min(row0 + 16 * q + n, n_rows - 1);  // rows past the block repeat its last
         const long long fr = (long long)f0 + r;
         lim[q] = a.causal && seg >= 0 ? ctx + (rb + r) / H : key_end - 1;
+        const uint16_t* ql = a.q_latent + fr * KV + 8 * g;
+        const uint16_t* qr = a.q_rope + fr * RP;
 #pragma unroll
         for (int j = 0; j < KSM; ++j)
-            qv[q][j] = ok && j < ks
-                           ? *reinterpret_cast<const V8*>(a.q_latent + fr * KV + 32 * j + 8 * g)
-                           : V8{};
+            qv[q][j] = j < ks ? *reinterpret_cast<const V8*>(ql + 32 * j) : V8{};
 #pragma unroll
-        for (int j = 0; j < RSM; ++j)
-            qv[q][KSM + j] = ok && 32 * j + 8 * g < RP
-                                 ? *reinterpret_cast<const V8*>(a.q_rope + fr * RP + 32 * j + 8 * g)
-                                 : V8{};
+        for (int j = 0; j < RSM; ++j) {
+            const int c = 32 * j + 8 * g;
+            const V8 v = j < rs ? *reinterpret_cast<const V8*>(qr + min(c, RP - 8)) : V8{};
+            qv[q][KSM + j] = c < RP ? v : V8{};
+        }
     }
     {   // the last key that any of the wave's rows sees (-1: it has no rows)
         const int last = min(n_rows, row0 + 16 * QT) - 1;
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
     int rope_tt[NR], rope_ch[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        const int c = ROWS ? tid >> 4 : 4 * i + g;
+        const int c = ROWS ? tid >> 4 : 4 * i + g;  // (list R: 16 chunks, all of a unit's)
         rope_tt[i] = c >= rcs;
         rope_ch[i] = c < 2 * rcs ? (c >= rcs ? c - rcs : c) : -1;
     }
@@ -161,18 +166,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
         const int id = 16 * t < key_end ? __builtin_amdgcn_readfirstlane(ptab[t / tpp]) : -1;
         return (unsigned)id < (unsigned)a.num_pool_pages ? id : -1;
     };
+    // The unit's keys that exist: before key_end, on a page of the pool.
+    auto keys_of = [&](int t0, int pg0, int pg1) {
+        const int valid = min(32, key_end - 16 * t0);
+        uint32_t ok = valid >= 32 ? 0xffffffffu : (1u << valid) - 1u;
+        if (pg0 < 0)
+            ok &= 0xffff0000u;
+        if (pg1 < 0)
+            ok &= 0x0000ffffu;
+        return ok;
+    };
+    // (A missing tile loads page 0's, and is dropped when it is staged.)
     auto load_unit = [&](int t0, int pg0, int pg1) {
-        const uint8_t* base0 = a.pages + pg0 * rec;
-        const uint8_t* base1 = a.pages + pg1 * rec;
+        const uint8_t* base0 = a.pages + max(pg0, 0) * rec;
+        const uint8_t* base1 = a.pages + max(pg1, 0) * rec;
         const int in0 = t0 % tpp, in1 = (t0 + 1) % tpp;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int u = ROWS ? wave + 4 * i : i;
+            const int u = ROWS ? wave + NW * i : i;
             const int tt = u / UPT, k = u % UPT;
-            st[i] = u32x4{0, 0, 0, 0};
-            if constexpr (Q8)
-                sk[i] = 0;
-            if (u >= 2 * UPT || k >= upt || (tt ? pg1 : pg0) < 0)
+            if (u >= 2 * UPT || k >= upt)
                 continue;
             const uint8_t* base = tt ? base1 : base0;
             const int in = tt ? in1 : in0;
@@ -184,8 +197,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
                     sk[i] = ks & 1 ? sc[0] | sc[1] << 8 : *reinterpret_cast<const uint16_t*>(sc);
                 } else {
                     const u32x2 x = *reinterpret_cast<const u32x2*>(lat + lane * 8);
-                    st[i][0] = x[0];
-                    st[i][1] = x[1];
+                    st[i] = u32x4{x[0], x[1], 0, 0};
                     sk[i] = sc[0];
                 }
             } else {
@@ -193,30 +205,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
             }
         }
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            sr[i] = u32x4{0, 0, 0, 0};
-            if (rope_ch[i] >= 0 && (rope_tt[i] ? pg1 : pg0) >= 0)
+        for (int i = 0; i < NR; ++i)
+            if (rope_ch[i] >= 0)
                 sr[i] = *reinterpret_cast<const u32x4*>(
                     (rope_tt[i] ? base1 : base0) + (long long)PS * KV * (Q8 ? 1 : 2) +
                     ((rope_tt[i] ? in1 : in0) * rcs + rope_ch[i]) * 256 + n * 16);
-        }
     };
-    // Writes the loaded unit to `sp`; keys [valid, 32) become 0.  Returns the wave's marked keys.
-    auto stage_unit = [&](uint16_t* sp, int valid) {
+    // Writes the loaded unit to `sp`; keys outside `ok` become 0 (their slots, scales included, may
+    // hold anything).  Returns the wave's marked keys.
+    auto stage_unit = [&](uint16_t* sp, uint32_t ok) {
         uint32_t mark = 0;
+        int causal = a.causal;
+        asm("" : "+s"(causal));  // looked at anew each time: one copy of the loop, not two
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int u = ROWS ? wave + 4 * i : i;
+            const int u = ROWS ? wave + NW * i : i;
             const int tt = u / UPT, k = u % UPT;
             if (u >= 2 * UPT || k >= upt)
                 continue;
             u32x4 v = st[i];
             uint32_t k8 = Q8 ? sk[i] : 0;
-            if (valid < 32 && 16 * tt + n >= valid) {
-                v = u32x4{0, 0, 0, 0};
-                k8 = 0;  // a free slot's scale may be anything too
+            if (ok != 0xffffffffu) {
+                const uint32_t keep = -(ok >> (16 * tt + n) & 1);
+                v &= keep;
+                k8 &= keep;
             }
-            if (a.causal) {
+            if (causal) {
                 bool bad;
                 if constexpr (Q8)
                     bad = drop_nan8(v);
@@ -241,8 +255,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
         for (int i = 0; i < NR; ++i)
             if (rope_ch[i] >= 0) {
                 u32x4 v = sr[i];
-                if (valid < 32 && 16 * rope_tt[i] + n >= valid)
-                    v = u32x4{0, 0, 0, 0};
+                if (ok != 0xffffffffu)
+                    v &= -(ok >> (16 * rope_tt[i] + n) & 1);
                 *reinterpret_cast<u32x4*>(sp + 32 * KV + rope_tt[i] * 16 * RP + rope_ch[i] * 128 +
                                           n * 8) = v;
             }
@@ -276,28 +290,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
             for (int q = 0; q < QT; ++q)
                 sc[tt][q] = floatx4{0, 0, 0, 0};
+        // One k-step's operands are read while the step before it multiplies; the scheduler is held
+        // to that (it would read all of them ahead, and spill).
+        auto k_operand = [&](int tt, int j) {
+            return j < KSM ? *reinterpret_cast<const V8*>(sp + tt * 16 * KV + j * 512 + s_lane)
+                           : *reinterpret_cast<const V8*>(sp + 32 * KV + tt * 16 * RP +
+                                                          rope_off[j - KSM]);
+        };
+        V8 next[2] = {k_operand(0, 0), k_operand(1, 0)};
 #pragma unroll
-        for (int j = 0; j < KSM; ++j)
-            if (j < ks)
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const V8 ka =
-                        *reinterpret_cast<const V8*>(sp + tt * 16 * KV + j * 512 + s_lane);
-#pragma unroll
-                    for (int q = 0; q < QT; ++q)
-                        sc[tt][q] = T::mma32(ka, qv[q][j], sc[tt][q]);
+        for (int j = 0; j < KSM + RSM; ++j)
+            if (j < KSM ? j < ks : j - KSM < rs) {
+                const V8 now[2] = {next[0], next[1]};
+                const int after = j + 1 < ks ? j + 1 : (j < KSM ? KSM : j + 1);
+                if (after < KSM + rs) {
+                    next[0] = k_operand(0, after);
+                    next[1] = k_operand(1, after);
                 }
 #pragma unroll
-        for (int j = 0; j < RSM; ++j)
-            if (j < rs)
+                for (int q = 0; q < QT; ++q)
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const V8 ka = *reinterpret_cast<const V8*>(sp + 32 * KV + tt * 16 * RP +
-                                                               rope_off[j]);
-#pragma unroll
-                    for (int q = 0; q < QT; ++q)
-                        sc[tt][q] = T::mma32(ka, qv[q][KSM + j], sc[tt][q]);
-                }
+                    for (int tt = 0; tt < 2; ++tt)
+                        sc[tt][q] = T::mma32(now[tt], qv[q][j], sc[tt][q]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 
         V8 pb[QT];
 #pragma unroll
@@ -342,33 +358,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
                 }
             l_run[q] += psum;
         }
+        auto c_operand = [&](int rt) {  // latent columns 16rt.. of the unit's 32 keys
+            const int blk = ((rt >> 1) * 4 + 2 * (rt & 1)) * 128;
+            const u32x2 lo = read_tr16(sp + blk + tr_lane);
+            const u32x2 hi = read_tr16(sp + 16 * KV + blk + tr_lane);
+            return __builtin_bit_cast(V8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+        };
+        V8 cn[2] = {c_operand(0), c_operand(1)};
 #pragma unroll
-        for (int rt = 0; rt < RTM; ++rt)
+        for (int rt = 0; rt < RTM; rt += 2)
             if (rt < 2 * ks) {
-                const int blk = ((rt >> 1) * 4 + 2 * (rt & 1)) * 128;  // latent columns 16rt..
-                const u32x2 lo = read_tr16(sp + blk + tr_lane);
-                const u32x2 hi = read_tr16(sp + 16 * KV + blk + tr_lane);
-                const V8 ca = __builtin_bit_cast(V8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+                const V8 now[2] = {cn[0], cn[1]};
+                if (rt + 2 < 2 * ks) {
+                    cn[0] = c_operand(rt + 2);
+                    cn[1] = c_operand(rt + 3);
+                }
 #pragma unroll
                 for (int q = 0; q < QT; ++q)
-                    acc[q][rt] = T::mma32(ca, pb[q], acc[q][rt]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        acc[q][rt + i] = T::mma32(now[i], pb[q], acc[q][rt + i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
     };
-    // The unit's keys that exist: before key_end, on a page of the pool.
-    auto keys_of = [&](int t0, int pg0, int pg1) {
-        const int valid = min(32, key_end - 16 * t0);
-        uint32_t ok = valid >= 32 ? 0xffffffffu : (1u << valid) - 1u;
-        if (pg0 < 0)
-            ok &= 0xffff0000u;
-        if (pg1 < 0)
-            ok &= 0x0000ffffu;
-        return ok;
-    };
-
     // ---- the units: loaded one ahead, page ids two ahead ----
     constexpr int STEP = ROWS ? 1 : 4;
     const int first = ROWS ? 0 : wave, tile0 = key0 >> 4;
-    if (ROWS && a.causal) {
+    if constexpr (ROWS) {
         if (tid < 3)
             marks[tid] = 0;
         __syncthreads();
@@ -387,8 +403,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
         const int t0 = tile0 + 2 * u;
         uint16_t* sp = smem[ROWS ? u & 1 : wave];
         const uint32_t ok = keys_of(t0, pg0, pg1);
-        uint32_t mark = stage_unit(sp, min(32, key_end - 16 * t0));
-        if (ROWS && a.causal && mark && lane == 0)
+        uint32_t mark = stage_unit(sp, ok);
+        if (ROWS && mark && lane == 0)
             atomicOr(&marks[u % 3], mark);
         if (u + STEP < n_units) {
             load_unit(t0 + 2 * STEP, nx0, nx1);
@@ -404,11 +420,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
             // finished with it.  Likewise marks: unit u + 2's word, last read in unit u - 1, is
             // cleared behind this barrier and set again behind the next.
             __syncthreads();
-            if (a.causal) {
-                mark = marks[u % 3];
-                if (tid == 0)
-                    marks[(u + 2) % 3] = 0;
-            }
+            mark = marks[u % 3];
+            if (tid == 0)
+                marks[(u + 2) % 3] = 0;
         } else {
             wave_lds_fence();
         }
@@ -512,21 +526,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(
     }
 }
 
-template <typename T, bool Q8, int KSM, int QT, bool ROWS>
+template <typename T, bool Q8, int KSM, int QT, bool ROWS, int RP = -1>
 hipError_t launch_one(const LatentArgs& a, hipStream_t stream) {
     const int jobs = ROWS ? a.p.max_jobs_r : a.p.max_jobs_k;
-    hipLaunchKernelGGL((latent_attend_kernel<T, Q8, KSM, QT, ROWS>), dim3(jobs), dim3(256), 0,
-                       stream, a);
+    hipLaunchKernelGGL((latent_attend_kernel<T, Q8, KSM, QT, ROWS, RP>), dim3(jobs),
+                       dim3(ROWS ? 64 * kRowsR / (16 * QT) : 256), 0, stream, a);
     return hipGetLastError();
 }
 
 template <typename T, bool Q8>
 hipError_t launch_list(const LatentArgs& a, bool rows, hipStream_t stream) {
     const int ks = a.kv_rank / 32;
+    const bool base = ks == 4 && a.rope_dim == 16, wide = ks == 16 && a.rope_dim == 64;
+    if (rows && base)
+        return launch_one<T, Q8, 4, 2, true, 16>(a, stream);
+    if (rows && wide)
+        return launch_one<T, Q8, 16, 1, true, 64>(a, stream);
+    if (base)
+        return a.p.qt == 2 ? launch_one<T, Q8, 4, 2, false, 16>(a, stream)
+                           : launch_one<T, Q8, 4, 1, false, 16>(a, stream);
+    if (wide)
+        return launch_one<T, Q8, 16, 1, false, 64>(a, stream);
     if (rows)
         return ks <= 4   ? launch_one<T, Q8, 4, 2, true>(a, stream)
-               : ks <= 8 ? launch_one<T, Q8, 8, 2, true>(a, stream)
-                         : launch_one<T, Q8, 16, 2, true>(a, stream);
+               : ks <= 8 ? launch_one<T, Q8, 8, 1, true>(a, stream)
+                         : launch_one<T, Q8, 16, 1, true>(a, stream);
     if (a.p.qt == 2)
         return launch_one<T, Q8, 4, 2, false>(a, stream);
     return ks <= 4   ? launch_one<T, Q8, 4, 1, false>(a, stream)
