@@ -255,7 +255,8 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
     p.kv_rank = kv_rank;
     p.max_q_len = max_q_len;
     const long long flat = (long long)rows * H;
-    const long long own = std::min<long long>(kFewRows, (long long)max_q_len * H);
+    const long long own_most = std::min(flat, (long long)max_q_len * H);  // rows of a session
+    const long long own = std::min<long long>(kFewRows, own_most);
     p.qt = kv_rank <= 128 && own > 16 ? 2 : 1;
     p.target_k = kv_rank <= 128 ? 768 : 256;
     p.target_r = kv_rank <= 128 ? 512 : 256;
@@ -266,8 +267,10 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
     const long long blocks_k =
         std::min(segs * (kFewRows / (16 * p.qt)), sides * (flat / (16 * p.qt)) + segs);
     const long long blocks_r = sides * (flat / kRowsR) + std::min(segs, sides * (flat / (kFewRows + 1)));
-    p.max_jobs_k = (int)(p.target_k + blocks_k);
-    p.max_jobs_r = flat > kFewRows ? (int)(p.target_r + blocks_r) : 0;
+    // a list that no segment of these sizes can be on is not launched
+    const bool few = H <= kFewRows, many = own_most > kFewRows || (groups > 0 && flat > kFewRows);
+    p.max_jobs_k = few ? (int)(p.target_k + blocks_k) : 0;
+    p.max_jobs_r = many ? (int)(p.target_r + blocks_r) : 0;
     // rows of a segment cut into s >= 2 ranges: n s <= 2 (rows of a block) blocks tiles / len;
     // and one range each of the sessions behind a prefix, own keys and the prefix
     const long long cut = 2LL * 16 * p.qt * p.target_k + (p.max_jobs_r ? 2LL * kRowsR * p.target_r : 0);

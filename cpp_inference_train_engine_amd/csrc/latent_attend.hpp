@@ -124,7 +124,7 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     // ---- Q^T operands: row 16q + n, latent columns 32j + 8g .., then the rope key's ----
     V8 qv[QT][KSM + RSM];
     int lim[QT];  // lane's row n sees keys [0, lim] of the segment
-    int lim_wave = -1;
+    int lim_wave = -1, lim_all = key_end - 1;
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
         const int r = min(row0 + 16 * q + n, n_rows - 1);  // rows past the block repeat its last
@@ -142,10 +142,12 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
             qv[q][KSM + j] = c < RP ? v : V8{};
         }
     }
-    {   // the last key that any of the wave's rows sees (-1: it has no rows)
+    {   // the last key that any of the wave's rows sees (-1: it has no rows), and that all see
         const int last = min(n_rows, row0 + 16 * QT) - 1;
         if (last >= row0)
             lim_wave = a.causal && seg >= 0 ? ctx + (rb + last) / H : key_end - 1;
+        if (a.causal && seg >= 0)
+            lim_all = ctx + (rb + row0) / H;
     }
 
     // ---- a unit's way into LDS ----
@@ -315,26 +317,31 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
                 __builtin_amdgcn_sched_barrier(0);
             }
 
+        // Units that some row does not see in full: their scores are replaced.
+        if (ok != 0xffffffffu || mark != 0 || 16 * t0 + 31 > lim_all)
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = 16 * tt + 4 * g + i;
+                        if (mark >> key & 1)
+                            sc[tt][q][i] = NAN;
+                        if (!(ok >> key & 1) || 16 * t0 + key > lim[q])
+                            sc[tt][q][i] = -INFINITY;
+                    }
         V8 pb[QT];
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
-            bool rise = false;
-            float mp = -INFINITY;
+            float mp = -INFINITY;  // of the lane's eight scores (NaN is passed over)
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = 16 * tt + 4 * g + i;
-                    float x = sc[tt][q][i] * a.scale_log2;
-                    if (mark >> key & 1)
-                        x = NAN;
-                    if (!(ok >> key & 1) || 16 * t0 + key > lim[q])
-                        x = -INFINITY;
-                    sc[tt][q][i] = x;
-                    rise |= x > m_run[q] + kRise;
-                    mp = fmaxf(mp, x);
-                }
-            if (__builtin_amdgcn_ballot_w64(rise)) {
+                for (int i = 0; i < 4; ++i)
+                    mp = fmaxf(mp, sc[tt][q][i]);
+            mp *= a.scale_log2;
+            if (__builtin_amdgcn_ballot_w64(mp > m_run[q] + kRise)) {
                 const float m_new = fmaxf(m_run[q], rows_max(mp) - kHead);
                 const bool had = m_run[q] != -INFINITY;  // the row has accumulated state
                 if (__builtin_amdgcn_ballot_w64(had && m_new > m_run[q])) {
@@ -352,7 +359,8 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(sc[tt][q][i] - m_ref);
+                    const float e =
+                        __builtin_amdgcn_exp2f(fmaf(sc[tt][q][i], a.scale_log2, -m_ref));
                     psum += e;
                     pb[q][4 * tt + i] = static_cast<typename T::scalar>(e);
                 }

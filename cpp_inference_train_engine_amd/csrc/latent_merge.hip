@@ -1,7 +1,9 @@
 // Joins the partials of mla_latent_attention: a row's weighted sums over ranges of its shared
 // prefix and of its own keys, each with its reference maximum and mass, become the final row.
 //     M = max_i m_i,  L = sum_i l_i 2^(m_i - M),  row = sum_i o_i 2^(m_i - M) / L
-// One thread per 4 columns of a row.  Bound by the partials' bytes, or by latency for few rows.
+// One thread per 4 columns of a row and each of GROUPS groups; the groups split the row's partials,
+// each reads kFlight of them at once (a round trip to memory is what a row costs, a partial's bytes
+// are few), and their states meet in LDS.
 #include "mla_latent.hpp"
 #include "mla_common.hpp"
 
@@ -10,43 +12,95 @@
 namespace mla {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kFlight = 4;
+constexpr long long kFewElements = 1 << 20;
 
-template <typename T>
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(kThreads) void latent_merge_kernel(LatentArgs a) {
+    constexpr int PER = kThreads / GROUPS;  // threads of a group
+    __shared__ float so[GROUPS > 1 ? kThreads * 4 : 4], sml[GROUPS > 1 ? kThreads * 2 : 4];
     const int32_t* plan = a.plan;
-    if (plan[kPlanTag] != (int)a.p.tag || plan[kPlanParts] == 0)
-        return;
+    const int tid = threadIdx.x, group = tid / PER, me = tid % PER;
     const int per_row = a.kv_rank / 4, H = a.H;
-    const long long e = blockIdx.x * (long long)kThreads + threadIdx.x;
+    const long long e = blockIdx.x * (long long)PER + me;
     const long long fr = e / per_row;
     const int c = (int)(e - fr * per_row) * 4;
     const int row = (int)(fr / H);
-    if (row >= plan[kPlanRows])
-        return;
-    const int s = plan[a.p.session_at + row];
-    const int32_t* m = plan + a.p.merge_at + (long long)s * kMergeInts;
-    const int pre = m[0], mine = m[4];
-    if (pre + mine == 0)
-        return;  // one job wrote the row itself
-    const long long own_at = m[5] + fr - (long long)m[7] * H;
-    const long long pre_at = m[1] + m[3] + fr - (long long)m[7] * H;
-    const long long own_n = m[6], pre_n = m[2];
-    auto at = [&](int i) { return i < pre ? pre_at + i * pre_n : own_at + (i - pre) * own_n; };
-    float M = -INFINITY;
-    for (int i = 0; i < pre + mine; ++i)
-        M = fmaxf(M, a.part_ml[2 * at(i)]);
-    float L = 0.0f;
-    floatx4 o = {0, 0, 0, 0};
-    for (int i = 0; i < pre + mine; ++i) {
-        const long long p = at(i);
-        const float mi = a.part_ml[2 * p];
-        if (mi == -INFINITY)
-            continue;  // no key of the range is the row's
-        const float f = __builtin_amdgcn_exp2f(mi - M);
-        L += a.part_ml[2 * p + 1] * f;
-        o += *reinterpret_cast<const floatx4*>(a.part_o + p * a.kv_rank + c) * f;
+    int pre = 0, mine = 0;
+    long long own_at = 0, pre_at = 0, own_n = 0, pre_n = 0;
+    if (plan[kPlanTag] == (int)a.p.tag && plan[kPlanParts] > 0 && row < plan[kPlanRows]) {
+        const int s = plan[a.p.session_at + row];
+        const int32_t* m = plan + a.p.merge_at + (long long)s * kMergeInts;
+        pre = m[0];
+        mine = m[4];
+        const long long r = fr - (long long)m[7] * H;
+        own_at = m[5] + r;
+        pre_at = m[1] + m[3] + r;
+        own_n = m[6];
+        pre_n = m[2];
     }
+    const int parts = pre + mine;  // 0: no such row, or one job wrote it itself
+    float M = -INFINITY, L = 0.0f;
+    floatx4 o = {0, 0, 0, 0};
+    for (int i0 = group; i0 < parts; i0 += GROUPS * kFlight) {
+        float m[kFlight], l[kFlight];
+        floatx4 x[kFlight];
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const int i = min(i0 + k * GROUPS, parts - 1);
+            const long long p = i < pre ? pre_at + i * pre_n : own_at + (i - pre) * own_n;
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            const f2 ml = *reinterpret_cast<const f2*>(a.part_ml + 2 * p);
+            m[k] = ml[0];
+            l[k] = ml[1];
+            x[k] = *reinterpret_cast<const floatx4*>(a.part_o + p * a.kv_rank + c);
+        }
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            if (i0 + k * GROUPS >= parts) {  // read twice: counts once
+                m[k] = -INFINITY;
+                l[k] = 0.0f;
+                x[k] = floatx4{0, 0, 0, 0};
+            }
+            top = fmaxf(top, m[k]);
+        }
+        // A mass of NaN may come with a maximum of -inf (every score was NaN): weight 0 keeps it.
+        const float f0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - top);
+        L *= f0;
+        o *= f0;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const float f = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - top);
+            L += l[k] * f;
+            o += x[k] * f;
+        }
+        M = top;
+    }
+    if constexpr (GROUPS > 1) {
+        *reinterpret_cast<floatx4*>(so + 4 * tid) = o;
+        sml[2 * tid] = M;
+        sml[2 * tid + 1] = L;
+        __syncthreads();
+        if (group > 0)
+            return;
+#pragma unroll
+        for (int v = 1; v < GROUPS; ++v)
+            M = fmaxf(M, sml[2 * (tid + v * PER)]);
+        const float f0 = sml[2 * tid] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sml[2 * tid] - M);
+        L *= f0;
+        o *= f0;
+#pragma unroll
+        for (int v = 1; v < GROUPS; ++v) {
+            const int at = tid + v * PER;
+            const float m = sml[2 * at];
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+            L += sml[2 * at + 1] * f;
+            o += *reinterpret_cast<const floatx4*>(so + 4 * at) * f;
+        }
+    }
+    if (parts == 0)
+        return;
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
     typedef typename T::scalar s4 __attribute__((ext_vector_type(4)));
     s4 y;
@@ -56,6 +110,25 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(LatentArgs a) {
     *reinterpret_cast<s4*>(a.out + fr * a.kv_rank + c) = y;
     if (a.lse && c == 0)
         a.lse[fr] = (M + __log2f(L)) * kLn2;
+}
+
+template <typename T, int GROUPS>
+void launch_groups(const LatentArgs& a, hipStream_t stream) {
+    constexpr int per = kThreads / GROUPS;
+    const long long n = (long long)a.p.rows * a.H * (a.kv_rank / 4);
+    hipLaunchKernelGGL((latent_merge_kernel<T, GROUPS>), dim3((unsigned)((n + per - 1) / per)),
+                       dim3(kThreads), 0, stream, a);
+}
+
+template <typename T>
+hipError_t launch_merge_t(const LatentArgs& a, hipStream_t stream) {
+    // few rows: eight groups, so that one round of reads covers 32 partials; many: as many threads
+    // as columns already fill the GPU
+    if ((long long)a.p.rows * a.H * a.kv_rank <= kFewElements)
+        launch_groups<T, 8>(a, stream);
+    else
+        launch_groups<T, 1>(a, stream);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -74,13 +147,7 @@ hipError_t launch_latent_attention(const LatentArgs& a, int dtype, hipStream_t s
 }
 
 hipError_t launch_latent_merge(const LatentArgs& a, int dtype, hipStream_t stream) {
-    const long long n = (long long)a.p.rows * a.H * (a.kv_rank / 4);
-    const dim3 grid((unsigned)((n + kThreads - 1) / kThreads));
-    if (dtype == 0)
-        hipLaunchKernelGGL(latent_merge_kernel<F16>, grid, dim3(kThreads), 0, stream, a);
-    else
-        hipLaunchKernelGGL(latent_merge_kernel<BF16>, grid, dim3(kThreads), 0, stream, a);
-    return hipGetLastError();
+    return dtype == 0 ? launch_merge_t<F16>(a, stream) : launch_merge_t<BF16>(a, stream);
 }
 
 }  // namespace mla

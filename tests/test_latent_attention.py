@@ -239,7 +239,7 @@ def test_long_keys_and_many_sessions(gpu, H, kv, rope, page, sessions, groups, q
 @pytest.mark.parametrize("H,kv,rope,page", [(8, 128, 16, 64), (40, 64, 16, 32), (128, 512, 64, 64)])
 def test_nonfinite_latents_reach_only_the_rows_that_see_them(gpu, H, kv, rope, page, q8):
     """NaN (16-bit cache: infinities too) in a chunk's own tokens and in a prefix."""
-    sessions = [(40, 1), (200, 40), (0, 9), (70, 1), (5, 1)]
+    sessions = [(40, 1), (200, 40), (0, 9), (70, 1), (5, 1), (0, 1), (600, 1)]
     c = make(H, kv, rope, page, 0, q8, sessions, [(2, 100), (1, 70)], seed=5)
     lat, key = c.rows()
 
@@ -258,11 +258,13 @@ def test_nonfinite_latents_reach_only_the_rows_that_see_them(gpu, H, kv, rope, p
     spoil(c.flat(c.own_pages[2], 9)[[4]], 0x7E00)
     spoil(c.flat(c.own_pages[3], 71)[[30]], 0x7E00)
     spoil(c.flat(c.prefix_pages[1], 70)[[69]], 0x7E00)
+    spoil(c.flat(c.own_pages[5], 1), 0x7E00)                     # a row's only key
+    spoil(c.flat(c.own_pages[6], 601)[512:544], 0x7E00)          # all keys of a unit
     _say(f"non-finite H={H} kv={kv} q8={q8}")
     d = device(gpu, c)
     _, out, lse = call(gpu, c, d)
     check(c, out, lse)
-    assert np.isnan(out.double().cpu().numpy()).any(axis=(1, 2)).sum() == 20 + 9 + 1
+    assert np.isnan(out.double().cpu().numpy()).any(axis=(1, 2)).sum() == 20 + 9 + 1 + 1 + 1
     if not q8:
         want = expect(c)
         spoil(c.flat(c.own_pages[1], 240)[[220, 236]], 0x7C00)
