@@ -42,6 +42,13 @@ constexpr int kRot = 12;
 // clear of its subnormals.
 constexpr float kHead = 6.0f, kRise = 14.0f;
 
+// Tables that other kernels wrote are read through the scalar cache: a vector load of a page id
+// would be waited for together with the unit that was just sent for.
+typedef const __attribute__((address_space(4))) int32_t* table_ptr;
+__device__ __forceinline__ table_ptr table(const int32_t* p) {
+    return (table_ptr)reinterpret_cast<uintptr_t>(p);
+}
+
 __device__ __forceinline__ u32x2 read_tr16(const uint16_t* p) {
     typedef short s4 __attribute__((ext_vector_type(4)));
     const auto v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -103,11 +110,12 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     __shared__ __attribute__((aligned(16))) uint16_t smem[SLOTS][SLOT];
     __shared__ uint32_t marks[3];  // list R: keys of a unit with a non-finite latent
 
-    const int32_t* d = a.plan + (ROWS ? a.p.jobs_r_at : a.p.jobs_k_at) + (long long)blockIdx.x * kJobInts;
-    const int n_jobs = a.plan[ROWS ? kPlanJobsR : kPlanJobsK];
+    const table_ptr plan = table(a.plan);
+    const table_ptr d = plan + (ROWS ? a.p.jobs_r_at : a.p.jobs_k_at) + (long long)blockIdx.x * kJobInts;
+    const int n_jobs = plan[ROWS ? kPlanJobsR : kPlanJobsK], tag = plan[kPlanTag];
     const int seg = d[0], f0 = d[1], n_rows = d[2], rb = d[3], key0 = d[4], key_end = d[5],
               ctx = d[6], part = d[7];
-    if ((int)blockIdx.x >= n_jobs || a.plan[kPlanTag] != (int)a.p.tag)
+    if ((int)blockIdx.x >= n_jobs || tag != (int)a.p.tag)
         return;
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
@@ -116,8 +124,8 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     const int KV = ONE ? 32 * KSM : a.kv_rank, RP = ONE ? RP_ : a.rope_dim;
     const int ks = KV >> 5, rs = (RP + 31) >> 5, tpp = PS >> 4;
     const long long rec = Q8 ? q8_page_bytes(PS, KV, RP) : 2LL * PS * (KV + RP);
-    const int32_t* ptab = seg >= 0 ? a.page_table + (long long)seg * a.max_pages
-                                   : a.prefix_page_ids + a.cu_prefix_pages[~seg];
+    const table_ptr ptab = table(seg >= 0 ? a.page_table + (long long)seg * a.max_pages
+                                          : a.prefix_page_ids + table(a.cu_prefix_pages)[~seg]);
     const int n_units = key_end > key0 && a.num_pool_pages > 0 ? (key_end - key0 + 31) >> 5 : 0;
     const int row0 = ROWS ? 16 * QT * wave : 0;  // the wave's first row of the block
 
@@ -163,11 +171,15 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
         rope_tt[i] = c >= rcs;
         rope_ch[i] = c < 2 * rcs ? (c >= rcs ? c - rcs : c) : -1;
     }
-    // Tile t's page id, -1 past the keys or outside the pool.
+    // A tile's page and its place there (page sizes are mostly powers of two).
+    const int tpp_shift = (tpp & (tpp - 1)) == 0 ? __builtin_ctz(tpp) : -1;
+    auto page_of = [&](int t) { return tpp_shift >= 0 ? t >> tpp_shift : t / tpp; };
+    auto place_of = [&](int t) { return tpp_shift >= 0 ? t & (tpp - 1) : t % tpp; };
+    // Tile t's page id, some id past the keys; valid_page: -1 when it lies outside the pool.
     auto tile_page = [&](int t) {
-        const int id = 16 * t < key_end ? __builtin_amdgcn_readfirstlane(ptab[t / tpp]) : -1;
-        return (unsigned)id < (unsigned)a.num_pool_pages ? id : -1;
+        return ptab[page_of(min(t, (key_end - 1) >> 4))];
     };
+    auto valid_page = [&](int id) { return (unsigned)id < (unsigned)a.num_pool_pages ? id : -1; };
     // The unit's keys that exist: before key_end, on a page of the pool.
     auto keys_of = [&](int t0, int pg0, int pg1) {
         const int valid = min(32, key_end - 16 * t0);
@@ -182,7 +194,7 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     auto load_unit = [&](int t0, int pg0, int pg1) {
         const uint8_t* base0 = a.pages + max(pg0, 0) * rec;
         const uint8_t* base1 = a.pages + max(pg1, 0) * rec;
-        const int in0 = t0 % tpp, in1 = (t0 + 1) % tpp;
+        const int in0 = place_of(t0), in1 = place_of(t0 + 1);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int u = ROWS ? wave + NW * i : i;
@@ -399,13 +411,12 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     }
     int pg0 = -1, pg1 = -1, nx0 = -1, nx1 = -1;
     if (first < n_units) {
-        pg0 = tile_page(tile0 + 2 * first);
-        pg1 = tile_page(tile0 + 2 * first + 1);
-        load_unit(tile0 + 2 * first, pg0, pg1);
-        if (first + STEP < n_units) {
-            nx0 = tile_page(tile0 + 2 * (first + STEP));
-            nx1 = tile_page(tile0 + 2 * (first + STEP) + 1);
-        }
+        const int t0 = tile0 + 2 * first;
+        pg0 = valid_page(tile_page(t0));
+        pg1 = valid_page(tile_page(t0 + 1));
+        nx0 = tile_page(t0 + 2 * STEP);
+        nx1 = tile_page(t0 + 2 * STEP + 1);
+        load_unit(t0, pg0, pg1);
     }
     for (int u = first; u < n_units; u += STEP) {
         const int t0 = tile0 + 2 * u;
@@ -415,13 +426,11 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
         if (ROWS && mark && lane == 0)
             atomicOr(&marks[u % 3], mark);
         if (u + STEP < n_units) {
-            load_unit(t0 + 2 * STEP, nx0, nx1);
-            pg0 = nx0;
-            pg1 = nx1;
-            if (u + 2 * STEP < n_units) {
-                nx0 = tile_page(t0 + 4 * STEP);
-                nx1 = tile_page(t0 + 4 * STEP + 1);
-            }
+            pg0 = valid_page(nx0);
+            pg1 = valid_page(nx1);
+            load_unit(t0 + 2 * STEP, pg0, pg1);
+            nx0 = tile_page(t0 + 4 * STEP);
+            nx1 = tile_page(t0 + 4 * STEP + 1);
         }
         if constexpr (ROWS) {
             // The other buffer is free: every wave that passed the barrier before this one has
