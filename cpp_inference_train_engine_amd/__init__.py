@@ -83,7 +83,7 @@ _SIGNATURES = {
     "mla_read_plan_info": (C.c_int, [C.c_void_p] * 3),
     "mla_latent_attention": (C.c_int, [C.c_void_p] + [C.c_int] * 9 + [C.c_float, C.c_void_p] +
                              [C.c_int] * 2 + [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 3 +
-                             [C.c_size_t] + [C.c_void_p] * 3 + [C.c_size_t]),
+                             [C.c_size_t] + [C.c_void_p] * 4 + [C.c_size_t]),
     "mla_config_validate": (C.c_int, [C.c_void_p]),
     "mla_config_parameter_count": (C.c_size_t, [C.c_void_p]),
     "mla_model_create": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int,
@@ -188,10 +188,20 @@ def ptr(t) -> int | None:
     return t.ctypes.data
 
 
+_current_raw_stream = None
+
+
 def stream_handle(stream=None) -> int | None:
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    global _current_raw_stream
+    if _current_raw_stream is None:  # the handle alone costs 0.1 us, torch's Stream object 3 us
+        import torch
+        torch.cuda.current_stream()  # initialises the device
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _current_raw_stream = ((lambda: raw(torch.cuda.current_device())) if raw else
+                               (lambda: torch.cuda.current_stream().cuda_stream))
+    return _current_raw_stream()
 
 
 from .ops import (  # noqa: E402  (re-exported operator interface)

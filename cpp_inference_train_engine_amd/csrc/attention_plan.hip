@@ -1,11 +1,14 @@
 // The plan of mla_latent_attention: which workgroup takes which rows over which keys, built on
 // the GPU once for a batch and used by every layer's call.  No reference counterpart.
 //
-// One workgroup.  For each segment (mla_latent.hpp) it takes the row blocks and the 32-key tiles,
-// cuts the keys of all segments into ranges of one length per list, so that a list has about its
-// target of jobs, and lays out jobs, partial rows and, per session, what the merge has to add up.
-// Everything is scanned in one pass over the segments with a running carry, so any batch size
-// works; the tables live in the plan itself.
+// One workgroup, everything in LDS tables (in the plan's own for very large batches).  A segment
+// (mla_latent.hpp) has row blocks and 32-key tiles; the keys of all segments of a list are cut into
+// ranges of one length.  A GPU that holds `slots` workgroups of the list at once takes
+//     ceil(jobs / slots) * (length * time of a tile + time of a job's start and end)
+// so what counts is that the jobs fill one round or two and not a little more: the length is
+// the best of candidates between 1 and 2 times total / (rounds * slots).  Whether segments of many
+// rows go to list R or are taken apart for list K is decided by the same estimate: list K costs
+// more per row, but its jobs are small and there is one launch instead of two.
 #include "mla_latent.hpp"
 
 #include <algorithm>
@@ -14,6 +17,18 @@ namespace mla {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kLdsSegs = 3072;  // segments whose tables fit LDS (9 of 12 KB)
+constexpr int kTables = 9;
+constexpr int kFewRows = 64;    // segments up to this go to list K in any case
+constexpr int kRounds = 2, kSteps = 8, kTries = kRounds * kSteps;
+
+// Times in ns of a unit of 32 keys, by list, and of a job's start and end.
+struct Cost {
+    int tile_k, job_k, tile_r, job_r, launch;
+};
+__device__ __forceinline__ Cost cost_of(int kv_rank) {
+    return kv_rank <= 128 ? Cost{1500, 3500, 1100, 4000, 3000} : Cost{6000, 6000, 2200, 8000, 3000};
+}
 
 __device__ __forceinline__ long long wave_scan(long long v, int lane) {
     for (int d = 1; d < 64; d <<= 1) {
@@ -24,68 +39,89 @@ __device__ __forceinline__ long long wave_scan(long long v, int lane) {
     return v;
 }
 
-// Inclusive scan over the workgroup; `total` receives the sum.  `tmp`: kWaves values in LDS.
-__device__ long long block_scan(long long v, long long* tmp, long long& total) {
+// Inclusive scans of three values over the workgroup; `total` receives the sums.
+__device__ void block_scan3(long long (&v)[3], long long (*tmp)[3], long long (&total)[3]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v = wave_scan(v, lane);
     __syncthreads();
-    if (lane == 63)
-        tmp[wave] = v;
-    __syncthreads();
-    long long before = 0;
-    total = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        const long long x = tmp[w];
-        before += w < wave ? x : 0;
-        total += x;
+    for (int k = 0; k < 3; ++k) {
+        v[k] = wave_scan(v[k], lane);
+        if (lane == 63)
+            tmp[wave][k] = v[k];
     }
-    return v + before;
+    __syncthreads();
+    for (int k = 0; k < 3; ++k) {
+        long long before = 0;
+        total[k] = 0;
+        for (int w = 0; w < kWaves; ++w) {
+            const long long x = tmp[w][k];
+            before += w < wave ? x : 0;
+            total[k] += x;
+        }
+        v[k] += before;
+    }
 }
 
-struct Seg {
-    long long n;  // (query, head) rows
-    int tiles, keys, blocks, q0, q_len, few;
-};
+__device__ __forceinline__ long long wave_total(long long v) {
+    for (int d = 32; d > 0; d >>= 1)
+        v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
 
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
-    __shared__ long long tmp[kWaves];
+    __shared__ int32_t lds[kTables * kLdsSegs];
+    __shared__ long long tmp[kWaves][3];
+    __shared__ unsigned long long best[3];
     __shared__ int first_bad;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PlanShape& p = a.p;
     const int B = p.B, G = p.groups, S = G + B, H = p.H;
-    int32_t* head = a.plan;
-    int32_t* segs = a.plan + p.seg_at;
-    int32_t* merges = a.plan + p.merge_at;
-    int32_t* session_of = a.plan + p.session_at;
-    const int total_q = a.info[0] < 0 ? -1 : a.cu_q[B];
+    int32_t* const head = a.plan;
+    int32_t* const merges = a.plan + p.merge_at;
+    int32_t* const session_of = a.plan + p.session_at;
+    // tables of the segments: the groups' prefixes, then the sessions' own keys
+    int32_t* const t = S <= kLdsSegs ? lds : a.plan + p.seg_at;
+    int32_t *const q0 = t, *const ql = t + S, *const keys = t + 2LL * S, *const group = t + 3LL * S,
+            *const job_k = t + 4LL * S, *const job_r = t + 5LL * S, *const part = t + 6LL * S,
+            *const cuts = t + 7LL * S, *const len = t + 8LL * S;
 
-    // ---- checks: the metadata, the sessions' rows, the groups and their pages ----
+    // ---- checks and the segments' sizes ----
+    const int total_q = a.info[0] < 0 ? -1 : a.cu_q[B];
     if (tid == 0)
-        first_bad = 0x7fffffff;
+        first_bad = total_q < 0 || total_q > p.rows ? -1 : 0x7fffffff;
+    if (tid < 3)
+        best[tid] = ~0ull;
     __syncthreads();
-    if (total_q < 0 || total_q > p.rows) {
-        if (tid == 0)
-            first_bad = -1;  // a failed metadata build, or more rows than the call's
-    } else {
-        for (int s = tid; s < B; s += kThreads)
-            if (a.cu_q[s + 1] - a.cu_q[s] > p.max_q_len)
-                atomicMin(&first_bad, G + s);
-        for (int g = tid; g < G; g += kThreads) {
-            const int s0 = a.cu_groups[g], s1 = a.cu_groups[g + 1], len = a.prefix_len[g];
-            const int c0 = a.cu_prefix_pages[g], c1 = a.cu_prefix_pages[g + 1];
-            if (s0 < 0 || s1 < s0 || s1 > B || len < 0 || c0 < 0 || c1 < c0 ||
-                c1 > a.n_prefix_pages || (long long)(c1 - c0) * a.page_size < len)
-                atomicMin(&first_bad, g);
+    if (first_bad != -1) {
+        for (int i = tid; i < S; i += kThreads) {
+            bool ok;
+            int s0 = 0, s1 = 0, n = 0;
+            if (i < G) {
+                s0 = a.cu_groups[i];
+                s1 = a.cu_groups[i + 1];
+                n = a.prefix_len[i];
+                const int c0 = a.cu_prefix_pages[i], c1 = a.cu_prefix_pages[i + 1];
+                ok = s0 >= 0 && s1 >= s0 && s1 <= B && n >= 0 && c0 >= 0 && c1 >= c0 &&
+                     c1 <= a.n_prefix_pages && (long long)(c1 - c0) * a.page_size >= n;
+            } else {
+                s0 = i - G;
+                s1 = s0 + 1;
+                n = a.cu_k[s1] - a.cu_k[s0];
+                ok = a.cu_q[s1] - a.cu_q[s0] <= p.max_q_len;
+            }
+            if (!ok)
+                atomicMin(&first_bad, i);
+            q0[i] = ok ? a.cu_q[s0] : 0;
+            ql[i] = ok ? a.cu_q[s1] - a.cu_q[s0] : 0;
+            keys[i] = n;
+            group[i] = -1;
         }
-        __syncthreads();
-        for (int g = wave; g < G; g += kWaves) {  // a bad group's list may lie anywhere
-            const int c0 = a.cu_prefix_pages[g], c1 = a.cu_prefix_pages[g + 1];
-            if (c0 < 0 || c1 > a.n_prefix_pages)
-                continue;
-            for (int i = c0 + lane; i < c1; i += 64)
-                if ((unsigned)a.prefix_page_ids[i] >= (unsigned)a.num_pool_pages)
-                    atomicMin(&first_bad, g);
-        }
+        for (int i = tid; i < a.n_prefix_pages; i += kThreads)
+            if ((unsigned)a.prefix_page_ids[i] >= (unsigned)a.num_pool_pages)
+                for (int g = 0; g < G; ++g)  // only ids that some group lists count
+                    if (a.cu_prefix_pages[g] <= i && i < a.cu_prefix_pages[g + 1])
+                        atomicMin(&first_bad, g);
     }
     __syncthreads();
     if (first_bad != 0x7fffffff) {
@@ -93,101 +129,113 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             head[tid] = tid == kPlanStatus ? -1 : tid == kPlanBad ? first_bad : 0;
         return;
     }
-
-    // ---- which prefix a session has ----
-    for (int s = tid; s < B; s += kThreads)
-        for (int i = 0; i < kMergeInts; ++i)
-            merges[(long long)s * kMergeInts + i] = 0;
-    __syncthreads();
-    for (int g = wave; g < G; g += kWaves)
-        if (a.prefix_len[g] > 0)
+    for (int g = wave; g < G; g += kWaves)  // which prefix a session has
+        if (keys[g] > 0)
             for (int s = a.cu_groups[g] + lane; s < a.cu_groups[g + 1]; s += 64)
-                merges[(long long)s * kMergeInts] = 1;
+                group[G + s] = g;
     __syncthreads();
 
-    auto segment = [&](int i) {
-        Seg x{};
-        if (i < G) {
-            x.q0 = a.cu_q[a.cu_groups[i]];
-            x.q_len = a.cu_q[a.cu_groups[i + 1]] - x.q0;
-            x.keys = a.prefix_len[i];
-        } else {
-            x.q0 = a.cu_q[i - G];
-            x.q_len = a.cu_q[i - G + 1] - x.q0;
-            x.keys = a.cu_k[i - G + 1] - a.cu_k[i - G];
-        }
-        if (x.q_len <= 0 || x.keys <= 0)
-            return x;
-        x.n = (long long)x.q_len * H;
-        x.few = x.n <= kFewRows;
-        const int rows = x.few ? 16 * p.qt : kRowsR;
-        x.blocks = (int)((x.n + rows - 1) / rows);
-        x.tiles = (int)(((long long)x.keys + kTile - 1) / kTile);
-        return x;
+    auto flat = [&](int i) { return ql[i] > 0 && keys[i] > 0 ? ql[i] * H : 0; };  // its rows
+    auto tiles = [&](int i) { return (int)(((long long)keys[i] + kTile - 1) / kTile); };
+    const Cost cost = cost_of(p.kv_rank);
+    // Lists to estimate: 0 list K of the few, 1 list R of the others, 2 list K of all.
+    auto blocks_of = [&](int list, int i) {
+        const int n = flat(i);
+        if (list == 2 || (list == 0 && n <= kFewRows))
+            return ceil_div(n, kRowsK);
+        return list == 1 && n > kFewRows ? ceil_div(n, kRowsR) : 0;
     };
 
-    // ---- the length of a key range, per list: about target jobs in all ----
-    long long cost_k = 0, cost_r = 0, all;
-    for (int i = tid; i < S; i += kThreads) {
-        const Seg x = segment(i);
-        (x.few ? cost_k : cost_r) += (long long)x.blocks * x.tiles;
+    // ---- the range lengths ----
+    long long sums[3];
+    {
+        long long v[3] = {0, 0, 0};
+        for (int i = tid; i < S; i += kThreads)
+            for (int list = 0; list < 3; ++list)
+                v[list] += (long long)blocks_of(list, i) * tiles(i);
+        block_scan3(v, tmp, sums);
     }
-    block_scan(cost_k, tmp, all);
-    cost_k = all;
-    block_scan(cost_r, tmp, all);
-    cost_r = all;
-    auto range = [](long long cost, int target, int least) {
-        return std::max<long long>((cost + target - 1) / target, least);
+    auto tried = [&](int list, int c) {  // length of candidate c, in tiles
+        const int slots = list == 1 ? p.slots_r : p.slots_k;
+        const long long share = sums[list] / (slots * (1 + c / kSteps)) + 1;
+        long long n = share + share * (c % kSteps) / kSteps;
+        if (list != 1)
+            n = (n + 3) & ~3LL;  // a tile for each of the four waves
+        return (int)std::min<long long>(n, 1 << 26);
     };
-    const long long len_k = range(cost_k, p.target_k, p.least_k);
-    const long long len_r = range(cost_r, p.target_r, p.least_r);
+    for (int e = wave; e < 3 * kTries; e += kWaves) {
+        const int list = e / kTries, c = e % kTries, n = tried(list, c);
+        if (sums[list] == 0)
+            continue;
+        long long jobs = 0;
+        int longest = 0;
+        for (int i = lane; i < S; i += 64)
+            if (const int b = blocks_of(list, i)) {
+                jobs += (long long)b * ceil_div(tiles(i), n);
+                longest = std::max(longest, std::min(n, tiles(i)));
+            }
+        jobs = wave_total(jobs);
+        for (int d = 32; d > 0; d >>= 1)
+            longest = std::max(longest, __shfl_xor(longest, d, 64));
+        if (lane == 0) {
+            const int slots = list == 1 ? p.slots_r : p.slots_k;
+            const long long rounds = (jobs + slots - 1) / slots;
+            const long long each = list == 1 ? (long long)longest * cost.tile_r + cost.job_r
+                                             : (longest + 3LL) / 4 * cost.tile_k + cost.job_k;
+            const unsigned long long ns = std::min<long long>(rounds * each, 0xffffffffLL);
+            atomicMin(&best[list], ns << 32 | (unsigned)c);
+        }
+    }
+    __syncthreads();
+    auto ns_of = [&](int list) { return sums[list] == 0 ? 0 : (long long)(best[list] >> 32); };
+    const bool all_k = p.max_jobs_r == 0 || sums[1] == 0 ||
+                       (p.list_k_holds_all &&
+                        ns_of(2) < ns_of(0) + ns_of(1) + (sums[0] > 0 ? cost.launch : 0));
+    auto few = [&](int i) { return all_k || flat(i) <= kFewRows; };
+    const int list_k = all_k ? 2 : 0;
+    const int len_k = sums[list_k] == 0 ? 4 : tried(list_k, (int)(best[list_k] & 0xffffffffu));
+    const int len_r = all_k ? 1 : tried(1, (int)(best[1] & 0xffffffffu));
 
     // ---- jobs and partial rows of each segment ----
-    long long at_k = 0, at_r = 0, at_part = 0;
+    long long at[3] = {0, 0, 0};
     for (int i0 = 0; i0 < S; i0 += kThreads) {
         const int i = i0 + tid;
-        Seg x{};
-        if (i < S)
-            x = segment(i);
-        int splits = 0, len = 0;
-        if (x.blocks > 0) {
-            const long long most = x.few ? len_k : len_r;
-            splits = (int)((x.tiles + most - 1) / most);
-            len = (x.tiles + splits - 1) / splits;
-            if (x.few)
-                len = (len + 3) & ~3;  // the four waves of a list-K job take a tile each
-            splits = (x.tiles + len - 1) / len;
+        int n = 0, splits = 0, range = 0, blocks = 0;
+        bool f = false;
+        if (i < S && (n = flat(i)) > 0) {
+            f = few(i);
+            blocks = ceil_div(n, f ? kRowsK : kRowsR);
+            splits = ceil_div(tiles(i), f ? len_k : len_r);
+            range = ceil_div(tiles(i), splits);  // the segment's ranges as even as they go
+            if (f)
+                range = (range + 3) & ~3;
+            splits = ceil_div(tiles(i), range);
         }
-        const bool joined =
-            x.blocks > 0 && (splits > 1 || i < G || merges[(long long)(i - G) * kMergeInts] != 0);
-        const long long jobs = (long long)x.blocks * splits;
-        const long long parts = joined ? x.n * splits : 0;
-        long long sum;
-        const long long jk = block_scan(x.few ? jobs : 0, tmp, sum) + at_k - (x.few ? jobs : 0);
-        at_k += sum;
-        const long long jr = block_scan(x.few ? 0 : jobs, tmp, sum) + at_r - (x.few ? 0 : jobs);
-        at_r += sum;
-        const long long pt = block_scan(parts, tmp, sum) + at_part - parts;
-        at_part += sum;
+        const bool joined = n > 0 && (splits > 1 || i < G || group[i] >= 0);
+        const long long jobs = (long long)blocks * splits;
+        long long v[3] = {f ? jobs : 0, f ? 0 : jobs, joined ? (long long)n * splits : 0};
+        const long long mine[3] = {v[0], v[1], v[2]};
+        long long sum[3];
+        block_scan3(v, tmp, sum);
         if (i < S) {
-            int32_t* d = segs + (long long)i * kSegInts;
-            d[0] = x.few;
-            d[1] = (int)std::min<long long>(x.few ? jk : jr, 0x7fffffff);
-            d[2] = splits;
-            d[3] = len;
-            d[4] = joined ? (int)std::min<long long>(pt, 0x7fffffff) : -1;
-            d[5] = x.blocks;
+            job_k[i] = (int)std::min<long long>(at[0] + v[0] - mine[0], 0x7fffffff);
+            job_r[i] = (int)std::min<long long>(at[1] + v[1] - mine[1], 0x7fffffff);
+            part[i] = joined ? (int)std::min<long long>(at[2] + v[2] - mine[2], 0x7fffffff) : -1;
+            cuts[i] = splits;
+            len[i] = range;
         }
+        for (int k = 0; k < 3; ++k)
+            at[k] += sum[k];
     }
     __syncthreads();
-    const bool fits = at_k <= p.max_jobs_k && at_r <= p.max_jobs_r && at_part <= p.max_parts;
+    const bool fits = at[0] <= p.max_jobs_k && at[1] <= p.max_jobs_r && at[2] <= p.max_parts;
     if (tid < kPlanHead) {
         int v = 0;
         if (fits)
-            v = tid == kPlanStatus ? (int)(at_k + at_r)
-                : tid == kPlanJobsK ? (int)at_k
-                : tid == kPlanJobsR ? (int)at_r
-                : tid == kPlanParts ? (int)at_part
+            v = tid == kPlanStatus ? (int)(at[0] + at[1])
+                : tid == kPlanJobsK ? (int)at[0]
+                : tid == kPlanJobsR ? (int)at[1]
+                : tid == kPlanParts ? (int)at[2]
                 : tid == kPlanRows  ? total_q
                 : tid == kPlanTag   ? (int)p.tag
                                     : 0;
@@ -198,50 +246,53 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     if (!fits)
         return;
 
-    // ---- the jobs; what the merge adds up for a session; the session of each row ----
-    for (int i = wave; i < S; i += kWaves) {
-        const Seg x = segment(i);
-        const int32_t* d = segs + (long long)i * kSegInts;
-        const int job0 = d[1], splits = d[2], len = d[3], part0 = d[4], blocks = d[5];
-        if (i < G) {
-            for (int s = a.cu_groups[i] + lane; s < a.cu_groups[i + 1]; s += 64) {
-                int32_t* m = merges + (long long)s * kMergeInts;
-                m[0] = blocks > 0 ? splits : 0;
-                m[1] = part0;
-                m[2] = (int)x.n;
-                m[3] = (a.cu_q[s] - x.q0) * H;
+    // ---- the jobs ----
+    for (int list = 0; list < 2; ++list) {
+        const int32_t* first = list ? job_r : job_k;
+        int32_t* out = a.plan + (list ? p.jobs_r_at : p.jobs_k_at);
+        for (int j = tid; j < (int)at[list]; j += kThreads) {
+            int lo = 0, hi = S;  // the last segment that starts at or before the job
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (first[mid] <= j)
+                    lo = mid;
+                else
+                    hi = mid;
             }
-        } else {
-            if (lane == 0) {
-                int32_t* m = merges + (long long)(i - G) * kMergeInts;
-                m[4] = part0 >= 0 ? splits : 0;
-                m[5] = part0;
-                m[6] = (int)x.n;
-                m[7] = x.q0;
-            }
-            for (int r = lane; r < x.q_len; r += 64)
-                session_of[x.q0 + r] = i - G;
-        }
-        const int rows = x.few ? 16 * p.qt : kRowsR;
-        int32_t* list = a.plan + (x.few ? p.jobs_k_at : p.jobs_r_at);
-        const int ctx = i < G ? x.keys : x.keys - x.q_len;
-        for (int j = lane; j < blocks * splits; j += 64) {
-            const int sp = j / blocks, rb = (j - sp * blocks) * rows;
-            const int n = (int)std::min<long long>(rows, x.n - rb);
-            const long long k0 = (long long)sp * len * kTile;
+            const int i = lo, n = flat(i), rows = list ? kRowsR : kRowsK;
+            const int blocks = ceil_div(n, rows), in = j - first[i];
+            const int sp = in / blocks, rb = (in - sp * blocks) * rows;
+            const int m = std::min(rows, n - rb), ctx = i < G ? keys[i] : keys[i] - ql[i];
+            const long long k0 = (long long)sp * len[i] * kTile;
             // own keys: the block's last row sees keys up to its own token
-            const int seen = i < G ? x.keys : ctx + (rb + n - 1) / H + 1;
-            int32_t* o = list + (long long)(job0 + j) * kJobInts;
+            const int seen = i < G ? keys[i] : ctx + (rb + m - 1) / H + 1;
+            int32_t* o = out + (long long)j * kJobInts;
             o[0] = i < G ? ~i : i - G;
-            o[1] = (int)((long long)x.q0 * H + rb);
-            o[2] = n;
+            o[1] = q0[i] * H + rb;
+            o[2] = m;
             o[3] = rb;
             o[4] = (int)k0;
-            o[5] = (int)std::min<long long>(seen, k0 + (long long)len * kTile);
+            o[5] = (int)std::min<long long>(seen, k0 + (long long)len[i] * kTile);
             o[6] = ctx;
-            o[7] = part0 < 0 ? -1 : part0 + (int)(sp * x.n) + rb;
+            o[7] = part[i] < 0 ? -1 : part[i] + sp * n + rb;
         }
     }
+    // ---- what the merge adds up for a session; the session of each row ----
+    for (int s = tid; s < B; s += kThreads) {
+        const int i = G + s, g = group[i];
+        int32_t* m = merges + (long long)s * kMergeInts;
+        m[0] = g >= 0 && flat(g) > 0 ? cuts[g] : 0;
+        m[1] = g >= 0 ? part[g] : 0;
+        m[2] = g >= 0 ? flat(g) : 0;
+        m[3] = g >= 0 ? (q0[i] - q0[g]) * H : 0;
+        m[4] = part[i] >= 0 ? cuts[i] : 0;
+        m[5] = part[i];
+        m[6] = flat(i);
+        m[7] = q0[i];
+    }
+    for (int e = tid; e < 16 * B; e += kThreads)  // 16 threads a session
+        for (int r = e & 15; r < ql[G + (e >> 4)]; r += 16)
+            session_of[q0[G + (e >> 4)] + r] = e >> 4;
 }
 
 }  // namespace
@@ -255,29 +306,33 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
     p.kv_rank = kv_rank;
     p.max_q_len = max_q_len;
     const long long flat = (long long)rows * H;
-    const long long own_most = std::min(flat, (long long)max_q_len * H);  // rows of a session
-    const long long own = std::min<long long>(kFewRows, own_most);
-    p.qt = kv_rank <= 128 && own > 16 ? 2 : 1;
-    p.target_k = kv_rank <= 128 ? 768 : 256;
-    p.target_r = kv_rank <= 128 ? 512 : 256;
-    p.least_k = 4;
-    p.least_r = 8;
-    // a segment's jobs: blocks * ceil(tiles / len) <= cost / len + blocks
+    const long long own = std::min(flat, (long long)max_q_len * H);  // most rows of a session
+    // Workgroups that 256 compute units hold: by registers and LDS of the two lists' kernels.
+    p.slots_k = kv_rank <= 128 ? 1024 : kv_rank <= 256 ? 512 : 256;
+    p.slots_r = kv_rank <= 128 ? 512 : 256;
+    const bool few = H <= kFewRows, many = own > kFewRows || (groups > 0 && flat > kFewRows);
     const long long segs = (long long)B + groups, sides = groups > 0 ? 2 : 1;
-    const long long blocks_k =
-        std::min(segs * (kFewRows / (16 * p.qt)), sides * (flat / (16 * p.qt)) + segs);
-    const long long blocks_r = sides * (flat / kRowsR) + std::min(segs, sides * (flat / (kFewRows + 1)));
-    // a list that no segment of these sizes can be on is not launched
-    const bool few = H <= kFewRows, many = own_most > kFewRows || (groups > 0 && flat > kFewRows);
-    p.max_jobs_k = few ? (int)(p.target_k + blocks_k) : 0;
-    p.max_jobs_r = many ? (int)(p.target_r + blocks_r) : 0;
-    // rows of a segment cut into s >= 2 ranges: n s <= 2 (rows of a block) blocks tiles / len;
-    // and one range each of the sessions behind a prefix, own keys and the prefix
-    const long long cut = 2LL * 16 * p.qt * p.target_k + (p.max_jobs_r ? 2LL * kRowsR * p.target_r : 0);
+    // A list's ranges are at least sums / (kRounds slots) long (see tried), so a segment's jobs,
+    // blocks * ceil(tiles / length) <= blocks * tiles / length + blocks, add up to at most
+    // kRounds * slots + the blocks.
+    const long long blocks_k = sides * (flat / kRowsK) + segs;
+    const long long few_k = std::min(blocks_k, segs * (kFewRows / kRowsK));
+    const long long blocks_r =
+        sides * (flat / kRowsR) + std::min(segs, sides * (flat / (kFewRows + 1)));
+    // List K takes segments of many rows only while its table stays small: where it would pay.
+    p.list_k_holds_all = many && blocks_k <= 4LL * p.slots_k;
+    const long long most_k = p.list_k_holds_all ? blocks_k : few_k;
+    p.max_jobs_k = few || p.list_k_holds_all ? (int)(kRounds * p.slots_k + most_k) : 0;
+    p.max_jobs_r = many ? (int)(kRounds * p.slots_r + blocks_r) : 0;
+    // A segment of n rows cut into s >= 2 ranges has n s <= 2 (rows of a block) blocks tiles /
+    // length partial rows, 2 (rows of a block) kRounds slots in all; the sessions behind a prefix
+    // and the prefixes have n each even where they are not cut.
+    const long long cut = 2LL * kRounds * (kRowsK * (p.max_jobs_k ? p.slots_k : 0) +
+                                           kRowsR * (p.max_jobs_r ? p.slots_r : 0));
     p.max_parts = std::min(cut + (groups > 0 ? 2 * flat : 0),
-                           16LL * p.qt * p.max_jobs_k + (long long)kRowsR * p.max_jobs_r);
+                           (long long)kRowsK * p.max_jobs_k + (long long)kRowsR * p.max_jobs_r);
     p.seg_at = kPlanHead;
-    p.merge_at = p.seg_at + segs * kSegInts;
+    p.merge_at = p.seg_at + (segs > kLdsSegs ? segs * kTables : 0);
     p.session_at = p.merge_at + (long long)B * kMergeInts;
     p.jobs_k_at = (p.session_at + rows + 7) & ~7LL;
     p.jobs_r_at = p.jobs_k_at + (long long)p.max_jobs_k * kJobInts;

@@ -6,13 +6,12 @@
 // as the framework's other attention kernels (src/infer/inference.cpp:116-153 in the reference,
 // causal rows src/model/ops.cpp:109-142).
 //
-// latent_attend_kernel -- a workgroup of 4 waves takes a job: up to 16 QT rows (list K) or 128 rows
-//   (list R) of a segment over a range of its keys, 32 keys (a unit: two 16-token tiles, which may
-//   lie on different pages) at a time.  List K: every wave holds all rows and takes every 4th
-//   unit through a slot of its own; the waves' states meet in LDS at the end.  List R: every wave
-//   holds 32 rows, the four stage a unit together into one of two buffers (one barrier a unit), and
-//   no state is exchanged: each key is read once for 128 rows, which is what makes a shared prefix
-//   cheap.  A unit goes from memory to registers while the unit before it is computed, and from
+// latent_attend_kernel -- a workgroup takes a job: rows of a segment over a range of its keys, 32
+//   keys (a unit: two 16-token tiles, which may lie on different pages) at a time, a wave 16 rows.
+//   List K, 16 rows: each of four waves holds all of them and takes every 4th unit through a slot
+//   of its own; the waves' states meet in LDS at the end.  List R, 128 rows: each of eight waves
+//   holds 16, they stage a unit together into one of two buffers (one barrier a unit), and no
+//   state is exchanged: a key is fetched and converted once for 128 rows.  A unit goes from memory to registers while the unit before it is computed, and from
 //   there to LDS as 16-bit words in MFMA-operand order (8-bit latents: v_cvt_scalef32_pk_*, exact,
 //   see mla_q8.hpp), so that both formats share everything behind it:
 //     S^T = K . Q^T     v_mfma_f32_16x16x32, Q^T in registers for the whole job
@@ -91,12 +90,12 @@ __device__ __forceinline__ bool drop_nan8(u32x4& v) {
 }
 
 // T: 16-bit type of the queries, rope keys, 16-bit latents and rows; Q8: 8-bit latents; KSM: latent
-// k-steps (kv_rank / 32 <= KSM); QT: 16-row tiles of a wave; ROWS: list R; RP_: the rope columns of
-// an instantiation for one shape (kv_rank = 32 KSM, rope_dim = RP_), -1 for any.
-template <typename T, bool Q8, int KSM, int QT, bool ROWS, int RP_ = -1>
-__global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__((
+// k-steps (kv_rank / 32 <= KSM); ROWS: list R; RP_: the rope columns of an instantiation for one
+// shape (kv_rank = 32 KSM, rope_dim = RP_), -1 for any.
+template <typename T, bool Q8, int KSM, bool ROWS, int RP_ = -1>
+__global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     amdgpu_waves_per_eu(KSM >= 16 && !ROWS ? 1 : 2, 8))) void latent_attend_kernel(LatentArgs a) {
-    constexpr int NW = ROWS ? kRowsR / (16 * QT) : 4;   // waves
+    constexpr int NW = (ROWS ? kThreadsR : kThreadsK) / 64;  // waves
     constexpr bool ONE = RP_ >= 0;
     constexpr int RSM = ONE ? (RP_ + 31) / 32 : 2;      // rope k-steps (rope_dim <= 64)
     constexpr int RTM = 2 * KSM;                        // 16-row tiles of O^T
@@ -106,8 +105,13 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     constexpr int RCS = ONE ? RP_ / 8 : 8;              // rope chunks of a tile, at most
     constexpr int NR = ROWS ? 1 : (2 * RCS + 3) / 4;    // rope loads of a lane per unit
     constexpr int SLOTS = ROWS ? 2 : 4;
+    constexpr int DEPTH = ROWS && ONE && KSM == 4 ? 2 : 1;  // units in flight behind the one at work
+    // Q^T k-steps that stay in LDS, lane by lane, where the registers would spill (a reload waits
+    // for every load in flight): at kv 512 O^T takes 128 of a wave's 256 registers, Q^T 72.
+    constexpr int QL = KSM >= 16 && ROWS ? (ONE ? (Q8 ? 4 : 6) : 8) : 0;
     using V8 = typename T::vec8;
     __shared__ __attribute__((aligned(16))) uint16_t smem[SLOTS][SLOT];
+    __shared__ __attribute__((aligned(16))) uint16_t q_lds[QL > 0 ? NW * QL * 512 : 8];
     __shared__ uint32_t marks[3];  // list R: keys of a unit with a non-finite latent
 
     const table_ptr plan = table(a.plan);
@@ -115,6 +119,7 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     const int n_jobs = plan[ROWS ? kPlanJobsR : kPlanJobsK], tag = plan[kPlanTag];
     const int seg = d[0], f0 = d[1], n_rows = d[2], rb = d[3], key0 = d[4], key_end = d[5],
               ctx = d[6], part = d[7];
+    // no such job; or a plan for other sizes, or a failed one
     if ((int)blockIdx.x >= n_jobs || tag != (int)a.p.tag)
         return;
 
@@ -127,41 +132,55 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     const table_ptr ptab = table(seg >= 0 ? a.page_table + (long long)seg * a.max_pages
                                           : a.prefix_page_ids + table(a.cu_prefix_pages)[~seg]);
     const int n_units = key_end > key0 && a.num_pool_pages > 0 ? (key_end - key0 + 31) >> 5 : 0;
-    const int row0 = ROWS ? 16 * QT * wave : 0;  // the wave's first row of the block
+    const int row0 = ROWS ? 16 * wave : 0;  // the wave's first row of the block
 
-    // ---- Q^T operands: row 16q + n, latent columns 32j + 8g .., then the rope key's ----
-    V8 qv[QT][KSM + RSM];
-    int lim[QT];  // lane's row n sees keys [0, lim] of the segment
-    int lim_wave = -1, lim_all = key_end - 1;
-#pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        const int r = min(row0 + 16 * q + n, n_rows - 1);  // rows past the block repeat its last
+    // ---- Q^T operands: row n, latent columns 32j + 8g .., then the rope key's; the rows' limits ----
+    V8 qv[KSM + RSM - QL];
+    uint16_t* const my_q = q_lds + wave * QL * 512 + lane * 8;
+    const bool causal_seg = a.causal && seg >= 0;
+    int lim, lim_wave = -1, lim_all = key_end - 1;  // lane's row n sees keys [0, lim] of the segment
+    {
+        const int r = min(row0 + n, n_rows - 1);  // rows past the block repeat its last
         const long long fr = (long long)f0 + r;
-        lim[q] = a.causal && seg >= 0 ? ctx + (rb + r) / H : key_end - 1;
+        lim = causal_seg ? ctx + (rb + r) / H : key_end - 1;
         const uint16_t* ql = a.q_latent + fr * KV + 8 * g;
         const uint16_t* qr = a.q_rope + fr * RP;
 #pragma unroll
-        for (int j = 0; j < KSM; ++j)
-            qv[q][j] = j < ks ? *reinterpret_cast<const V8*>(ql + 32 * j) : V8{};
-#pragma unroll
-        for (int j = 0; j < RSM; ++j) {
-            const int c = 32 * j + 8 * g;
-            const V8 v = j < rs ? *reinterpret_cast<const V8*>(qr + min(c, RP - 8)) : V8{};
-            qv[q][KSM + j] = c < RP ? v : V8{};
+        for (int j = 0; j < KSM + RSM; ++j) {
+            V8 v = {};
+            if (j < KSM) {
+                if (j < ks)
+                    v = *reinterpret_cast<const V8*>(ql + 32 * j);
+            } else if (j - KSM < rs) {
+                const int c = 32 * (j - KSM) + 8 * g;
+                v = *reinterpret_cast<const V8*>(qr + min(c, RP - 8));
+                v = c < RP ? v : V8{};
+            }
+            if (j < KSM + RSM - QL)
+                qv[j] = v;
+            else
+                *reinterpret_cast<V8*>(my_q + (j - (KSM + RSM - QL)) * 512) = v;
         }
-    }
-    {   // the last key that any of the wave's rows sees (-1: it has no rows), and that all see
-        const int last = min(n_rows, row0 + 16 * QT) - 1;
+        // the last key that any of the wave's rows sees (-1: it has no rows), and that all see
+        const int last = min(n_rows, row0 + 16) - 1;
         if (last >= row0)
-            lim_wave = a.causal && seg >= 0 ? ctx + (rb + last) / H : key_end - 1;
-        if (a.causal && seg >= 0)
+            lim_wave = causal_seg ? ctx + (rb + last) / H : key_end - 1;
+        if (causal_seg)
             lim_all = ctx + (rb + row0) / H;
     }
+    auto q_operand = [&](int j) {
+        return j < KSM + RSM - QL
+                   ? qv[j]
+                   : *reinterpret_cast<const V8*>(my_q + (j - (KSM + RSM - QL)) * 512);
+    };
 
     // ---- a unit's way into LDS ----
     const int s_lane = g * 128 + (n ^ ((g & 1) * kRot)) * 8;
-    u32x4 st[NL], sr[NR];
-    uint32_t sk[Q8 ? NL : 1];  // scale bytes of a load's one or two k-steps
+    struct Loaded {
+        u32x4 st[NL], sr[NR];
+        uint32_t sk[Q8 ? NL : 1];  // scale bytes of a load's one or two k-steps
+        int pg0, pg1;              // pages of the unit's tiles, -1 outside the pool
+    };
     const int upt = Q8 ? (ks + 1) >> 1 : ks;
     const int rcs = RP >> 3;
     int rope_tt[NR], rope_ch[NR];
@@ -191,7 +210,8 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
         return ok;
     };
     // (A missing tile loads page 0's, and is dropped when it is staged.)
-    auto load_unit = [&](int t0, int pg0, int pg1) {
+    auto load_unit = [&](Loaded& x, int t0, int id0, int id1) {
+        const int pg0 = x.pg0 = valid_page(id0), pg1 = x.pg1 = valid_page(id1);
         const uint8_t* base0 = a.pages + max(pg0, 0) * rec;
         const uint8_t* base1 = a.pages + max(pg1, 0) * rec;
         const int in0 = place_of(t0), in1 = place_of(t0 + 1);
@@ -207,27 +227,27 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
                 const uint8_t* lat = base + in * 16 * KV + k * 1024;
                 const uint8_t* sc = base + (long long)PS * (KV + 2 * RP) + (in * 16 + n) * ks + 2 * k;
                 if (2 * k + 1 < ks) {
-                    st[i] = *reinterpret_cast<const u32x4*>(lat + lane * 16);
-                    sk[i] = ks & 1 ? sc[0] | sc[1] << 8 : *reinterpret_cast<const uint16_t*>(sc);
+                    x.st[i] = *reinterpret_cast<const u32x4*>(lat + lane * 16);
+                    x.sk[i] = ks & 1 ? sc[0] | sc[1] << 8 : *reinterpret_cast<const uint16_t*>(sc);
                 } else {
-                    const u32x2 x = *reinterpret_cast<const u32x2*>(lat + lane * 8);
-                    st[i] = u32x4{x[0], x[1], 0, 0};
-                    sk[i] = sc[0];
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(lat + lane * 8);
+                    x.st[i] = u32x4{w[0], w[1], 0, 0};
+                    x.sk[i] = sc[0];
                 }
             } else {
-                st[i] = *reinterpret_cast<const u32x4*>(base + in * 32 * KV + k * 1024 + lane * 16);
+                x.st[i] = *reinterpret_cast<const u32x4*>(base + in * 32 * KV + k * 1024 + lane * 16);
             }
         }
 #pragma unroll
         for (int i = 0; i < NR; ++i)
             if (rope_ch[i] >= 0)
-                sr[i] = *reinterpret_cast<const u32x4*>(
+                x.sr[i] = *reinterpret_cast<const u32x4*>(
                     (rope_tt[i] ? base1 : base0) + (long long)PS * KV * (Q8 ? 1 : 2) +
                     ((rope_tt[i] ? in1 : in0) * rcs + rope_ch[i]) * 256 + n * 16);
     };
     // Writes the loaded unit to `sp`; keys outside `ok` become 0 (their slots, scales included, may
     // hold anything).  Returns the wave's marked keys.
-    auto stage_unit = [&](uint16_t* sp, uint32_t ok) {
+    auto stage_unit = [&](const Loaded& x, uint16_t* sp, uint32_t ok) {
         uint32_t mark = 0;
         int causal = a.causal;
         asm("" : "+s"(causal));  // looked at anew each time: one copy of the loop, not two
@@ -237,8 +257,8 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
             const int tt = u / UPT, k = u % UPT;
             if (u >= 2 * UPT || k >= upt)
                 continue;
-            u32x4 v = st[i];
-            uint32_t k8 = Q8 ? sk[i] : 0;
+            u32x4 v = x.st[i];
+            uint32_t k8 = Q8 ? x.sk[i] : 0;
             if (ok != 0xffffffffu) {
                 const uint32_t keep = -(ok >> (16 * tt + n) & 1);
                 v &= keep;
@@ -268,7 +288,7 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
 #pragma unroll
         for (int i = 0; i < NR; ++i)
             if (rope_ch[i] >= 0) {
-                u32x4 v = sr[i];
+                u32x4 v = x.sr[i];
                 if (ok != 0xffffffffu)
                     v &= -(ok >> (16 * rope_tt[i] + n) & 1);
                 *reinterpret_cast<u32x4*>(sp + 32 * KV + rope_tt[i] * 16 * RP + rope_ch[i] * 128 +
@@ -284,26 +304,16 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
     for (int j = 0; j < RSM; ++j)
         rope_off[j] = (32 * j + 8 * g < RP ? 4 * j + g : 0) * 128 + n * 8;
 
-    float m_run[QT], l_run[QT];
-    floatx4 acc[QT][RTM];
+    float m_run = -INFINITY, l_run = 0.0f;
+    floatx4 acc[RTM];
 #pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        m_run[q] = -INFINITY;
-        l_run[q] = 0.0f;
-#pragma unroll
-        for (int rt = 0; rt < RTM; ++rt)
-            acc[q][rt] = floatx4{0, 0, 0, 0};
-    }
+    for (int rt = 0; rt < RTM; ++rt)
+        acc[rt] = floatx4{0, 0, 0, 0};
 
     // ---- scores, softmax and product of the unit at `sp`, whose first tile is t0; `ok`: keys of
     // the unit that exist, `mark`: those with a non-finite latent ----
     auto compute_unit = [&](const uint16_t* sp, int t0, uint32_t ok, uint32_t mark) {
-        floatx4 sc[2][QT];
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int q = 0; q < QT; ++q)
-                sc[tt][q] = floatx4{0, 0, 0, 0};
+        floatx4 sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         // One k-step's operands are read while the step before it multiplies; the scheduler is held
         // to that (it would read all of them ahead, and spill).
         auto k_operand = [&](int tt, int j) {
@@ -311,73 +321,67 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
                            : *reinterpret_cast<const V8*>(sp + 32 * KV + tt * 16 * RP +
                                                           rope_off[j - KSM]);
         };
-        V8 next[2] = {k_operand(0, 0), k_operand(1, 0)};
+        V8 next[2] = {k_operand(0, 0), k_operand(1, 0)}, q_next = {};
 #pragma unroll
         for (int j = 0; j < KSM + RSM; ++j)
             if (j < KSM ? j < ks : j - KSM < rs) {
                 const V8 now[2] = {next[0], next[1]};
+                const V8 q_now = ONE && j >= KSM + RSM - QL ? q_next : q_operand(j);
                 const int after = j + 1 < ks ? j + 1 : (j < KSM ? KSM : j + 1);
                 if (after < KSM + rs) {
                     next[0] = k_operand(0, after);
                     next[1] = k_operand(1, after);
                 }
-#pragma unroll
-                for (int q = 0; q < QT; ++q)
-#pragma unroll
-                    for (int tt = 0; tt < 2; ++tt)
-                        sc[tt][q] = T::mma32(now[tt], qv[q][j], sc[tt][q]);
+                if (ONE && j + 1 >= KSM + RSM - QL && j + 1 < KSM + RSM)
+                    q_next = q_operand(j + 1);
+                sc[0] = T::mma32(now[0], q_now, sc[0]);
+                sc[1] = T::mma32(now[1], q_now, sc[1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
 
         // Units that some row does not see in full: their scores are replaced.
         if (ok != 0xffffffffu || mark != 0 || 16 * t0 + 31 > lim_all)
 #pragma unroll
-            for (int q = 0; q < QT; ++q)
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = 16 * tt + 4 * g + i;
-                        if (mark >> key & 1)
-                            sc[tt][q][i] = NAN;
-                        if (!(ok >> key & 1) || 16 * t0 + key > lim[q])
-                            sc[tt][q][i] = -INFINITY;
-                    }
-        V8 pb[QT];
-#pragma unroll
-        for (int q = 0; q < QT; ++q) {
-            float mp = -INFINITY;  // of the lane's eight scores (NaN is passed over)
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    mp = fmaxf(mp, sc[tt][q][i]);
-            mp *= a.scale_log2;
-            if (__builtin_amdgcn_ballot_w64(mp > m_run[q] + kRise)) {
-                const float m_new = fmaxf(m_run[q], rows_max(mp) - kHead);
-                const bool had = m_run[q] != -INFINITY;  // the row has accumulated state
-                if (__builtin_amdgcn_ballot_w64(had && m_new > m_run[q])) {
-                    const float alpha = had ? __builtin_amdgcn_exp2f(m_run[q] - m_new) : 1.0f;
-                    l_run[q] *= alpha;
-#pragma unroll
-                    for (int rt = 0; rt < RTM; ++rt)
-                        acc[q][rt] *= alpha;
-                }
-                m_run[q] = m_new;
-            }
-            const float m_ref = m_run[q] == -INFINITY ? 0.0f : m_run[q];
-            float psum = 0.0f;
-#pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e =
-                        __builtin_amdgcn_exp2f(fmaf(sc[tt][q][i], a.scale_log2, -m_ref));
-                    psum += e;
-                    pb[q][4 * tt + i] = static_cast<typename T::scalar>(e);
+                    const int key = 16 * tt + 4 * g + i;
+                    if (mark >> key & 1)
+                        sc[tt][i] = NAN;
+                    if (!(ok >> key & 1) || 16 * t0 + key > lim)
+                        sc[tt][i] = -INFINITY;
                 }
-            l_run[q] += psum;
+        float mp = -INFINITY;  // of the lane's eight scores (NaN is passed over)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                mp = fmaxf(mp, sc[tt][i]);
+        mp *= a.scale_log2;
+        if (__builtin_amdgcn_ballot_w64(mp > m_run + kRise)) {
+            const float m_new = fmaxf(m_run, rows_max(mp) - kHead);
+            const bool had = m_run != -INFINITY;  // the row has accumulated state
+            if (__builtin_amdgcn_ballot_w64(had && m_new > m_run)) {
+                const float alpha = had ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                l_run *= alpha;
+#pragma unroll
+                for (int rt = 0; rt < RTM; ++rt)
+                    acc[rt] *= alpha;
+            }
+            m_run = m_new;
         }
+        const float m_ref = m_run == -INFINITY ? 0.0f : m_run;
+        float psum = 0.0f;
+        V8 pb;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(sc[tt][i], a.scale_log2, -m_ref));
+                psum += e;
+                pb[4 * tt + i] = static_cast<typename T::scalar>(e);
+            }
+        l_run += psum;
         auto c_operand = [&](int rt) {  // latent columns 16rt.. of the unit's 32 keys
             const int blk = ((rt >> 1) * 4 + 2 * (rt & 1)) * 128;
             const u32x2 lo = read_tr16(sp + blk + tr_lane);
@@ -393,15 +397,13 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
                     cn[0] = c_operand(rt + 2);
                     cn[1] = c_operand(rt + 3);
                 }
-#pragma unroll
-                for (int q = 0; q < QT; ++q)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        acc[q][rt + i] = T::mma32(now[i], pb[q], acc[q][rt + i]);
+                acc[rt] = T::mma32(now[0], pb, acc[rt]);
+                acc[rt + 1] = T::mma32(now[1], pb, acc[rt + 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
-    // ---- the units: loaded one ahead, page ids two ahead ----
+
+    // ---- the units: loaded DEPTH ahead, page ids one further ----
     constexpr int STEP = ROWS ? 1 : 4;
     const int first = ROWS ? 0 : wave, tile0 = key0 >> 4;
     if constexpr (ROWS) {
@@ -409,170 +411,160 @@ __global__ __launch_bounds__(ROWS ? 64 * kRowsR / (16 * QT) : 256) __attribute__
             marks[tid] = 0;
         __syncthreads();
     }
-    int pg0 = -1, pg1 = -1, nx0 = -1, nx1 = -1;
+    Loaded x[DEPTH];
+    int id0 = -1, id1 = -1;  // pages of the next unit to load
+    auto next_ids = [&](int u) {
+        id0 = tile_page(tile0 + 2 * u);
+        id1 = tile_page(tile0 + 2 * u + 1);
+    };
     if (first < n_units) {
-        const int t0 = tile0 + 2 * first;
-        pg0 = valid_page(tile_page(t0));
-        pg1 = valid_page(tile_page(t0 + 1));
-        nx0 = tile_page(t0 + 2 * STEP);
-        nx1 = tile_page(t0 + 2 * STEP + 1);
-        load_unit(t0, pg0, pg1);
+        next_ids(first);
+#pragma unroll
+        for (int k = 0; k < DEPTH; ++k)
+            if (first + k * STEP < n_units) {
+                const int a0 = id0, a1 = id1;
+                next_ids(first + (k + 1) * STEP);
+                load_unit(x[k], tile0 + 2 * (first + k * STEP), a0, a1);
+            }
     }
-    for (int u = first; u < n_units; u += STEP) {
-        const int t0 = tile0 + 2 * u;
-        uint16_t* sp = smem[ROWS ? u & 1 : wave];
-        const uint32_t ok = keys_of(t0, pg0, pg1);
-        uint32_t mark = stage_unit(sp, ok);
-        if (ROWS && mark && lane == 0)
-            atomicOr(&marks[u % 3], mark);
-        if (u + STEP < n_units) {
-            pg0 = valid_page(nx0);
-            pg1 = valid_page(nx1);
-            load_unit(t0 + 2 * STEP, pg0, pg1);
-            nx0 = tile_page(t0 + 4 * STEP);
-            nx1 = tile_page(t0 + 4 * STEP + 1);
+    for (int u0 = first; u0 < n_units; u0 += DEPTH * STEP) {
+#pragma unroll
+        for (int k = 0; k < DEPTH; ++k) {
+            const int u = u0 + k * STEP;
+            if (u >= n_units)
+                break;
+            const int t0 = tile0 + 2 * u;
+            uint16_t* sp = smem[ROWS ? u & 1 : wave];
+            const uint32_t ok = keys_of(t0, x[k].pg0, x[k].pg1);
+            uint32_t mark = stage_unit(x[k], sp, ok);
+            if (ROWS && mark && lane == 0)
+                atomicOr(&marks[u % 3], mark);
+            if (u + DEPTH * STEP < n_units) {
+                load_unit(x[k], t0 + 2 * DEPTH * STEP, id0, id1);
+                next_ids(u + (DEPTH + 1) * STEP);
+            }
+            if constexpr (ROWS) {
+                // The other buffer is free: every wave that passed the barrier before this one has
+                // finished with it.  Likewise marks: unit u + 2's word, last read in unit u - 1, is
+                // cleared behind this barrier and set again behind the next.
+                __syncthreads();
+                mark = __builtin_amdgcn_readfirstlane(marks[u % 3]);
+                if (tid == 0)
+                    marks[(u + 2) % 3] = 0;
+            } else {
+                wave_lds_fence();
+            }
+            if (16 * t0 <= lim_wave)
+                compute_unit(sp, t0, ok, mark);
+            if constexpr (!ROWS)
+                wave_lds_fence();  // the slot's reads are done before the next unit's writes
         }
-        if constexpr (ROWS) {
-            // The other buffer is free: every wave that passed the barrier before this one has
-            // finished with it.  Likewise marks: unit u + 2's word, last read in unit u - 1, is
-            // cleared behind this barrier and set again behind the next.
-            __syncthreads();
-            mark = marks[u % 3];
-            if (tid == 0)
-                marks[(u + 2) % 3] = 0;
-        } else {
-            wave_lds_fence();
-        }
-        if (16 * t0 <= lim_wave)
-            compute_unit(sp, t0, ok, mark);
-        if constexpr (!ROWS)
-            wave_lds_fence();  // the slot's reads are done before the next unit's writes
     }
 
     // ---- final rows, or partials ----
+    typedef typename T::scalar s4 __attribute__((ext_vector_type(4)));
+    auto rounded = [](floatx4 v) {
+        s4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            x[i] = static_cast<typename T::scalar>(v[i]);
+        return x;
+    };
+    const float l = rows_sum(l_run);
     if constexpr (ROWS) {
-#pragma unroll
-        for (int q = 0; q < QT; ++q) {
-            const float l = rows_sum(l_run[q]);
-            const int r = row0 + 16 * q + n;
-            if (r >= n_rows)
-                continue;
-            if (part < 0) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                uint16_t* o = a.out + ((long long)f0 + r) * KV;
-#pragma unroll
-                for (int rt = 0; rt < RTM; ++rt)
-                    if (rt < 2 * ks) {
-                        typedef typename T::scalar s4 __attribute__((ext_vector_type(4)));
-                        s4 x;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            x[i] = static_cast<typename T::scalar>(acc[q][rt][i] * inv);
-                        *reinterpret_cast<s4*>(o + 16 * rt + 4 * g) = x;
-                    }
-                if (a.lse && g == 0)
-                    a.lse[(long long)f0 + r] = (m_run[q] + __log2f(l)) * kLn2;
-            } else {
-                float* o = a.part_o + ((long long)part + r) * KV;
-#pragma unroll
-                for (int rt = 0; rt < RTM; ++rt)
-                    if (rt < 2 * ks)
-                        *reinterpret_cast<floatx4*>(o + 16 * rt + 4 * g) = acc[q][rt];
-                if (g == 0) {
-                    a.part_ml[2 * ((long long)part + r)] = m_run[q];
-                    a.part_ml[2 * ((long long)part + r) + 1] = l;
-                }
-            }
-        }
-    } else {
-        // A wave parks a row tile in its own slot: 16 rows of KV + 4 floats, then m and l.
-        const int pitch = KV + 4;
-#pragma unroll
-        for (int q = 0; q < QT; ++q) {
-            const float l = rows_sum(l_run[q]);
-            float* mine = reinterpret_cast<float*>(smem[wave]);
-            if (q > 0)
-                __syncthreads();  // the previous tile's rows have been read
+        const int r = row0 + n;
+        if (r >= n_rows)
+            return;
+        if (part < 0) {
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            uint16_t* o = a.out + ((long long)f0 + r) * KV;
 #pragma unroll
             for (int rt = 0; rt < RTM; ++rt)
                 if (rt < 2 * ks)
-                    *reinterpret_cast<floatx4*>(mine + n * pitch + 16 * rt + 4 * g) = acc[q][rt];
+                    *reinterpret_cast<s4*>(o + 16 * rt + 4 * g) = rounded(acc[rt] * inv);
+            if (a.lse && g == 0)
+                a.lse[(long long)f0 + r] = (m_run + __log2f(l)) * kLn2;
+        } else {
+            float* o = a.part_o + ((long long)part + r) * KV;
+#pragma unroll
+            for (int rt = 0; rt < RTM; ++rt)
+                if (rt < 2 * ks)
+                    *reinterpret_cast<floatx4*>(o + 16 * rt + 4 * g) = acc[rt];
             if (g == 0) {
-                mine[16 * pitch + n] = m_run[q];
-                mine[16 * pitch + 16 + n] = l;
+                a.part_ml[2 * ((long long)part + r)] = m_run;
+                a.part_ml[2 * ((long long)part + r) + 1] = l;
             }
-            __syncthreads();
-            const int per_row = KV / 4;
-            for (int e = tid; e < 16 * per_row; e += 256) {
-                const int r = e / per_row, c = (e % per_row) * 4, row = 16 * q + r;
-                if (row >= n_rows)
-                    break;
-                float M = -INFINITY;
+        }
+    } else {
+        // A wave parks its rows in its own slot: 16 rows of KV + 4 floats, then m and l.
+        const int pitch = KV + 4;
+        float* mine = reinterpret_cast<float*>(smem[wave]);
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    M = fmaxf(M, reinterpret_cast<const float*>(smem[v])[16 * pitch + r]);
-                float L = 0.0f;
-                floatx4 o = {0, 0, 0, 0};
+        for (int rt = 0; rt < RTM; ++rt)
+            if (rt < 2 * ks)
+                *reinterpret_cast<floatx4*>(mine + n * pitch + 16 * rt + 4 * g) = acc[rt];
+        if (g == 0) {
+            mine[16 * pitch + n] = m_run;
+            mine[16 * pitch + 16 + n] = l;
+        }
+        __syncthreads();
+        const int per_row = KV / 4;
+        for (int e = tid; e < n_rows * per_row; e += kThreadsK) {
+            const int r = e / per_row, c = (e % per_row) * 4;
+            float M = -INFINITY;
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const float* x = reinterpret_cast<const float*>(smem[v]);
-                    const float mv = x[16 * pitch + r];
-                    const float f = mv == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mv - M);
-                    L += x[16 * pitch + 16 + r] * f;
-                    o += *reinterpret_cast<const floatx4*>(x + r * pitch + c) * f;
-                }
-                if (part < 0) {
-                    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-                    typedef typename T::scalar s4 __attribute__((ext_vector_type(4)));
-                    s4 y;
+            for (int v = 0; v < 4; ++v)
+                M = fmaxf(M, reinterpret_cast<const float*>(smem[v])[16 * pitch + r]);
+            float L = 0.0f;
+            floatx4 o = {0, 0, 0, 0};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        y[i] = static_cast<typename T::scalar>(o[i] * inv);
-                    *reinterpret_cast<s4*>(a.out + ((long long)f0 + row) * KV + c) = y;
-                    if (a.lse && c == 0)
-                        a.lse[(long long)f0 + row] = (M + __log2f(L)) * kLn2;
-                } else {
-                    *reinterpret_cast<floatx4*>(a.part_o + ((long long)part + row) * KV + c) = o;
-                    if (c == 0) {
-                        a.part_ml[2 * ((long long)part + row)] = M;
-                        a.part_ml[2 * ((long long)part + row) + 1] = L;
-                    }
+            for (int v = 0; v < 4; ++v) {
+                const float* w = reinterpret_cast<const float*>(smem[v]);
+                const float mv = w[16 * pitch + r];
+                // A sum of NaN may come with a maximum of -inf (all scores NaN): weight 0 keeps it.
+                const float f = mv == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mv - M);
+                L += w[16 * pitch + 16 + r] * f;
+                o += *reinterpret_cast<const floatx4*>(w + r * pitch + c) * f;
+            }
+            if (part < 0) {
+                const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+                *reinterpret_cast<s4*>(a.out + ((long long)f0 + r) * KV + c) = rounded(o * inv);
+                if (a.lse && c == 0)
+                    a.lse[(long long)f0 + r] = (M + __log2f(L)) * kLn2;
+            } else {
+                *reinterpret_cast<floatx4*>(a.part_o + ((long long)part + r) * KV + c) = o;
+                if (c == 0) {
+                    a.part_ml[2 * ((long long)part + r)] = M;
+                    a.part_ml[2 * ((long long)part + r) + 1] = L;
                 }
             }
         }
     }
 }
 
-template <typename T, bool Q8, int KSM, int QT, bool ROWS, int RP = -1>
+template <typename T, bool Q8, int KSM, bool ROWS, int RP = -1>
 hipError_t launch_one(const LatentArgs& a, hipStream_t stream) {
-    const int jobs = ROWS ? a.p.max_jobs_r : a.p.max_jobs_k;
-    hipLaunchKernelGGL((latent_attend_kernel<T, Q8, KSM, QT, ROWS, RP>), dim3(jobs),
-                       dim3(ROWS ? 64 * kRowsR / (16 * QT) : 256), 0, stream, a);
+    hipLaunchKernelGGL((latent_attend_kernel<T, Q8, KSM, ROWS, RP>),
+                       dim3(ROWS ? a.jobs_r : a.jobs_k), dim3(ROWS ? kThreadsR : kThreadsK), 0,
+                       stream, a);
     return hipGetLastError();
+}
+
+template <typename T, bool Q8, bool ROWS>
+hipError_t launch_shape(const LatentArgs& a, hipStream_t stream) {
+    const int ks = a.kv_rank / 32;
+    if (ks == 4 && a.rope_dim == 16)
+        return launch_one<T, Q8, 4, ROWS, 16>(a, stream);
+    if (ks == 16 && a.rope_dim == 64)
+        return launch_one<T, Q8, 16, ROWS, 64>(a, stream);
+    return ks <= 4   ? launch_one<T, Q8, 4, ROWS>(a, stream)
+           : ks <= 8 ? launch_one<T, Q8, 8, ROWS>(a, stream)
+                     : launch_one<T, Q8, 16, ROWS>(a, stream);
 }
 
 template <typename T, bool Q8>
 hipError_t launch_list(const LatentArgs& a, bool rows, hipStream_t stream) {
-    const int ks = a.kv_rank / 32;
-    const bool base = ks == 4 && a.rope_dim == 16, wide = ks == 16 && a.rope_dim == 64;
-    if (rows && base)
-        return launch_one<T, Q8, 4, 2, true, 16>(a, stream);
-    if (rows && wide)
-        return launch_one<T, Q8, 16, 1, true, 64>(a, stream);
-    if (base)
-        return a.p.qt == 2 ? launch_one<T, Q8, 4, 2, false, 16>(a, stream)
-                           : launch_one<T, Q8, 4, 1, false, 16>(a, stream);
-    if (wide)
-        return launch_one<T, Q8, 16, 1, false, 64>(a, stream);
-    if (rows)
-        return ks <= 4   ? launch_one<T, Q8, 4, 2, true>(a, stream)
-               : ks <= 8 ? launch_one<T, Q8, 8, 1, true>(a, stream)
-                         : launch_one<T, Q8, 16, 1, true>(a, stream);
-    if (a.p.qt == 2)
-        return launch_one<T, Q8, 4, 2, false>(a, stream);
-    return ks <= 4   ? launch_one<T, Q8, 4, 1, false>(a, stream)
-           : ks <= 8 ? launch_one<T, Q8, 8, 1, false>(a, stream)
-                     : launch_one<T, Q8, 16, 1, false>(a, stream);
+    return rows ? launch_shape<T, Q8, true>(a, stream) : launch_shape<T, Q8, false>(a, stream);
 }
 
 }  // namespace

@@ -195,8 +195,8 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
                          const int32_t* page_table, int max_pages, int num_pool_pages,
                          const void* pages, const void* q_latent, const void* q_rope, int n_groups,
                          const int32_t* cu_prefix_pages, const int32_t* prefix_page_ids,
-                         const void* plan, size_t plan_bytes, void* out, float* lse,
-                         void* workspace, size_t workspace_bytes) {
+                         const void* plan, size_t plan_bytes, const int32_t* host_info, void* out,
+                         float* lse, void* workspace, size_t workspace_bytes) {
     const char* fn = "mla_latent_attention";
     if (int st = plan_scalars(fn, B, rows, n_heads, kv_rank, page_size, max_q_len, n_groups))
         return st;
@@ -217,6 +217,16 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
     a.p = plan_shape(B, n_groups, rows, n_heads, kv_rank, max_q_len);
     if (plan_bytes < (size_t)a.p.words * sizeof(int32_t))
         return invalid(fn, "the plan was made for other sizes");
+    a.jobs_k = a.p.max_jobs_k;
+    a.jobs_r = a.p.max_jobs_r;
+    if (host_info) {
+        if (host_info[kPlanTag] != (int)a.p.tag || host_info[kPlanJobsK] < 0 ||
+            host_info[kPlanJobsK] > a.jobs_k || host_info[kPlanJobsR] < 0 ||
+            host_info[kPlanJobsR] > a.jobs_r)
+            return invalid(fn, "host_info is not that of a plan for these sizes");
+        a.jobs_k = host_info[kPlanJobsK];
+        a.jobs_r = host_info[kPlanJobsR];
+    }
     if (workspace_bytes < workspace_size(a.p))
         return invalid(fn, "workspace needs " + std::to_string(workspace_size(a.p)) + " bytes");
     a.H = n_heads;

@@ -136,7 +136,7 @@ hipError_t launch_merge_t(const LatentArgs& a, hipStream_t stream) {
 hipError_t launch_latent_attention(const LatentArgs& a, int dtype, hipStream_t stream) {
     // List R first: its jobs are the longer ones.
     for (const bool rows : {true, false}) {
-        if ((rows ? a.p.max_jobs_r : a.p.max_jobs_k) == 0)
+        if ((rows ? a.jobs_r : a.jobs_k) == 0)
             continue;
         const hipError_t e = a.q8 ? launch_attend_q8(a, dtype, rows, stream)
                                   : launch_attend_16(a, dtype, rows, stream);

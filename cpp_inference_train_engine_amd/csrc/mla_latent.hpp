@@ -8,15 +8,14 @@ namespace mla {
 
 // A segment is a run of keys that a set of consecutive query rows sees: a session's own pages
 // with its rows, or a group's shared prefix with the rows of all of the group's sessions.  A job
-// is one block of a segment's (query, head) rows over one range of its keys.  Segments of at most
-// kFewRows rows go to list K (a workgroup's four waves split the keys), the others to list R (they
-// split the rows).
-constexpr int kFewRows = 64;
-constexpr int kRowsR = 128;  // rows of a block of list R
+// is one block of a segment's (query, head) rows over one range of its keys.  Segments with few
+// rows go to list K (16 rows a job; its four waves split the keys), the others to list R (128 rows;
+// its eight waves split them).
+constexpr int kRowsK = 16, kRowsR = 128;  // rows of a block
+constexpr int kThreadsK = 256, kThreadsR = 512;
 constexpr int kTile = 32;    // keys a wave takes at a time
 constexpr int kJobInts = 8;  // segment (>= 0 session, ~group), first flat row, rows, first row's
                              // index in the segment, first key, last key + 1, ctx, partial row
-constexpr int kSegInts = 8;
 constexpr int kMergeInts = 8;
 constexpr int kPlanHead = 64;  // words
 enum { kPlanStatus, kPlanBad, kPlanJobsK, kPlanJobsR, kPlanParts, kPlanRows, kPlanTag };
@@ -24,11 +23,10 @@ enum { kPlanStatus, kPlanBad, kPlanJobsK, kPlanJobsR, kPlanParts, kPlanRows, kPl
 // What a plan and the calls over it derive from the same scalars.
 struct PlanShape {
     int B, groups, rows, H, kv_rank, max_q_len;
-    int qt;                 // 16-row tiles of a list-K block
-    int target_k, target_r; // workgroups that the lists aim at
-    int least_k, least_r;   // tiles that a job takes at least
-    int max_jobs_k, max_jobs_r;
-    long long max_parts;    // (query, head) rows of partials
+    int slots_k, slots_r;        // workgroups of a list that the GPU holds at once
+    bool list_k_holds_all;       // list K has room for the segments of many rows, too
+    int max_jobs_k, max_jobs_r;  // 0: no segment of these sizes can be on the list
+    long long max_parts;         // (query, head) rows of partials
     long long seg_at, merge_at, session_at, jobs_k_at, jobs_r_at, words;  // word offsets
     uint32_t tag;
 };
@@ -48,6 +46,7 @@ struct LatentArgs {
     int H, kv_rank, rope_dim, page_size, max_pages, num_pool_pages;
     int causal;        // the rows of a block may see different keys
     int q8;
+    int jobs_k, jobs_r;  // workgroups to launch: the plan's jobs, or as many as it could have
     float scale_log2;  // softmax scale * log2(e)
     const int32_t *plan, *page_table, *cu_prefix_pages, *prefix_page_ids;
     const uint8_t* pages;

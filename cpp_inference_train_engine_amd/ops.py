@@ -271,13 +271,14 @@ def _dtype_of(code: int):
 def _check(what: str, t, shape, dtype) -> None:
     """A contiguous tensor of this shape (None: any size) and type on the current GPU, or
     ValueError: the kernels see addresses only."""
-    torch = _torch()
-    if (t.dtype != dtype or len(t.shape) != len(shape) or not t.is_contiguous() or
-            any(n is not None and n != m for n, m in zip(shape, t.shape))):
-        raise ValueError(f"{what}: wanted a contiguous {dtype} tensor of shape {tuple(shape)}, got "
-                         f"{t.dtype} {tuple(t.shape)}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if (t.dtype is dtype and t.is_contiguous() and
+            (t.shape == shape or (len(t.shape) == len(shape) and
+                                  all(n is None or n == m for n, m in zip(shape, t.shape))))):
+        if t.is_cuda and t.get_device() == _torch().cuda.current_device():
+            return
         raise ValueError(f"{what}: wanted on the current GPU, is on {t.device}")
+    raise ValueError(f"{what}: wanted a contiguous {dtype} tensor of shape {tuple(shape)}, got "
+                     f"{t.dtype} {tuple(t.shape)}")
 
 
 class QuantizedLatentCache:
@@ -376,17 +377,20 @@ class AttentionPlan:
     max_q_len: int
     prefixes: SharedPrefixes | None
     words: object  # the plan itself (device int32)
+    info: object = None  # host copy of its info once read_info has been called
 
     @property
     def n_groups(self) -> int:
         return self.prefixes.n_groups if self.prefixes is not None else 0
 
     def read_info(self, stream=None):
-        """Synchronise and return [jobs, 0, jobs of few rows, jobs of many rows, partial rows,
-        query rows, ..]; raises when the batch or the prefixes are invalid."""
+        """Synchronise and return [jobs, 0, jobs of 16 rows, jobs of 128 rows, partial rows, query
+        rows, ..]; raises when the batch or the prefixes are invalid.  Calls after it launch no
+        more workgroups than the plan has jobs."""
         import numpy as np
         h = np.zeros(PLAN_INFO_INTS, np.int32)
         check(lib().mla_read_plan_info(stream_handle(stream), ptr(self.words), h.ctypes.data))
+        self.info = h
         return h.tolist()
 
 
@@ -461,7 +465,8 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
         CACHE_Q8 if q8 else CACHE_16BIT, float(scale), ptr(b.page_table), b.max_pages,
         b.num_pool_pages, ptr(pages), ptr(q_latent), ptr(q_rope), plan.n_groups,
         ptr(x.cu_pages) if x else None, ptr(x.page_ids) if x else None, ptr(plan.words),
-        plan.words.numel() * 4, ptr(out), ptr(lse), ptr(workspace), workspace.numel()))
+        plan.words.numel() * 4, ptr(plan.info), ptr(out), ptr(lse), ptr(workspace),
+        workspace.numel()))
     return out
 
 

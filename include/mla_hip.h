@@ -395,14 +395,16 @@ int mla_plan_attention(void* stream, int B, int rows, int n_heads, int kv_rank, 
                        const int32_t* prefix_len, const int32_t* cu_prefix_pages,
                        const int32_t* prefix_page_ids, int n_prefix_pages, int num_pool_pages,
                        void* plan, size_t plan_bytes);
-/* Synchronises `stream` and copies host_info[MLA_PLAN_INFO_INTS]: {jobs, 0, jobs of few rows, jobs
- * of many rows, partial rows, query rows, 0 or more of no meaning}, or {-1, first bad entry, ..}
+/* Synchronises `stream` and copies host_info[MLA_PLAN_INFO_INTS]: {jobs, 0, jobs of 16 rows, jobs
+ * of 128 rows, partial rows, query rows, a tag of the plan's sizes, 0}, or {-1, first bad entry, ..}
  * with MLA_ERR_INVALID_ARGUMENT and a message. */
 int mla_read_plan_info(void* stream, const void* plan, int32_t* host_info);
 /* The attention.  page_table and max_pages are those of the metadata, cache_format one of
  * MLA_CACHE_*, q_latent [rows x n_heads x kv_rank], q_rope [rows x n_heads x rope_dim] and out
- * [rows x n_heads x kv_rank] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.  Shapes
- * as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace at multiples of 16
+ * [rows x n_heads x kv_rank] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.
+ * host_info is what mla_read_plan_info returned for this very plan, or NULL: with it the call
+ * launches as many workgroups as the plan has jobs, without it as many as a plan of these sizes can
+ * have, whose rest returns at once (a few us).  Shapes as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace at multiples of 16
  * bytes.  The workspace needs no initialisation; calls that share one must be ordered on one
  * stream.  Page ids outside the pool are skipped, with the keys on them.  A non-finite latent
  * makes the rows that see its key NaN, and no others. */
@@ -411,8 +413,8 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
                          const int32_t* page_table, int max_pages, int num_pool_pages,
                          const void* pages, const void* q_latent, const void* q_rope, int n_groups,
                          const int32_t* cu_prefix_pages, const int32_t* prefix_page_ids,
-                         const void* plan, size_t plan_bytes, void* out, float* lse,
-                         void* workspace, size_t workspace_bytes);
+                         const void* plan, size_t plan_bytes, const int32_t* host_info, void* out,
+                         float* lse, void* workspace, size_t workspace_bytes);
 
 /* ------------------------------------------------------------------ model
  * The batched decode step around the attention: everything of

@@ -229,9 +229,12 @@ def test_shared_prefixes(gpu, H, kv, rope, page, dtype, q8):
 def test_long_keys_and_many_sessions(gpu, H, kv, rope, page, sessions, groups, q8):
     c = make(H, kv, rope, page, 0, q8, sessions, groups, seed=len(sessions))
     _say(f"long H={H} kv={kv} sessions={len(sessions)} groups={groups} q8={q8}")
-    plan, out, lse = call(gpu, c, device(gpu, c))
-    _say(plan.read_info())
+    d = device(gpu, c)
+    plan, out, lse = call(gpu, c, d)
     check(c, out, lse)
+    _say(plan.read_info())  # from here on the exact number of workgroups
+    _, out2, lse2 = call(gpu, c, d, plan)
+    assert (out2 == out).all() and (lse2 == lse).all()
 
 
 @pytest.mark.gpu
@@ -426,6 +429,10 @@ def test_a_plan_for_other_sizes_writes_nothing(gpu):
     other = dataclasses.replace(plan, max_q_len=1)  # tables of the same size
     _, out, lse = call(gpu, c, d, other, workspace=gpu.attention_workspace(plan))
     assert (out == 5).all() and (lse == 5).all()
+    plan.read_info()
+    with pytest.raises(gpu.MlaError, match="host_info"):
+        call(gpu, c, d, dataclasses.replace(other, info=plan.info),
+             workspace=gpu.attention_workspace(plan))
     small = dataclasses.replace(plan, words=plan.words[:64])
     with pytest.raises(gpu.MlaError, match="other sizes"):
         call(gpu, c, d, small, workspace=gpu.attention_workspace(plan))
@@ -458,11 +465,11 @@ def test_refusals_of_planned_attention():
         assert plan(**kw) == 1, kw
     names2 = ("stream", "B", "rows", "H", "kv", "rope", "page", "max_q", "dtype", "fmt", "scale",
               "table", "max_pages", "pool", "pages", "ql", "qr", "groups", "cu_pages", "ids",
-              "plan", "plan_bytes", "out", "lse", "ws", "ws_bytes")
+              "plan", "plan_bytes", "info", "out", "lse", "ws", "ws_bytes")
 
     def attend(**kw):
         v = dict(zip(names2, (None, 4, 4, 8, 128, 16, 64, 1, 0, 1, 0.1, a, 4, 10, a, a, a, 1, a, a,
-                              a, 1 << 30, a, None, a, 1 << 40)), **kw)
+                              a, 1 << 30, None, a, None, a, 1 << 40)), **kw)
         return L.mla_latent_attention(*[v[n] for n in names2])
 
     for kw in (dict(B=-1), dict(rows=-1), dict(H=0), dict(kv=0), dict(rope=-1), dict(page=0),
@@ -471,7 +478,7 @@ def test_refusals_of_planned_attention():
                dict(table=None), dict(pages=None), dict(ql=None), dict(qr=None), dict(plan=None),
                dict(out=None), dict(ws=None), dict(cu_pages=None), dict(pages=a + 8),
                dict(ql=a + 2), dict(qr=a + 8), dict(out=a + 8), dict(plan=a + 8), dict(ws=a + 4),
-               dict(plan_bytes=16), dict(ws_bytes=16)):
+               dict(plan_bytes=16), dict(ws_bytes=16), dict(info=a)):
         assert attend(**kw) == 1, kw
     for kw in (dict(kv=100), dict(kv=544), dict(rope=4), dict(rope=72), dict(page=40)):
         assert attend(**kw) == 3, kw
