@@ -94,7 +94,7 @@ __device__ __forceinline__ bool drop_nan8(u32x4& v) {
 // shape (kv_rank = 32 KSM, rope_dim = RP_), -1 for any.
 template <typename T, bool Q8, int KSM, bool ROWS, int RP_ = -1>
 __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
-    amdgpu_waves_per_eu(KSM >= 16 && !ROWS ? 1 : 2, 8))) void latent_attend_kernel(LatentArgs a) {
+    amdgpu_waves_per_eu(KSM >= 16 && !ROWS ? 1 : RP_ == 16 ? 4 : 2, 8))) void latent_attend_kernel(LatentArgs a) {
     constexpr int NW = (ROWS ? kThreadsR : kThreadsK) / 64;  // waves
     constexpr bool ONE = RP_ >= 0;
     constexpr int RSM = ONE ? (RP_ + 31) / 32 : 2;      // rope k-steps (rope_dim <= 64)
@@ -108,7 +108,8 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     constexpr int DEPTH = ROWS && ONE && KSM == 4 ? 2 : 1;  // units in flight behind the one at work
     // Q^T k-steps that stay in LDS, lane by lane, where the registers would spill (a reload waits
     // for every load in flight): at kv 512 O^T takes 128 of a wave's 256 registers, Q^T 72.
-    constexpr int QL = KSM >= 16 && ROWS ? (ONE ? (Q8 ? 4 : 6) : 8) : 0;
+    constexpr int AHEAD = ONE && KSM >= 16 ? 2 : 1;  // steps that LDS reads run ahead of their use
+    constexpr int QL = KSM >= 16 && ROWS ? (ONE ? (Q8 ? 8 : 10) : 8) : 0;
     using V8 = typename T::vec8;
     __shared__ __attribute__((aligned(16))) uint16_t smem[SLOTS][SLOT];
     __shared__ __attribute__((aligned(16))) uint16_t q_lds[QL > 0 ? NW * QL * 512 : 8];
@@ -321,22 +322,54 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                            : *reinterpret_cast<const V8*>(sp + 32 * KV + tt * 16 * RP +
                                                           rope_off[j - KSM]);
         };
-        V8 next[2] = {k_operand(0, 0), k_operand(1, 0)}, q_next = {};
+        if constexpr (ONE) {
+            // Step j's operands are read AHEAD steps before (an LDS read takes about as long as
+            // that many steps' products); the first of the second product before the softmax.
+            V8 ring[AHEAD][2], q_ring[AHEAD];
 #pragma unroll
-        for (int j = 0; j < KSM + RSM; ++j)
-            if (j < KSM ? j < ks : j - KSM < rs) {
-                const V8 now[2] = {next[0], next[1]};
-                const V8 q_now = ONE && j >= KSM + RSM - QL ? q_next : q_operand(j);
-                const int after = j + 1 < ks ? j + 1 : (j < KSM ? KSM : j + 1);
-                if (after < KSM + rs) {
-                    next[0] = k_operand(0, after);
-                    next[1] = k_operand(1, after);
+            for (int j = 0; j < KSM + RSM + AHEAD; ++j) {
+                if (j >= AHEAD) {
+                    const int i = j - AHEAD;
+                    const V8 q_now = i < KSM + RSM - QL ? qv[i < KSM + RSM - QL ? i : 0] : q_ring[i % AHEAD];
+                    sc[0] = T::mma32(ring[i % AHEAD][0], q_now, sc[0]);
+                    sc[1] = T::mma32(ring[i % AHEAD][1], q_now, sc[1]);
                 }
-                if (ONE && j + 1 >= KSM + RSM - QL && j + 1 < KSM + RSM)
-                    q_next = q_operand(j + 1);
-                sc[0] = T::mma32(now[0], q_now, sc[0]);
-                sc[1] = T::mma32(now[1], q_now, sc[1]);
+                if (j < KSM + RSM) {
+                    ring[j % AHEAD][0] = k_operand(0, j);
+                    ring[j % AHEAD][1] = k_operand(1, j);
+                    if (j >= KSM + RSM - QL)
+                        q_ring[j % AHEAD] = q_operand(j);
+                }
                 __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            V8 next[2] = {k_operand(0, 0), k_operand(1, 0)};
+#pragma unroll
+            for (int j = 0; j < KSM + RSM; ++j)
+                if (j < KSM ? j < ks : j - KSM < rs) {
+                    const V8 now[2] = {next[0], next[1]}, q_now = q_operand(j);
+                    const int after = j + 1 < ks ? j + 1 : (j < KSM ? KSM : j + 1);
+                    if (after < KSM + rs) {
+                        next[0] = k_operand(0, after);
+                        next[1] = k_operand(1, after);
+                    }
+                    sc[0] = T::mma32(now[0], q_now, sc[0]);
+                    sc[1] = T::mma32(now[1], q_now, sc[1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+        auto c_operand = [&](int rt) {  // latent columns 16rt.. of the unit's 32 keys
+            const int blk = ((rt >> 1) * 4 + 2 * (rt & 1)) * 128;
+            const u32x2 lo = read_tr16(sp + blk + tr_lane);
+            const u32x2 hi = read_tr16(sp + 16 * KV + blk + tr_lane);
+            return __builtin_bit_cast(V8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+        };
+        V8 cring[AHEAD][2];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (2 * k < 2 * ks) {
+                cring[k][0] = c_operand(2 * k);
+                cring[k][1] = c_operand(2 * k + 1);
             }
 
         // Units that some row does not see in full: their scores are replaced.
@@ -382,23 +415,15 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                 pb[4 * tt + i] = static_cast<typename T::scalar>(e);
             }
         l_run += psum;
-        auto c_operand = [&](int rt) {  // latent columns 16rt.. of the unit's 32 keys
-            const int blk = ((rt >> 1) * 4 + 2 * (rt & 1)) * 128;
-            const u32x2 lo = read_tr16(sp + blk + tr_lane);
-            const u32x2 hi = read_tr16(sp + 16 * KV + blk + tr_lane);
-            return __builtin_bit_cast(V8, u32x4{lo[0], lo[1], hi[0], hi[1]});
-        };
-        V8 cn[2] = {c_operand(0), c_operand(1)};
 #pragma unroll
-        for (int rt = 0; rt < RTM; rt += 2)
-            if (rt < 2 * ks) {
-                const V8 now[2] = {cn[0], cn[1]};
-                if (rt + 2 < 2 * ks) {
-                    cn[0] = c_operand(rt + 2);
-                    cn[1] = c_operand(rt + 3);
+        for (int k = 0; k < KSM; ++k)
+            if (k < ks) {
+                acc[2 * k] = T::mma32(cring[k % AHEAD][0], pb, acc[2 * k]);
+                acc[2 * k + 1] = T::mma32(cring[k % AHEAD][1], pb, acc[2 * k + 1]);
+                if (k + AHEAD < ks) {
+                    cring[k % AHEAD][0] = c_operand(2 * (k + AHEAD));
+                    cring[k % AHEAD][1] = c_operand(2 * (k + AHEAD) + 1);
                 }
-                acc[rt] = T::mma32(now[0], pb, acc[rt]);
-                acc[rt + 1] = T::mma32(now[1], pb, acc[rt + 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
