@@ -268,17 +268,31 @@ def _dtype_of(code: int):
     return torch.float16 if code == DTYPE_F16 else torch.bfloat16
 
 
-def _check(what: str, t, shape, dtype) -> None:
-    """A contiguous tensor of this shape (None: any size) and type on the current GPU, or
-    ValueError: the kernels see addresses only."""
-    if (t.dtype is dtype and t.is_contiguous() and
-            (t.shape == shape or (len(t.shape) == len(shape) and
-                                  all(n is None or n == m for n, m in zip(shape, t.shape))))):
-        if t.is_cuda and t.get_device() == _torch().cuda.current_device():
-            return
+_current_device = None
+
+
+def _gpu() -> int:
+    """Index of the current GPU (0.2 us; torch is imported once)."""
+    global _current_device
+    if _current_device is None:
+        _current_device = _torch().cuda.current_device
+    return _current_device()
+
+
+def _check(what: str, t, shape, dtype, gpu: int) -> int:
+    """Address of a contiguous tensor of this shape and type on GPU ``gpu``, or ValueError: the
+    kernels see addresses only."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: wanted a contiguous {dtype} tensor of shape {tuple(shape)}, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    if t.get_device() != gpu:
         raise ValueError(f"{what}: wanted on the current GPU, is on {t.device}")
-    raise ValueError(f"{what}: wanted a contiguous {dtype} tensor of shape {tuple(shape)}, got "
-                     f"{t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _check_list(what: str, t, gpu: int) -> int:
+    """The same of a one-dimensional int32 tensor of any length."""
+    return _check(what, t, (t.numel(),), _torch().int32, gpu)
 
 
 class QuantizedLatentCache:
@@ -310,23 +324,28 @@ class QuantizedLatentCache:
     def record_bytes(self) -> int:
         return int(self.pages.shape[2])
 
+    def _layer_address(self, l: int, gpu: int) -> int:
+        if self.pages.get_device() != gpu:
+            raise ValueError(f"cache: wanted on the current GPU, is on {self.pages.device}")
+        if not -self.n_layers <= l < self.n_layers:
+            raise IndexError(f"layer {l} of {self.n_layers}")
+        return self.pages.data_ptr() + l % self.n_layers * self.pages.stride(0)
+
 
 def append_latent_q8(cache: QuantizedLatentCache, layer: int, ckv, krope, slot_mapping,
                      stream=None) -> None:
     """(d) Quantise ckv [T x kv_rank] (fp32) to 8 bits, round krope [T x rope_dim] (fp32) to the
     cache's 16-bit dtype, and write row t to flat slot slot_mapping[t] of ``layer``'s pool.  Slots
     outside the pool are skipped; the others are distinct."""
-    torch = _torch()
-    T, pages = int(ckv.shape[0]), cache.layer(layer)
-    _check("ckv", ckv, (T, cache.kv_rank), torch.float32)
-    _check("krope", krope, (T, cache.rope_dim), torch.float32)
-    _check("slot_mapping", slot_mapping, (None,), torch.int32)
-    _check("cache", pages, (None, None), torch.uint8)
-    if slot_mapping.shape[0] < T:
-        raise ValueError(f"slot_mapping: {slot_mapping.shape[0]} slots for {T} rows")
+    f32, gpu, T = _torch().float32, _gpu(), int(ckv.shape[0])
+    x = _check("ckv", ckv, (T, cache.kv_rank), f32, gpu)
+    k = _check("krope", krope, (T, cache.rope_dim), f32, gpu)
+    slots = _check_list("slot_mapping", slot_mapping, gpu)
+    if slot_mapping.numel() < T:
+        raise ValueError(f"slot_mapping: {slot_mapping.numel()} slots for {T} rows")
     check(lib().mla_append_latent_q8(stream_handle(stream), T, cache.kv_rank, cache.rope_dim,
-                                     cache.page_size, cache.dtype, ptr(ckv), ptr(krope),
-                                     ptr(slot_mapping), cache.num_pages, ptr(pages)))
+                                     cache.page_size, cache.dtype, x, k, slots, cache.num_pages,
+                                     cache._layer_address(layer, gpu)))
 
 
 def read_latent_q8(cache: QuantizedLatentCache, layer: int, slot_mapping, ckv=None, krope=None,
@@ -334,19 +353,17 @@ def read_latent_q8(cache: QuantizedLatentCache, layer: int, slot_mapping, ckv=No
     """(d) The tokens at flat slots slot_mapping[T] of ``layer``'s pool as 16-bit rows of the
     cache's dtype: (ckv [T x kv_rank], krope [T x rope_dim]), exact.  Rows whose slot lies outside
     the pool are left as they were (zero in tensors that this call makes)."""
-    torch = _torch()
-    T, pages, dt = int(slot_mapping.shape[0]), cache.layer(layer), _dtype_of(cache.dtype)
+    gpu, T, dt = _gpu(), int(slot_mapping.shape[0]), _dtype_of(cache.dtype)
+    slots = _check_list("slot_mapping", slot_mapping, gpu)
     if ckv is None:
-        ckv = torch.zeros((T, cache.kv_rank), dtype=dt, device=pages.device)
+        ckv = _torch().zeros((T, cache.kv_rank), dtype=dt, device=cache.pages.device)
     if krope is None:
-        krope = torch.zeros((T, cache.rope_dim), dtype=dt, device=pages.device)
-    _check("slot_mapping", slot_mapping, (T,), torch.int32)
-    _check("ckv", ckv, (T, cache.kv_rank), dt)
-    _check("krope", krope, (T, cache.rope_dim), dt)
-    _check("cache", pages, (None, None), torch.uint8)
+        krope = _torch().zeros((T, cache.rope_dim), dtype=dt, device=cache.pages.device)
+    x = _check("ckv", ckv, (T, cache.kv_rank), dt, gpu)
+    k = _check("krope", krope, (T, cache.rope_dim), dt, gpu)
     check(lib().mla_read_latent_q8(stream_handle(stream), T, cache.kv_rank, cache.rope_dim,
-                                   cache.page_size, cache.dtype, ptr(slot_mapping),
-                                   cache.num_pages, ptr(pages), ptr(ckv), ptr(krope)))
+                                   cache.page_size, cache.dtype, slots, cache.num_pages,
+                                   cache._layer_address(layer, gpu), x, k))
     return ckv, krope
 
 
@@ -366,22 +383,32 @@ class SharedPrefixes:
         return int(self.prefix_len.shape[0])
 
 
-@dataclass
 class AttentionPlan:
     """What ``plan_attention`` built, for ``latent_attention`` calls over the same batch."""
 
-    batch: RaggedBatch
-    n_heads: int
-    kv_rank: int
-    rows: int
-    max_q_len: int
-    prefixes: SharedPrefixes | None
-    words: object  # the plan itself (device int32)
-    info: object = None  # host copy of its info once read_info has been called
+    def __init__(self, batch: RaggedBatch, n_heads: int, kv_rank: int, rows: int, max_q_len: int,
+                 prefixes: SharedPrefixes | None, words):
+        self.batch, self.n_heads, self.kv_rank = batch, n_heads, kv_rank
+        self.rows, self.max_q_len, self.prefixes = rows, max_q_len, prefixes
+        self.words = words  # the plan itself (device int32)
+        self.n_groups = prefixes.n_groups if prefixes is not None else 0
+        self.info = None    # host copy of its info once read_info has been called
+        # the arguments of a call that are the plan's
+        self._table = ptr(batch.page_table)
+        self._shared = ((ptr(prefixes.cu_pages), ptr(prefixes.page_ids)) if self.n_groups else
+                        (None, None))
+        self._words = (ptr(words), 4 * words.numel())
+        self._records = {}
 
-    @property
-    def n_groups(self) -> int:
-        return self.prefixes.n_groups if self.prefixes is not None else 0
+    def record_words(self, rope_dim: int, q8: bool) -> int:
+        """Bytes of an 8-bit page record, or 16-bit words of a 16-bit one."""
+        n = self._records.get((rope_dim, q8))
+        if n is None:
+            page = self.batch.page_size
+            n = (int(lib().mla_q8_page_bytes(page, self.kv_rank, rope_dim)) if q8 else
+                 page * (self.kv_rank + rope_dim))
+            self._records[rope_dim, q8] = n
+        return n
 
     def read_info(self, stream=None):
         """Synchronise and return [jobs, 0, jobs of 16 rows, jobs of 128 rows, partial rows, query
@@ -389,9 +416,12 @@ class AttentionPlan:
         more workgroups than the plan has jobs."""
         import numpy as np
         h = np.zeros(PLAN_INFO_INTS, np.int32)
-        check(lib().mla_read_plan_info(stream_handle(stream), ptr(self.words), h.ctypes.data))
+        check(lib().mla_read_plan_info(stream_handle(stream), self._words[0], h.ctypes.data))
         self.info = h
+        self._info = h.ctypes.data
         return h.tolist()
+
+    _info = None
 
 
 def plan_attention(batch: RaggedBatch, n_heads: int, kv_rank: int, *, rows: int | None = None,
@@ -400,28 +430,26 @@ def plan_attention(batch: RaggedBatch, n_heads: int, kv_rank: int, *, rows: int 
     """(e) Plan the attention of a batch (one launch): which workgroup takes which query rows over
     which keys.  ``rows``: query rows of the calls (default the batch's max_rows); ``max_q_len``:
     at least every session's q_len.  The plan serves every layer's ``latent_attention``."""
-    torch = _torch()
+    torch, gpu = _torch(), _gpu()
     rows = batch.max_rows if rows is None else rows
-    groups = 0
+    groups, shared = 0, (None, None, None, None)
     if prefixes is not None:
-        groups = prefixes.n_groups
-        _check("cu_groups", prefixes.cu_groups, (groups + 1,), torch.int32)
-        _check("prefix_len", prefixes.prefix_len, (groups,), torch.int32)
-        _check("cu_pages", prefixes.cu_pages, (groups + 1,), torch.int32)
-        _check("page_ids", prefixes.page_ids, (None,), torch.int32)
+        x = prefixes
+        groups = x.n_groups
+        shared = (_check("cu_groups", x.cu_groups, (groups + 1,), torch.int32, gpu),
+                  _check("prefix_len", x.prefix_len, (groups,), torch.int32, gpu),
+                  _check("cu_pages", x.cu_pages, (groups + 1,), torch.int32, gpu),
+                  _check_list("page_ids", x.page_ids, gpu))
     n = int(lib().mla_attention_plan_bytes(batch.B, rows, n_heads, kv_rank, max_q_len, groups))
     if n == 0:
         raise ValueError(f"plan_attention: no plan for B={batch.B}, rows={rows}, n_heads={n_heads}, "
                          f"kv_rank={kv_rank}, max_q_len={max_q_len}, groups={groups}")
+    info = _check_list("batch", batch.info, gpu)
     words = torch.empty(n // 4, dtype=torch.int32, device=batch.info.device)
-    _check("batch", batch.info, (None,), torch.int32)
-    x = prefixes
     check(lib().mla_plan_attention(
         stream_handle(stream), batch.B, rows, n_heads, kv_rank, batch.page_size, max_q_len,
-        ptr(batch.cu_seqlens_q), ptr(batch.cu_seqlens_k), ptr(batch.info), groups,
-        ptr(x.cu_groups) if x else None, ptr(x.prefix_len) if x else None,
-        ptr(x.cu_pages) if x else None, ptr(x.page_ids) if x else None,
-        int(x.page_ids.shape[0]) if x else 0, batch.num_pool_pages, ptr(words), n))
+        ptr(batch.cu_seqlens_q), ptr(batch.cu_seqlens_k), info, groups, *shared,
+        prefixes.page_ids.numel() if groups else 0, batch.num_pool_pages, ptr(words), n))
     return AttentionPlan(batch, n_heads, kv_rank, rows, max_q_len, prefixes, words)
 
 
@@ -442,31 +470,24 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
     q_latent [rows, H, kv_rank] and q_rope [rows, H, rope_dim] in ``dtype``; returns out
     [rows, H, kv_rank] in ``dtype`` (and fills lse [rows, H], fp32, if given).  Rows past the
     batch's are left as they were."""
-    torch = _torch()
-    b, rows, H, kv, x = plan.batch, plan.rows, plan.n_heads, plan.kv_rank, plan.prefixes
-    dt = _dtype_of(dtype)
+    torch, gpu = _torch(), _gpu()
+    b, rows, H, kv = plan.batch, plan.rows, plan.n_heads, plan.kv_rank
+    dt = torch.float16 if dtype == DTYPE_F16 else torch.bfloat16
     if out is None:
         out = torch.zeros((rows, H, kv), dtype=dt, device=q_latent.device)
     if workspace is None:
         workspace = attention_workspace(plan)
-    _check("q_latent", q_latent, (rows, H, kv), dt)
-    _check("q_rope", q_rope, (rows, H, rope_dim), dt)
-    _check("out", out, (rows, H, kv), dt)
-    _check("workspace", workspace, (None,), torch.uint8)
-    if lse is not None:
-        _check("lse", lse, (rows, H), torch.float32)
-    if q8:
-        rec = int(lib().mla_q8_page_bytes(b.page_size, kv, rope_dim))
-        _check("pages", pages, (b.num_pool_pages, rec), torch.uint8)
-    else:
-        _check("pages", pages, (b.num_pool_pages, b.page_size * (kv + rope_dim)), dt)
     check(lib().mla_latent_attention(
         stream_handle(stream), b.B, rows, H, kv, rope_dim, b.page_size, plan.max_q_len, dtype,
-        CACHE_Q8 if q8 else CACHE_16BIT, float(scale), ptr(b.page_table), b.max_pages,
-        b.num_pool_pages, ptr(pages), ptr(q_latent), ptr(q_rope), plan.n_groups,
-        ptr(x.cu_pages) if x else None, ptr(x.page_ids) if x else None, ptr(plan.words),
-        plan.words.numel() * 4, ptr(plan.info), ptr(out), ptr(lse), ptr(workspace),
-        workspace.numel()))
+        CACHE_Q8 if q8 else CACHE_16BIT, scale, plan._table, b.max_pages, b.num_pool_pages,
+        _check("pages", pages, (b.num_pool_pages, plan.record_words(rope_dim, q8)),
+               torch.uint8 if q8 else dt, gpu),
+        _check("q_latent", q_latent, (rows, H, kv), dt, gpu),
+        _check("q_rope", q_rope, (rows, H, rope_dim), dt, gpu),
+        plan.n_groups, *plan._shared, *plan._words, plan._info,
+        _check("out", out, (rows, H, kv), dt, gpu),
+        None if lse is None else _check("lse", lse, (rows, H), torch.float32, gpu),
+        _check("workspace", workspace, (workspace.numel(),), torch.uint8, gpu), workspace.numel()))
     return out
 
 

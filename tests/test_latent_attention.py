@@ -420,20 +420,19 @@ def test_bad_batches_and_prefixes_fail_the_plan_and_write_nothing(gpu):
 
 @pytest.mark.gpu
 def test_a_plan_for_other_sizes_writes_nothing(gpu):
-    import dataclasses
-    import torch
     c = make(8, 128, 16, 64, 0, False, [(10, 1), (20, 1)], seed=7)
     d = device(gpu, c)
     _say("plan of other sizes")
     plan = gpu.plan_attention(d["batch"], 8, 128, rows=2, max_q_len=2)
-    other = dataclasses.replace(plan, max_q_len=1)  # tables of the same size
+    replan = lambda q, words: gpu.AttentionPlan(d["batch"], 8, 128, 2, q, None, words)
+    other = replan(1, plan.words)  # tables of the same size
     _, out, lse = call(gpu, c, d, other, workspace=gpu.attention_workspace(plan))
     assert (out == 5).all() and (lse == 5).all()
     plan.read_info()
     with pytest.raises(gpu.MlaError, match="host_info"):
-        call(gpu, c, d, dataclasses.replace(other, info=plan.info),
-             workspace=gpu.attention_workspace(plan))
-    small = dataclasses.replace(plan, words=plan.words[:64])
+        other._info = plan._info
+        call(gpu, c, d, other, workspace=gpu.attention_workspace(plan))
+    small = replan(2, plan.words[:64])
     with pytest.raises(gpu.MlaError, match="other sizes"):
         call(gpu, c, d, small, workspace=gpu.attention_workspace(plan))
 
@@ -487,7 +486,7 @@ def test_refusals_of_planned_attention():
     assert st == 1
 
 
-def test_python_wrappers_refuse_wrong_tensors():
+def test_python_wrappers_refuse_wrong_tensors(monkeypatch):
     import torch
     import cpp_inference_train_engine_amd as mla
     i = torch.zeros(8, dtype=torch.int32)
@@ -496,6 +495,7 @@ def test_python_wrappers_refuse_wrong_tensors():
                                            "slot_mapping", "num_splits", "cu_splits",
                                            "work_session", "work_split", "work_desc",
                                            "work_pages", "info")})
+    monkeypatch.setattr(mla.ops, "_gpu", lambda: 0)
     with pytest.raises(ValueError, match="no plan"):
         mla.plan_attention(rb, 0, 128)
     with pytest.raises(ValueError, match="GPU"):
@@ -504,10 +504,20 @@ def test_python_wrappers_refuse_wrong_tensors():
         mla.plan_attention(rb, 8, 128, prefixes=mla.SharedPrefixes(i, i[:1], i[:2], i))
     plan = mla.AttentionPlan(rb, 8, 128, 2, 1, None, i)
     q = torch.zeros((2, 8, 128), dtype=torch.float16)
+    monkeypatch.setattr(mla.ops, "stream_handle", lambda stream=None: None)
+    for pages in (q, torch.zeros((2, 9216)), torch.zeros((2, 9216), dtype=torch.float16)):
+        with pytest.raises(ValueError, match="pages"):
+            mla.latent_attention(plan, pages, q, q[:, :, :16], 0.1, rope_dim=16,
+                                 out=q, workspace=i.view(torch.uint8))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    pages = torch.zeros((2, 9216), dtype=torch.float16)
     for ql in (q[:1], q.bfloat16(), q.transpose(0, 1)):
         with pytest.raises(ValueError, match="q_latent"):
-            mla.latent_attention(plan, q, ql, q[:, :, :16], 0.1, rope_dim=16,
+            mla.latent_attention(plan, pages, ql, q[:, :, :16], 0.1, rope_dim=16,
                                  out=q, workspace=i.view(torch.uint8))
+    with pytest.raises(ValueError, match="q_rope"):
+        mla.latent_attention(plan, pages, q, q[:, :, :16], 0.1, rope_dim=16,  # not contiguous
+                             out=q, workspace=i.view(torch.uint8))
 
 
 @pytest.mark.gpu

@@ -92,9 +92,10 @@ def test_refusals_of_the_8_bit_cache():
     assert read(ckv=a + 2) == 1 and read(krope=a + 8) == 1
 
 
-def test_python_wrappers_refuse_wrong_tensors():
+def test_python_wrappers_refuse_wrong_tensors(monkeypatch):
     import torch
     import cpp_inference_train_engine_amd as mla
+    monkeypatch.setattr(mla.ops, "_gpu", lambda: 0)
     with pytest.raises(ValueError, match="multiple of 16"):
         mla.QuantizedLatentCache(1, 2, 60, 128, 16, device="cpu")
     with pytest.raises(ValueError, match="storage"):
