@@ -5,6 +5,7 @@
 // (mla_latent.hpp) has row blocks and 32-key tiles; the keys of all segments of a list are cut into
 // ranges of one length.  A GPU that holds `slots` workgroups of the list at once takes
 //     ceil(jobs / slots) * (length * time of a tile + time of a job's start and end)
+//     + the time of writing and reading the jobs' partial rows, where there are any
 // so what counts is that the jobs fill one round or two and not a little more: the length is
 // the best of candidates between 1 and 2 times total / (rounds * slots).  Whether segments of many
 // rows go to list R or are taken apart for list K is decided by the same estimate: list K costs
@@ -159,22 +160,25 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         const int slots = list == 1 ? p.slots_r : p.slots_k;
         const long long share = sums[list] / (slots * (1 + c / kSteps)) + 1;
         long long n = share + share * (c % kSteps) / kSteps;
-        if (list != 1)
-            n = (n + 3) & ~3LL;  // a tile for each of the four waves
+        n = list == 1 ? (n + 1) & ~1LL : (n + 3) & ~3LL;  // a tile for each of the four waves
         return (int)std::min<long long>(n, 1 << 26);
     };
     for (int e = wave; e < 3 * kTries; e += kWaves) {
         const int list = e / kTries, c = e % kTries, n = tried(list, c);
         if (sums[list] == 0)
             continue;
-        long long jobs = 0;
+        long long jobs = 0, parts = 0;
         int longest = 0;
         for (int i = lane; i < S; i += 64)
             if (const int b = blocks_of(list, i)) {
-                jobs += (long long)b * ceil_div(tiles(i), n);
+                const int splits = ceil_div(tiles(i), n);
+                jobs += (long long)b * splits;
+                if (splits > 1 || i < G || group[i] >= 0)
+                    parts += (long long)b * splits;
                 longest = std::max(longest, std::min(n, tiles(i)));
             }
         jobs = wave_total(jobs);
+        parts = wave_total(parts);
         for (int d = 32; d > 0; d >>= 1)
             longest = std::max(longest, __shfl_xor(longest, d, 64));
         if (lane == 0) {
@@ -182,7 +186,9 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             const long long rounds = (jobs + slots - 1) / slots;
             const long long each = list == 1 ? (long long)longest * cost.tile_r + cost.job_r
                                              : (longest + 3LL) / 4 * cost.tile_k + cost.job_k;
-            const unsigned long long ns = std::min<long long>(rounds * each, 0xffffffffLL);
+            // fp32 rows written and read back, at about 4 TB/s
+            const long long rows = parts * (list == 1 ? kRowsR : kRowsK) * p.kv_rank * 8 / 4000;
+            const unsigned long long ns = std::min<long long>(rounds * each + rows, 0xffffffffLL);
             atomicMin(&best[list], ns << 32 | (unsigned)c);
         }
     }
@@ -207,8 +213,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             blocks = ceil_div(n, f ? kRowsK : kRowsR);
             splits = ceil_div(tiles(i), f ? len_k : len_r);
             range = ceil_div(tiles(i), splits);  // the segment's ranges as even as they go
-            if (f)
-                range = (range + 3) & ~3;
+            range = f ? (range + 3) & ~3 : (range + 1) & ~1;  // (list R stages two units at once)
             splits = ceil_div(tiles(i), range);
         }
         const bool joined = n > 0 && (splits > 1 || i < G || group[i] >= 0);

@@ -21,14 +21,15 @@
 //                       step of that type each, and is itself rounded to it in the end
 // A key past a row's position adds nothing to the row, whatever it holds: its rope key only enters
 // the score, which is replaced, and a non-finite latent is staged as zero with the key marked, and
-// makes the scores of the rows that see it NaN.  (Without causal rows every row of a job sees all
-// of its keys, and such a latent spreads to them by itself.)
+// makes the scores of the rows that see it NaN.  (Where every row of a job sees the key, such a
+// latent spreads to them by itself, and is not looked for.)
 #pragma once
 
 #include "mla_latent.hpp"
 #include "mla_q8.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace mla {
 namespace {
@@ -99,13 +100,16 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     constexpr bool ONE = RP_ >= 0;
     constexpr int RSM = ONE ? (RP_ + 31) / 32 : 2;      // rope k-steps (rope_dim <= 64)
     constexpr int RTM = 2 * KSM;                        // 16-row tiles of O^T
+    // 32-key units that are fetched and staged together: two on list R where LDS has room, which
+    // halves the barriers and what else a unit costs besides its products
+    constexpr int SUB = ROWS && KSM <= 8 ? 2 : 1;
+    constexpr int NT = 2 * SUB, KEYS = 32 * SUB;
     constexpr int SLOT = 32 * 32 * (KSM + RSM);         // words of a unit
     constexpr int UPT = Q8 ? (KSM + 1) / 2 : KSM;       // 16-byte loads of a lane per tile
-    constexpr int NL = ROWS ? (2 * UPT + NW - 1) / NW : 2 * UPT;
+    constexpr int NL = ROWS ? (NT * UPT + NW - 1) / NW : NT * UPT;
     constexpr int RCS = ONE ? RP_ / 8 : 8;              // rope chunks of a tile, at most
-    constexpr int NR = ROWS ? 1 : (2 * RCS + 3) / 4;    // rope loads of a lane per unit
-    constexpr int SLOTS = ROWS ? 2 : 4;
-    constexpr int DEPTH = ROWS && ONE && KSM == 4 ? 2 : 1;  // units in flight behind the one at work
+    constexpr int NR = ROWS ? (NT * RCS + 4 * NW - 1) / (4 * NW) : (NT * RCS + 3) / 4;
+    constexpr int SLOTS = ROWS ? 2 * SUB : 4;
     // Q^T k-steps that stay in LDS, lane by lane, where the registers would spill (a reload waits
     // for every load in flight): at kv 512 O^T takes 128 of a wave's 256 registers, Q^T 72.
     constexpr int AHEAD = ONE && KSM >= 16 ? 2 : 1;  // steps that LDS reads run ahead of their use
@@ -113,7 +117,7 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     using V8 = typename T::vec8;
     __shared__ __attribute__((aligned(16))) uint16_t smem[SLOTS][SLOT];
     __shared__ __attribute__((aligned(16))) uint16_t q_lds[QL > 0 ? NW * QL * 512 : 8];
-    __shared__ uint32_t marks[3];  // list R: keys of a unit with a non-finite latent
+    __shared__ uint32_t marks[3 * SUB];  // list R: keys of a unit with a non-finite latent
 
     const table_ptr plan = table(a.plan);
     const table_ptr d = plan + (ROWS ? a.p.jobs_r_at : a.p.jobs_k_at) + (long long)blockIdx.x * kJobInts;
@@ -132,7 +136,7 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     const long long rec = Q8 ? q8_page_bytes(PS, KV, RP) : 2LL * PS * (KV + RP);
     const table_ptr ptab = table(seg >= 0 ? a.page_table + (long long)seg * a.max_pages
                                           : a.prefix_page_ids + table(a.cu_prefix_pages)[~seg]);
-    const int n_units = key_end > key0 && a.num_pool_pages > 0 ? (key_end - key0 + 31) >> 5 : 0;
+    const int n_units = key_end > key0 && a.num_pool_pages > 0 ? (key_end - key0 + KEYS - 1) / KEYS : 0;
     const int row0 = ROWS ? 16 * wave : 0;  // the wave's first row of the block
 
     // ---- Q^T operands: row n, latent columns 32j + 8g .., then the rope key's; the rows' limits ----
@@ -140,6 +144,9 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     uint16_t* const my_q = q_lds + wave * QL * 512 + lane * 8;
     const bool causal_seg = a.causal && seg >= 0;
     int lim, lim_wave = -1, lim_all = key_end - 1;  // lane's row n sees keys [0, lim] of the segment
+    // The last key that every row of the block sees: from there on a non-finite latent has to be
+    // kept from the rows before it.
+    const int seen_by_all = causal_seg ? ctx + rb / H : 0x7fffffff;
     {
         const int r = min(row0 + n, n_rows - 1);  // rows past the block repeat its last
         const long long fr = (long long)f0 + r;
@@ -180,102 +187,162 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     struct Loaded {
         u32x4 st[NL], sr[NR];
         uint32_t sk[Q8 ? NL : 1];  // scale bytes of a load's one or two k-steps
-        int pg0, pg1;              // pages of the unit's tiles, -1 outside the pool
+        uint32_t has;              // tiles whose page lies in the pool
     };
     const int upt = Q8 ? (ks + 1) >> 1 : ks;
+    const int lat_tile = (Q8 ? 16 : 32) * KV, key_tile = 32 * RP, sc_tile = 16 * ks;  // bytes
+    const long long key_at = (long long)PS * (Q8 ? 1 : 2) * KV, sc_at = (long long)PS * (KV + 2 * RP);
+    // This lane's rope chunks: tile, and bytes from the first tile's keys (-1: none).
     const int rcs = RP >> 3;
-    int rope_tt[NR], rope_ch[NR];
+    int rope_tt[NR], rope_in[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        const int c = ROWS ? tid >> 4 : 4 * i + g;  // (list R: 16 chunks, all of a unit's)
-        rope_tt[i] = c >= rcs;
-        rope_ch[i] = c < 2 * rcs ? (c >= rcs ? c - rcs : c) : -1;
+        const int c = ROWS ? (tid >> 4) + 4 * NW * i : 4 * i + g;
+        const int tt = ONE ? c / (RCS > 0 ? RCS : 1) : (rcs > 0 ? c / rcs : 0);
+        rope_tt[i] = tt;
+        rope_in[i] = tt < NT && rcs > 0 ? tt * key_tile + (c - tt * rcs) * 256 + n * 16 : -1;
     }
-    // A tile's page and its place there (page sizes are mostly powers of two).
-    const int tpp_shift = (tpp & (tpp - 1)) == 0 ? __builtin_ctz(tpp) : -1;
-    auto page_of = [&](int t) { return tpp_shift >= 0 ? t >> tpp_shift : t / tpp; };
-    auto place_of = [&](int t) { return tpp_shift >= 0 ? t & (tpp - 1) : t % tpp; };
-    // Tile t's page id, some id past the keys; valid_page: -1 when it lies outside the pool.
-    auto tile_page = [&](int t) {
-        return ptab[page_of(min(t, (key_end - 1) >> 4))];
+    // A tile's page (number in the list) and place there: t / tpp by a product, one too small at most.
+    auto page_of = [&](int t, int& in) {
+        int q = (int)(((unsigned long long)(unsigned)t * a.tpp_inverse) >> 32), r = t - q * tpp;
+        if (r >= tpp) {
+            ++q;
+            r -= tpp;
+        }
+        in = r;
+        return q;
     };
-    auto valid_page = [&](int id) { return (unsigned)id < (unsigned)a.num_pool_pages ? id : -1; };
-    // The unit's keys that exist: before key_end, on a page of the pool.
-    auto keys_of = [&](int t0, int pg0, int pg1) {
-        const int valid = min(32, key_end - 16 * t0);
-        uint32_t ok = valid >= 32 ? 0xffffffffu : (1u << valid) - 1u;
-        if (pg0 < 0)
-            ok &= 0xffff0000u;
-        if (pg1 < 0)
-            ok &= 0x0000ffffu;
-        return ok;
+    const int last_tile = (key_end - 1) >> 4;
+    const bool one_page = ONE && PS % KEYS == 0;  // a unit lies on one page
+    // Page ids and first place of the unit at tile t (past the keys: the last page's).
+    struct Pages {
+        int id[NT], in[NT];
     };
-    // (A missing tile loads page 0's, and is dropped when it is staged.)
-    auto load_unit = [&](Loaded& x, int t0, int id0, int id1) {
-        const int pg0 = x.pg0 = valid_page(id0), pg1 = x.pg1 = valid_page(id1);
-        const uint8_t* base0 = a.pages + max(pg0, 0) * rec;
-        const uint8_t* base1 = a.pages + max(pg1, 0) * rec;
-        const int in0 = place_of(t0), in1 = place_of(t0 + 1);
+    auto find_pages = [&](int t) {
+        Pages p;
+        if (one_page) {
+            p.id[0] = ptab[page_of(min(t, last_tile), p.in[0])];
+        } else {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int u = ROWS ? wave + NW * i : i;
-            const int tt = u / UPT, k = u % UPT;
-            if (u >= 2 * UPT || k >= upt)
-                continue;
-            const uint8_t* base = tt ? base1 : base0;
-            const int in = tt ? in1 : in0;
+            for (int k = 0; k < NT; ++k)
+                p.id[k] = ptab[page_of(min(t + k, last_tile), p.in[k])];
+        }
+        return p;
+    };
+    auto load_unit = [&](Loaded& x, const Pages& p) {
+        x.has = 0;
+        auto fetch = [&](int i, int k, const uint8_t* base, int in) {  // a lane's 16 bytes of a tile
             if constexpr (Q8) {
-                const uint8_t* lat = base + in * 16 * KV + k * 1024;
-                const uint8_t* sc = base + (long long)PS * (KV + 2 * RP) + (in * 16 + n) * ks + 2 * k;
+                const uint8_t* lat = base + in * lat_tile + k * 1024;
+                const uint8_t* sc = base + sc_at + in * sc_tile + 2 * k;
                 if (2 * k + 1 < ks) {
                     x.st[i] = *reinterpret_cast<const u32x4*>(lat + lane * 16);
-                    x.sk[i] = ks & 1 ? sc[0] | sc[1] << 8 : *reinterpret_cast<const uint16_t*>(sc);
+                    x.sk[i] = ks & 1 ? sc[n * ks] | sc[n * ks + 1] << 8
+                                     : *reinterpret_cast<const uint16_t*>(sc + n * ks);
                 } else {
                     const u32x2 w = *reinterpret_cast<const u32x2*>(lat + lane * 8);
                     x.st[i] = u32x4{w[0], w[1], 0, 0};
-                    x.sk[i] = sc[0];
+                    x.sk[i] = sc[n * ks];
                 }
             } else {
-                x.st[i] = *reinterpret_cast<const u32x4*>(base + in * 32 * KV + k * 1024 + lane * 16);
+                x.st[i] = *reinterpret_cast<const u32x4*>(base + in * lat_tile + k * 1024 + lane * 16);
+            }
+        };
+        if (one_page) {
+            // (an id outside the pool loads page 0, and the unit is dropped when it is staged)
+            const bool ok = (unsigned)p.id[0] < (unsigned)a.num_pool_pages;
+            const uint8_t* base = a.pages + (ok ? p.id[0] : 0) * rec;
+            x.has = ok ? (1u << NT) - 1 : 0;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int u = ROWS ? wave + NW * i : i, tt = u / UPT, k = u % UPT;
+                if (u < NT * UPT && k < upt)
+                    fetch(i, k, base, p.in[0] + tt);
+            }
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (rope_in[i] >= 0)
+                    x.sr[i] = *reinterpret_cast<const u32x4*>(base + key_at + p.in[0] * key_tile +
+                                                              rope_in[i]);
+        } else {
+            const uint8_t* bases[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const bool ok = (unsigned)p.id[t] < (unsigned)a.num_pool_pages;
+                bases[t] = a.pages + (ok ? p.id[t] : 0) * rec;
+                x.has |= ok ? 1u << t : 0;
+            }
+            auto base_of = [&](int tt, int& in) {
+                const uint8_t* base = bases[0];
+                in = p.in[0];
+#pragma unroll
+                for (int t = 1; t < NT; ++t) {
+                    base = tt == t ? bases[t] : base;
+                    in = tt == t ? p.in[t] : in;
+                }
+                return base;
+            };
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int u = ROWS ? wave + NW * i : i, tt = u / UPT, k = u % UPT;
+                int in;
+                const uint8_t* base = base_of(tt, in);
+                if (u < NT * UPT && k < upt)
+                    fetch(i, k, base, in);
+            }
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                int in;
+                const uint8_t* base = base_of(rope_tt[i], in);
+                if (rope_in[i] >= 0)
+                    x.sr[i] = *reinterpret_cast<const u32x4*>(
+                        base + key_at + (in - rope_tt[i]) * key_tile + rope_in[i]);
             }
         }
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-            if (rope_ch[i] >= 0)
-                x.sr[i] = *reinterpret_cast<const u32x4*>(
-                    (rope_tt[i] ? base1 : base0) + (long long)PS * KV * (Q8 ? 1 : 2) +
-                    ((rope_tt[i] ? in1 : in0) * rcs + rope_ch[i]) * 256 + n * 16);
     };
-    // Writes the loaded unit to `sp`; keys outside `ok` become 0 (their slots, scales included, may
-    // hold anything).  Returns the wave's marked keys.
-    auto stage_unit = [&](const Loaded& x, uint16_t* sp, uint32_t ok) {
-        uint32_t mark = 0;
-        int causal = a.causal;
-        asm("" : "+s"(causal));  // looked at anew each time: one copy of the loop, not two
+    // The keys of 32-key part `sub` of a unit that exist: before key_end, on a page of the pool.
+    auto keys_of = [&](int t0, int sub, uint32_t has) {
+        const int valid = key_end - 16 * t0 - 32 * sub;
+        uint32_t ok = valid >= 32 ? 0xffffffffu : valid <= 0 ? 0u : (1u << valid) - 1u;
+        if (!(has >> (2 * sub) & 1))
+            ok &= 0xffff0000u;
+        if (!(has >> (2 * sub) & 2))
+            ok &= 0x0000ffffu;
+        return ok;
+    };
+    // Writes the loaded unit to `sp` and behind.  PLAIN: all of its keys exist and it needs no look
+    // for non-finite latents; else keys outside `ok` become 0 (their slots, scales included, may
+    // hold anything), and the keys that the wave found to have such a latent are left in `mark`.
+    auto stage_unit = [&]<bool PLAIN>(std::bool_constant<PLAIN>, const Loaded& x, uint16_t* sp,
+                                      const uint32_t (&ok)[SUB], uint32_t (&mark)[SUB], bool look) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int u = ROWS ? wave + NW * i : i;
-            const int tt = u / UPT, k = u % UPT;
-            if (u >= 2 * UPT || k >= upt)
+            const int u = ROWS ? wave + NW * i : i, tt = u / UPT, k = u % UPT;
+            if (u >= NT * UPT || k >= upt)
                 continue;
             u32x4 v = x.st[i];
             uint32_t k8 = Q8 ? x.sk[i] : 0;
-            if (ok != 0xffffffffu) {
-                const uint32_t keep = -(ok >> (16 * tt + n) & 1);
+            if constexpr (!PLAIN) {
+                const uint32_t of = SUB == 1 || tt < 2 ? ok[0] : ok[SUB - 1];
+                const uint32_t keep = -(of >> (16 * (tt & 1) + n) & 1);
                 v &= keep;
                 k8 &= keep;
+                if (look) {
+                    bool bad;
+                    if constexpr (Q8)
+                        bad = drop_nan8(v);
+                    else
+                        bad = drop_nonfinite16<T>(v);
+                    const uint64_t b = __builtin_amdgcn_ballot_w64(bad);
+                    const uint32_t m = (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff)
+                                       << (16 * (tt & 1));
+                    if (SUB == 1 || tt < 2)
+                        mark[0] |= m;
+                    else
+                        mark[SUB - 1] |= m;
+                }
             }
-            if (causal) {
-                bool bad;
-                if constexpr (Q8)
-                    bad = drop_nan8(v);
-                else
-                    bad = drop_nonfinite16<T>(v);
-                const uint64_t b = __builtin_amdgcn_ballot_w64(bad);
-                if (b)
-                    mark |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff) << (16 * tt);
-            }
-            uint16_t* dst = sp + tt * 16 * KV + s_lane;
+            uint16_t* dst = sp + (tt >> 1) * SLOT + (tt & 1) * 16 * KV + s_lane;
             if constexpr (Q8) {
                 *reinterpret_cast<u32x4*>(dst + 2 * k * 512) =
                     q8_decode8<T>(v[0], v[1], q8_scale(k8 & 0xff));
@@ -288,14 +355,17 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         }
 #pragma unroll
         for (int i = 0; i < NR; ++i)
-            if (rope_ch[i] >= 0) {
+            if (rope_in[i] >= 0) {
+                const int tt = rope_tt[i];
                 u32x4 v = x.sr[i];
-                if (ok != 0xffffffffu)
-                    v &= -(ok >> (16 * rope_tt[i] + n) & 1);
-                *reinterpret_cast<u32x4*>(sp + 32 * KV + rope_tt[i] * 16 * RP + rope_ch[i] * 128 +
-                                          n * 8) = v;
+                if constexpr (!PLAIN) {
+                    const uint32_t of = SUB == 1 || tt < 2 ? ok[0] : ok[SUB - 1];
+                    v &= -(of >> (16 * (tt & 1) + n) & 1);
+                }
+                // (a tile's key rows take as many bytes here as in the record)
+                *reinterpret_cast<u32x4*>(sp + (tt >> 1) * SLOT + 32 * KV +
+                                          (rope_in[i] - (tt >> 1) * 2 * key_tile) / 2) = v;
             }
-        return mark;
     };
 
     const int tr_par = (n & 3) >> 1;
@@ -372,8 +442,37 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                 cring[k][1] = c_operand(2 * k + 1);
             }
 
+        float mp = -INFINITY;  // of the lane's eight scores (NaN is passed over)
+        auto take_max = [&]() {
+            mp = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    mp = fmaxf(mp, sc[tt][i]);
+        };
+        take_max();
+        if constexpr (!Q8) {
+            // An infinite latent that every row sees has not been looked for, and a score of -inf
+            // would give it the weight 0: such keys are marked now.  (NaN scores need no mark.)
+            float mn = INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    mn = fminf(mn, sc[tt][i]);
+            if (__builtin_amdgcn_ballot_w64(mp == INFINITY || mn == -INFINITY)) {
+#pragma unroll 1
+                for (int j = 0; j < 2 * ks; ++j) {
+                    const int tt = j >= ks;
+                    u32x4 v = *reinterpret_cast<const u32x4*>(sp + j * 512 + s_lane);
+                    const uint64_t b = __builtin_amdgcn_ballot_w64(drop_nonfinite16<T>(v));
+                    mark |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff) << (16 * tt);
+                }
+            }
+        }
         // Units that some row does not see in full: their scores are replaced.
-        if (ok != 0xffffffffu || mark != 0 || 16 * t0 + 31 > lim_all)
+        if (ok != 0xffffffffu || mark != 0 || 16 * t0 + 31 > lim_all) {
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -384,12 +483,8 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                     if (!(ok >> key & 1) || 16 * t0 + key > lim)
                         sc[tt][i] = -INFINITY;
                 }
-        float mp = -INFINITY;  // of the lane's eight scores (NaN is passed over)
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                mp = fmaxf(mp, sc[tt][i]);
+            take_max();
+        }
         mp *= a.scale_log2;
         if (__builtin_amdgcn_ballot_w64(mp > m_run + kRise)) {
             const float m_new = fmaxf(m_run, rows_max(mp) - kHead);
@@ -428,62 +523,64 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
             }
     };
 
-    // ---- the units: loaded DEPTH ahead, page ids one further ----
+    // ---- the units: loaded one ahead, page ids two ahead ----
     constexpr int STEP = ROWS ? 1 : 4;
     const int first = ROWS ? 0 : wave, tile0 = key0 >> 4;
     if constexpr (ROWS) {
-        if (tid < 3)
+        if (tid < 3 * SUB)
             marks[tid] = 0;
         __syncthreads();
     }
-    Loaded x[DEPTH];
-    int id0 = -1, id1 = -1;  // pages of the next unit to load
-    auto next_ids = [&](int u) {
-        id0 = tile_page(tile0 + 2 * u);
-        id1 = tile_page(tile0 + 2 * u + 1);
-    };
+    Loaded x;
+    Pages pages{};
     if (first < n_units) {
-        next_ids(first);
-#pragma unroll
-        for (int k = 0; k < DEPTH; ++k)
-            if (first + k * STEP < n_units) {
-                const int a0 = id0, a1 = id1;
-                next_ids(first + (k + 1) * STEP);
-                load_unit(x[k], tile0 + 2 * (first + k * STEP), a0, a1);
-            }
+        pages = find_pages(tile0 + NT * first);
+        load_unit(x, pages);
+        pages = find_pages(tile0 + NT * (first + STEP));
     }
-    for (int u0 = first; u0 < n_units; u0 += DEPTH * STEP) {
+    for (int u = first; u < n_units; u += STEP) {
+        const int t0 = tile0 + NT * u;
+        uint16_t* sp = smem[ROWS ? (u & 1) * SUB : wave];
+        const bool look = 16 * t0 + KEYS - 1 > seen_by_all;
+        uint32_t ok[SUB], mark[SUB] = {};
 #pragma unroll
-        for (int k = 0; k < DEPTH; ++k) {
-            const int u = u0 + k * STEP;
-            if (u >= n_units)
-                break;
-            const int t0 = tile0 + 2 * u;
-            uint16_t* sp = smem[ROWS ? u & 1 : wave];
-            const uint32_t ok = keys_of(t0, x[k].pg0, x[k].pg1);
-            uint32_t mark = stage_unit(x[k], sp, ok);
-            if (ROWS && mark && lane == 0)
-                atomicOr(&marks[u % 3], mark);
-            if (u + DEPTH * STEP < n_units) {
-                load_unit(x[k], t0 + 2 * DEPTH * STEP, id0, id1);
-                next_ids(u + (DEPTH + 1) * STEP);
-            }
-            if constexpr (ROWS) {
-                // The other buffer is free: every wave that passed the barrier before this one has
-                // finished with it.  Likewise marks: unit u + 2's word, last read in unit u - 1, is
-                // cleared behind this barrier and set again behind the next.
-                __syncthreads();
-                mark = __builtin_amdgcn_readfirstlane(marks[u % 3]);
-                if (tid == 0)
-                    marks[(u + 2) % 3] = 0;
-            } else {
-                wave_lds_fence();
-            }
-            if (16 * t0 <= lim_wave)
-                compute_unit(sp, t0, ok, mark);
-            if constexpr (!ROWS)
-                wave_lds_fence();  // the slot's reads are done before the next unit's writes
+        for (int k = 0; k < SUB; ++k)
+            ok[k] = keys_of(t0, k, x.has);
+        if ((ok[0] & ok[SUB - 1]) == 0xffffffffu && !look) {
+            stage_unit(std::true_type{}, x, sp, ok, mark, false);
+        } else {
+            stage_unit(std::false_type{}, x, sp, ok, mark, look);
+            if (ROWS && lane == 0)
+#pragma unroll
+                for (int k = 0; k < SUB; ++k)
+                    if (mark[k])
+                        atomicOr(&marks[u % 3 * SUB + k], mark[k]);
         }
+        if (u + STEP < n_units) {
+            load_unit(x, pages);
+            pages = find_pages(t0 + 2 * NT * STEP);
+        }
+        if constexpr (ROWS) {
+            // The other buffer is free: every wave that passed the barrier before this one has
+            // finished with it.  Likewise marks: unit u + 2's words, last read in unit u - 1, are
+            // cleared behind this barrier and set again behind the next.
+            __syncthreads();
+            if (look) {
+#pragma unroll
+                for (int k = 0; k < SUB; ++k)
+                    mark[k] = __builtin_amdgcn_readfirstlane(marks[u % 3 * SUB + k]);
+            }
+            if (causal_seg && tid < SUB)
+                marks[(u + 2) % 3 * SUB + tid] = 0;
+        } else {
+            wave_lds_fence();
+        }
+#pragma unroll
+        for (int k = 0; k < SUB; ++k)
+            if (16 * t0 + 32 * k <= lim_wave)
+                compute_unit(sp + k * SLOT, t0 + 2 * k, ok[k], mark[k]);
+        if constexpr (!ROWS)
+            wave_lds_fence();  // the slot's reads are done before the next unit's writes
     }
 
     // ---- final rows, or partials ----

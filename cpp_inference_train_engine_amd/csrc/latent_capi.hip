@@ -5,6 +5,7 @@
 #include "mla_latent.hpp"
 #include "mla_q8.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <string>
@@ -219,6 +220,7 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
         return invalid(fn, "the plan was made for other sizes");
     a.jobs_k = a.p.max_jobs_k;
     a.jobs_r = a.p.max_jobs_r;
+    a.merge = true;
     if (host_info) {
         if (host_info[kPlanTag] != (int)a.p.tag || host_info[kPlanJobsK] < 0 ||
             host_info[kPlanJobsK] > a.jobs_k || host_info[kPlanJobsR] < 0 ||
@@ -226,6 +228,7 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
             return invalid(fn, "host_info is not that of a plan for these sizes");
         a.jobs_k = host_info[kPlanJobsK];
         a.jobs_r = host_info[kPlanJobsR];
+        a.merge = host_info[kPlanParts] > 0;
     }
     if (workspace_bytes < workspace_size(a.p))
         return invalid(fn, "workspace needs " + std::to_string(workspace_size(a.p)) + " bytes");
@@ -235,6 +238,7 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
     a.page_size = page_size;
     a.max_pages = max_pages;
     a.num_pool_pages = num_pool_pages;
+    a.tpp_inverse = (uint32_t)std::min<uint64_t>((1ULL << 32) / (page_size / 16), 0xffffffffULL);
     a.causal = max_q_len > 1;
     a.q8 = cache_format == MLA_CACHE_Q8;
     a.scale_log2 = scale * 1.4426950408889634f;

@@ -143,7 +143,7 @@ hipError_t launch_latent_attention(const LatentArgs& a, int dtype, hipStream_t s
         if (e != hipSuccess)
             return e;
     }
-    return launch_latent_merge(a, dtype, stream);
+    return a.merge ? launch_latent_merge(a, dtype, stream) : hipSuccess;
 }
 
 hipError_t launch_latent_merge(const LatentArgs& a, int dtype, hipStream_t stream) {

@@ -272,6 +272,8 @@ def test_nonfinite_latents_reach_only_the_rows_that_see_them(gpu, H, kv, rope, p
         want = expect(c)
         spoil(c.flat(c.own_pages[1], 240)[[220, 236]], 0x7C00)
         spoil(c.flat(c.own_pages[2], 9)[[4]], 0xFC00)
+        spoil(c.flat(c.own_pages[3], 71)[[30]], 0xFC00)
+        spoil(c.flat(c.own_pages[5], 1), 0x7C00)
         d = device(gpu, c)
         _, out, lse = call(gpu, c, d)
         check(c, out, lse, want)
