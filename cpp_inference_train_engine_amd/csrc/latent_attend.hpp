@@ -187,20 +187,20 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     struct Loaded {
         u32x4 st[NL], sr[NR];
         uint32_t sk[Q8 ? NL : 1];  // scale bytes of a load's one or two k-steps
-        uint32_t has;              // tiles whose page lies in the pool
     };
     const int upt = Q8 ? (ks + 1) >> 1 : ks;
     const int lat_tile = (Q8 ? 16 : 32) * KV, key_tile = 32 * RP, sc_tile = 16 * ks;  // bytes
     const long long key_at = (long long)PS * (Q8 ? 1 : 2) * KV, sc_at = (long long)PS * (KV + 2 * RP);
-    // This lane's rope chunks: tile, and bytes from the first tile's keys (-1: none).
+    // This lane's rope chunks: tile, and bytes from the unit's first keys (-1: none).
     const int rcs = RP >> 3;
     int rope_tt[NR], rope_in[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
         const int c = ROWS ? (tid >> 4) + 4 * NW * i : 4 * i + g;
         const int tt = ONE ? c / (RCS > 0 ? RCS : 1) : (rcs > 0 ? c / rcs : 0);
-        rope_tt[i] = tt;
-        rope_in[i] = tt < NT && rcs > 0 ? tt * key_tile + (c - tt * rcs) * 256 + n * 16 : -1;
+        const bool some = tt < NT && rcs > 0;
+        rope_tt[i] = some ? tt : 0;
+        rope_in[i] = some ? tt * key_tile + (c - tt * rcs) * 256 + n * 16 : -1;
     }
     // A tile's page (number in the list) and place there: t / tpp by a product, one too small at most.
     auto page_of = [&](int t, int& in) {
@@ -213,15 +213,22 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         return q;
     };
     const int last_tile = (key_end - 1) >> 4;
-    const bool one_page = ONE && PS % KEYS == 0;  // a unit lies on one page
-    // Page ids and first place of the unit at tile t (past the keys: the last page's).
+    const bool one_page = PS % KEYS == 0;  // a unit lies on one page
+    // Page ids of the unit at tile t, and the places of its tiles there.  Tiles past the keys take
+    // the last one's: they are read, so that no load hangs on a branch (the compiler would load
+    // into other registers, and wait to move), and dropped when they are staged.
     struct Pages {
         int id[NT], in[NT];
     };
     auto find_pages = [&](int t) {
         Pages p;
         if (one_page) {
-            p.id[0] = ptab[page_of(min(t, last_tile), p.in[0])];
+            const int id = ptab[page_of(min(t, last_tile), p.in[0])];
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                p.id[k] = id;
+                p.in[k] = p.in[0] + (t + k <= last_tile ? k : 0);
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < NT; ++k)
@@ -229,86 +236,68 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         }
         return p;
     };
+    // (Ids were checked by the builds of the metadata and the plan; the bound is for memory's sake.)
+    auto page_base = [&](int id) {
+        return a.pages + (long long)min((unsigned)id, (unsigned)a.num_pool_pages - 1) * rec;
+    };
     auto load_unit = [&](Loaded& x, const Pages& p) {
-        x.has = 0;
-        auto fetch = [&](int i, int k, const uint8_t* base, int in) {  // a lane's 16 bytes of a tile
+        const uint8_t* base[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            base[t] = one_page && t > 0 ? base[0] : page_base(p.id[t]);
+        auto base_of = [&](int tt, int& in) {
+            const uint8_t* b = base[0];
+            in = p.in[0];
+#pragma unroll
+            for (int t = 1; t < NT; ++t) {
+                b = tt == t ? base[t] : b;
+                in = tt == t ? p.in[t] : in;
+            }
+            return b;
+        };
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            // (indexes past the unit's loads, in shapes that do not fill them, read its first again)
+            int u = ROWS ? wave + NW * i : i, tt = u / UPT, k = u % UPT;
+            if (!ONE || ROWS) {
+                const bool some = u < NT * UPT && k < upt;
+                tt = some ? tt : 0;
+                k = some ? k : 0;
+            }
+            int in;
+            const uint8_t* b = base_of(tt, in);
             if constexpr (Q8) {
-                const uint8_t* lat = base + in * lat_tile + k * 1024;
-                const uint8_t* sc = base + sc_at + in * sc_tile + 2 * k;
-                if (2 * k + 1 < ks) {
+                const uint8_t* lat = b + in * lat_tile + k * 1024;
+                const uint8_t* sc = b + sc_at + in * sc_tile + 2 * k + n * ks;
+                if constexpr (ONE) {
                     x.st[i] = *reinterpret_cast<const u32x4*>(lat + lane * 16);
-                    x.sk[i] = ks & 1 ? sc[n * ks] | sc[n * ks + 1] << 8
-                                     : *reinterpret_cast<const uint16_t*>(sc + n * ks);
+                    x.sk[i] = *reinterpret_cast<const uint16_t*>(sc);
                 } else {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(lat + lane * 8);
-                    x.st[i] = u32x4{w[0], w[1], 0, 0};
-                    x.sk[i] = sc[n * ks];
+                    // an odd last k-step has 8 bytes a lane, and one scale
+                    const bool pair = 2 * k + 1 < ks;
+                    const u32x2 lo = *reinterpret_cast<const u32x2*>(lat + lane * (pair ? 16 : 8));
+                    const u32x2 hi =
+                        *reinterpret_cast<const u32x2*>(lat + (pair ? lane * 16 + 8 : lane * 8));
+                    x.st[i] = u32x4{lo[0], lo[1], pair ? hi[0] : 0, pair ? hi[1] : 0};
+                    x.sk[i] = sc[0] | (uint32_t)sc[pair ? 1 : 0] << 8;
                 }
             } else {
-                x.st[i] = *reinterpret_cast<const u32x4*>(base + in * lat_tile + k * 1024 + lane * 16);
-            }
-        };
-        if (one_page) {
-            // (an id outside the pool loads page 0, and the unit is dropped when it is staged)
-            const bool ok = (unsigned)p.id[0] < (unsigned)a.num_pool_pages;
-            const uint8_t* base = a.pages + (ok ? p.id[0] : 0) * rec;
-            x.has = ok ? (1u << NT) - 1 : 0;
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int u = ROWS ? wave + NW * i : i, tt = u / UPT, k = u % UPT;
-                if (u < NT * UPT && k < upt)
-                    fetch(i, k, base, p.in[0] + tt);
-            }
-#pragma unroll
-            for (int i = 0; i < NR; ++i)
-                if (rope_in[i] >= 0)
-                    x.sr[i] = *reinterpret_cast<const u32x4*>(base + key_at + p.in[0] * key_tile +
-                                                              rope_in[i]);
-        } else {
-            const uint8_t* bases[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const bool ok = (unsigned)p.id[t] < (unsigned)a.num_pool_pages;
-                bases[t] = a.pages + (ok ? p.id[t] : 0) * rec;
-                x.has |= ok ? 1u << t : 0;
-            }
-            auto base_of = [&](int tt, int& in) {
-                const uint8_t* base = bases[0];
-                in = p.in[0];
-#pragma unroll
-                for (int t = 1; t < NT; ++t) {
-                    base = tt == t ? bases[t] : base;
-                    in = tt == t ? p.in[t] : in;
-                }
-                return base;
-            };
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int u = ROWS ? wave + NW * i : i, tt = u / UPT, k = u % UPT;
-                int in;
-                const uint8_t* base = base_of(tt, in);
-                if (u < NT * UPT && k < upt)
-                    fetch(i, k, base, in);
-            }
-#pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                int in;
-                const uint8_t* base = base_of(rope_tt[i], in);
-                if (rope_in[i] >= 0)
-                    x.sr[i] = *reinterpret_cast<const u32x4*>(
-                        base + key_at + (in - rope_tt[i]) * key_tile + rope_in[i]);
+                x.st[i] = *reinterpret_cast<const u32x4*>(b + in * lat_tile + k * 1024 + lane * 16);
             }
         }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            int in;
+            const uint8_t* b = base_of(rope_tt[i], in);
+            x.sr[i] = *reinterpret_cast<const u32x4*>(b + (RP > 0 ? key_at : 0) +
+                                                      (in - rope_tt[i]) * key_tile +
+                                                      max(rope_in[i], rope_tt[i] * key_tile));
+        }
     };
-    // The keys of 32-key part `sub` of a unit that exist: before key_end, on a page of the pool.
-    auto keys_of = [&](int t0, int sub, uint32_t has) {
+    // The keys of 32-key part `sub` of the unit at tile t0 that exist.
+    auto keys_of = [&](int t0, int sub) {
         const int valid = key_end - 16 * t0 - 32 * sub;
-        uint32_t ok = valid >= 32 ? 0xffffffffu : valid <= 0 ? 0u : (1u << valid) - 1u;
-        if (!(has >> (2 * sub) & 1))
-            ok &= 0xffff0000u;
-        if (!(has >> (2 * sub) & 2))
-            ok &= 0x0000ffffu;
-        return ok;
+        return valid >= 32 ? 0xffffffffu : valid <= 0 ? 0u : (1u << valid) - 1u;
     };
     // Writes the loaded unit to `sp` and behind.  PLAIN: all of its keys exist and it needs no look
     // for non-finite latents; else keys outside `ok` become 0 (their slots, scales included, may
@@ -545,7 +534,7 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         uint32_t ok[SUB], mark[SUB] = {};
 #pragma unroll
         for (int k = 0; k < SUB; ++k)
-            ok[k] = keys_of(t0, k, x.has);
+            ok[k] = keys_of(t0, k);
         if ((ok[0] & ok[SUB - 1]) == 0xffffffffu && !look) {
             stage_unit(std::true_type{}, x, sp, ok, mark, false);
         } else {
@@ -556,10 +545,8 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                     if (mark[k])
                         atomicOr(&marks[u % 3 * SUB + k], mark[k]);
         }
-        if (u + STEP < n_units) {
-            load_unit(x, pages);
-            pages = find_pages(t0 + 2 * NT * STEP);
-        }
+        load_unit(x, pages);  // (the last one once more, at the end)
+        pages = find_pages(t0 + 2 * NT * STEP);
         if constexpr (ROWS) {
             // The other buffer is free: every wave that passed the barrier before this one has
             // finished with it.  Likewise marks: unit u + 2's words, last read in unit u - 1, are

@@ -406,8 +406,8 @@ int mla_read_plan_info(void* stream, const void* plan, int32_t* host_info);
  * launches as many workgroups as the plan has jobs, without it as many as a plan of these sizes can
  * have, whose rest returns at once (a few us).  Shapes as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace at multiples of 16
  * bytes.  The workspace needs no initialisation; calls that share one must be ordered on one
- * stream.  Page ids outside the pool are skipped, with the keys on them.  A non-finite latent
- * makes the rows that see its key NaN, and no others. */
+ * stream.  Page ids are those that mla_build_metadata and mla_plan_attention have checked.  A
+ * non-finite latent makes the rows that see its key NaN, and no others. */
 int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank, int rope_dim,
                          int page_size, int max_q_len, int dtype, int cache_format, float scale,
                          const int32_t* page_table, int max_pages, int num_pool_pages,
