@@ -104,11 +104,13 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     // halves the barriers and what else a unit costs besides its products
     constexpr int SUB = ROWS && KSM <= 8 ? 2 : 1;
     constexpr int NT = 2 * SUB, KEYS = 32 * SUB;
-    constexpr int SLOT = 32 * 32 * (KSM + RSM);         // words of a unit
+    // Words of a unit in LDS: 32 keys' latents, on list R (whose waves take each other's keys) their
+    // rope keys too, on list K (see the end) room for 16 rows of O^T in fp32 and their m and l.
+    constexpr int SLOT = ROWS ? 32 * 32 * (KSM + RSM) : 2 * (16 * (32 * KSM + 4) + 32);
     constexpr int UPT = Q8 ? (KSM + 1) / 2 : KSM;       // 16-byte loads of a lane per tile
     constexpr int NL = ROWS ? (NT * UPT + NW - 1) / NW : NT * UPT;
-    constexpr int RCS = ONE ? RP_ / 8 : 8;              // rope chunks of a tile, at most
-    constexpr int NR = ROWS ? (NT * RCS + 4 * NW - 1) / (4 * NW) : (NT * RCS + 3) / 4;
+    constexpr int RCS = ONE ? RP_ / 8 : 8;              // 8-column rope chunks of a tile, at most
+    constexpr int NR = ROWS ? (NT * RCS + 4 * NW - 1) / (4 * NW) : 2 * RSM;  // rope loads of a lane
     constexpr int SLOTS = ROWS ? 2 * SUB : 4;
     // Q^T k-steps that stay in LDS, lane by lane, where the registers would spill (a reload waits
     // for every load in flight): at kv 512 O^T takes 128 of a wave's 256 registers, Q^T 72.
@@ -191,16 +193,23 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     const int upt = Q8 ? (ks + 1) >> 1 : ks;
     const int lat_tile = (Q8 ? 16 : 32) * KV, key_tile = 32 * RP, sc_tile = 16 * ks;  // bytes
     const long long key_at = (long long)PS * (Q8 ? 1 : 2) * KV, sc_at = (long long)PS * (KV + 2 * RP);
-    // This lane's rope chunks: tile, and bytes from the unit's first keys (-1: none).
+    // This lane's rope chunks: tile, and bytes from the unit's first keys (-1: none).  List K: the
+    // operands of (tile, k-step) i; lanes past the rope columns take a valid chunk (their Q^T is 0).
     const int rcs = RP >> 3;
     int rope_tt[NR], rope_in[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        const int c = ROWS ? (tid >> 4) + 4 * NW * i : 4 * i + g;
-        const int tt = ONE ? c / (RCS > 0 ? RCS : 1) : (rcs > 0 ? c / rcs : 0);
-        const bool some = tt < NT && rcs > 0;
-        rope_tt[i] = some ? tt : 0;
-        rope_in[i] = some ? tt * key_tile + (c - tt * rcs) * 256 + n * 16 : -1;
+        if constexpr (ROWS) {
+            const int c = (tid >> 4) + 4 * NW * i;
+            const int tt = ONE ? c / (RCS > 0 ? RCS : 1) : (rcs > 0 ? c / rcs : 0);
+            const bool some = tt < NT && rcs > 0;
+            rope_tt[i] = some ? tt : 0;
+            rope_in[i] = some ? tt * key_tile + (c - tt * rcs) * 256 + n * 16 : -1;
+        } else {
+            const int tt = i / RSM, j = i % RSM;
+            rope_tt[i] = tt;
+            rope_in[i] = tt * key_tile + (32 * j + 8 * g < RP ? 4 * j + g : 0) * 256 + n * 16;
+        }
     }
     // A tile's page (number in the list) and place there: t / tpp by a product, one too small at most.
     auto page_of = [&](int t, int& in) {
@@ -289,9 +298,10 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         for (int i = 0; i < NR; ++i) {
             int in;
             const uint8_t* b = base_of(rope_tt[i], in);
-            x.sr[i] = *reinterpret_cast<const u32x4*>(b + (RP > 0 ? key_at : 0) +
-                                                      (in - rope_tt[i]) * key_tile +
-                                                      max(rope_in[i], rope_tt[i] * key_tile));
+            if (ROWS || RP > 0)
+                x.sr[i] = *reinterpret_cast<const u32x4*>(b + (RP > 0 ? key_at : 0) +
+                                                          (in - rope_tt[i]) * key_tile +
+                                                          max(rope_in[i], rope_tt[i] * key_tile));
         }
     };
     // The keys of 32-key part `sub` of the unit at tile t0 that exist.
@@ -299,45 +309,56 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         const int valid = key_end - 16 * t0 - 32 * sub;
         return valid >= 32 ? 0xffffffffu : valid <= 0 ? 0u : (1u << valid) - 1u;
     };
-    // Writes the loaded unit to `sp` and behind.  PLAIN: all of its keys exist and it needs no look
-    // for non-finite latents; else keys outside `ok` become 0 (their slots, scales included, may
-    // hold anything), and the keys that the wave found to have such a latent are left in `mark`.
-    auto stage_unit = [&]<bool PLAIN>(std::bool_constant<PLAIN>, const Loaded& x, uint16_t* sp,
-                                      const uint32_t (&ok)[SUB], uint32_t (&mark)[SUB], bool look) {
+    // Keys of the loaded unit outside `ok` become 0 (their slots, scales included, may hold
+    // anything).  look: non-finite latents become 0 as well, and the wave's `mark` names their keys.
+    auto clean_unit = [&](Loaded& x, const uint32_t (&ok)[SUB], uint32_t (&mark)[SUB], bool look) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int u = ROWS ? wave + NW * i : i, tt = u / UPT, k = u % UPT;
-            if (u >= NT * UPT || k >= upt)
-                continue;
-            u32x4 v = x.st[i];
-            uint32_t k8 = Q8 ? x.sk[i] : 0;
-            if constexpr (!PLAIN) {
-                const uint32_t of = SUB == 1 || tt < 2 ? ok[0] : ok[SUB - 1];
-                const uint32_t keep = -(of >> (16 * (tt & 1) + n) & 1);
-                v &= keep;
-                k8 &= keep;
-                if (look) {
-                    bool bad;
-                    if constexpr (Q8)
-                        bad = drop_nan8(v);
-                    else
-                        bad = drop_nonfinite16<T>(v);
-                    const uint64_t b = __builtin_amdgcn_ballot_w64(bad);
-                    const uint32_t m = (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff)
-                                       << (16 * (tt & 1));
+            const int u = ROWS ? wave + NW * i : i, tt = u / UPT;
+            const uint32_t of = SUB == 1 || tt < 2 ? ok[0] : ok[SUB - 1];
+            const uint32_t keep = -(of >> (16 * (tt & 1) + n) & 1);
+            x.st[i] &= keep;
+            if constexpr (Q8)
+                x.sk[i] &= keep;
+            if (look) {
+                bool bad;
+                if constexpr (Q8)
+                    bad = drop_nan8(x.st[i]);
+                else
+                    bad = drop_nonfinite16<T>(x.st[i]);
+                const uint64_t b = __builtin_amdgcn_ballot_w64(bad);
+                const uint32_t m = (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff)
+                                   << (16 * (tt & 1));
+                if (u < NT * UPT && u % UPT < upt) {
                     if (SUB == 1 || tt < 2)
                         mark[0] |= m;
                     else
                         mark[SUB - 1] |= m;
                 }
             }
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int tt = rope_tt[i];
+            const uint32_t of = SUB == 1 || tt < 2 ? ok[0] : ok[SUB - 1];
+            x.sr[i] &= -(of >> (16 * (tt & 1) + n) & 1);
+        }
+    };
+    // List R: writes the loaded unit to `sp` and behind.
+    auto stage_unit = [&](const Loaded& x, uint16_t* sp) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int u = wave + NW * i, tt = u / UPT, k = u % UPT;
+            if (u >= NT * UPT || k >= upt)
+                continue;
             uint16_t* dst = sp + (tt >> 1) * SLOT + (tt & 1) * 16 * KV + s_lane;
+            const u32x4 v = x.st[i];
             if constexpr (Q8) {
                 *reinterpret_cast<u32x4*>(dst + 2 * k * 512) =
-                    q8_decode8<T>(v[0], v[1], q8_scale(k8 & 0xff));
+                    q8_decode8<T>(v[0], v[1], q8_scale(x.sk[i] & 0xff));
                 if (2 * k + 1 < ks)
                     *reinterpret_cast<u32x4*>(dst + (2 * k + 1) * 512) =
-                        q8_decode8<T>(v[2], v[3], q8_scale(k8 >> 8));
+                        q8_decode8<T>(v[2], v[3], q8_scale(x.sk[i] >> 8));
             } else {
                 *reinterpret_cast<u32x4*>(dst + k * 512) = v;
             }
@@ -346,15 +367,40 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         for (int i = 0; i < NR; ++i)
             if (rope_in[i] >= 0) {
                 const int tt = rope_tt[i];
-                u32x4 v = x.sr[i];
-                if constexpr (!PLAIN) {
-                    const uint32_t of = SUB == 1 || tt < 2 ? ok[0] : ok[SUB - 1];
-                    v &= -(of >> (16 * (tt & 1) + n) & 1);
-                }
                 // (a tile's key rows take as many bytes here as in the record)
                 *reinterpret_cast<u32x4*>(sp + (tt >> 1) * SLOT + 32 * KV +
-                                          (rope_in[i] - (tt >> 1) * 2 * key_tile) / 2) = v;
+                                          (rope_in[i] - (tt >> 1) * 2 * key_tile) / 2) = x.sr[i];
             }
+    };
+    // List K: a wave loads its units in the order of the score product's operands, and so takes
+    // the scores from its registers; the latents go to `sp` for the second product.
+    auto stage_scores = [&](const Loaded& x, uint16_t* sp, floatx4 (&sc)[2]) {
+        auto step = [&](int tt, int j, u32x4 v) {
+            sc[tt] = T::mma32(__builtin_bit_cast(V8, v), qv[j], sc[tt]);
+            *reinterpret_cast<u32x4*>(sp + tt * 16 * KV + j * 512 + s_lane) = v;
+        };
+#pragma unroll
+        for (int k = 0; k < UPT; ++k)
+            if (k < upt)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    const int i = tt * UPT + k;
+                    const u32x4 v = x.st[i];
+                    if constexpr (Q8) {
+                        step(tt, 2 * k, q8_decode8<T>(v[0], v[1], q8_scale(x.sk[i] & 0xff)));
+                        if (2 * k + 1 < ks)
+                            step(tt, 2 * k + 1 < KSM ? 2 * k + 1 : 0,
+                                 q8_decode8<T>(v[2], v[3], q8_scale(x.sk[i] >> 8)));
+                    } else {
+                        step(tt, k, v);
+                    }
+                }
+#pragma unroll
+        for (int j = 0; j < RSM; ++j)
+            if (j < rs)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+                    sc[tt] = T::mma32(__builtin_bit_cast(V8, x.sr[tt * RSM + j]), qv[KSM + j], sc[tt]);
     };
 
     const int tr_par = (n & 3) >> 1;
@@ -370,10 +416,8 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     for (int rt = 0; rt < RTM; ++rt)
         acc[rt] = floatx4{0, 0, 0, 0};
 
-    // ---- scores, softmax and product of the unit at `sp`, whose first tile is t0; `ok`: keys of
-    // the unit that exist, `mark`: those with a non-finite latent ----
-    auto compute_unit = [&](const uint16_t* sp, int t0, uint32_t ok, uint32_t mark) {
-        floatx4 sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    // ---- list R: scores of the unit at `sp` ----
+    auto take_scores = [&](const uint16_t* sp, floatx4 (&sc)[2]) {
         // One k-step's operands are read while the step before it multiplies; the scheduler is held
         // to that (it would read all of them ahead, and spill).
         auto k_operand = [&](int tt, int j) {
@@ -417,6 +461,10 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
+    };
+    // ---- softmax and product of the unit at `sp`, whose first tile is t0; `ok`: keys of the unit
+    // that exist, `mark`: those with a non-finite latent ----
+    auto finish_unit = [&](floatx4 (&sc)[2], const uint16_t* sp, int t0, uint32_t ok, uint32_t mark) {
         auto c_operand = [&](int rt) {  // latent columns 16rt.. of the unit's 32 keys
             const int blk = ((rt >> 1) * 4 + 2 * (rt & 1)) * 128;
             const u32x2 lo = read_tr16(sp + blk + tr_lane);
@@ -535,19 +583,17 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
 #pragma unroll
         for (int k = 0; k < SUB; ++k)
             ok[k] = keys_of(t0, k);
-        if ((ok[0] & ok[SUB - 1]) == 0xffffffffu && !look) {
-            stage_unit(std::true_type{}, x, sp, ok, mark, false);
-        } else {
-            stage_unit(std::false_type{}, x, sp, ok, mark, look);
-            if (ROWS && lane == 0)
+        if ((ok[0] & ok[SUB - 1]) != 0xffffffffu || look)
+            clean_unit(x, ok, mark, look);
+        if constexpr (ROWS) {
+            if (look && lane == 0)
 #pragma unroll
                 for (int k = 0; k < SUB; ++k)
                     if (mark[k])
                         atomicOr(&marks[u % 3 * SUB + k], mark[k]);
-        }
-        load_unit(x, pages);  // (the last one once more, at the end)
-        pages = find_pages(t0 + 2 * NT * STEP);
-        if constexpr (ROWS) {
+            stage_unit(x, sp);
+            load_unit(x, pages);  // (the last one once more, at the end)
+            pages = find_pages(t0 + 2 * NT * STEP);
             // The other buffer is free: every wave that passed the barrier before this one has
             // finished with it.  Likewise marks: unit u + 2's words, last read in unit u - 1, are
             // cleared behind this barrier and set again behind the next.
@@ -559,15 +605,22 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
             }
             if (causal_seg && tid < SUB)
                 marks[(u + 2) % 3 * SUB + tid] = 0;
-        } else {
-            wave_lds_fence();
-        }
 #pragma unroll
-        for (int k = 0; k < SUB; ++k)
-            if (16 * t0 + 32 * k <= lim_wave)
-                compute_unit(sp + k * SLOT, t0 + 2 * k, ok[k], mark[k]);
-        if constexpr (!ROWS)
+            for (int k = 0; k < SUB; ++k)
+                if (16 * t0 + 32 * k <= lim_wave) {
+                    floatx4 sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                    take_scores(sp + k * SLOT, sc);
+                    finish_unit(sc, sp + k * SLOT, t0 + 2 * k, ok[k], mark[k]);
+                }
+        } else {
+            floatx4 sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            stage_scores(x, sp, sc);
+            load_unit(x, pages);
+            pages = find_pages(t0 + 2 * NT * STEP);
+            wave_lds_fence();
+            finish_unit(sc, sp, t0, ok[0], mark[0]);
             wave_lds_fence();  // the slot's reads are done before the next unit's writes
+        }
     }
 
     // ---- final rows, or partials ----
