@@ -17,8 +17,8 @@
 namespace mla {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kLdsSegs = 3072;  // segments whose tables fit LDS (9 of 12 KB)
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kLdsSegs = 3000;  // segments whose tables fit LDS (9 of 12 KB)
 constexpr int kTables = 9;
 constexpr int kFewRows = 64;    // segments up to this go to list K in any case
 constexpr int kRounds = 2, kSteps = 8, kTries = kRounds * kSteps;
@@ -31,30 +31,26 @@ __device__ __forceinline__ Cost cost_of(int kv_rank) {
     return kv_rank <= 128 ? Cost{1500, 3500, 1100, 4000, 3000} : Cost{6000, 6000, 2200, 8000, 3000};
 }
 
-__device__ __forceinline__ long long wave_scan(long long v, int lane) {
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long u = __shfl_up(v, d, 64);
-        if (lane >= d)
-            v += u;
-    }
-    return v;
-}
-
-// Inclusive scans of three values over the workgroup; `total` receives the sums.
-__device__ void block_scan3(long long (&v)[3], long long (*tmp)[3], long long (&total)[3]) {
+// Inclusive scans of three counts over the workgroup; `total` receives the sums.  (Jobs and partial
+// rows of a plan's sizes stay below 2^31, see plan_shape.)
+__device__ void block_scan3(int (&v)[3], int (*tmp)[3], int (&total)[3]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = 1; d < 64; d <<= 1)
+        for (int k = 0; k < 3; ++k) {
+            const int u = __shfl_up(v[k], d, 64);
+            if (lane >= d)
+                v[k] += u;
+        }
     __syncthreads();
-    for (int k = 0; k < 3; ++k) {
-        v[k] = wave_scan(v[k], lane);
-        if (lane == 63)
+    if (lane == 63)
+        for (int k = 0; k < 3; ++k)
             tmp[wave][k] = v[k];
-    }
     __syncthreads();
     for (int k = 0; k < 3; ++k) {
-        long long before = 0;
+        int before = 0;
         total[k] = 0;
         for (int w = 0; w < kWaves; ++w) {
-            const long long x = tmp[w][k];
+            const int x = tmp[w][k];
             before += w < wave ? x : 0;
             total[k] += x;
         }
@@ -72,8 +68,8 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)
 
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     __shared__ int32_t lds[kTables * kLdsSegs];
-    __shared__ long long tmp[kWaves][3];
-    __shared__ unsigned long long best[3];
+    __shared__ int tmp[kWaves][3];
+    __shared__ unsigned long long best[3], cost_sum[3];
     __shared__ int first_bad;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PlanShape& p = a.p;
@@ -91,8 +87,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     const int total_q = a.info[0] < 0 ? -1 : a.cu_q[B];
     if (tid == 0)
         first_bad = total_q < 0 || total_q > p.rows ? -1 : 0x7fffffff;
-    if (tid < 3)
+    if (tid < 3) {
         best[tid] = ~0ull;
+        cost_sum[tid] = 0;
+    }
     __syncthreads();
     if (first_bad != -1) {
         for (int i = tid; i < S; i += kThreads) {
@@ -154,7 +152,14 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         for (int i = tid; i < S; i += kThreads)
             for (int list = 0; list < 3; ++list)
                 v[list] += (long long)blocks_of(list, i) * tiles(i);
-        block_scan3(v, tmp, sums);
+        for (int list = 0; list < 3; ++list) {
+            v[list] = wave_total(v[list]);
+            if (lane == 0 && v[list] != 0)
+                atomicAdd(&cost_sum[list], (unsigned long long)v[list]);
+        }
+        __syncthreads();
+        for (int list = 0; list < 3; ++list)
+            sums[list] = (long long)cost_sum[list];
     }
     auto tried = [&](int list, int c) {  // length of candidate c, in tiles
         const int slots = list == 1 ? p.slots_r : p.slots_k;
@@ -203,7 +208,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     const int len_r = all_k ? 1 : tried(1, (int)(best[1] & 0xffffffffu));
 
     // ---- jobs and partial rows of each segment ----
-    long long at[3] = {0, 0, 0};
+    int at[3] = {0, 0, 0};
     for (int i0 = 0; i0 < S; i0 += kThreads) {
         const int i = i0 + tid;
         int n = 0, splits = 0, range = 0, blocks = 0;
@@ -217,15 +222,14 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             splits = ceil_div(tiles(i), range);
         }
         const bool joined = n > 0 && (splits > 1 || i < G || group[i] >= 0);
-        const long long jobs = (long long)blocks * splits;
-        long long v[3] = {f ? jobs : 0, f ? 0 : jobs, joined ? (long long)n * splits : 0};
-        const long long mine[3] = {v[0], v[1], v[2]};
-        long long sum[3];
+        const int jobs = blocks * splits;
+        const int mine[3] = {f ? jobs : 0, f ? 0 : jobs, joined ? n * splits : 0};
+        int v[3] = {mine[0], mine[1], mine[2]}, sum[3];
         block_scan3(v, tmp, sum);
         if (i < S) {
-            job_k[i] = (int)std::min<long long>(at[0] + v[0] - mine[0], 0x7fffffff);
-            job_r[i] = (int)std::min<long long>(at[1] + v[1] - mine[1], 0x7fffffff);
-            part[i] = joined ? (int)std::min<long long>(at[2] + v[2] - mine[2], 0x7fffffff) : -1;
+            job_k[i] = at[0] + v[0] - mine[0];
+            job_r[i] = at[1] + v[1] - mine[1];
+            part[i] = joined ? at[2] + v[2] - mine[2] : -1;
             cuts[i] = splits;
             len[i] = range;
         }
@@ -237,10 +241,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     if (tid < kPlanHead) {
         int v = 0;
         if (fits)
-            v = tid == kPlanStatus ? (int)(at[0] + at[1])
-                : tid == kPlanJobsK ? (int)at[0]
-                : tid == kPlanJobsR ? (int)at[1]
-                : tid == kPlanParts ? (int)at[2]
+            v = tid == kPlanStatus ? at[0] + at[1]
+                : tid == kPlanJobsK ? at[0]
+                : tid == kPlanJobsR ? at[1]
+                : tid == kPlanParts ? at[2]
                 : tid == kPlanRows  ? total_q
                 : tid == kPlanTag   ? (int)p.tag
                                     : 0;
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     for (int list = 0; list < 2; ++list) {
         const int32_t* first = list ? job_r : job_k;
         int32_t* out = a.plan + (list ? p.jobs_r_at : p.jobs_k_at);
-        for (int j = tid; j < (int)at[list]; j += kThreads) {
+        for (int j = tid; j < at[list]; j += kThreads) {
             int lo = 0, hi = S;  // the last segment that starts at or before the job
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
