@@ -33,18 +33,24 @@ int q8_shape(const char* fn, int kv_rank, int rope_dim, int page_size, int dtype
         return invalid(fn, "invalid argument");
     if (!q8_supported(page_size, kv_rank, rope_dim))
         return fail(MLA_ERR_UNSUPPORTED,
-                    std::string(fn) + ": page_size must be a multiple of 16, kv_rank of 32 up to "
-                                      "512, rope_dim of 8 up to 64");
+                    std::string(fn) + ": page_size must be a multiple of 16 up to 65,536, kv_rank of "
+                                      "32 up to 512, rope_dim of 8 up to 64");
     return MLA_OK;
 }
+
+constexpr long long kMaxSegments = 1 << 22;
 
 int plan_scalars(const char* fn, int B, int rows, int n_heads, int kv_rank, int page_size,
                  int max_q_len, int n_groups) {
     if (B < 0 || rows < 0 || n_heads < 1 || kv_rank < 1 || page_size < 1 || max_q_len < 1 ||
-        n_groups < 0 || n_groups > B || (long long)rows * n_heads > (1LL << 30))
+        n_groups < 0 || n_groups > B || (long long)B + n_groups > kMaxSegments ||
+        (long long)rows * n_heads > (1LL << 30))
         return invalid(fn, "invalid argument");
     const PlanShape p = plan_shape(B, n_groups, rows, n_heads, kv_rank, max_q_len);
-    if (p.max_parts > 0x7fffffffLL || p.words > (1LL << 40))
+    // (a launch has fewer than 2^32 threads)
+    if (p.max_parts > 0x7fffffffLL || p.words > (1LL << 40) ||
+        (long long)p.max_jobs_k * kThreadsK > 0xffffffffLL ||
+        (long long)p.max_jobs_r * kThreadsR > 0xffffffffLL)
         return invalid(fn, "the batch is too large for one plan");
     return MLA_OK;
 }

@@ -7,6 +7,7 @@
 #include "mla_latent.hpp"
 #include "mla_common.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace mla {
@@ -14,6 +15,7 @@ namespace {
 
 constexpr int kThreads = 256, kFlight = 4;
 constexpr long long kFewElements = 1 << 20;
+constexpr long long kBlocksX = 1 << 20;  // a grid's x: it has fewer than 2^32 threads there
 
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(kThreads) void latent_merge_kernel(LatentArgs a) {
@@ -22,10 +24,10 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(LatentArgs a) {
     const int32_t* plan = a.plan;
     const int tid = threadIdx.x, group = tid / PER, me = tid % PER;
     const int per_row = a.kv_rank / 4, H = a.H;
-    const long long e = blockIdx.x * (long long)PER + me;
+    const long long block = blockIdx.y * (long long)gridDim.x + blockIdx.x, e = block * PER + me;
     const long long fr = e / per_row;
     const int c = (int)(e - fr * per_row) * 4;
-    const int row = (int)(fr / H);
+    const int row = (int)(fr / H);  // (past the rows in the last blocks)
     int pre = 0, mine = 0;
     long long own_at = 0, pre_at = 0, own_n = 0, pre_n = 0;
     if (plan[kPlanTag] == (int)a.p.tag && plan[kPlanParts] > 0 && row < plan[kPlanRows]) {
@@ -115,8 +117,9 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(LatentArgs a) {
 template <typename T, int GROUPS>
 void launch_groups(const LatentArgs& a, hipStream_t stream) {
     constexpr int per = kThreads / GROUPS;
-    const long long n = (long long)a.p.rows * a.H * (a.kv_rank / 4);
-    hipLaunchKernelGGL((latent_merge_kernel<T, GROUPS>), dim3((unsigned)((n + per - 1) / per)),
+    const long long blocks = ((long long)a.p.rows * a.H * (a.kv_rank / 4) + per - 1) / per;
+    const unsigned x = (unsigned)std::min(blocks, kBlocksX);
+    hipLaunchKernelGGL((latent_merge_kernel<T, GROUPS>), dim3(x, (unsigned)((blocks + x - 1) / x)),
                        dim3(kThreads), 0, stream, a);
 }
 

@@ -23,9 +23,10 @@
 namespace mla {
 
 constexpr int kQ8MaxRank = 512, kQ8MaxRope = 64;
+constexpr int kQ8MaxPage = 65536;  // offsets within a page's record stay below 2^31
 
 __host__ __device__ inline bool q8_supported(int page_size, int kv_rank, int rope_dim) {
-    return page_size >= 16 && kv_rank >= 32 && rope_dim >= 0 &&
+    return page_size >= 16 && page_size <= kQ8MaxPage && kv_rank >= 32 && rope_dim >= 0 &&
            page_tiled(page_size, kv_rank, rope_dim) && kv_rank <= kQ8MaxRank &&
            rope_dim <= kQ8MaxRope;
 }

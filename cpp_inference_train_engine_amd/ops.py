@@ -13,6 +13,7 @@ current torch stream unless ``stream`` is given.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass, field
 
 from . import (CACHE_16BIT, CACHE_Q8, DECODE_FUSED_MERGE, DTYPE_BF16, DTYPE_F16, INFO_INTS, MAX_WORK,
@@ -295,6 +296,12 @@ def _check_list(what: str, t, gpu: int) -> int:
     return _check(what, t, (t.numel(),), _torch().int32, gpu)
 
 
+def _allocating_on(stream):
+    """Tensors that a call makes belong to the stream it works on: their fill comes before the
+    call's kernels, and their memory is not given to another stream's work while those run."""
+    return nullcontext() if stream is None else _torch().cuda.stream(stream)
+
+
 class QuantizedLatentCache:
     """Device page pool of the 8-bit latent cache: uint8 [layers, pages, record bytes], a record
     as mla_hip.h lays it out (e4m3 latents with a power-of-two scale for each 32 columns, rope
@@ -307,8 +314,8 @@ class QuantizedLatentCache:
         self.kv_rank, self.rope_dim, self.dtype = kv_rank, rope_dim, dtype
         rec = int(lib().mla_q8_page_bytes(page_size, kv_rank, rope_dim))
         if rec == 0:
-            raise ValueError("8-bit latent cache: page_size must be a multiple of 16, kv_rank of "
-                             "32 up to 512, rope_dim of 8 up to 64")
+            raise ValueError("8-bit latent cache: page_size must be a multiple of 16 up to 65,536, "
+                             "kv_rank of 32 up to 512, rope_dim of 8 up to 64")
         if storage is None:
             storage = torch.zeros((n_layers, num_pages, rec), dtype=torch.uint8, device=device)
         if (tuple(storage.shape) != (n_layers, num_pages, rec) or storage.dtype != torch.uint8 or
@@ -355,10 +362,12 @@ def read_latent_q8(cache: QuantizedLatentCache, layer: int, slot_mapping, ckv=No
     the pool are left as they were (zero in tensors that this call makes)."""
     gpu, T, dt = _gpu(), int(slot_mapping.shape[0]), _dtype_of(cache.dtype)
     slots = _check_list("slot_mapping", slot_mapping, gpu)
-    if ckv is None:
-        ckv = _torch().zeros((T, cache.kv_rank), dtype=dt, device=cache.pages.device)
-    if krope is None:
-        krope = _torch().zeros((T, cache.rope_dim), dtype=dt, device=cache.pages.device)
+    if ckv is None or krope is None:
+        with _allocating_on(stream):
+            if ckv is None:
+                ckv = _torch().zeros((T, cache.kv_rank), dtype=dt, device=cache.pages.device)
+            if krope is None:
+                krope = _torch().zeros((T, cache.rope_dim), dtype=dt, device=cache.pages.device)
     x = _check("ckv", ckv, (T, cache.kv_rank), dt, gpu)
     k = _check("krope", krope, (T, cache.rope_dim), dt, gpu)
     check(lib().mla_read_latent_q8(stream_handle(stream), T, cache.kv_rank, cache.rope_dim,
@@ -413,7 +422,8 @@ class AttentionPlan:
     def read_info(self, stream=None):
         """Synchronise and return [jobs, 0, jobs of 16 rows, jobs of 128 rows, partial rows, query
         rows, ..]; raises when the batch or the prefixes are invalid.  Calls after it launch no
-        more workgroups than the plan has jobs."""
+        more workgroups than the plan has jobs; so it is not for a plan that a captured graph
+        builds anew at each replay, whose jobs change."""
         import numpy as np
         h = np.zeros(PLAN_INFO_INTS, np.int32)
         check(lib().mla_read_plan_info(stream_handle(stream), self._words[0], h.ctypes.data))
@@ -445,7 +455,8 @@ def plan_attention(batch: RaggedBatch, n_heads: int, kv_rank: int, *, rows: int 
         raise ValueError(f"plan_attention: no plan for B={batch.B}, rows={rows}, n_heads={n_heads}, "
                          f"kv_rank={kv_rank}, max_q_len={max_q_len}, groups={groups}")
     info = _check_list("batch", batch.info, gpu)
-    words = torch.empty(n // 4, dtype=torch.int32, device=batch.info.device)
+    with _allocating_on(stream):
+        words = torch.empty(n // 4, dtype=torch.int32, device=batch.info.device)
     check(lib().mla_plan_attention(
         stream_handle(stream), batch.B, rows, n_heads, kv_rank, batch.page_size, max_q_len,
         ptr(batch.cu_seqlens_q), ptr(batch.cu_seqlens_k), info, groups, *shared,
@@ -473,10 +484,12 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
     torch, gpu = _torch(), _gpu()
     b, rows, H, kv = plan.batch, plan.rows, plan.n_heads, plan.kv_rank
     dt = torch.float16 if dtype == DTYPE_F16 else torch.bfloat16
-    if out is None:
-        out = torch.zeros((rows, H, kv), dtype=dt, device=q_latent.device)
-    if workspace is None:
-        workspace = attention_workspace(plan)
+    if out is None or workspace is None:
+        with _allocating_on(stream):
+            if out is None:
+                out = torch.zeros((rows, H, kv), dtype=dt, device=q_latent.device)
+            if workspace is None:
+                workspace = attention_workspace(plan)
     check(lib().mla_latent_attention(
         stream_handle(stream), b.B, rows, H, kv, rope_dim, b.page_size, plan.max_q_len, dtype,
         CACHE_Q8 if q8 else CACHE_16BIT, scale, plan._table, b.max_pages, b.num_pool_pages,

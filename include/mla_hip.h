@@ -333,7 +333,7 @@ int mla_prefill_attention(void* stream, int B, int n_heads, int kv_rank, int rop
  *             (J odd, j = J-1: t*16*kv_rank + j*512 + (16 g + n)*8 + e)
  *     rope    word (t*(rope_dim/8) + c/8)*128 + n*8 + c%8 of the section at byte page_size*kv_rank
  *     scale   byte page_size*(kv_rank + 2 rope_dim) + slot*J + j, holding k + 127
- * Shapes: page_size % 16 == 0, kv_rank % 32 == 0 up to 512, rope_dim % 8 == 0 up to 64
+ * Shapes: page_size % 16 == 0 up to 65,536, kv_rank % 32 == 0 up to 512, rope_dim % 8 == 0 up to 64
  * (MLA_ERR_UNSUPPORTED otherwise); pages at a multiple of 16 bytes. */
 /* Bytes of a page record, 0 for a shape outside the above. */
 size_t mla_q8_page_bytes(int page_size, int kv_rank, int rope_dim);
@@ -379,7 +379,8 @@ int mla_read_latent_q8(void* stream, int T, int kv_rank, int rope_dim, int page_
 #define MLA_CACHE_Q8 1    /* those of mla_append_latent_q8 */
 #define MLA_PLAN_INFO_INTS 8
 /* Sizes of a plan and of a call's workspace, 0 for sizes that no plan takes (a plan takes
- * rows * n_heads up to 2^30). */
+ * rows * n_heads up to 2^30, B + n_groups up to 2^22, and as many jobs as one launch of fewer than
+ * 2^32 threads). */
 size_t mla_attention_plan_bytes(int B, int rows, int n_heads, int kv_rank, int max_q_len,
                                 int n_groups);
 size_t mla_attention_workspace_bytes(int B, int rows, int n_heads, int kv_rank, int max_q_len,
@@ -402,10 +403,11 @@ int mla_read_plan_info(void* stream, const void* plan, int32_t* host_info);
 /* The attention.  page_table and max_pages are those of the metadata, cache_format one of
  * MLA_CACHE_*, q_latent [rows x n_heads x kv_rank], q_rope [rows x n_heads x rope_dim] and out
  * [rows x n_heads x kv_rank] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.
- * host_info is what mla_read_plan_info returned for this very plan, or NULL: with it the call
- * launches as many workgroups as the plan has jobs, without it as many as a plan of these sizes can
- * have, whose rest returns at once (a few us).  Shapes as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace at multiples of 16
- * bytes.  The workspace needs no initialisation; calls that share one must be ordered on one
+ * host_info is what mla_read_plan_info returned for this very plan, not built anew since, or NULL:
+ * with it the call launches as many workgroups as the plan has jobs, without it as many as a plan
+ * of these sizes can have, whose rest returns at once (a few us).  A captured graph that builds the
+ * plan takes NULL.  Shapes as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace
+ * at multiples of 16 bytes.  The workspace needs no initialisation; calls that share one must be ordered on one
  * stream.  Page ids are those that mla_build_metadata and mla_plan_attention have checked.  A
  * non-finite latent makes the rows that see its key NaN, and no others. */
 int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank, int rope_dim,

@@ -1,7 +1,7 @@
 """Planned attention over the 16-bit and the 8-bit latent cache, with and without shared prefixes,
 against the definition in 64 bits."""
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 import pytest
@@ -378,6 +378,122 @@ def test_one_plan_many_calls_streams_and_graphs(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,kv,rope,page,dtype,q8", [(2, 32, 8, 16, 1, False), (8, 128, 16, 64, 0, True)])
+def test_more_sessions_than_the_plan_keeps_on_chip(gpu, H, kv, rope, page, dtype, q8):
+    """The plan's tables of the segments lie in its own memory; sessions behind a prefix and
+    without one, the longest own keys at the end."""
+    rng = np.random.default_rng(12)
+    sessions = [(int(k), 1) for k in rng.integers(0, 60, 3100)]
+    sessions[7], sessions[1900], sessions[3099] = (9, 12), (20, 0), (63, 1)
+    c = make(H, kv, rope, page, dtype, q8, sessions, [(5, 70), (2200, 200), (1, 3)], seed=13)
+    _say(f"3100 sessions H={H} kv={kv} q8={q8}")
+    d = device(gpu, c)
+    plan, out, lse = call(gpu, c, d)
+    check(c, out, lse)
+    plan.read_info()
+    _, out2, lse2 = call(gpu, c, d, plan)
+    assert (out2 == out).all() and (lse2 == lse).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,kv,rope,page", [(8, 128, 16, 64), (128, 512, 64, 64)])
+def test_a_batch_without_rows_or_without_sessions(gpu, H, kv, rope, page):
+    import torch
+    c = make(H, kv, rope, page, 0, True, [(30, 0), (100, 0)], [(2, 70)], seed=14)
+    _say(f"no rows H={H}")
+    d = device(gpu, c, rows=3, max_q_len=1)
+    plan, out, lse = call(gpu, c, d)
+    assert plan.read_info()[:1] == [0]
+    assert (out == 5).all() and (lse == 5).all()
+    _, out, lse = call(gpu, c, d, plan)
+    assert (out == 5).all() and (lse == 5).all()
+    _say("no sessions")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    batch = gpu.build_metadata(none, none, zero, zero, page, 1, len(c.pool), max_rows=3)
+    d = dict(d, batch=batch, shared=None)
+    plan, out, lse = call(gpu, c, d)
+    assert plan.read_info()[:1] == [0]
+    assert (out == 5).all() and (lse == 5).all()
+
+
+@pytest.mark.gpu
+def test_a_graph_that_plans_a_growing_batch(gpu):
+    """Metadata, plan and attention captured together: each replay is that of the lengths that the
+    batch has then, eager calls between."""
+    import torch
+    rng = np.random.default_rng(15)
+    full = [int(k) for k in rng.integers(60, 900, 12)]
+    c = make(8, 128, 16, 64, 0, True, [(k, 1) for k in full], [(5, 300), (3, 10)], seed=16)
+    d = device(gpu, c)
+    need = [len(p) for p in c.own_pages]
+    i32 = lambda x: torch.tensor(np.asarray(x, np.int64).astype(np.int32), device="cuda")
+    ctx, q = i32(c.ctx), i32(c.q)
+    cu_pages, ids = i32(np.concatenate([[0], np.cumsum(need)])), i32(np.concatenate(c.own_pages))
+    out = torch.zeros((12, 8, 128), dtype=torch.float16, device="cuda")
+    lse = torch.zeros((12, 8), device="cuda")
+
+    def step(out, lse, ws=None):
+        # (a session's page list may be longer than its keys need)
+        batch = gpu.build_metadata(ctx, q, cu_pages, ids, c.page, max(need), len(c.pool),
+                                   split_pages=4, max_work=4096, max_rows=12)
+        plan = gpu.plan_attention(batch, 8, 128, rows=12, max_q_len=1, prefixes=d["shared"])
+        gpu.latent_attention(plan, d["pages"], d["ql"], d["qr"], c.scale, rope_dim=16, q8=True,
+                             out=out, lse=lse, workspace=ws)
+        return plan
+
+    _say("graph of a growing batch")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ws = gpu.attention_workspace(step(out, lse))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(out, lse, ws)
+    for share in (0.0, 0.3, 1.0, 0.6):
+        now = (np.array(full) * share).astype(int)
+        ctx.copy_(torch.from_numpy(now.astype(np.int32)))
+        eager, elses = torch.zeros_like(out), torch.zeros_like(lse)
+        step(eager, elses)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.equal(lse, elses), share
+        want = expect(replace(c, ctx=now))
+        check(c, out, lse, want)
+
+
+@pytest.mark.gpu
+def test_tensors_made_by_a_call_belong_to_its_stream(gpu):
+    """Without out and workspace, on a stream that is not the current one: what the call makes is
+    filled before its kernels run, however far behind the current stream is."""
+    import torch
+    c = make(8, 128, 16, 64, 0, True, [(k * 50, 1) for k in range(20)], [(12, 500)], seed=17)
+    d = device(gpu, c)
+    plan, want, _ = call(gpu, c, d)
+    slots = torch.arange(64, dtype=torch.int32, device="cuda")
+    cache = gpu.QuantizedLatentCache(1, len(c.pool), 64, 128, 16, storage=d["pages"][None])
+    lat, key = gpu.read_latent_q8(cache, 0, slots)
+    a = torch.randn(4096, 4096, device="cuda", dtype=torch.float16)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    _say("made on a side stream")
+    for _ in range(20):
+        b = a @ a  # the current stream is busy
+    sided = gpu.plan_attention(d["batch"], 8, 128, rows=20, max_q_len=1, prefixes=d["shared"],
+                               stream=side)
+    got = gpu.latent_attention(sided, d["pages"], d["ql"], d["qr"], c.scale, rope_dim=16, q8=True,
+                               stream=side)
+    lat2, key2 = gpu.read_latent_q8(cache, 0, slots, stream=side)
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert torch.equal(lat.view(torch.int16), lat2.view(torch.int16))
+    assert torch.equal(key.view(torch.int16), key2.view(torch.int16))
+
+
+@pytest.mark.gpu
 def test_bad_batches_and_prefixes_fail_the_plan_and_write_nothing(gpu):
     """Every error that only the device arrays hold: the plan says which entry, and the call over
     it leaves its outputs alone."""
@@ -449,7 +565,8 @@ def test_refusals_of_planned_attention():
     assert size(4, 4, 8, 128, 1, 0) > 0
     for bad in ((-1, 4, 8, 128, 1, 0), (4, -1, 8, 128, 1, 0), (4, 4, 0, 128, 1, 0),
                 (4, 4, 8, 0, 1, 0), (4, 4, 8, 128, 0, 0), (4, 4, 8, 128, 1, -1),
-                (4, 4, 8, 128, 1, 5), (4, 1 << 28, 8, 128, 1, 0)):
+                (4, 4, 8, 128, 1, 5), (4, 1 << 28, 8, 128, 1, 0), (1 << 22, 4, 8, 128, 1, 1),
+                (2**31 - 1, 4, 8, 128, 1, 0), (4, 1 << 24, 64, 128, 1 << 24, 4)):
         assert size(*bad) == 0 and L.mla_attention_workspace_bytes(*bad) == 0
     names = ("stream", "B", "rows", "H", "kv", "page", "max_q", "cu_q", "cu_k", "info", "groups",
              "cu_groups", "prefix_len", "cu_pages", "ids", "n_ids", "pool", "plan", "bytes")
@@ -481,7 +598,7 @@ def test_refusals_of_planned_attention():
                dict(ql=a + 2), dict(qr=a + 8), dict(out=a + 8), dict(plan=a + 8), dict(ws=a + 4),
                dict(plan_bytes=16), dict(ws_bytes=16), dict(info=a)):
         assert attend(**kw) == 1, kw
-    for kw in (dict(kv=100), dict(kv=544), dict(rope=4), dict(rope=72), dict(page=40)):
+    for kw in (dict(kv=100), dict(kv=544), dict(rope=4), dict(rope=72), dict(page=40), dict(page=65552)):
         assert attend(**kw) == 3, kw
     assert attend(rows=0) == 0  # nothing to do
     st = L.mla_read_plan_info(None, None, a)
