@@ -6,10 +6,16 @@
 // ranges of one length.  A GPU that holds `slots` workgroups of the list at once takes
 //     ceil(jobs / slots) * (length * time of a tile + time of a job's start and end)
 //     + the time of writing and reading the jobs' partial rows, where there are any
-// so what counts is that the jobs fill one round or two and not a little more: the length is
-// the best of candidates between 1 and 2 times total / (rounds * slots).  Whether segments of many
-// rows go to list R or are taken apart for list K is decided by the same estimate: list K costs
-// more per row, but its jobs are small and there is one launch instead of two.
+// where a tile takes its full time with all slots taken and half of it with half of them or fewer
+// (a wave alone is bound by its latencies).  So what counts is that the jobs fill one round or two
+// and not a little more, and that small batches are not cut finer than pays for the partial rows:
+// the length is the best of candidates between half and four times a slot's share.  (200 sessions
+// behind 5 prefixes, 8 heads, kv 128: 470 jobs in 17.3 us; 801 jobs, a share each, 18.4.)
+// Whether segments of many rows go to list R or are taken apart for list K is decided by the same
+// estimate: list K costs more per row, but its jobs are small and there is one launch instead of
+// two.  (4 chunks of 509 rows, 8 heads, kv 128: list K 26.8 us, list R 36.)
+// The kernel is a chain of short phases of one workgroup: 16 us for one session, 31 for 200 with
+// prefixes.  512 threads: twice as many only wait longer at the barriers (23-35 us).
 #include "mla_latent.hpp"
 
 #include <algorithm>
@@ -20,10 +26,11 @@ namespace {
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kLdsSegs = 3000;  // segments whose tables fit LDS (9 of 12 KB)
 constexpr int kTables = 9;
+constexpr int kUnits = 256;     // compute units
 constexpr int kFewRows = 64;    // segments up to this go to list K in any case
-constexpr int kRounds = 2, kSteps = 8, kTries = kRounds * kSteps;
+constexpr int kRounds = 2, kSteps = 6, kTries = (kRounds + 1) * kSteps;
 
-// Times in ns of a unit of 32 keys, by list, and of a job's start and end.
+// Times in ns of a unit of 32 keys, by list, with all slots taken, and of a job's start and end.
 struct Cost {
     int tile_k, job_k, tile_r, job_r, launch;
 };
@@ -163,7 +170,8 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     }
     auto tried = [&](int list, int c) {  // length of candidate c, in tiles
         const int slots = list == 1 ? p.slots_r : p.slots_k;
-        const long long share = sums[list] / (slots * (1 + c / kSteps)) + 1;
+        const int k = c / kSteps;  // 0: twice a slot's share or more, 1: its share, 2: half of it
+        const long long share = (sums[list] * kRounds >> k) / slots + 1;
         long long n = share + share * (c % kSteps) / kSteps;
         n = list == 1 ? (n + 1) & ~1LL : (n + 3) & ~3LL;  // a tile for each of the four waves
         return (int)std::min<long long>(n, 1 << 26);
@@ -189,8 +197,12 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         if (lane == 0) {
             const int slots = list == 1 ? p.slots_r : p.slots_k;
             const long long rounds = (jobs + slots - 1) / slots;
-            const long long each = list == 1 ? (long long)longest * cost.tile_r + cost.job_r
-                                             : (longest + 3LL) / 4 * cost.tile_k + cost.job_k;
+            // workgroups that share a compute unit share its time, down to half of them
+            const int most = slots / kUnits, here = (int)std::min<long long>(most, (jobs + kUnits - 1) / kUnits);
+            const long long share = std::max(2 * here, most);
+            const long long each =
+                list == 1 ? longest * share * cost.tile_r / (2 * most) + cost.job_r
+                          : (longest + 3LL) / 4 * share * cost.tile_k / (2 * most) + cost.job_k;
             // fp32 rows written and read back, at about 4 TB/s
             const long long rows = parts * (list == 1 ? kRowsR : kRowsK) * p.kv_rank * 8 / 4000;
             const unsigned long long ns = std::min<long long>(rounds * each + rows, 0xffffffffLL);
