@@ -14,8 +14,10 @@
 // Whether segments of many rows go to list R or are taken apart for list K is decided by the same
 // estimate: list K costs more per row, but its jobs are small and there is one launch instead of
 // two.  (4 chunks of 509 rows, 8 heads, kv 128: list K 26.8 us, list R 36.)
-// The kernel is a chain of short phases of one workgroup: 16 us for one session, 31 for 200 with
-// prefixes.  512 threads: twice as many only wait longer at the barriers (23-35 us).
+// The kernel is a chain of short phases of one workgroup: 11 us for one session, 23 for 200 with
+// prefixes.  Two things cost it most and were taken out: 64-bit divisions, and sums across lanes
+// for each candidate where a lane can have a candidate of its own (16-31 us).  512 threads: twice
+// as many only wait longer at the barriers.
 #include "mla_latent.hpp"
 
 #include <algorithm>
@@ -28,7 +30,7 @@ constexpr int kLdsSegs = 3000;  // segments whose tables fit LDS (9 of 12 KB)
 constexpr int kTables = 9;
 constexpr int kUnits = 256;     // compute units
 constexpr int kFewRows = 64;    // segments up to this go to list K in any case
-constexpr int kRounds = 2, kSteps = 6, kTries = (kRounds + 1) * kSteps;
+constexpr int kRounds = 2, kSteps = 8, kTries = (kRounds + 1) * kSteps;
 
 // Times in ns of a unit of 32 keys, by list, with all slots taken, and of a job's start and end.
 struct Cost {
@@ -73,11 +75,13 @@ __device__ __forceinline__ long long wave_total(long long v) {
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
 
+// ON_CHIP: the tables lie in LDS (known to the compiler: generic loads take three times as long)
+template <bool ON_CHIP>
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
-    __shared__ int32_t lds[kTables * kLdsSegs];
+    __shared__ int32_t lds[ON_CHIP ? kTables * kLdsSegs : 1];
     __shared__ int tmp[kWaves][3];
-    __shared__ unsigned long long best[3], cost_sum[3];
-    __shared__ int first_bad;
+    __shared__ unsigned long long best[3], tile_sum[3];
+    __shared__ int first_bad, tries[3][3 * kTries];  // jobs, their partial rows' blocks, the longest
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PlanShape& p = a.p;
     const int B = p.B, G = p.groups, S = G + B, H = p.H;
@@ -85,7 +89,11 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     int32_t* const merges = a.plan + p.merge_at;
     int32_t* const session_of = a.plan + p.session_at;
     // tables of the segments: the groups' prefixes, then the sessions' own keys
-    int32_t* const t = S <= kLdsSegs ? lds : a.plan + p.seg_at;
+    int32_t* t;
+    if constexpr (ON_CHIP)
+        t = lds;
+    else
+        t = a.plan + p.seg_at;
     int32_t *const q0 = t, *const ql = t + S, *const keys = t + 2LL * S, *const group = t + 3LL * S,
             *const job_k = t + 4LL * S, *const job_r = t + 5LL * S, *const part = t + 6LL * S,
             *const cuts = t + 7LL * S, *const len = t + 8LL * S;
@@ -96,8 +104,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         first_bad = total_q < 0 || total_q > p.rows ? -1 : 0x7fffffff;
     if (tid < 3) {
         best[tid] = ~0ull;
-        cost_sum[tid] = 0;
+        tile_sum[tid] = 0;
     }
+    if (tid < 3 * kTries)
+        tries[0][tid] = tries[1][tid] = tries[2][tid] = 0;
     __syncthreads();
     if (first_bad != -1) {
         for (int i = tid; i < S; i += kThreads) {
@@ -142,72 +152,84 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     __syncthreads();
 
     auto flat = [&](int i) { return ql[i] > 0 && keys[i] > 0 ? ql[i] * H : 0; };  // its rows
-    auto tiles = [&](int i) { return (int)(((long long)keys[i] + kTile - 1) / kTile); };
+    auto tiles = [&](int i) { return ceil_div(std::max(keys[i], 0), kTile); };
     const Cost cost = cost_of(p.kv_rank);
     // Lists to estimate: 0 list K of the few, 1 list R of the others, 2 list K of all.
-    auto blocks_of = [&](int list, int i) {
-        const int n = flat(i);
-        if (list == 2 || (list == 0 && n <= kFewRows))
-            return ceil_div(n, kRowsK);
-        return list == 1 && n > kFewRows ? ceil_div(n, kRowsR) : 0;
+    auto blocks_of = [&](int list, int n) {  // blocks of n rows
+        const int k = ceil_div(n, kRowsK), r = ceil_div(n, kRowsR);
+        return list == 2 ? k : list == 0 ? (n <= kFewRows ? k : 0) : (n > kFewRows ? r : 0);
     };
 
     // ---- the range lengths ----
     long long sums[3];
     {
         long long v[3] = {0, 0, 0};
-        for (int i = tid; i < S; i += kThreads)
+        for (int i = tid; i < S; i += kThreads) {
+            const int n = flat(i), t = tiles(i);
             for (int list = 0; list < 3; ++list)
-                v[list] += (long long)blocks_of(list, i) * tiles(i);
+                v[list] += (long long)blocks_of(list, n) * t;
+            cuts[i] = n;  // for the estimates: rows, tiles, and whether there is more to join
+            len[i] = i < G || group[i] >= 0 ? -1 - t : t;
+        }
         for (int list = 0; list < 3; ++list) {
             v[list] = wave_total(v[list]);
             if (lane == 0 && v[list] != 0)
-                atomicAdd(&cost_sum[list], (unsigned long long)v[list]);
+                atomicAdd(&tile_sum[list], (unsigned long long)v[list]);
         }
         __syncthreads();
         for (int list = 0; list < 3; ++list)
-            sums[list] = (long long)cost_sum[list];
+            sums[list] = (long long)tile_sum[list];
     }
+    const int log_k = __builtin_ctz(p.slots_k), log_r = __builtin_ctz(p.slots_r);  // powers of two
     auto tried = [&](int list, int c) {  // length of candidate c, in tiles
-        const int slots = list == 1 ? p.slots_r : p.slots_k;
         const int k = c / kSteps;  // 0: twice a slot's share or more, 1: its share, 2: half of it
-        const long long share = (sums[list] * kRounds >> k) / slots + 1;
+        const long long share = (sums[list] * kRounds >> (k + (list == 1 ? log_r : log_k))) + 1;
         long long n = share + share * (c % kSteps) / kSteps;
         n = list == 1 ? (n + 1) & ~1LL : (n + 3) & ~3LL;  // a tile for each of the four waves
         return (int)std::min<long long>(n, 1 << 26);
     };
-    for (int e = wave; e < 3 * kTries; e += kWaves) {
-        const int list = e / kTries, c = e % kTries, n = tried(list, c);
-        if (sums[list] == 0)
+    // A lane estimates a candidate, over every kWaves-th segment in each wave.
+    auto wanted = [&](int list) {  // (without segments of many rows lists 0 and 2 are the same)
+        return sums[list] > 0 && !(list == 0 && sums[1] == 0) &&
+               !(list == 2 && sums[1] > 0 && !p.list_k_holds_all);
+    };
+    for (int e = lane; e < 3 * kTries; e += 64) {
+        const int list = e / kTries;
+        if (!wanted(list))
             continue;
-        long long jobs = 0, parts = 0;
-        int longest = 0;
-        for (int i = lane; i < S; i += 64)
-            if (const int b = blocks_of(list, i)) {
-                const int splits = ceil_div(tiles(i), n);
-                jobs += (long long)b * splits;
-                if (splits > 1 || i < G || group[i] >= 0)
-                    parts += (long long)b * splits;
-                longest = std::max(longest, std::min(n, tiles(i)));
-            }
-        jobs = wave_total(jobs);
-        parts = wave_total(parts);
-        for (int d = 32; d > 0; d >>= 1)
-            longest = std::max(longest, __shfl_xor(longest, d, 64));
-        if (lane == 0) {
-            const int slots = list == 1 ? p.slots_r : p.slots_k;
-            const long long rounds = (jobs + slots - 1) / slots;
-            // workgroups that share a compute unit share its time, down to half of them
-            const int most = slots / kUnits, here = (int)std::min<long long>(most, (jobs + kUnits - 1) / kUnits);
-            const long long share = std::max(2 * here, most);
-            const long long each =
-                list == 1 ? longest * share * cost.tile_r / (2 * most) + cost.job_r
-                          : (longest + 3LL) / 4 * share * cost.tile_k / (2 * most) + cost.job_k;
-            // fp32 rows written and read back, at about 4 TB/s
-            const long long rows = parts * (list == 1 ? kRowsR : kRowsK) * p.kv_rank * 8 / 4000;
-            const unsigned long long ns = std::min<long long>(rounds * each + rows, 0xffffffffLL);
-            atomicMin(&best[list], ns << 32 | (unsigned)c);
+        const int n = tried(list, e % kTries);
+        const float inv = 1.0f / (float)n;  // an estimate may be a range off where it just fits
+        int jobs = 0, parts = 0, longest = 0;
+#pragma unroll 4
+        for (int i = wave; i < S; i += kWaves) {
+            const int b = blocks_of(list, cuts[i]);
+            const bool joined = len[i] < 0;
+            const int t = joined ? -1 - len[i] : len[i];
+            const int splits = (int)__builtin_ceilf((float)t * inv);
+            jobs += b * splits;
+            parts += splits > 1 || joined ? b * splits : 0;
+            longest = b > 0 ? std::max(longest, std::min(n, t)) : longest;
         }
+        atomicAdd(&tries[0][e], jobs);
+        atomicAdd(&tries[1][e], parts);
+        atomicMax(&tries[2][e], longest);
+    }
+    __syncthreads();
+    if (const int list = tid / kTries; list < 3 && wanted(list)) {
+        const int jobs = tries[0][tid], parts = tries[1][tid], longest = tries[2][tid];
+        const int slots = list == 1 ? p.slots_r : p.slots_k, most = slots / kUnits;
+        const float rounds = (float)ceil_div(jobs, slots);
+        // workgroups that share a compute unit share its time, down to half of them
+        const float share =
+            std::max((float)std::min(most, ceil_div(jobs, kUnits)) / (float)most, 0.5f);
+        const float each = list == 1
+                               ? (float)longest * share * cost.tile_r + cost.job_r
+                               : (float)((longest + 3) / 4) * share * cost.tile_k + cost.job_k;
+        // fp32 rows written and read back, at about 4 TB/s
+        const float rows =
+            (float)parts * ((list == 1 ? kRowsR : kRowsK) * p.kv_rank) * (8.0f / 4000);
+        const unsigned long long ns = (unsigned long long)std::min(rounds * each + rows, 4e9f);
+        atomicMin(&best[list], ns << 32 | (unsigned)(tid - list * kTries));
     }
     __syncthreads();
     auto ns_of = [&](int list) { return sums[list] == 0 ? 0 : (long long)(best[list] >> 32); };
@@ -366,7 +388,10 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
 }
 
 hipError_t launch_plan(const PlanArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+    if (a.p.B + a.p.groups <= kLdsSegs)
+        hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(kThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL(plan_kernel<false>, dim3(1), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
