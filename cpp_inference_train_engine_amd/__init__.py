@@ -199,7 +199,8 @@ def stream_handle(stream=None) -> int | None:
         import torch
         torch.cuda.current_stream()  # initialises the device
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        _current_raw_stream = ((lambda: raw(torch.cuda.current_device())) if raw else
+        device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _current_raw_stream = ((lambda: raw(device())) if raw else
                                (lambda: torch.cuda.current_stream().cuda_stream))
     return _current_raw_stream()
 
