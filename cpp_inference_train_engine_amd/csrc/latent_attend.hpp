@@ -204,9 +204,23 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
 
     // ---- a unit's way into LDS ----
     const int s_lane = g * 128 + (n ^ ((g & 1) * kRot)) * 8;
+    // Nothing is done to what was loaded before it is staged (taking a scale's byte out of its word
+    // would wait for the load): scales stay as they lie in memory, the words of a tile's token
+    // (WORDS), or those of a load's two k-steps in one word or in two.
+    constexpr bool WORDS = Q8 && ONE && !ROWS;
     struct Loaded {
         u32x4 st[NL], sr[NR];
-        uint32_t sk[Q8 ? NL : 1];  // scale bytes of a load's one or two k-steps
+        uint32_t sk[WORDS ? KSM / 2 : Q8 ? (ONE ? NL : 2 * NL) : 1];
+    };
+    auto scale_of = [](const Loaded& x, int i, int half) {  // of k-step `half` of load i
+        if constexpr (WORDS) {
+            const int b = 2 * (i % UPT) + half;
+            return q8_scale(x.sk[i / UPT * (KSM / 4) + b / 4] >> (8 * (b % 4)) & 0xff);
+        } else if constexpr (ONE) {
+            return q8_scale(half ? x.sk[i] >> 8 : x.sk[i] & 0xff);
+        } else {
+            return q8_scale(x.sk[2 * i + half]);
+        }
     };
     const int upt = Q8 ? (ks + 1) >> 1 : ks;
     const int lat_tile = (Q8 ? 16 : 32) * KV, key_tile = 32 * RP, sc_tile = 16 * ks;  // bytes
@@ -298,20 +312,30 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                 const uint8_t* sc = b + sc_at + in * sc_tile + 2 * k + n * ks;
                 if constexpr (ONE) {
                     x.st[i] = *reinterpret_cast<const u32x4*>(lat + lane * 16);
-                    x.sk[i] = *reinterpret_cast<const uint16_t*>(sc);
+                    if constexpr (!WORDS)
+                        x.sk[i] = *reinterpret_cast<const uint16_t*>(sc);
                 } else {
-                    // an odd last k-step has 8 bytes a lane, and one scale
+                    // an odd last k-step has 8 bytes a lane, and one scale: read twice
                     const bool pair = 2 * k + 1 < ks;
                     const u32x2 lo = *reinterpret_cast<const u32x2*>(lat + lane * (pair ? 16 : 8));
                     const u32x2 hi =
                         *reinterpret_cast<const u32x2*>(lat + (pair ? lane * 16 + 8 : lane * 8));
-                    x.st[i] = u32x4{lo[0], lo[1], pair ? hi[0] : 0, pair ? hi[1] : 0};
-                    x.sk[i] = sc[0] | (uint32_t)sc[pair ? 1 : 0] << 8;
+                    x.st[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                    x.sk[2 * i] = sc[0];
+                    x.sk[2 * i + 1] = sc[pair ? 1 : 0];
                 }
             } else {
                 x.st[i] = *reinterpret_cast<const u32x4*>(b + in * lat_tile + k * 1024 + lane * 16);
             }
         }
+        if constexpr (WORDS)
+#pragma unroll
+            for (int i = 0; i < KSM / 2; ++i) {
+                int in;
+                const uint8_t* b = base_of(i / (KSM / 4), in);
+                x.sk[i] = reinterpret_cast<const uint32_t*>(b + sc_at + in * sc_tile +
+                                                            n * ks)[i % (KSM / 4)];
+            }
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             int in;
@@ -336,8 +360,10 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
             const uint32_t of = SUB == 1 || tt < 2 ? ok[0] : ok[SUB - 1];
             const uint32_t keep = -(of >> (16 * (tt & 1) + n) & 1);
             x.st[i] &= keep;
-            if constexpr (Q8)
-                x.sk[i] &= keep;
+            if constexpr (Q8 && !ONE)
+                x.sk[2 * i + 1] &= keep;
+            if constexpr (Q8 && !WORDS)
+                x.sk[ONE ? i : 2 * i] &= keep;
             if (look) {
                 bool bad;
                 if constexpr (Q8)
@@ -355,6 +381,10 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                 }
             }
         }
+        if constexpr (WORDS)
+#pragma unroll
+            for (int i = 0; i < KSM / 2; ++i)
+                x.sk[i] &= -(ok[0] >> (16 * (i / (KSM / 4)) + n) & 1);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             const int tt = rope_tt[i];
@@ -373,10 +403,10 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
             const u32x4 v = x.st[i];
             if constexpr (Q8) {
                 *reinterpret_cast<u32x4*>(dst + 2 * k * 512) =
-                    q8_decode8<T>(v[0], v[1], q8_scale(x.sk[i] & 0xff));
+                    q8_decode8<T>(v[0], v[1], scale_of(x, i, 0));
                 if (2 * k + 1 < ks)
                     *reinterpret_cast<u32x4*>(dst + (2 * k + 1) * 512) =
-                        q8_decode8<T>(v[2], v[3], q8_scale(x.sk[i] >> 8));
+                        q8_decode8<T>(v[2], v[3], scale_of(x, i, 1));
             } else {
                 *reinterpret_cast<u32x4*>(dst + k * 512) = v;
             }
@@ -392,7 +422,11 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     };
     // List K: a wave loads its units in the order of the score product's operands, and so takes
     // the scores from its registers; the latents go to `sp` for the second product.
-    auto stage_scores = [&](const Loaded& x, uint16_t* sp, floatx4 (&sc)[2]) {
+    auto stage_scores = [&](Loaded& x, uint16_t* sp, floatx4 (&sc)[2]) {
+        if constexpr (WORDS)
+#pragma unroll
+            for (int i = 0; i < KSM / 2; ++i)
+                asm volatile("" : "+v"(x.sk[i]));  // (bytes are taken from here on)
         auto step = [&](int tt, int j, u32x4 v) {
             sc[tt] = T::mma32(__builtin_bit_cast(V8, v), qv[j], sc[tt]);
             *reinterpret_cast<u32x4*>(sp + tt * 16 * KV + j * 512 + s_lane) = v;
@@ -405,10 +439,10 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
                     const int i = tt * UPT + k;
                     const u32x4 v = x.st[i];
                     if constexpr (Q8) {
-                        step(tt, 2 * k, q8_decode8<T>(v[0], v[1], q8_scale(x.sk[i] & 0xff)));
+                        step(tt, 2 * k, q8_decode8<T>(v[0], v[1], scale_of(x, i, 0)));
                         if (2 * k + 1 < ks)
                             step(tt, 2 * k + 1 < KSM ? 2 * k + 1 : 0,
-                                 q8_decode8<T>(v[2], v[3], q8_scale(x.sk[i] >> 8)));
+                                 q8_decode8<T>(v[2], v[3], scale_of(x, i, 1)));
                     } else {
                         step(tt, k, v);
                     }
