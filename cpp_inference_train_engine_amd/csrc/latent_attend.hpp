@@ -67,6 +67,18 @@ __device__ __forceinline__ table_ptr table(const int32_t* p) {
     return (table_ptr)reinterpret_cast<uintptr_t>(p);
 }
 
+// n / d and the rest by a product with floor(2^32 / d) (2^32 - 1 for d = 1): one too small at most
+// for n < 2^32.
+__device__ __forceinline__ int quotient(int n, int d, uint32_t inverse, int& rest) {
+    int q = (int)(((unsigned long long)(unsigned)n * inverse) >> 32);
+    rest = n - q * d;
+    if (rest >= d) {
+        ++q;
+        rest -= d;
+    }
+    return q;
+}
+
 __device__ __forceinline__ u32x2 read_tr16(const uint16_t* p) {
     typedef short s4 __attribute__((ext_vector_type(4)));
     const auto v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -166,11 +178,15 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
     int lim, lim_wave = -1, lim_all = key_end - 1;  // lane's row n sees keys [0, lim] of the segment
     // The last key that every row of the block sees: from there on a non-finite latent has to be
     // kept from the rows before it.
-    const int seen_by_all = causal_seg ? ctx + rb / H : 0x7fffffff;
+    auto token_of = [&](int row) {  // row / H
+        int r;
+        return quotient(row, H, a.h_inverse, r);
+    };
+    const int seen_by_all = causal_seg ? ctx + token_of(rb) : 0x7fffffff;
     {
         const int r = min(row0 + n, n_rows - 1);  // rows past the block repeat its last
         const long long fr = (long long)f0 + r;
-        lim = causal_seg ? ctx + (rb + r) / H : key_end - 1;
+        lim = causal_seg ? ctx + token_of(rb + r) : key_end - 1;
         const uint16_t* ql = a.q_latent + fr * KV + 8 * g;
         const uint16_t* qr = a.q_rope + fr * RP;
 #pragma unroll
@@ -192,9 +208,9 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         // the last key that any of the wave's rows sees (-1: it has no rows), and that all see
         const int last = min(n_rows, row0 + 16) - 1;
         if (last >= row0)
-            lim_wave = causal_seg ? ctx + (rb + last) / H : key_end - 1;
+            lim_wave = causal_seg ? ctx + token_of(rb + last) : key_end - 1;
         if (causal_seg)
-            lim_all = ctx + (rb + row0) / H;
+            lim_all = ctx + token_of(rb + row0);
     }
     auto q_operand = [&](int j) {
         return j < KSM + RSM - QL
@@ -243,16 +259,8 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
             rope_in[i] = tt * key_tile + (32 * j + 8 * g < RP ? 4 * j + g : 0) * 256 + n * 16;
         }
     }
-    // A tile's page (number in the list) and place there: t / tpp by a product, one too small at most.
-    auto page_of = [&](int t, int& in) {
-        int q = (int)(((unsigned long long)(unsigned)t * a.tpp_inverse) >> 32), r = t - q * tpp;
-        if (r >= tpp) {
-            ++q;
-            r -= tpp;
-        }
-        in = r;
-        return q;
-    };
+    // A tile's page (number in the list) and place there.
+    auto page_of = [&](int t, int& in) { return quotient(t, tpp, a.tpp_inverse, in); };
     const int last_tile = (key_end - 1) >> 4;
     const bool one_page = PS % KEYS == 0;  // a unit lies on one page
     // Page ids of the unit at tile t, and the places of its tiles there.  Tiles past the keys take

@@ -244,7 +244,9 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
     a.page_size = page_size;
     a.max_pages = max_pages;
     a.num_pool_pages = num_pool_pages;
-    a.tpp_inverse = (uint32_t)std::min<uint64_t>((1ULL << 32) / (page_size / 16), 0xffffffffULL);
+    auto inverse = [](int n) { return (uint32_t)std::min<uint64_t>((1ULL << 32) / n, 0xffffffffULL); };
+    a.tpp_inverse = inverse(page_size / 16);
+    a.h_inverse = inverse(n_heads);
     a.causal = max_q_len > 1;
     a.q8 = cache_format == MLA_CACHE_Q8;
     a.scale_log2 = scale * 1.4426950408889634f;

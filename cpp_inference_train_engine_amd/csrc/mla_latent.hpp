@@ -46,7 +46,7 @@ struct LatentArgs {
     int H, kv_rank, rope_dim, page_size, max_pages, num_pool_pages;
     int causal;        // the rows of a block may see different keys
     int q8;
-    uint32_t tpp_inverse;  // floor(2^32 / tiles of a page) (2^32 - 1 for one)
+    uint32_t tpp_inverse, h_inverse;  // floor(2^32 / n) of a page's tiles and of H (2^32 - 1 for 1)
     int jobs_k, jobs_r;  // workgroups to launch: the plan's jobs, or as many as it could have
     bool merge;          // there may be partial rows
     float scale_log2;  // softmax scale * log2(e)
