@@ -86,8 +86,6 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     const PlanShape& p = a.p;
     const int B = p.B, G = p.groups, S = G + B, H = p.H;
     int32_t* const head = a.plan;
-    int32_t* const merges = a.plan + p.merge_at;
-    int32_t* const session_of = a.plan + p.session_at;
     // tables of the segments: the groups' prefixes, then the sessions' own keys
     int32_t* t;
     if constexpr (ON_CHIP)
@@ -320,22 +318,21 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             o[7] = part[i] < 0 ? -1 : part[i] + sp * n + rb;
         }
     }
-    // ---- what the merge adds up for a session; the session of each row ----
-    for (int s = tid; s < B; s += kThreads) {
-        const int i = G + s, g = group[i];
-        int32_t* m = merges + (long long)s * kMergeInts;
-        m[0] = g >= 0 && flat(g) > 0 ? cuts[g] : 0;
-        m[1] = g >= 0 ? part[g] : 0;
-        m[2] = g >= 0 ? flat(g) : 0;
-        m[3] = g >= 0 ? (q0[i] - q0[g]) * H : 0;
-        m[4] = part[i] >= 0 ? cuts[i] : 0;
-        m[5] = part[i];
-        m[6] = flat(i);
-        m[7] = q0[i];
+    // ---- what the merge adds up for each row ----
+    if (at[2] == 0)
+        return;
+    for (int e = tid; e < 16 * B; e += kThreads) {  // 16 threads a session
+        const int i = G + (e >> 4), g = group[i], rows = ql[i];
+        const int pre = g >= 0 && flat(g) > 0 ? cuts[g] : 0, mine = part[i] >= 0 ? cuts[i] : 0;
+        const int pre_n = pre > 0 ? flat(g) : 0;
+        const int pre_at = pre > 0 ? part[g] + (q0[i] - q0[g]) * H : 0;
+        for (int r = e & 15; r < rows; r += 16) {
+            i32x4* m = reinterpret_cast<i32x4*>(a.plan + p.merge_at +
+                                                (long long)(q0[i] + r) * kMergeInts);
+            m[0] = i32x4{pre, mine, pre_at + r * H, part[i] + r * H};
+            m[1] = i32x4{pre_n, flat(i), 0, 0};
+        }
     }
-    for (int e = tid; e < 16 * B; e += kThreads)  // 16 threads a session
-        for (int r = e & 15; r < ql[G + (e >> 4)]; r += 16)
-            session_of[q0[G + (e >> 4)] + r] = e >> 4;
 }
 
 }  // namespace
@@ -375,9 +372,8 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
     p.max_parts = std::min(cut + (groups > 0 ? 2 * flat : 0),
                            (long long)kRowsK * p.max_jobs_k + (long long)kRowsR * p.max_jobs_r);
     p.seg_at = kPlanHead;
-    p.merge_at = p.seg_at + (segs > kLdsSegs ? segs * kTables : 0);
-    p.session_at = p.merge_at + (long long)B * kMergeInts;
-    p.jobs_k_at = (p.session_at + rows + 7) & ~7LL;
+    p.merge_at = p.seg_at + (segs > kLdsSegs ? (segs * kTables + 7) & ~7LL : 0);
+    p.jobs_k_at = p.merge_at + (long long)rows * kMergeInts;
     p.jobs_r_at = p.jobs_k_at + (long long)p.max_jobs_k * kJobInts;
     p.words = p.jobs_r_at + (long long)p.max_jobs_r * kJobInts;
     uint32_t h = 2166136261u;

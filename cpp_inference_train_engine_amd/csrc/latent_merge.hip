@@ -31,19 +31,14 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(LatentArgs a) {
     const long long fr = e / per_row;
     const int c = (int)(e - fr * per_row) * 4;
     const int row = (int)(fr / H);  // (past the rows in the last blocks)
-    int pre = 0, mine = 0;
-    long long own_at = 0, pre_at = 0, own_n = 0, pre_n = 0;
-    if (plan[kPlanTag] == (int)a.p.tag && plan[kPlanParts] > 0 && row < plan[kPlanRows]) {
-        const int s = plan[a.p.session_at + row];
-        const int32_t* m = plan + a.p.merge_at + (long long)s * kMergeInts;
-        pre = m[0];
-        mine = m[4];
-        const long long r = fr - (long long)m[7] * H;
-        own_at = m[5] + r;
-        pre_at = m[1] + m[3] + r;
-        own_n = m[6];
-        pre_n = m[2];
-    }
+    // A row's entry is read with the plan's head, not behind it, and dropped if that does not fit.
+    const i32x4* entry = reinterpret_cast<const i32x4*>(
+        plan + a.p.merge_at + (long long)min(row, a.p.rows - 1) * kMergeInts);
+    const i32x4 m0 = entry[0], m1 = entry[1];
+    const int tag = plan[kPlanTag], all = plan[kPlanParts], rows = plan[kPlanRows];
+    const bool some = tag == (int)a.p.tag && all > 0 && row < rows;
+    const int pre = some ? m0[0] : 0, mine = some ? m0[1] : 0, head = (int)(fr - (long long)row * H);
+    const long long pre_at = m0[2] + head, own_at = m0[3] + head, pre_n = m1[0], own_n = m1[1];
     const int parts = pre + mine;  // 0: no such row, or one job wrote it itself
     float M = -INFINITY, L = 0.0f;
     floatx4 o = {0, 0, 0, 0};

@@ -16,7 +16,10 @@ constexpr int kThreadsK = 256, kThreadsR = 512;
 constexpr int kTile = 32;    // keys of a unit
 constexpr int kJobInts = 8;  // segment (>= 0 session, ~group), first flat row, rows, first row's
                              // index in the segment, first key, last key + 1, ctx, partial row
+// A row's partials: how many of its prefix, of its own keys, the first of either (of its head 0), and
+// from one to the next of either.
 constexpr int kMergeInts = 8;
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kPlanHead = 64;  // words
 enum { kPlanStatus, kPlanBad, kPlanJobsK, kPlanJobsR, kPlanParts, kPlanRows, kPlanTag };
 
@@ -27,7 +30,7 @@ struct PlanShape {
     bool list_k_holds_all;       // list K has room for the segments of many rows, too
     int max_jobs_k, max_jobs_r;  // 0: no segment of these sizes can be on the list
     long long max_parts;         // (query, head) rows of partials
-    long long seg_at, merge_at, session_at, jobs_k_at, jobs_r_at, words;  // word offsets
+    long long seg_at, merge_at, jobs_k_at, jobs_r_at, words;  // word offsets
     uint32_t tag;
 };
 PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_len);
