@@ -10,7 +10,7 @@
 // (a wave alone is bound by its latencies).  So what counts is that the jobs fill one round or two
 // and not a little more, and that small batches are not cut finer than pays for the partial rows:
 // the length is the best of candidates between half and four times a slot's share.  (200 sessions
-// behind 5 prefixes, 8 heads, kv 128: 470 jobs in 17.3 us; 801 jobs, a share each, 18.4.)
+// behind 5 prefixes, 8 heads, kv 128: 470 jobs took 17.3 us, 801, a share each, 18.4.)
 // Whether segments of many rows go to list R or are taken apart for list K is decided by the same
 // estimate: list K costs more per row, but its jobs are small and there is one launch instead of
 // two.  (4 chunks of 509 rows, 8 heads, kv 128: list K 26.8 us, list R 36.)

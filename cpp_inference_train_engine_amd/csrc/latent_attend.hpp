@@ -24,12 +24,14 @@
 //
 // What bounds it, and what was measured (MI355X; a large copy reaches 4.8 TB/s there, a large bf16
 // product 1,350 TFLOP/s):
-//   kv 128, 8 heads, 64 sessions of 128 .. 4,096 tokens in 8 bits (23.7 MB): 8.8 us, of which 2 us
-//     are the launch and the rest three dependent trips to memory (job, page ids, unit) and the
-//     chain of the 3 units that a wave gets: latency.  9.8 us behind one 4,000-token prefix of 64
-//     sessions, 16 bits.
+//   kv 128, 8 heads, 64 sessions of 128 .. 4,096 tokens in 8 bits (23.7 MB): 8.2 us, of which 2.4
+//     us are the launch, 1.7 three dependent trips to memory (job, page ids, unit), 2.6 the chain of
+//     the 3 or 4 units that a wave gets, 0.8 the waves' merge and the stores: latency.  10.0 us
+//     for 64 sessions behind one 4,000-token prefix, 16 bits.
 //   kv 128, chunks of 509 rows: 27 us, 0.33 PFLOP/s.  List K fetches and converts every key for 16
-//     rows: 160 vector and 120 scalar instructions for a unit's 18 MFMAs; instruction issue.
+//     rows: 160 vector and 120 scalar instructions for a unit's 18 MFMAs.  Instruction issue while
+//     all jobs run (1.3 us a unit), latency when the shorter ones have ended (a job ends after 16
+//     us on the average, the last after 25).
 //   kv 512, 128 heads, list R: 64 decode rows over 534,000 8-bit tokens (149 GFLOP) 190-208 us with
 //     the merge, 0.72-0.78 PFLOP/s; 48 sessions behind an 8,191-token prefix, 16 bits (117 GFLOP),
 //     163-168 us, 0.70-0.72.  LDS: eight waves read each unit twice (scores, weighted sum), 550 KB

@@ -4,9 +4,10 @@
 // One thread per 4 columns of a row and each of GROUPS groups; the groups split the row's partials,
 // each reads kFlight of them at once (a round trip to memory is what a row costs, a partial's bytes
 // are few), and their states meet in LDS.
-// Bound by the trips to memory (the plan's head, the row's session, its ranges, the partials) where
-// rows are few: 3.3-5.5 us for 4,000 to 10,000 partial rows of 128 columns; by HBM where they
-// are many: 32,512 partial rows of 512 columns into 8,192 rows 15.5 us, 4.8 TB/s, the rate of a copy.
+// Bound by the launch and two trips to memory (the plan's head with the row's ranges, the partials)
+// where rows are few: 3.6-4.2 us for up to 6,400 partial rows of 128 columns (the ranges by session,
+// a trip more, 4.0-4.6); by HBM where they are many: 32,512 partial rows of 512 columns into 8,192
+// rows 14.3 us, 5.2 TB/s, more than a large copy's rate.
 #include "mla_latent.hpp"
 #include "mla_common.hpp"
 
