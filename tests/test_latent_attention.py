@@ -465,6 +465,41 @@ def test_a_graph_that_plans_a_growing_batch(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+def test_pages_past_32_bit_offsets(gpu, q8):
+    """A session on the last pages of a pool of more than 4 GiB, and a prefix there, give the bits
+    that the same contents give on its first pages; read back too."""
+    import torch
+    H, kv, rope, page, n = 16, 512, 64, 64, 300
+    P = (1 << 32) // (page * ((kv + 2 * rope + kv // 32) if q8 else 2 * (kv + rope))) + 40
+    _say(f"a pool of {P} pages q8={q8}")
+    cache = (gpu.QuantizedLatentCache if q8 else gpu.PagedLatentCache)(1, P, page, kv, rope)
+    append = gpu.append_latent_q8 if q8 else gpu.append_latent
+    i32 = lambda x: torch.tensor(np.asarray(x, np.int64).astype(np.int32), device="cuda")
+    torch.manual_seed(18)
+    x, key = torch.randn(n, kv, device="cuda"), torch.randn(n, rope, device="cuda")
+    lists = [np.arange(5), P - 1 - np.arange(5)]
+    t = np.arange(n)
+    for l in lists:
+        append(cache, 0, x, key, i32(l[t // page] * page + t % page))
+    if q8:
+        got = [gpu.read_latent_q8(cache, 0, i32(l[t // page] * page + t % page)) for l in lists]
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+        assert (got[0][0].float() - x).abs().max() < 0.5  # e4m3 of |x| < 8
+    ql = torch.randn(1, H, kv, device="cuda").half().repeat(2, 1, 1)
+    qr = torch.randn(1, H, rope, device="cuda").half().repeat(2, 1, 1)
+    batch = gpu.build_metadata(i32([n - 1] * 2), i32([1, 1]), i32([0, 5, 10]),
+                               i32(np.concatenate(lists)), page, 5, P, max_rows=2)
+    shared = gpu.SharedPrefixes(i32([0, 1, 2]), i32([n, n]), i32([0, 5, 10]),
+                                i32(np.concatenate(lists)))
+    for prefixes in (None, shared):
+        plan = gpu.plan_attention(batch, H, kv, rows=2, prefixes=prefixes)
+        plan.read_info()
+        out = gpu.latent_attention(plan, cache.layer(0), ql, qr, 0.05, rope_dim=rope, q8=q8)
+        assert torch.equal(out[0], out[1]) and out.isfinite().all() and (out != 0).any()
+
+
+@pytest.mark.gpu
 def test_tensors_made_by_a_call_belong_to_its_stream(gpu):
     """Without out and workspace, on a stream that is not the current one: what the call makes is
     filled before its kernels run, however far behind the current stream is."""
