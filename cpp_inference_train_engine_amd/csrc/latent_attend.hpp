@@ -18,9 +18,8 @@
 //     S^T = K . Q^T     v_mfma_f32_16x16x32, Q^T in registers for the whole job; list K's keys
 //                       come from the registers that they were loaded into, list R's from LDS
 //     online softmax    log2 domain in 32 bits, the reference maximum raised lazily
-//     O^T += C^T . P^T  C^T by transpose reads (ds_read_b64_tr_b16); P^T rounded to the 16-bit type
-//                       of the cache: the row is a weighted mean whose weights are off by half a
-//                       step of that type each, and is itself rounded to it in the end
+//     O^T += C^T . P^T  C^T by transpose reads (ds_read_b64_tr_b16); P^T in two 16-bit parts
+//                       (see finish_unit)
 //
 // What bounds it, and what was measured (MI355X; a large copy reaches 4.8 TB/s there, a large bf16
 // product 1,350 TFLOP/s):
@@ -598,15 +597,20 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
             m_run = m_new;
         }
         const float m_ref = m_run == -INFINITY ? 0.0f : m_run;
+        // A weight enters the product as two parts of the 16-bit type, e = hi + lo, off by 2^-17 of
+        // it (bf16) or 2^-23 (fp16) at most: as one part it would be off by up to 2^-8 or 2^-11, all
+        // weights of keys of one score the same way, while the mass sums them in 32 bits.
         float psum = 0.0f;
-        V8 pb;
+        V8 pb, pl;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(sc[tt][i], a.scale_log2, -m_ref));
                 psum += e;
-                pb[4 * tt + i] = static_cast<typename T::scalar>(e);
+                const auto hi = static_cast<typename T::scalar>(e);
+                pb[4 * tt + i] = hi;
+                pl[4 * tt + i] = static_cast<typename T::scalar>(e - static_cast<float>(hi));
             }
         l_run += psum;
 #pragma unroll
@@ -614,6 +618,8 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
             if (k < ks) {
                 acc[2 * k] = T::mma32(cring[k % AHEAD][0], pb, acc[2 * k]);
                 acc[2 * k + 1] = T::mma32(cring[k % AHEAD][1], pb, acc[2 * k + 1]);
+                acc[2 * k] = T::mma32(cring[k % AHEAD][0], pl, acc[2 * k]);
+                acc[2 * k + 1] = T::mma32(cring[k % AHEAD][1], pl, acc[2 * k + 1]);
                 if (k + AHEAD < ks) {
                     cring[k % AHEAD][0] = c_operand(2 * (k + AHEAD));
                     cring[k % AHEAD][1] = c_operand(2 * (k + AHEAD) + 1);

@@ -361,8 +361,8 @@ int mla_read_latent_q8(void* stream, int T, int kv_rank, int rope_dim, int page_
  *     out[h] = sum_j softmax(s)_j c_j,   lse[h] = ln(sum_j exp(s_j)):
  * mla_decode_attention and mla_prefill_attention of the concatenated cache (the reference's
  * src/infer/inference.cpp:116-153 and src/model/ops.cpp:109-142).  `out` holds 16-bit words of
- * `dtype`, as the queries do: sums, maxima and masses are fp32, the softmax weights are rounded to
- * `dtype` where they enter the product, and the row once at the end.
+ * `dtype`, as the queries do: sums, maxima and masses are fp32, a softmax weight enters the product
+ * as the sum of two values of `dtype` (within 2^-17 of it), and the row is rounded once at the end.
  *
  * The plan says which workgroup takes which rows over which keys, and what is added up in the end.
  * It is built on the device from one mla_build_metadata call's cu_seqlens_q, cu_seqlens_k and
