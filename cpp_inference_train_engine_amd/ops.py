@@ -401,7 +401,9 @@ class SharedPrefixes:
 
 
 class AttentionPlan:
-    """What ``plan_attention`` built, for ``latent_attention`` calls over the same batch."""
+    """What ``plan_attention`` built, for ``latent_attention`` calls over the same batch.  It keeps
+    the tensors and sizes that it was made of: setting a field of the batch or of the prefixes
+    later changes nothing for its calls."""
 
     def __init__(self, batch: RaggedBatch, n_heads: int, kv_rank: int, rows: int, max_q_len: int,
                  prefixes: SharedPrefixes | None, words):
@@ -410,10 +412,14 @@ class AttentionPlan:
         self.words = words  # the plan itself (device int32)
         self.n_groups = prefixes.n_groups if prefixes is not None else 0
         self.info = None    # host copy of its info once read_info has been called
-        # the arguments of a call that are the plan's
+        # the arguments of a call that are the plan's: sizes, and addresses with their tensors
+        self._B, self._page_size = batch.B, batch.page_size
+        self._max_pages, self._pool_pages = batch.max_pages, batch.num_pool_pages
+        lists = (prefixes.cu_pages, prefixes.page_ids) if self.n_groups else (None, None)
+        self._tensors = (batch.page_table, *lists, words)
+        self._device = words.device
         self._table = ptr(batch.page_table)
-        self._shared = ((ptr(prefixes.cu_pages), ptr(prefixes.page_ids)) if self.n_groups else
-                        (None, None))
+        self._shared = (ptr(lists[0]), ptr(lists[1]))
         self._words = (ptr(words), 4 * words.numel())
         self._records = {}
 
@@ -421,7 +427,7 @@ class AttentionPlan:
         """Bytes of an 8-bit page record, or 16-bit words of a 16-bit one."""
         n = self._records.get((rope_dim, q8))
         if n is None:
-            page = self.batch.page_size
+            page = self._page_size
             n = (int(lib().mla_q8_page_bytes(page, self.kv_rank, rope_dim)) if q8 else
                  page * (self.kv_rank + rope_dim))
             self._records[rope_dim, q8] = n
@@ -476,9 +482,9 @@ def attention_workspace(plan: AttentionPlan):
     """Workspace of ``latent_attention`` calls with this plan (or one of the same sizes).  Calls
     that share one are ordered on one stream."""
     torch = _torch()
-    n = int(lib().mla_attention_workspace_bytes(plan.batch.B, plan.rows, plan.n_heads,
-                                                plan.kv_rank, plan.max_q_len, plan.n_groups))
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=plan.words.device)
+    n = int(lib().mla_attention_workspace_bytes(plan._B, plan.rows, plan.n_heads, plan.kv_rank,
+                                                plan.max_q_len, plan.n_groups))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=plan._device)
 
 
 def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float, *,
@@ -490,7 +496,7 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
     [rows, H, kv_rank] in ``dtype`` (and fills lse [rows, H], fp32, if given).  Rows past the
     batch's are left as they were."""
     torch, gpu = _torch(), _gpu()
-    b, rows, H, kv = plan.batch, plan.rows, plan.n_heads, plan.kv_rank
+    rows, H, kv = plan.rows, plan.n_heads, plan.kv_rank
     dt = torch.float16 if dtype == DTYPE_F16 else torch.bfloat16
     if out is None or workspace is None:
         with _allocating_on(stream):
@@ -499,9 +505,9 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
             if workspace is None:
                 workspace = attention_workspace(plan)
     check(lib().mla_latent_attention(
-        stream_handle(stream), b.B, rows, H, kv, rope_dim, b.page_size, plan.max_q_len, dtype,
-        CACHE_Q8 if q8 else CACHE_16BIT, scale, plan._table, b.max_pages, b.num_pool_pages,
-        _check("pages", pages, (b.num_pool_pages, plan.record_words(rope_dim, q8)),
+        stream_handle(stream), plan._B, rows, H, kv, rope_dim, plan._page_size, plan.max_q_len, dtype,
+        CACHE_Q8 if q8 else CACHE_16BIT, scale, plan._table, plan._max_pages, plan._pool_pages,
+        _check("pages", pages, (plan._pool_pages, plan.record_words(rope_dim, q8)),
                torch.uint8 if q8 else dt, gpu),
         _check("q_latent", q_latent, (rows, H, kv), dt, gpu),
         _check("q_rope", q_rope, (rows, H, rope_dim), dt, gpu),
