@@ -154,11 +154,12 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
 
     const table_ptr plan = table(a.plan);
     const table_ptr d = plan + (ROWS ? a.p.jobs_r_at : a.p.jobs_k_at) + (long long)blockIdx.x * kJobInts;
-    const int n_jobs = plan[ROWS ? kPlanJobsR : kPlanJobsK], tag = plan[kPlanTag];
+    const int jobs_k = plan[kPlanJobsK], jobs_r = plan[kPlanJobsR], parts = plan[kPlanParts],
+              tag = plan[kPlanTag];
     const int seg = d[0], f0 = d[1], n_rows = d[2], rb = d[3], key0 = d[4], key_end = d[5],
               ctx = d[6], part = d[7];
-    // no such job; or a plan for other sizes, or a failed one
-    if ((int)blockIdx.x >= n_jobs || tag != (int)a.p.tag)
+    // no such job; or a plan for other sizes, or a failed one, or not the build that the host knows
+    if ((int)blockIdx.x >= (ROWS ? jobs_r : jobs_k) || !plan_fits(a, tag, jobs_k, jobs_r, parts))
         return;
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;

@@ -226,15 +226,15 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
         return invalid(fn, "the plan was made for other sizes");
     a.jobs_k = a.p.max_jobs_k;
     a.jobs_r = a.p.max_jobs_r;
-    a.merge = true;
+    a.parts = -1;
     if (host_info) {
         if (host_info[kPlanTag] != (int)a.p.tag || host_info[kPlanJobsK] < 0 ||
             host_info[kPlanJobsK] > a.jobs_k || host_info[kPlanJobsR] < 0 ||
-            host_info[kPlanJobsR] > a.jobs_r)
+            host_info[kPlanJobsR] > a.jobs_r || host_info[kPlanParts] < 0)
             return invalid(fn, "host_info is not that of a plan for these sizes");
         a.jobs_k = host_info[kPlanJobsK];
         a.jobs_r = host_info[kPlanJobsR];
-        a.merge = host_info[kPlanParts] > 0;
+        a.parts = host_info[kPlanParts];
     }
     if (workspace_bytes < workspace_size(a.p))
         return invalid(fn, "workspace needs " + std::to_string(workspace_size(a.p)) + " bytes");

@@ -36,8 +36,9 @@ __global__ __launch_bounds__(kThreads) void latent_merge_kernel(LatentArgs a) {
     const i32x4* entry = reinterpret_cast<const i32x4*>(
         plan + a.p.merge_at + (long long)min(row, a.p.rows - 1) * kMergeInts);
     const i32x4 m0 = entry[0], m1 = entry[1];
-    const int tag = plan[kPlanTag], all = plan[kPlanParts], rows = plan[kPlanRows];
-    const bool some = tag == (int)a.p.tag && all > 0 && row < rows;
+    const int all = plan[kPlanParts], rows = plan[kPlanRows];
+    const bool some = plan_fits(a, plan[kPlanTag], plan[kPlanJobsK], plan[kPlanJobsR], all) &&
+                      all > 0 && row < rows;
     const int pre = some ? m0[0] : 0, mine = some ? m0[1] : 0, head = (int)(fr - (long long)row * H);
     const long long pre_at = m0[2] + head, own_at = m0[3] + head, pre_n = m1[0], own_n = m1[1];
     const int parts = pre + mine;  // 0: no such row, or one job wrote it itself
@@ -145,7 +146,7 @@ hipError_t launch_latent_attention(const LatentArgs& a, int dtype, hipStream_t s
         if (e != hipSuccess)
             return e;
     }
-    return a.merge ? launch_latent_merge(a, dtype, stream) : hipSuccess;
+    return a.parts != 0 ? launch_latent_merge(a, dtype, stream) : hipSuccess;
 }
 
 hipError_t launch_latent_merge(const LatentArgs& a, int dtype, hipStream_t stream) {

@@ -51,7 +51,7 @@ struct LatentArgs {
     int q8;
     uint32_t tpp_inverse, h_inverse;  // floor(2^32 / n) of a page's tiles and of H (2^32 - 1 for 1)
     int jobs_k, jobs_r;  // workgroups to launch: the plan's jobs, or as many as it could have
-    bool merge;          // there may be partial rows
+    int parts;           // the plan's partial rows, -1: not known (there may be some)
     float scale_log2;  // softmax scale * log2(e)
     const int32_t *plan, *page_table, *cu_prefix_pages, *prefix_page_ids;
     const uint8_t* pages;
@@ -59,6 +59,13 @@ struct LatentArgs {
     uint16_t* out;
     float *lse, *part_o, *part_ml;
 };
+// Whether the call is for this plan (its head): made for the same sizes, and where the host knows
+// its counts, with those.
+__host__ __device__ inline bool plan_fits(const LatentArgs& a, int tag, int jobs_k, int jobs_r,
+                                          int parts) {
+    return tag == (int)a.p.tag &&
+           (a.parts < 0 || (jobs_k == a.jobs_k && jobs_r == a.jobs_r && parts == a.parts));
+}
 hipError_t launch_latent_attention(const LatentArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_latent_merge(const LatentArgs& a, int dtype, hipStream_t stream);
 // The lists' kernels, one translation unit for each cache format (latent_attend_*.hip).

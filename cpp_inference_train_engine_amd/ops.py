@@ -436,16 +436,18 @@ class AttentionPlan:
     def read_info(self, stream=None):
         """Synchronise and return [jobs, 0, jobs of 16 rows, jobs of 128 rows, partial rows, query
         rows, ..]; raises when the batch or the prefixes are invalid.  Calls after it launch no
-        more workgroups than the plan has jobs; so it is not for a plan that a captured graph
-        builds anew at each replay, whose jobs change."""
+        more workgroups than the plan has jobs, unless the plan was made in a captured graph: each
+        replay builds that one anew, and its jobs change."""
         import numpy as np
         h = np.zeros(PLAN_INFO_INTS, np.int32)
         check(lib().mla_read_plan_info(stream_handle(stream), self._words[0], h.ctypes.data))
-        self.info = h
-        self._info = h.ctypes.data
+        if not self._captured:
+            self.info = h
+            self._info = h.ctypes.data
         return h.tolist()
 
     _info = None
+    _captured = False  # made in a captured graph
 
 
 def plan_attention(batch: RaggedBatch, n_heads: int, kv_rank: int, *, rows: int | None = None,
@@ -471,11 +473,14 @@ def plan_attention(batch: RaggedBatch, n_heads: int, kv_rank: int, *, rows: int 
     info = _check_list("batch", batch.info, gpu)
     with _allocating_on(stream):
         words = torch.empty(n // 4, dtype=torch.int32, device=batch.info.device)
+        captured = words.is_cuda and torch.cuda.is_current_stream_capturing()
     check(lib().mla_plan_attention(
         stream_handle(stream), batch.B, rows, n_heads, kv_rank, batch.page_size, max_q_len,
         ptr(batch.cu_seqlens_q), ptr(batch.cu_seqlens_k), info, groups, *shared,
         prefixes.page_ids.numel() if groups else 0, batch.num_pool_pages, ptr(words), n))
-    return AttentionPlan(batch, n_heads, kv_rank, rows, max_q_len, prefixes, words)
+    plan = AttentionPlan(batch, n_heads, kv_rank, rows, max_q_len, prefixes, words)
+    plan._captured = captured
+    return plan
 
 
 def attention_workspace(plan: AttentionPlan):

@@ -405,8 +405,8 @@ int mla_read_plan_info(void* stream, const void* plan, int32_t* host_info);
  * [rows x n_heads x kv_rank] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.
  * host_info is what mla_read_plan_info returned for this very plan, not built anew since, or NULL:
  * with it the call launches as many workgroups as the plan has jobs, without it as many as a plan
- * of these sizes can have, whose rest returns at once (a few us).  A captured graph that builds the
- * plan takes NULL.  Shapes as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace
+ * of these sizes can have, whose rest returns at once (a few us).  A call with the info of another
+ * build, whose counts differ, writes nothing.  A captured graph that builds the plan takes NULL.  Shapes as for the 8-bit cache; pages, q_latent, q_rope, plan, out and workspace
  * at multiples of 16 bytes.  The workspace needs no initialisation; calls that share one must be ordered on one
  * stream.  Page ids are those that mla_build_metadata and mla_plan_attention have checked.  A
  * non-finite latent makes the rows that see its key NaN, and no others. */

@@ -69,3 +69,73 @@ def test_a_plan_keeps_the_tensors_that_its_calls_read(recorded):
     for at in (11, 18, 19, 20):  # page table, prefix lists, plan
         assert first[at] == second[at] and first[at] in where
     assert first[5:14] == second[5:14]  # rope, page size, .., max_pages, pool pages
+
+
+def lengths_batch(gpu, ctx, per, page=64):
+    """(device lengths, function that builds their metadata): one row a session, ``per`` pages each."""
+    B = len(ctx)
+    i32 = lambda x: torch.tensor(np.asarray(x, np.int64).astype(np.int32), device="cuda")
+    lens, one, cu, ids = i32(ctx), i32([1] * B), i32(np.arange(B + 1) * per), i32(np.arange(B * per))
+    return lens, lambda: gpu.build_metadata(lens, one, cu, ids, page, per, B * per, split_pages=4,
+                                            max_work=4096, max_rows=B)
+
+
+@pytest.mark.gpu
+def test_info_of_a_plan_that_a_graph_builds_anew(gpu):
+    """read_info on such a plan says whether the last replay's was sound; calls after it, over a plan
+    that has grown since, lose no job."""
+    long, short = [4000, 3000, 2500, 3500], [5, 3, 60, 9]
+    lens, build = lengths_batch(gpu, long, 64)
+    torch.manual_seed(1)
+    pages = torch.randn((256, 64 * 144), device="cuda").half()
+    ql, qr = torch.randn((4, 8, 128), device="cuda").half(), torch.randn((4, 8, 16), device="cuda").half()
+    out = torch.zeros((4, 8, 128), device="cuda", dtype=torch.float16)
+    step = lambda plan, out, ws: gpu.latent_attention(plan, pages, ql, qr, 0.1, rope_dim=16, out=out,
+                                                      workspace=ws)
+    ws = gpu.attention_workspace(gpu.plan_attention(build(), 8, 128, rows=4, max_q_len=1))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = gpu.plan_attention(build(), 8, 128, rows=4, max_q_len=1)
+        step(plan, out, ws)
+    lens.copy_(torch.tensor(short))
+    graph.replay()
+    few = plan.read_info()
+    lens.copy_(torch.tensor(long))
+    graph.replay()
+    torch.cuda.synchronize()
+    want = out.clone()
+    again = step(plan, torch.full_like(out, 5.0), ws)
+    print("jobs", few, plan.read_info(), flush=True)
+    assert plan.read_info()[0] > few[0] and want.isfinite().all()
+    assert torch.equal(again, want)
+    lens.fill_(70 * 64)  # more than the page table holds: the build and the plan fail
+    graph.replay()
+    with pytest.raises(gpu.MlaError, match="metadata"):
+        plan.read_info()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,kv,rope", [(8, 128, 16), (128, 512, 64)])
+@pytest.mark.parametrize("first,then", [([5, 3], [4000, 3000]), ([4000, 3000], [5, 3])])
+def test_host_info_of_an_earlier_build_writes_nothing(gpu, H, kv, rope, first, then):
+    """Part of the jobs is never done: with the info of a build with other counts, none is."""
+    lens, build = lengths_batch(gpu, first, 64)
+    pages = torch.zeros((128, 64 * (kv + rope)), device="cuda", dtype=torch.float16)
+    ql = torch.zeros((2, H, kv), device="cuda", dtype=torch.float16)
+    qr = torch.zeros((2, H, rope), device="cuda", dtype=torch.float16)
+    out, lse = torch.full_like(ql, 5.0), torch.full((2, H), 5.0, device="cuda")
+    plan = gpu.plan_attention(build(), H, kv, rows=2, max_q_len=1)
+    old = plan.read_info()
+    call = lambda: gpu.latent_attention(plan, pages, ql, qr, 0.1, rope_dim=rope, out=out, lse=lse)
+    lens.copy_(torch.tensor(then))
+    b = build()
+    L = gpu.lib()
+    gpu.check(L.mla_plan_attention(gpu.stream_handle(), 2, 2, H, kv, 64, 1, b.cu_seqlens_q.data_ptr(),
+                                   b.cu_seqlens_k.data_ptr(), b.info.data_ptr(), 0, None, None, None,
+                                   None, 0, 128, *plan._words))
+    call()
+    assert (out == 5).all() and (lse == 5).all()
+    print("jobs", old, plan.read_info(), flush=True)
+    call()
+    assert (out == 0).all() and torch.allclose(lse, torch.tensor(then, device="cuda")[:, None].add(1).float().log())
