@@ -376,11 +376,14 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
     p.jobs_k_at = p.merge_at + (long long)rows * kMergeInts;
     p.jobs_r_at = p.jobs_k_at + (long long)p.max_jobs_k * kJobInts;
     p.words = p.jobs_r_at + (long long)p.max_jobs_r * kJobInts;
-    uint32_t h = 2166136261u;
-    for (const int v : {B, groups, rows, H, kv_rank, max_q_len})
-        h = (h ^ (uint32_t)v) * 16777619u;
-    p.tag = h | 1u;
     return p;
+}
+
+uint32_t plan_tag(const PlanShape& p, int page_size, bool prefix_pages) {
+    uint32_t h = 2166136261u;
+    for (const int v : {p.B, p.groups, p.rows, p.H, p.kv_rank, p.max_q_len, page_size, (int)prefix_pages})
+        h = (h ^ (uint32_t)v) * 16777619u;
+    return h | 1u;
 }
 
 hipError_t launch_plan(const PlanArgs& a, hipStream_t stream) {

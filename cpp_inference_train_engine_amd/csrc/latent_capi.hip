@@ -156,6 +156,7 @@ int mla_plan_attention(void* stream, int B, int rows, int n_heads, int kv_rank, 
         return invalid(fn, "null buffer");
     PlanArgs a{};
     a.p = plan_shape(B, n_groups, rows, n_heads, kv_rank, max_q_len);
+    a.p.tag = plan_tag(a.p, page_size, n_groups > 0 && prefix_page_ids);
     const size_t need = (size_t)a.p.words * sizeof(int32_t);
     if (plan_bytes < need || misaligned({plan}))
         return invalid(fn, "the plan needs " + std::to_string(need) +
@@ -222,6 +223,7 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
                            "of 16 bytes");
     LatentArgs a{};
     a.p = plan_shape(B, n_groups, rows, n_heads, kv_rank, max_q_len);
+    a.p.tag = plan_tag(a.p, page_size, n_groups > 0 && prefix_page_ids);
     if (plan_bytes < (size_t)a.p.words * sizeof(int32_t))
         return invalid(fn, "the plan was made for other sizes");
     a.jobs_k = a.p.max_jobs_k;

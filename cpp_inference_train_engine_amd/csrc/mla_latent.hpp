@@ -31,9 +31,12 @@ struct PlanShape {
     int max_jobs_k, max_jobs_r;  // 0: no segment of these sizes can be on the list
     long long max_parts;         // (query, head) rows of partials
     long long seg_at, merge_at, jobs_k_at, jobs_r_at, words;  // word offsets
-    uint32_t tag;
+    uint32_t tag;  // plan_tag
 };
 PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_len);
+// What a plan and its calls have to agree on: the sizes, the page size (page lists are indexed by
+// it), and whether there is a list of prefix pages to index.
+uint32_t plan_tag(const PlanShape& p, int page_size, bool prefix_pages);
 
 struct PlanArgs {
     PlanShape p;

@@ -368,8 +368,9 @@ int mla_read_latent_q8(void* stream, int T, int kv_rank, int rope_dim, int page_
  * It is built on the device from one mla_build_metadata call's cu_seqlens_q, cu_seqlens_k and
  * info, once for a batch, and serves any number of calls (all layers of a step).  Plan and calls
  * take the same B, rows (the rows of q_latent; at least the batch's, rows past those are left as
- * they were), n_heads, kv_rank, max_q_len (at least every session's q_len) and n_groups; a call
- * with a plan made for others writes nothing.
+ * they were), n_heads, kv_rank, page_size, max_q_len (at least every session's q_len), n_groups and
+ * prefix lists (prefix_page_ids NULL in both or in neither); a call with a plan made for others
+ * writes nothing.  The pool of a call has at least the pages that plan and metadata were given.
  *
  * Shared prefixes: group g is the sessions [cu_groups[g], cu_groups[g+1]) (n_groups <= B; sessions
  * outside every group have no prefix); its prefix is prefix_len[g] tokens on the pool's pages

@@ -139,3 +139,38 @@ def test_host_info_of_an_earlier_build_writes_nothing(gpu, H, kv, rope, first, t
     print("jobs", old, plan.read_info(), flush=True)
     call()
     assert (out == 0).all() and torch.allclose(lse, torch.tensor(then, device="cuda")[:, None].add(1).float().log())
+
+
+@pytest.mark.gpu
+def test_a_plan_for_another_page_size_or_without_its_prefix_pages_writes_nothing(gpu):
+    """A page list would be indexed past its end, or where there is none."""
+    lens, build = lengths_batch(gpu, [40, 100], 4)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    b, shared = build(), gpu.SharedPrefixes(i32(0, 2), i32(100), i32(0, 2), i32(6, 7))
+    plan = gpu.plan_attention(b, 8, 128, rows=2, max_q_len=1, prefixes=shared)
+    info = np.array(plan.read_info(), np.int32)
+    pages = torch.zeros((8, 64 * 144), device="cuda", dtype=torch.float16)
+    ql = torch.zeros((2, 8, 128), device="cuda", dtype=torch.float16)
+    qr = torch.zeros((2, 8, 16), device="cuda", dtype=torch.float16)
+    ws = gpu.attention_workspace(plan)
+
+    def call(page=64, ids=shared.page_ids.data_ptr(), host=None):
+        out = torch.full_like(ql, 5.0)
+        status = gpu.lib().mla_latent_attention(
+            gpu.stream_handle(), 2, 2, 8, 128, 16, page, 1, 0, 0, 0.1, b.page_table.data_ptr(), 4, 8,
+            pages.data_ptr(), ql.data_ptr(), qr.data_ptr(), 1, shared.cu_pages.data_ptr(), ids,
+            *plan._words, host, out.data_ptr(), None, ws.data_ptr(), ws.numel())
+        return status, out.cpu()
+
+    for host in (None, info.ctypes.data):
+        status, out = call(host=host)
+        assert status == 0 and (out == 0).all()
+    for kw in (dict(page=16), dict(page=128), dict(ids=None)):
+        status, out = call(**kw)
+        assert status == 0 and (out == 5).all(), kw
+        status, out = call(**kw, host=info.ctypes.data)
+        assert status == 1 and (out == 5).all(), kw
+    none = gpu.SharedPrefixes(i32(0, 2), i32(0), i32(0, 0), i32())  # a group without a prefix
+    plan = gpu.plan_attention(b, 8, 128, rows=2, max_q_len=1, prefixes=none)
+    out = gpu.latent_attention(plan, pages, ql, qr, 0.1, rope_dim=16, out=torch.full_like(ql, 5.0))
+    assert plan.read_info()[0] > 0 and (out == 0).all()
