@@ -451,13 +451,16 @@ class AttentionPlan:
 
 
 def plan_attention(batch: RaggedBatch, n_heads: int, kv_rank: int, *, rows: int | None = None,
-                   max_q_len: int = 1, prefixes: SharedPrefixes | None = None,
+                   max_q_len: int | None = None, prefixes: SharedPrefixes | None = None,
                    stream=None) -> AttentionPlan:
     """(e) Plan the attention of a batch (one launch): which workgroup takes which query rows over
     which keys.  ``rows``: query rows of the calls (default the batch's max_rows); ``max_q_len``:
-    at least every session's q_len.  The plan serves every layer's ``latent_attention``."""
+    at least every session's q_len (default ``rows``; a tighter bound makes a smaller plan, and
+    calls without ``read_info`` launch fewer workgroups).  The plan serves every layer's
+    ``latent_attention``."""
     torch, gpu = _torch(), _gpu()
     rows = batch.max_rows if rows is None else rows
+    max_q_len = max(rows, 1) if max_q_len is None else max_q_len
     groups, shared = 0, (None, None, None, None)
     if prefixes is not None:
         x = prefixes

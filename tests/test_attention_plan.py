@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import cpp_inference_train_engine_amd as mla
+from test_latent_attention import call, check, device, make
 
 
 class Recorder:
@@ -174,3 +175,23 @@ def test_a_plan_for_another_page_size_or_without_its_prefix_pages_writes_nothing
     plan = gpu.plan_attention(b, 8, 128, rows=2, max_q_len=1, prefixes=none)
     out = gpu.latent_attention(plan, pages, ql, qr, 0.1, rope_dim=16, out=torch.full_like(ql, 5.0))
     assert plan.read_info()[0] > 0 and (out == 0).all()
+
+
+def test_max_q_len_left_out_covers_every_session(recorded):
+    for rows, want in ((5, 5), (None, 7), (0, 1)):
+        plan = mla.plan_attention(small_batch(rows=7), 8, 128, rows=rows)
+        assert recorded.calls[-1][1][6] == plan.max_q_len == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [[], [(2, 100)]])
+def test_a_plan_without_max_q_len(gpu, groups):
+    """The rows are those of a plan that was told the largest q_len; left out, one row a session
+    was assumed, and a session with more made every row of the batch zero."""
+    c = make(8, 128, 16, 64, 0, False, [(40, 1), (100, 3), (7, 20)], groups, seed=3)
+    d = device(gpu, c)
+    _, want, lse = call(gpu, c, d)
+    check(c, want, lse)
+    plan = gpu.plan_attention(d["batch"], 8, 128, prefixes=d["shared"])
+    out = gpu.latent_attention(plan, d["pages"], d["ql"], d["qr"], c.scale, rope_dim=16)
+    assert torch.equal(out, want)
