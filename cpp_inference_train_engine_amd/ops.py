@@ -417,7 +417,7 @@ class AttentionPlan:
         self._max_pages, self._pool_pages = batch.max_pages, batch.num_pool_pages
         lists = (prefixes.cu_pages, prefixes.page_ids) if self.n_groups else (None, None)
         self._tensors = (batch.page_table, *lists, words)
-        self._device = words.device
+        self._device, self._gpu = words.device, words.get_device()
         self._table = ptr(batch.page_table)
         self._shared = (ptr(lists[0]), ptr(lists[1]))
         self._words = (ptr(words), 4 * words.numel())
@@ -512,7 +512,7 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
                 out = torch.zeros((rows, H, kv), dtype=dt, device=q_latent.device)
             if workspace is None:
                 workspace = attention_workspace(plan)
-    check(lib().mla_latent_attention(
+    args = (
         stream_handle(stream), plan._B, rows, H, kv, rope_dim, plan._page_size, plan.max_q_len, dtype,
         CACHE_Q8 if q8 else CACHE_16BIT, scale, plan._table, plan._max_pages, plan._pool_pages,
         _check("pages", pages, (plan._pool_pages, plan.record_words(rope_dim, q8)),
@@ -522,7 +522,10 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
         plan.n_groups, *plan._shared, *plan._words, plan._info,
         _check("out", out, (rows, H, kv), dt, gpu),
         None if lse is None else _check("lse", lse, (rows, H), torch.float32, gpu),
-        _check("workspace", workspace, (workspace.numel(),), torch.uint8, gpu), workspace.numel()))
+        _check("workspace", workspace, (workspace.numel(),), torch.uint8, gpu), workspace.numel())
+    if plan._gpu != gpu:
+        raise ValueError(f"plan: wanted on the current GPU, is on {plan._device}")
+    check(lib().mla_latent_attention(*args))
     return out
 
 

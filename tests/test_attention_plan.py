@@ -195,3 +195,14 @@ def test_a_plan_without_max_q_len(gpu, groups):
     plan = gpu.plan_attention(d["batch"], 8, 128, prefixes=d["shared"])
     out = gpu.latent_attention(plan, d["pages"], d["ql"], d["qr"], c.scale, rope_dim=16)
     assert torch.equal(out, want)
+
+
+def test_a_plan_of_another_gpu_is_refused(recorded, monkeypatch):
+    """The plan, the page table and the prefixes would be read from another GPU's memory."""
+    plan = mla.plan_attention(small_batch(), 8, 128, rows=2, max_q_len=1)
+    attend(plan)
+    monkeypatch.setattr(mla.ops, "_gpu", lambda: 1)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1)
+    with pytest.raises(ValueError, match="plan: wanted on the current GPU"):
+        attend(plan)
+    assert len(recorded.calls) == 2
