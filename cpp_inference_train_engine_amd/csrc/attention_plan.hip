@@ -81,6 +81,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     __shared__ int32_t lds[ON_CHIP ? kTables * kLdsSegs : 1];
     __shared__ int tmp[kWaves][3];
     __shared__ unsigned long long best[3], tile_sum[3];
+    __shared__ int listed[2];  // the prefix pages that groups list: first, behind the last
     __shared__ int first_bad, tries[3][3 * kTries];  // jobs, their partial rows' blocks, the longest
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PlanShape& p = a.p;
@@ -98,6 +99,8 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
 
     // ---- checks and the segments' sizes ----
     const int total_q = a.info[0] < 0 ? -1 : a.cu_q[B];
+    if (tid < 2)
+        listed[tid] = tid == 0 ? a.n_prefix_pages : 0;
     if (tid == 0)
         first_bad = total_q < 0 || total_q > p.rows ? -1 : 0x7fffffff;
     if (tid < 3) {
@@ -118,6 +121,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
                 const int c0 = a.cu_prefix_pages[i], c1 = a.cu_prefix_pages[i + 1];
                 ok = s0 >= 0 && s1 >= s0 && s1 <= B && n >= 0 && c0 >= 0 && c1 >= c0 &&
                      c1 <= a.n_prefix_pages && (long long)(c1 - c0) * a.page_size >= n;
+                if (ok && c1 > c0) {
+                    atomicMin(&listed[0], c0);
+                    atomicMax(&listed[1], c1);
+                }
             } else {
                 s0 = i - G;
                 s1 = s0 + 1;
@@ -131,11 +138,17 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             keys[i] = n;
             group[i] = -1;
         }
-        for (int i = tid; i < a.n_prefix_pages; i += kThreads)
+        // Only ids that some group lists count.  (Behind the lists there may be anything, -1 in a
+        // buffer of fixed length: a bad id costs a pass over the groups, 2.4 ms for 65,536 behind
+        // 200 groups.)
+        __syncthreads();
+        for (long long i = listed[0] + (long long)tid; i < listed[1]; i += kThreads)
             if ((unsigned)a.prefix_page_ids[i] >= (unsigned)a.num_pool_pages)
-                for (int g = 0; g < G; ++g)  // only ids that some group lists count
-                    if (a.cu_prefix_pages[g] <= i && i < a.cu_prefix_pages[g + 1])
+                for (int g = 0; g < G; ++g)
+                    if (a.cu_prefix_pages[g] <= i && i < a.cu_prefix_pages[g + 1]) {
                         atomicMin(&first_bad, g);
+                        break;
+                    }
     }
     __syncthreads();
     if (first_bad != 0x7fffffff) {

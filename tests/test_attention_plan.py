@@ -206,3 +206,39 @@ def test_a_plan_of_another_gpu_is_refused(recorded, monkeypatch):
     with pytest.raises(ValueError, match="plan: wanted on the current GPU"):
         attend(plan)
     assert len(recorded.calls) == 2
+
+
+@pytest.mark.gpu
+def test_page_ids_behind_the_prefix_lists_are_not_looked_at(gpu):
+    """A list buffer of fixed length ends in ids that no group lists.  They made the plan of 200
+    groups 65 times as long: it may take twice as long now, and a bad id that a group lists counts."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    _, build = lengths_batch(gpu, [100] * 200, 2)
+    b = build()
+
+    def timed(ids):
+        p = gpu.SharedPrefixes(i32(range(201)), i32([100] * 200), i32(range(0, 401, 2)), i32(ids))
+        make = lambda: gpu.plan_attention(b, 8, 128, rows=200, max_q_len=1, prefixes=p)
+        make()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan = make()
+        e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        times = []
+        for _ in range(9):
+            e[0].record()
+            graph.replay()
+            e[1].record()
+            torch.cuda.synchronize()
+            times.append(e[0].elapsed_time(e[1]) * 1e3)
+        return plan, sorted(times)[4]
+
+    ids = list(range(400))
+    (plan, alone), (padded, behind) = timed(ids), timed(ids + [-1] * 65536)
+    print(f"plan {alone:.1f} us, with ids behind the lists {behind:.1f}", flush=True)
+    assert padded.read_info() == plan.read_info()
+    assert behind < 2 * alone
+    ids[317] = -1
+    with pytest.raises(gpu.MlaError, match="entry 158"):
+        timed(ids + [-1] * 10)[0].read_info()
