@@ -14,7 +14,7 @@
 // Whether segments of many rows go to list R or are taken apart for list K is decided by the same
 // estimate: list K costs more per row, but its jobs are small and there is one launch instead of
 // two.  (4 chunks of 509 rows, 8 heads, kv 128: list K 26.8 us, list R 36.)
-// The kernel is a chain of short phases of one workgroup: 11 us for one session, 23 for 200 with
+// The kernel is a chain of short phases of one workgroup: 10 us for one session, 24 for 200 with
 // prefixes.  Two things cost it most and were taken out: 64-bit divisions, and sums across lanes
 // for each candidate where a lane can have a candidate of its own (16-31 us).  512 threads: twice
 // as many only wait longer at the barriers.
@@ -32,7 +32,10 @@ constexpr int kUnits = 256;     // compute units
 constexpr int kFewRows = 64;    // segments up to this go to list K in any case
 constexpr int kRounds = 2, kSteps = 8, kTries = (kRounds + 1) * kSteps;
 
-// Times in ns of a unit of 32 keys, by list, with all slots taken, and of a job's start and end.
+// Times in ns of a unit of 32 keys, by list, with all slots taken, and of a job's start and end:
+// those of kv 128 (for up to 128) and 512 with fixed rope columns, and with the softmax weights in
+// one part, as the other times of jobs here.  (In two parts a unit takes 13-18 % longer.  With that in the table,
+// eleven batches at kv 128 to 512 got the same jobs.)
 struct Cost {
     int tile_k, job_k, tile_r, job_r, launch;
 };
@@ -360,7 +363,8 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
     p.max_q_len = max_q_len;
     const long long flat = (long long)rows * H;
     const long long own = std::min(flat, (long long)max_q_len * H);  // most rows of a session
-    // Workgroups that 256 compute units hold: by registers and LDS of the two lists' kernels.
+    // Workgroups that 256 compute units hold: by registers and LDS of the two lists' kernels with
+    // fixed rope columns.  (The others hold half as many of list K at kv 128.)
     p.slots_k = kv_rank <= 128 ? 1024 : kv_rank <= 256 ? 512 : 256;
     p.slots_r = kv_rank <= 128 ? 512 : 256;
     const bool few = H <= kFewRows, many = own > kFewRows || (groups > 0 && flat > kFewRows);

@@ -21,23 +21,28 @@
 //     O^T += C^T . P^T  C^T by transpose reads (ds_read_b64_tr_b16); P^T in two 16-bit parts
 //                       (see finish_unit)
 //
-// What bounds it, and what was measured (MI355X; a large copy reaches 4.8 TB/s there, a large bf16
-// product 1,350 TFLOP/s):
-//   kv 128, 8 heads, 64 sessions of 128 .. 4,096 tokens in 8 bits (23.7 MB): 8.2 us, of which 2.4
-//     us are the launch, 1.7 three dependent trips to memory (job, page ids, unit), 2.6 the chain of
-//     the 3 or 4 units that a wave gets, 0.8 the waves' merge and the stores: latency.  10.0 us
+// What bounds it, and what was measured (MI355X, kernels in a trace; a large copy reaches 4.8 TB/s
+// there, a large bf16 product 1,350 TFLOP/s; operations of the formula, the second part of P^T not
+// counted):
+//   kv 128, 8 heads, 64 sessions of 128 .. 4,096 tokens in 8 bits (23.7 MB): 9.4 us: the launch,
+//     three dependent trips to memory (job, page ids, unit), the chain of the 3 or 4 units that a
+//     wave gets, the waves' merge.  Latency: half of the waves' time is waiting for memory.  10.6 us
 //     for 64 sessions behind one 4,000-token prefix, 16 bits.
-//   kv 128, chunks of 509 rows: 27 us, 0.33 PFLOP/s.  List K fetches and converts every key for 16
-//     rows: 160 vector and 120 scalar instructions for a unit's 18 MFMAs.  Instruction issue while
-//     all jobs run (1.3 us a unit), latency when the shorter ones have ended (a job ends after 16
-//     us on the average, the last after 25).
-//   kv 512, 128 heads, list R: 64 decode rows over 534,000 8-bit tokens (149 GFLOP) 190-208 us with
-//     the merge, 0.72-0.78 PFLOP/s; 48 sessions behind an 8,191-token prefix, 16 bits (117 GFLOP),
-//     163-168 us, 0.70-0.72.  LDS: eight waves read each unit twice (scores, weighted sum), 550 KB
-//     a unit and CU, at 180 of the 200-220 bytes a clock that a loop of such reads alone reaches.
-//     Of the 205 us the weighted sum is 44, the scores 49, the staging 22, the barrier 8, Q^T from
-//     LDS 8, the merge 15.  32 rows a wave would halve the reads, and take 256 registers for O^T
-//     alone: at one wave a SIMD it spills 210 registers (940 us).
+//   kv 128, chunks of 509 rows: 30 us, 0.29 PFLOP/s.  List K fetches and converts every key for 16
+//     rows: 191 vector and 122 scalar instructions for a unit's 26 MFMAs.  37 % of the waves' time
+//     waits for issue, 29 % for memory.
+//   kv 512, 128 heads, list R: 64 decode rows over 534,000 8-bit tokens (149 GFLOP) 232-238 us with
+//     the merge, 0.63 PFLOP/s; 48 sessions behind an 8,191-token prefix, 16 bits (117 GFLOP),
+//     192-195 us, 0.60.  Over the whole dispatch the matrix cores are busy 42 and 38 % of the time,
+//     LDS 36 and 33 % (eight waves read each unit twice, for the scores and for the weighted sum):
+//     neither is full, a unit's phases follow one another in a wave, and with two waves a SIMD
+//     little else is there to run.  The longest job is 13-17 % above the mean.  32 rows a wave
+//     would halve the LDS reads, and take 256 registers for O^T alone: at one wave a SIMD it spilled
+//     210 registers (940 us).
+//   With P^T in one part (in error, see finish_unit): 8.2 us, 10.2, 26.7, 202 and 168.
+// Registers: of the instantiations for one shape, those over the 16-bit cache spill 3 to 35 (list K
+// at kv 512 the most); of the others, 8-bit list K 97-104 above kv 256 and 16 at kv 256, the rest
+// above kv 256 12 to 28.
 // A key past a row's position adds nothing to the row, whatever it holds: its rope key only enters
 // the score, which is replaced, and a non-finite latent is staged as zero with the key marked, and
 // makes the scores of the rows that see it NaN.  (Where every row of a job sees the key, such a

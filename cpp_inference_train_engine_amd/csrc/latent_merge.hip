@@ -5,9 +5,10 @@
 // each reads kFlight of them at once (a round trip to memory is what a row costs, a partial's bytes
 // are few), and their states meet in LDS.
 // Bound by the launch and two trips to memory (the plan's head with the row's ranges, the partials)
-// where rows are few: 3.6-4.2 us for up to 6,400 partial rows of 128 columns (the ranges by session,
-// a trip more, 4.0-4.6); by HBM where they are many: 32,512 partial rows of 512 columns into 8,192
-// rows 14.3 us, 5.2 TB/s, more than a large copy's rate.
+// where rows are few: 3.4-5.0 us for up to 6,400 partial rows of 128 columns; by its bytes where they
+// are many: 32,512 partial rows of 512 columns into 8,192 rows 14.2 us, 5.3 TB/s.  (That is more
+// than a copy from HBM reaches: the 67 MB were written just before and partly lie in the last
+// cache.)
 #include "mla_latent.hpp"
 #include "mla_common.hpp"
 
