@@ -364,7 +364,7 @@ PlanShape plan_shape(int B, int groups, int rows, int H, int kv_rank, int max_q_
     const long long flat = (long long)rows * H;
     const long long own = std::min(flat, (long long)max_q_len * H);  // most rows of a session
     // Workgroups that 256 compute units hold: by registers and LDS of the two lists' kernels with
-    // fixed rope columns.  (The others hold half as many of list K at kv 128.)
+    // fixed rope columns.  (The others hold half as many at kv 128.)
     p.slots_k = kv_rank <= 128 ? 1024 : kv_rank <= 256 ? 512 : 256;
     p.slots_r = kv_rank <= 128 ? 512 : 256;
     const bool few = H <= kFewRows, many = own > kFewRows || (groups > 0 && flat > kFewRows);

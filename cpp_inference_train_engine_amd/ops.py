@@ -437,7 +437,7 @@ class AttentionPlan:
         """Synchronise and return [jobs, 0, jobs of 16 rows, jobs of 128 rows, partial rows, query
         rows, ..]; raises when the batch or the prefixes are invalid.  Calls after it launch no
         more workgroups than the plan has jobs, unless the plan was made in a captured graph: each
-        replay builds that one anew, and its jobs change."""
+        replay builds that one anew, and its jobs change (before the first one it holds nothing)."""
         import numpy as np
         h = np.zeros(PLAN_INFO_INTS, np.int32)
         check(lib().mla_read_plan_info(stream_handle(stream), self._words[0], h.ctypes.data))
@@ -502,7 +502,8 @@ def latent_attention(plan: AttentionPlan, pages, q_latent, q_rope, scale: float,
     ``pages`` is a layer of a PagedLatentCache or, with ``q8``, of a QuantizedLatentCache.
     q_latent [rows, H, kv_rank] and q_rope [rows, H, rope_dim] in ``dtype``; returns out
     [rows, H, kv_rank] in ``dtype`` (and fills lse [rows, H], fp32, if given).  Rows past the
-    batch's are left as they were."""
+    batch's are left as they were, and over a failed plan (``AttentionPlan.read_info`` raises) all
+    of them: zero in a tensor that the call makes."""
     torch, gpu = _torch(), _gpu()
     rows, H, kv = plan.rows, plan.n_heads, plan.kv_rank
     dt = torch.float16 if dtype == DTYPE_F16 else torch.bfloat16
