@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(PKG, "libmla_hip.so")
 MLA_OK = 0
 ERROR_NAMES = {1: "invalid_argument", 2: "io_error", 3: "unsupported", 4: "out_of_memory",
                5: "gpu_error", 6: "numerical_error", 7: "unavailable"}
-DTYPE_F16, DTYPE_BF16 = 0, 1
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 WORK_DESC_INTS, WORK_PAGES, MAX_WORK, INFO_INTS = 8, 8, 65535, 8
 DECODE_FORCE_GENERIC = 1
 DECODE_FUSED_MERGE = 2
@@ -84,6 +84,18 @@ _SIGNATURES = {
     "mla_latent_attention": (C.c_int, [C.c_void_p] + [C.c_int] * 9 + [C.c_float, C.c_void_p] +
                              [C.c_int] * 2 + [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 3 +
                              [C.c_size_t] + [C.c_void_p] * 4 + [C.c_size_t]),
+    "mla_kv_page_words": (C.c_size_t, [C.c_int] * 4),
+    "mla_append_kv": (C.c_int, [C.c_void_p] + [C.c_int] * 8 +
+                      [C.c_void_p, C.c_longlong, C.c_longlong] * 3 + [C.c_void_p] * 2 +
+                      [C.c_int] * 3 + [C.c_void_p, C.c_int] + [C.c_void_p] * 2),
+    "mla_kv_plan_bytes": (C.c_size_t, [C.c_int] * 10),
+    "mla_kv_workspace_bytes": (C.c_size_t, [C.c_int] * 10),
+    "mla_plan_kv_attention": (C.c_int, [C.c_void_p] + [C.c_int] * 10 + [C.c_void_p] * 4 +
+                              [C.c_size_t]),
+    "mla_read_kv_plan_info": (C.c_int, [C.c_void_p] * 3),
+    "mla_kv_attention": (C.c_int, [C.c_void_p] + [C.c_int] * 11 + [C.c_float, C.c_void_p] +
+                         [C.c_int] * 2 + [C.c_void_p] * 3 + [C.c_size_t] + [C.c_void_p] * 4 +
+                         [C.c_size_t]),
     "mla_config_validate": (C.c_int, [C.c_void_p]),
     "mla_config_parameter_count": (C.c_size_t, [C.c_void_p]),
     "mla_model_create": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int,
@@ -212,6 +224,9 @@ from .ops import (  # noqa: E402  (re-exported operator interface)
     latent_attention, placed_work_slots, plan_attention, prefill_attention, read_latent_q8,
     xcd_count)
 from . import ops  # noqa: E402
+from .kv import (  # noqa: E402
+    KVAttentionPlan, PagedKVCache, Rotation, append_kv, kv_attention, kv_attention_workspace,
+    plan_kv_attention)
 
 from .model import (HipModel, ModelConfig, config_hash, config_parameter_count,  # noqa: E402
                     config_validate, read_export)
@@ -230,4 +245,5 @@ __all__ = ["MlaError", "lib", "check", "build_metadata", "append_latent", "decod
            "decode_workspace_bytes", "RaggedBatch", "PagedLatentCache", "DTYPE_F16",
            "DTYPE_BF16", "QuantizedLatentCache", "append_latent_q8", "read_latent_q8",
            "SharedPrefixes", "AttentionPlan", "plan_attention", "attention_workspace",
-           "latent_attention"]
+           "latent_attention", "PagedKVCache", "Rotation", "append_kv", "KVAttentionPlan",
+           "plan_kv_attention", "kv_attention_workspace", "kv_attention"]

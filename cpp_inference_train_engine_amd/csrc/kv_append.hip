@@ -1,0 +1,169 @@
+// The paged key-value cache's append: new tokens' keys, rotated by their positions, and values,
+// rounded to 16 bits, into their slots; the step's queries, rotated the same way, into rows of
+// their own.  No reference counterpart (its caches hold latents); the rotation is that of
+// src/model/ops.cpp:88-108, and with it the one over split halves.
+//   (a, b) of pair i at position p:  (a cos t - b sin t, a sin t + b cos t),  t = p f_i
+//
+// append_kv_kernel -- a workgroup takes a token: its threads turn the positions into rotations
+//   while the first rows are on their way, then each takes 8 columns of a head at a time.
+//   t is taken in 64 bits, in revolutions, and only the rest of the last one rounded to 32: at
+//   position 131,071 a 32-bit product would be off by up to 2^-8 rad.
+#include "mla_common.hpp"
+#include "mla_kv.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mla {
+namespace {
+
+constexpr int kMaxPairs = 128;  // dim <= 256
+typedef float f8 __attribute__((ext_vector_type(8)));
+
+struct F32Row {
+    using scalar = float;
+    __device__ static float to_float(float x) { return x; }
+};
+struct F16Row {
+    using scalar = uint16_t;
+    __device__ static float to_float(uint16_t x) { return F16::to_float(x); }
+};
+struct BF16Row {
+    using scalar = uint16_t;
+    __device__ static float to_float(uint16_t x) { return BF16::to_float(x); }
+};
+
+// Eight elements from p, 16-byte loads where WIDE.
+template <typename R, bool WIDE>
+__device__ __forceinline__ f8 load8(const typename R::scalar* p) {
+    f8 x;
+    if constexpr (!WIDE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] = R::to_float(p[i]);
+    } else if constexpr (sizeof(typename R::scalar) == 4) {
+        const floatx4 lo = *reinterpret_cast<const floatx4*>(p);
+        const floatx4 hi = *reinterpret_cast<const floatx4*>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = lo[i];
+            x[4 + i] = hi[i];
+        }
+    } else {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = R::to_float((uint16_t)v[i]);
+            x[2 * i + 1] = R::to_float((uint16_t)(v[i] >> 16));
+        }
+    }
+    return x;
+}
+
+template <typename T, typename R, bool WIDE>
+__global__ __launch_bounds__(256) void append_kv_kernel(KvAppendArgs a) {
+    __shared__ float2 turn[kMaxPairs];
+    const int tid = threadIdx.x;
+    const int qc = a.q ? a.heads * (a.dim / 8) : 0, kc = a.kv_heads * (a.dim / 8);
+    const int chunks = qc + kc + a.kv_heads * (a.v_dim / 8);
+    const long long rec = kv_record(a.kv_heads, a.page_size, a.dim, a.v_dim);
+    const int P = a.pairs, first = a.start, behind = a.start + 2 * P;
+
+    for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
+        if (P > 0) {
+            const double p = (double)a.positions[t];
+            __syncthreads();  // the token before has been turned
+            for (int i = tid; i < P; i += blockDim.x) {
+                const double r = p * a.frequencies[i] * 0.15915494309189533577;  // 1 / (2 pi)
+                float s, c;
+                sincospif((float)(2.0 * (r - rint(r))), &s, &c);
+                turn[i] = float2{c, s};
+            }
+            __syncthreads();
+        }
+        const int flat = a.slot_mapping[t];
+        const int page = flat / a.page_size, slot = flat - page * a.page_size;
+        const bool inside = flat >= 0 && page < a.num_pool_pages;
+        uint16_t* const record = a.pages + (inside ? page : 0) * rec;
+        for (int e = tid; e < chunks; e += blockDim.x) {
+            const bool is_q = e < qc, is_v = e >= qc + kc;
+            const int f = is_q ? e : is_v ? e - qc - kc : e - qc;
+            const int width = is_v ? a.v_dim : a.dim, per = width / 8;
+            const int h = f / per, c = (f - h * per) * 8;
+            const auto* src = static_cast<const typename R::scalar*>(is_q ? a.q : is_v ? a.v : a.k) +
+                              t * (is_q ? a.q_row : is_v ? a.v_row : a.k_row) +
+                              h * (is_q ? a.q_head : is_v ? a.v_head : a.k_head);
+            f8 x = load8<R, WIDE>(src + c);
+            if (!is_v && c + 8 > first && c < behind) {
+                if (a.adjacent) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const int j = c + i - first;
+                        if (j >= 0 && j < 2 * P) {
+                            const float2 w = turn[j >> 1];
+                            const float y = x[i], z = x[i + 1];
+                            x[i] = y * w.x - z * w.y;
+                            x[i + 1] = y * w.y + z * w.x;
+                        }
+                    }
+                } else if (WIDE) {  // the partners are one chunk, too
+                    const int j = c - first;
+                    const bool low = j < P;
+                    const f8 z = load8<R, true>(src + c + (low ? P : -P));
+                    const float2* w = turn + (low ? j : j - P);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        x[i] = low ? x[i] * w[i].x - z[i] * w[i].y : z[i] * w[i].y + x[i] * w[i].x;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int j = c + i - first;
+                        if (j >= 0 && j < 2 * P) {
+                            const bool low = j < P;
+                            const float z = R::to_float(src[c + i + (low ? P : -P)]);
+                            const float2 w = turn[low ? j : j - P];
+                            x[i] = low ? x[i] * w.x - z * w.y : z * w.y + x[i] * w.x;
+                        }
+                    }
+                }
+            }
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = T::from_float(x[2 * i]) | (uint32_t)T::from_float(x[2 * i + 1]) << 16;
+            if (is_q)
+                *reinterpret_cast<u32x4*>(a.q_out + ((long long)t * a.heads + h) * a.dim + c) = v;
+            else if (inside)
+                *reinterpret_cast<u32x4*>(
+                    record + (is_v ? (long long)a.kv_heads * a.page_size * a.dim : 0) +
+                    ((long long)h * a.page_size + slot) * width + c) = v;
+        }
+    }
+}
+
+template <typename T, typename R>
+hipError_t launch_rows(const KvAppendArgs& a, hipStream_t stream) {
+    const int chunks = (a.q ? a.heads * (a.dim / 8) : 0) + a.kv_heads * ((a.dim + a.v_dim) / 8);
+    const int threads = std::min(256, (chunks + 63) / 64 * 64);
+    const dim3 grid(std::min(a.T, 1 << 20));
+    if (a.wide)
+        hipLaunchKernelGGL((append_kv_kernel<T, R, true>), grid, dim3(threads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((append_kv_kernel<T, R, false>), grid, dim3(threads), 0, stream, a);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_type(const KvAppendArgs& a, int row_dtype, hipStream_t stream) {
+    return row_dtype == kKvF32 ? launch_rows<T, F32Row>(a, stream)
+           : row_dtype == 0     ? launch_rows<T, F16Row>(a, stream)
+                                : launch_rows<T, BF16Row>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_kv_append(const KvAppendArgs& a, int dtype, int row_dtype, hipStream_t stream) {
+    return dtype == 0 ? launch_type<F16>(a, row_dtype, stream) : launch_type<BF16>(a, row_dtype, stream);
+}
+
+}  // namespace mla

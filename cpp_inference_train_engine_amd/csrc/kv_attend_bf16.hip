@@ -1,0 +1,10 @@
+// bf16 instantiations of kv_attend.hpp.
+#include "kv_attend.hpp"
+
+namespace mla {
+
+hipError_t launch_kv_attend_bf16(const KvArgs& a, bool many, hipStream_t stream) {
+    return launch_list<BF16>(a, many, stream);
+}
+
+}  // namespace mla

@@ -1,0 +1,291 @@
+// The plan of mla_kv_attention: which workgroup takes which query rows over which keys, built on
+// the GPU once for a batch, a window and its sinks, and used by every such layer's call.  No
+// reference counterpart.
+//
+// One workgroup, its tables in LDS (in the plan for large batches).  A session's flat rows
+// (mla_kv.hpp) are cut into blocks, and the units of 32 keys that a block sees into ranges: of a
+// length that gives every slot of the GPU one range where there are fewer blocks than slots, and
+// of twice a slot's share (so that only blocks well above it are cut) where there are more.
+#include "mla_kv.hpp"
+
+#include <algorithm>
+#include <climits>
+
+namespace mla {
+namespace {
+
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kLdsBlocks = 2800, kLdsSessions = 1400;
+constexpr int kTables = 4, kTries = 24;
+constexpr int kMinF = 4, kMinM = 16;  // least units of a range
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
+
+// Inclusive scans of two counts over the workgroup; `total` receives the sums.
+__device__ void block_scan2(int (&v)[2], int (*tmp)[2], int (&total)[2]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = 1; d < 64; d <<= 1)
+        for (int k = 0; k < 2; ++k) {
+            const int u = __shfl_up(v[k], d, 64);
+            if (lane >= d)
+                v[k] += u;
+        }
+    __syncthreads();
+    if (lane == 63)
+        for (int k = 0; k < 2; ++k)
+            tmp[wave][k] = v[k];
+    __syncthreads();
+    for (int k = 0; k < 2; ++k) {
+        int before = 0;
+        total[k] = 0;
+        for (int w = 0; w < kWaves; ++w) {
+            const int x = tmp[w][k];
+            before += w < wave ? x : 0;
+            total[k] += x;
+        }
+        v[k] += before;
+    }
+}
+
+// The last of n starts that lies at or before i.
+__device__ __forceinline__ int find(const int32_t* starts, int n, int i) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= i)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+template <bool ON_CHIP>
+__global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
+    __shared__ int32_t lds[ON_CHIP ? kTables * kLdsBlocks + 2 * kLdsSessions : 1];
+    __shared__ int tmp[kWaves][2], tries[kTries], first_bad;
+    __shared__ unsigned long long sum;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const KvShape& p = a.p;
+    const int B = p.B, G = p.group, NB = p.max_blocks;
+    int32_t* const head = a.plan;
+    int32_t* t;
+    if constexpr (ON_CHIP)
+        t = lds;
+    else
+        t = a.plan + p.tables_at;
+    int32_t *const session = t, *const units = t + NB, *const job = t + 2LL * NB,
+            *const part = t + 3LL * NB, *const start = t + (long long)kTables * NB;
+
+    // ---- checks ----
+    const int total_q = a.info[0] < 0 ? -1 : a.cu_q[B];
+    if (tid == 0)
+        first_bad = total_q < 0 || total_q > p.rows ? -1 : INT_MAX;
+    __syncthreads();
+    if (first_bad != -1)
+        for (int s = tid; s < B; s += kThreads)
+            if (a.cu_q[s + 1] - a.cu_q[s] > p.max_q_len)
+                atomicMin(&first_bad, s);
+    __syncthreads();
+    if (first_bad != INT_MAX) {
+        if (tid < kKvHead)
+            head[tid] = tid == kKvStatus ? -1 : tid == kKvBad ? first_bad : 0;
+        return;
+    }
+
+    int jobs[2] = {0, 0}, parts = 0;
+    for (int list = 0; list < 2; ++list) {
+        const int per = list ? kv_many_rows(p.width) : kKvFewRows;
+        const int slots = list ? p.slots_m : p.slots_f;
+        const int most_jobs = list ? p.max_jobs_m : p.max_jobs_f;
+        if (most_jobs == 0)
+            continue;
+        auto flat = [&](int s) { return (a.cu_q[s + 1] - a.cu_q[s]) * G; };
+        // ---- the sessions' blocks ----
+        int blocks = 0;
+        for (int s0 = 0; s0 < B; s0 += kThreads) {
+            const int s = s0 + tid;
+            const int n = s < B ? flat(s) : 0;
+            const int mine = (n <= kKvFew) == (list == 0) ? ceil_div(n, per) : 0;
+            int v[2] = {mine, 0}, total[2];
+            block_scan2(v, tmp, total);
+            if (s < B)
+                start[s] = blocks + v[0] - mine;
+            blocks += total[0];
+        }
+        if (tid < kTries)
+            tries[tid] = 0;
+        if (tid == 0)
+            sum = 0;
+        __syncthreads();
+        // ---- the units that each sees ----
+        unsigned long long mine = 0;
+        for (int b = tid; b < blocks; b += kThreads) {
+            const int s = find(start, B, b), f0 = (b - start[s]) * per, n = flat(s);
+            const int keys = a.cu_k[s + 1] - a.cu_k[s], ctx = keys - n / G;
+            const int last = std::min(f0 + per, n) - 1;
+            session[b] = s;
+            units[b] = kv_units(ctx + f0 / G, ctx + last / G, p.window, p.sinks).count;
+            mine += units[b];
+        }
+        for (int d = 32; d > 0; d >>= 1)
+            mine += __shfl_xor(mine, d, 64);
+        if (lane == 0 && mine != 0)
+            atomicAdd(&sum, mine);
+        __syncthreads();
+        // ---- the length of a range ----
+        const int share = (int)std::min<unsigned long long>((sum + slots - 1) / slots, 1 << 26);
+        const int least = list ? kMinM : kMinF;
+        auto length = [&](int c) { return (std::max(share + (int)((long long)share * c / 8), least) + 3) & ~3; };
+        int len = length(8);
+        if (blocks <= slots) {
+            // the shortest candidate, from a slot's share on, whose ranges all run at once
+            if (lane < kTries) {
+                const float inv = 1.0f / (float)length(lane);
+                int n = 0;
+                for (int b = wave; b < blocks; b += kWaves)
+                    n += (int)__builtin_ceilf((float)units[b] * inv);
+                atomicAdd(&tries[lane], n);
+            }
+            __syncthreads();
+            int c = 0;
+            while (c < kTries - 1 && tries[c] > slots)
+                ++c;
+            len = length(c);
+        }
+        // ---- jobs and partial rows of each block ----
+        int at = 0;
+        for (int b0 = 0; b0 < blocks; b0 += kThreads) {
+            const int b = b0 + tid;
+            int n = 0, splits = 0, range = 0;
+            if (b < blocks) {
+                const int s = session[b];
+                n = std::min(per, flat(s) - (b - start[s]) * per);
+                splits = ceil_div(units[b], len);
+                range = (ceil_div(units[b], splits) + 3) & ~3;  // a block's ranges as even as they go
+                splits = ceil_div(units[b], range);
+            }
+            const int rows = splits > 1 ? n * splits : 0;
+            int v[2] = {splits, rows}, total[2];
+            block_scan2(v, tmp, total);
+            if (b < blocks) {
+                job[b] = at + v[0] - splits;
+                part[b] = rows > 0 ? parts + v[1] - rows : -1;
+                units[b] = range;  // (what a block sees is computed anew where it is needed)
+            }
+            at += total[0];
+            parts += total[1];
+        }
+        __syncthreads();
+        jobs[list] = at;
+        if (at > most_jobs || parts > p.max_parts)
+            break;  // (the bounds hold for every batch of these sizes: never)
+        // ---- the jobs, the last rows' first: a prompt's later blocks see more ----
+        int32_t* out = a.plan + (list ? p.jobs_m_at : p.jobs_f_at);
+        for (int j = tid; j < at; j += kThreads) {
+            const int b = find(job, blocks, j), s = session[b], range = units[b];
+            const int f0 = (b - start[s]) * per, n = flat(s), m = std::min(per, n - f0);
+            const int ctx = a.cu_k[s + 1] - a.cu_k[s] - n / G, sp = j - job[b];
+            const int seen = kv_units(ctx + f0 / G, ctx + (f0 + m - 1) / G, p.window, p.sinks).count;
+            int32_t* o = out + (long long)(at - 1 - j) * kKvJobInts;
+            o[0] = s;
+            o[1] = a.cu_q[s];
+            o[2] = f0;
+            o[3] = m;
+            o[4] = sp * range;
+            o[5] = std::min(seen, (sp + 1) * range);
+            o[6] = ctx;
+            o[7] = part[b] < 0 ? -1 : part[b] + sp * m;
+        }
+        // ---- what the merge adds up for each row ----
+        for (int e = tid >> 4; e < blocks; e += kThreads / 16) {
+            const int s = session[e], f0 = (e - start[s]) * per, n = flat(s), m = std::min(per, n - f0);
+            const int splits = part[e] < 0 ? 0 : (e + 1 < blocks ? job[e + 1] : at) - job[e];
+            for (int r = tid & 15; r < m; r += 16) {
+                int32_t* o = a.plan + p.rows_at +
+                             ((long long)a.cu_q[s] * G + f0 + r) * kKvRowInts;
+                o[0] = part[e] + r;
+                o[1] = splits;
+                o[2] = m;
+            }
+        }
+        __syncthreads();
+    }
+    const bool fits = jobs[0] <= p.max_jobs_f && jobs[1] <= p.max_jobs_m && parts <= p.max_parts;
+    if (tid < kKvHead) {
+        int v = 0;
+        if (fits)
+            v = tid == kKvStatus ? jobs[0] + jobs[1]
+                : tid == kKvJobsF ? jobs[0]
+                : tid == kKvJobsM ? jobs[1]
+                : tid == kKvParts ? parts
+                : tid == kKvRows  ? total_q
+                : tid == kKvTag   ? (int)p.tag
+                                  : 0;
+        else
+            v = tid == kKvStatus ? -1 : tid == kKvBad ? -2 : 0;
+        head[tid] = v;
+    }
+}
+
+}  // namespace
+
+KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int page_size,
+                 int max_q_len, int window, int sinks) {
+    KvShape p{};
+    p.B = B;
+    p.rows = rows;
+    p.H = H;
+    p.kv_heads = kv_heads;
+    p.group = H / kv_heads;
+    p.dim = dim;
+    p.v_dim = v_dim;
+    p.width = kv_width(dim, v_dim);
+    p.page_size = page_size;
+    p.max_q_len = max_q_len;
+    p.window = window;
+    p.sinks = sinks;
+    const long long flat = (long long)rows * p.group;  // of one kv head
+    const long long own = std::min(flat, (long long)max_q_len * p.group);
+    // Workgroups that 256 compute units hold.
+    const int at_once_f = p.width == 64 ? 1536 : p.width == 128 ? 768 : 512;
+    const int at_once_m = 512;
+    p.slots_f = std::max(1, at_once_f / kv_heads);
+    p.slots_m = std::max(1, at_once_m / kv_heads);
+    const int many = kv_many_rows(p.width);
+    const bool few = p.group <= kKvFew;
+    const long long blocks_f =
+        few ? std::min<long long>((long long)B * (kKvFew / kKvFewRows), flat / kKvFewRows + B) : 0;
+    const long long blocks_m =
+        own > kKvFew ? flat / many + std::min<long long>(B, flat / (kKvFew + 1)) : 0;
+    // A range is at least a slot's share long, so that a list's blocks have at most
+    // units / share + blocks <= slots + blocks ranges; those that are cut have fewer than twice
+    // units / share, of a block's rows each.
+    p.max_jobs_f = (int)std::min<long long>(blocks_f ? blocks_f + p.slots_f : 0, INT_MAX);
+    p.max_jobs_m = (int)std::min<long long>(blocks_m ? blocks_m + p.slots_m : 0, INT_MAX);
+    p.max_blocks = (int)std::min<long long>(std::max(blocks_f, blocks_m), INT_MAX);
+    p.max_parts = (p.max_jobs_f ? 2LL * p.slots_f * kKvFewRows : 0) +
+                  (p.max_jobs_m ? 2LL * p.slots_m * many : 0);
+    p.tables_at = kKvHead;
+    const bool on_chip = p.max_blocks <= kLdsBlocks && B <= kLdsSessions;
+    p.rows_at = p.tables_at +
+                (on_chip ? 0 : (((long long)p.max_blocks * kTables + B + 7) & ~7LL));
+    p.jobs_f_at = p.rows_at + flat * kKvRowInts;
+    p.jobs_m_at = p.jobs_f_at + (long long)p.max_jobs_f * kKvJobInts;
+    p.words = p.jobs_m_at + (long long)p.max_jobs_m * kKvJobInts;
+    uint32_t h = 2166136261u;
+    for (const int v : {B, rows, H, kv_heads, dim, v_dim, page_size, max_q_len, window, sinks})
+        h = (h ^ (uint32_t)v) * 16777619u;
+    p.tag = h | 1u;
+    return p;
+}
+
+hipError_t launch_kv_plan(const KvPlanArgs& a, hipStream_t stream) {
+    if (a.p.rows_at == a.p.tables_at)
+        hipLaunchKernelGGL(kv_plan_kernel<true>, dim3(1), dim3(kThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL(kv_plan_kernel<false>, dim3(1), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace mla

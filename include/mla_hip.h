@@ -419,6 +419,79 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
                          const void* plan, size_t plan_bytes, const int32_t* host_info, void* out,
                          float* lse, void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------------ (f)
+ * The paged key-value cache, for layers whose heads have keys and values of their own or share them
+ * in groups, beside the latent caches above: the same metadata, pages and slots.  No reference
+ * counterpart (its MLA caches hold latents, src/infer/inference.cpp:15-18; the Gemma engine's
+ * contiguous key-value cache is another program's, src/infer/gemma.cpp:318-478).  Page p of a
+ * layer's pool is one record of mla_kv_page_words 16-bit words of `dtype`: keys
+ * [n_kv_heads][page_size][head_dim], then values [n_kv_heads][page_size][v_dim].  page_size is a
+ * multiple of 16 up to 65,536, head_dim and v_dim multiples of 16 up to 256
+ * (MLA_ERR_UNSUPPORTED otherwise).  Query head h reads key-value head h / (n_heads / n_kv_heads). */
+#define MLA_DTYPE_F32 2 /* type of appended rows only */
+/* 16-bit words of a page record; 0 for shapes outside the above. */
+size_t mla_kv_page_words(int n_kv_heads, int head_dim, int v_dim, int page_size);
+/* Row t of k [T x n_kv_heads x head_dim], rotated, and of v [T x n_kv_heads x v_dim] is rounded once
+ * to `dtype` and written to flat slot slot_mapping[t]; slots outside the pool are skipped, the others
+ * are distinct.  With q [T x n_heads x head_dim] (NULL: none) row t of q is rotated the same way,
+ * rounded and written to q_out [T x n_heads x head_dim], whatever its slot.  Rows are of row_dtype
+ * (MLA_DTYPE_*); *_row and *_head are strides in elements (columns lie one behind the other), so
+ * that slices of one projection's rows can be given; rows, and strides, at multiples of 16 bytes
+ * are read faster.
+ * The rotation turns pair i of a head at position p = positions[t] by the angle p * frequencies[i]
+ * (device fp64, radians; taken in 64 bits): (a, b) -> (a cos - b sin, a sin + b cos).  The pairs'
+ * columns are rotary_start + (2i, 2i + 1) with adjacent = 1 (src/model/ops.cpp:88-108), rotary_start
+ * + (i, pairs + i) with 0; the others stay.  rotary_start is even; pairs = 0: no rotation. */
+int mla_append_kv(void* stream, int T, int n_heads, int n_kv_heads, int head_dim, int v_dim,
+                  int page_size, int dtype, int row_dtype, const void* k, long long k_row,
+                  long long k_head, const void* v, long long v_row, long long v_head, const void* q,
+                  long long q_row, long long q_head, const int32_t* positions,
+                  const double* frequencies, int pairs, int rotary_start, int adjacent,
+                  const int32_t* slot_mapping, int num_pool_pages, void* pages, void* q_out);
+/* Attention of every query row of a batch over its session's cached keys and values: row i of a
+ * session, at position p = k_len - q_len + i, sees the keys j <= p, and with window > 0 of these only
+ * those with p - j < window or j < sinks:
+ *     s_j = (q . k_j) * scale,   out = sum_j softmax(s)_j v_j,   lse = ln sum_j exp(s_j)
+ * for decode rows, drafted tokens and prompt chunks alike.  Only pages with keys that some row sees
+ * are read.  A plan, built on the GPU once for a batch and one (window, sinks), says which workgroup
+ * takes which rows over which keys and serves every such layer's call.  The rows' own keys and
+ * values must already be appended. */
+size_t mla_kv_plan_bytes(int B, int rows, int n_heads, int n_kv_heads, int head_dim, int v_dim,
+                         int page_size, int max_q_len, int window, int sinks);
+/* Bytes of the workspace of calls with a plan of these sizes. */
+size_t mla_kv_workspace_bytes(int B, int rows, int n_heads, int n_kv_heads, int head_dim, int v_dim,
+                              int page_size, int max_q_len, int window, int sinks);
+/* Builds the plan (one launch) of mla_kv_plan_bytes bytes at a multiple of 16.  cu_seqlens_q,
+ * cu_seqlens_k and info are those of mla_build_metadata; rows: query rows of the calls (at least the
+ * batch's); max_q_len: at least every session's q_len.  What only the device arrays show to be wrong
+ * (a failed metadata build, more rows than `rows`, a session past max_q_len) fails the plan: calls
+ * with it write nothing, and mla_read_kv_plan_info reports it. */
+int mla_plan_kv_attention(void* stream, int B, int rows, int n_heads, int n_kv_heads, int head_dim,
+                          int v_dim, int page_size, int max_q_len, int window, int sinks,
+                          const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                          const int32_t* info, void* plan, size_t plan_bytes);
+/* Synchronises `stream` and copies host_info[MLA_PLAN_INFO_INTS]: {jobs, 0, jobs of few rows, jobs of
+ * many, partial rows (each of one key-value head), query rows, a tag of the plan's sizes, 0}, or {-1,
+ * first bad session, ..} with MLA_ERR_INVALID_ARGUMENT and a message. */
+int mla_read_kv_plan_info(void* stream, const void* plan, int32_t* host_info);
+/* The attention.  page_table and max_pages are those of the metadata; q [rows x n_heads x head_dim]
+ * and out [rows x n_heads x v_dim] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.  Rows
+ * past the batch's are left as they were, and over a failed plan all.  host_info is what
+ * mla_read_kv_plan_info returned for this very plan, not built anew since, or NULL: with it the call
+ * launches as many workgroups as the plan has jobs, without it as many as a plan of these sizes can
+ * have, whose rest returns at once.  A call with the info of another build, whose counts differ,
+ * writes nothing; a captured graph that builds the plan takes NULL.  pages, q, plan, out and
+ * workspace at multiples of 16 bytes.  The workspace needs no initialisation; calls that share one
+ * must be ordered on one stream.  Rows are rounded once, to `dtype`.  A key or value that a row does
+ * not see adds nothing to it, whatever it holds.  A value that is not finite makes its column of the
+ * rows that see it infinite or NaN, a NaN key those rows. */
+int mla_kv_attention(void* stream, int B, int rows, int n_heads, int n_kv_heads, int head_dim,
+                     int v_dim, int page_size, int max_q_len, int window, int sinks, int dtype,
+                     float scale, const int32_t* page_table, int max_pages, int num_pool_pages,
+                     const void* pages, const void* q, const void* plan, size_t plan_bytes,
+                     const int32_t* host_info, void* out, float* lse, void* workspace,
+                     size_t workspace_bytes);
+
 /* ------------------------------------------------------------------ model
  * The batched decode step around the attention: everything of
  * CpuDecoder::decode (src/infer/inference.cpp:76-173) for B sessions at once,
