@@ -360,7 +360,8 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 }
 
 template <typename T, int HD, bool EXACT>
-__global__ __launch_bounds__(kKvThreads) void kv_few_kernel(KvArgs a) {
+__global__ __launch_bounds__(kKvThreads) __attribute__((
+    amdgpu_waves_per_eu(HD == 64 ? 4 : HD == 128 ? 3 : 2, 8))) void kv_few_kernel(KvArgs a) {
     constexpr int CW = HD >= 128 ? 8 : 4, PITCH = HD + 4;
     using A = Attend<T, HD, EXACT, CW, 1>;
     using V8 = typename T::vec8;
@@ -485,7 +486,8 @@ __global__ __launch_bounds__(kKvThreads) void kv_few_kernel(KvArgs a) {
 }
 
 template <typename T, int HD, bool EXACT>
-__global__ __launch_bounds__(kKvThreads) void kv_many_kernel(KvArgs a) {
+__global__ __launch_bounds__(kKvThreads) __attribute__((
+    amdgpu_waves_per_eu(2, 8))) void kv_many_kernel(KvArgs a) {
     constexpr int N = HD == 256 ? 1 : 2, CW = 4;
     constexpr int SU = HD == 64 ? 4 : HD == 128 ? 2 : 1;  // units of a stage
     using A = Attend<T, HD, EXACT, CW, N>;
