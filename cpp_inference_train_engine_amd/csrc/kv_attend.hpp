@@ -20,9 +20,10 @@
 // kv_few_kernel -- a job of at most 16 rows: each of four waves holds all of them and takes every
 //   4th unit, straight from memory into the operands' registers; the waves' states meet in LDS at
 //   the end.
-// kv_many_kernel -- a job of 128 rows (64 above width 128): each of four waves holds 32 (16).  They
-//   stage 64 keys (128 at width 64, 32 at 256) together in LDS, in operand order, into one of two
-//   buffers: one barrier a stage, and every LDS access is 16 bytes a lane in a row.
+// kv_many_kernel -- a job of 128 rows: each of four waves holds 32 (of eight 16 above width 128).
+//   They stage 32 keys (64 at width 64) together in LDS, in operand order, into one of three
+//   buffers: one barrier a stage, and every LDS access is 16 bytes a lane in a row.  The scores of a
+//   stage are computed beside the weights of the one before it.
 //
 // A key past a row's position, or between its sinks and its window, adds nothing to the row,
 // whatever it holds: its score is replaced, and its value is taken as zero where no row of the
@@ -60,6 +61,14 @@ __device__ __forceinline__ int quotient(int n, int d, uint32_t inverse, int& res
         rest -= d;
     }
     return q;
+}
+
+// Two values rounded to 16 bits (to nearest even) in one word: one instruction.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef typename T::scalar s2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), s2));
 }
 
 template <typename T>
@@ -111,9 +120,30 @@ __device__ __forceinline__ int first_key(const Job& j, int u) {
     return (u < j.units.sink_units ? u : u + j.units.skip) * kKvTile;
 }
 
+// The units that rows at positions from `first` on, the last of them with a window from `lo` on, all
+// see in full: some of the sinks', some of the window's.
+struct Full {
+    int sinks, from, to;
+    __device__ __forceinline__ Full(const Job& j, int first, int lo, int held) {
+        const int behind = (first + 1) / kKvTile;
+        sinks = min(min(held / kKvTile, behind), j.units.sink_units);
+        from = (int)(((unsigned)lo + kKvTile - 1) / kKvTile) - j.units.skip;
+        to = behind - j.units.skip;
+    }
+    __device__ __forceinline__ bool has(int u) const { return u < sinks || (u >= from && u < to); }
+};
+
+// An element at a uniform address and the lane's 32-bit distance in bytes.
+template <typename E>
+__device__ __forceinline__ E fetch(const uint16_t* base, uint32_t bytes) {
+    return *reinterpret_cast<const E*>(reinterpret_cast<const char*>(base) + bytes);
+}
+
 // Page ids of a unit's two tiles, and their places there.
 struct Pages {
-    int id[2], in[2];
+    int id0, id1, in0, in1;
+    __device__ __forceinline__ int id(int tt) const { return tt ? id1 : id0; }
+    __device__ __forceinline__ int in(int tt) const { return tt ? in1 : in0; }
 };
 
 // What both kernels share: T 16-bit type, HD width (head sizes are HD in EXACT instantiations, at
@@ -172,10 +202,10 @@ struct Attend {
     __device__ __forceinline__ Pages find_pages(int u) const {
         Pages p;
         const int t = first_key(job, min(u, job.u1 - 1)) >> 4, tpp = a.p.page_size >> 4;
-        p.id[0] = ptab[quotient(t, tpp, a.tpp_inverse, p.in[0])];
+        p.id0 = ptab[quotient(t, tpp, a.tpp_inverse, p.in0)];
         // a tile behind the last key is not on a page: the one before it is read again
         const int t1 = min(t + 1, job.pb >> 4);
-        p.id[1] = ptab[quotient(t1, tpp, a.tpp_inverse, p.in[1])];
+        p.id1 = ptab[quotient(t1, tpp, a.tpp_inverse, p.in1)];
         return p;
     }
     // (Ids were checked by the metadata's build; the bound is for memory's sake.)
@@ -183,36 +213,35 @@ struct Attend {
         return (long long)min((unsigned)id, (unsigned)a.num_pool_pages - 1) * record;
     }
     __device__ __forceinline__ const uint16_t* keys_at(const Pages& p, int tt) const {
-        return keys_of_head + page_at(p.id[tt]) + (long long)p.in[tt] * 16 * D;
+        return keys_of_head + page_at(p.id(tt)) + (long long)p.in(tt) * 16 * D;
     }
     __device__ __forceinline__ const uint16_t* values_at(const Pages& p, int tt) const {
-        return values_of_head + page_at(p.id[tt]) + (long long)p.in[tt] * 16 * DV;
+        return values_of_head + page_at(p.id(tt)) + (long long)p.in(tt) * 16 * DV;
     }
     // Key operand of a tile's step s: columns 32s + 8g .. of key n.
     __device__ __forceinline__ u32x4 load_key(const uint16_t* tile, int s) const {
         const int c = 32 * s + 8 * g;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(tile + n * D + (EXACT ? c : min(c, D - 8)));
-        return EXACT || c < D ? v : u32x4{0, 0, 0, 0};
+        if constexpr (EXACT)
+            return fetch<u32x4>(tile + 32 * s, (uint32_t)(n * HD + 8 * g) * 2);
+        const u32x4 v = fetch<u32x4>(tile, (uint32_t)(n * D + min(c, D - 8)) * 2);
+        return c < D ? v : u32x4{0, 0, 0, 0};
     }
     // The lane's columns of chunk c of a tile's row 4g + i.
     struct Row {
         uint32_t w[CW / 2];
     };
     __device__ __forceinline__ Row load_value(const uint16_t* tile, int c, int i) const {
+        typedef uint32_t words __attribute__((ext_vector_type(CW / 2)));
         const int col = 16 * CW * c + CW * n;
-        const uint16_t* p = tile + (4 * g + i) * DV + (EXACT ? col : min(col, DV - CW));
         Row r;
-        if constexpr (CW == 8) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+        words v;
+        if constexpr (EXACT)
+            v = fetch<words>(tile + 16 * CW * c + i * HD, (uint32_t)(4 * g * HD + CW * n) * 2);
+        else
+            v = fetch<words>(tile + i * DV, (uint32_t)(4 * g * DV + min(col, DV - CW)) * 2);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                r.w[k] = EXACT || col < DV ? v[k] : 0;
-        } else {
-            const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-                r.w[k] = EXACT || col < DV ? v[k] : 0;
-        }
+        for (int k = 0; k < CW / 2; ++k)
+            r.w[k] = EXACT || col < DV ? v[k] : 0;
         return r;
     }
     // Operand e of eight rows: their columns e, two keys a word.
@@ -227,11 +256,6 @@ struct Attend {
     // Whether some row of the block sees the key.
     __device__ __forceinline__ bool some_row_sees(int key) const {
         return key <= job.pb && (key >= job.lo_a || key < a.p.sinks);
-    }
-    // Whether every row of the block sees the unit's keys.
-    __device__ __forceinline__ bool all_rows_see(int key0) const {
-        return key0 + kKvTile - 1 <= job.pa &&
-               (key0 >= job.lo_b || key0 + kKvTile - 1 < a.p.sinks);
     }
     // The lane's rows (tile r / 4, row 4g + r % 4) of a unit that not every row of the block sees:
     // values that no row sees become zero.  With several positions in the block non-finite ones
@@ -251,63 +275,72 @@ struct Attend {
         return bad;
     }
 
-    // Scores become weights: masks, maximum, exponentials and their sum, in two parts.
-    __device__ __forceinline__ void weights(floatx4 (&sc)[N][2], int key0, bool full, V8 (&hi)[N],
-                                            V8 (&lw)[N]) {
-        float mp[N];
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-            if (!full)
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = key0 + 16 * tt + 4 * g + i;
-                        if (key > pos[t] || (key < lo[t] && key >= a.p.sinks))
-                            sc[t][tt][i] = -INFINITY;
-                    }
-            mp[t] = -INFINITY;  // of the lane's eight scores (NaN is passed over)
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    mp[t] = fmaxf(mp[t], sc[t][tt][i]);
-            mp[t] *= a.scale_log2;
-        }
-        bool raise = false;
+    // Scores of keys that a row does not see are replaced.
+    __device__ __forceinline__ void mask(floatx4 (&sc)[N][2], int key0) const {
 #pragma unroll
         for (int t = 0; t < N; ++t)
-            raise |= mp[t] > m[t] + kRise;
-        if (__builtin_amdgcn_ballot_w64(raise)) {
-#pragma unroll
-            for (int t = 0; t < N; ++t) {
-                const float top = rows_max(mp[t]) - kHead;
-                const float m_new = top > m[t] + (kRise - kHead) ? top : m[t];
-                const bool had = m[t] != -INFINITY;  // the row has accumulated state
-                if (__builtin_amdgcn_ballot_w64(had && m_new > m[t])) {
-                    const float alpha = had ? __builtin_amdgcn_exp2f(m[t] - m_new) : 1.0f;
-                    l[t] *= alpha;
-#pragma unroll
-                    for (int k = 0; k < NT; ++k)
-                        acc[t][k] *= alpha;
-                }
-                m[t] = m_new;
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-            const float ref = m[t] == -INFINITY ? 0.0f : m[t];
-            float sum = 0.0f;
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[t][tt][i], a.scale_log2, -ref));
-                    sum += e;
-                    const auto h = static_cast<typename T::scalar>(e);
-                    hi[t][4 * tt + i] = h;
-                    lw[t][4 * tt + i] = static_cast<typename T::scalar>(e - static_cast<float>(h));
+                    const int key = key0 + 16 * tt + 4 * g + i;
+                    const bool sees = (key <= pos[t]) & ((key >= lo[t]) | (key < a.p.sinks));
+                    sc[t][tt][i] = sees ? sc[t][tt][i] : -INFINITY;
                 }
+    }
+    // The rows' reference maxima, and what was summed under lower ones, follow the scores of U units.
+    template <int U>
+    __device__ __forceinline__ void raise(const floatx4 (&sc)[U][N][2]) {
+        float mp[N];
+        bool above = false;
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            mp[t] = -INFINITY;  // of the lane's scores (NaN is passed over)
+#pragma unroll
+            for (int x = 0; x < U; ++x)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mp[t] = fmaxf(mp[t], sc[x][t][tt][i]);
+            mp[t] *= a.scale_log2;
+            above |= mp[t] > m[t] + kRise;
+        }
+        if (__builtin_amdgcn_ballot_w64(above) == 0)
+            return;
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const float top = rows_max(mp[t]) - kHead;
+            const float m_new = top > m[t] + (kRise - kHead) ? top : m[t];
+            const bool had = m[t] != -INFINITY;  // the row has accumulated state
+            if (__builtin_amdgcn_ballot_w64(had && m_new > m[t])) {
+                const float alpha = had ? __builtin_amdgcn_exp2f(m[t] - m_new) : 1.0f;
+                l[t] *= alpha;
+#pragma unroll
+                for (int k = 0; k < NT; ++k)
+                    acc[t][k] *= alpha;
+            }
+            m[t] = m_new;
+        }
+    }
+    // Scores become weights, in two parts, and are summed.
+    __device__ __forceinline__ void weights(const floatx4 (&sc)[N][2], V8 (&hi)[N], V8 (&lw)[N]) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const float ref = m[t] == -INFINITY ? 0.0f : m[t];
+            float sum = 0.0f;
+            u32x4 h, w;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const floatx4 y = sc[t][x >> 1];
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(y[2 * (x & 1)], a.scale_log2, -ref));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(y[2 * (x & 1) + 1], a.scale_log2, -ref));
+                sum += e0 + e1;
+                h[x] = pack2<T>(e0, e1);
+                w[x] = pack2<T>(e0 - T::to_float((uint16_t)h[x]), e1 - T::to_float((uint16_t)(h[x] >> 16)));
+            }
+            hi[t] = __builtin_bit_cast(V8, h);
+            lw[t] = __builtin_bit_cast(V8, w);
             l[t] += sum;
         }
     }
@@ -354,11 +387,6 @@ struct Attend {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-    return T::from_float(x) | (uint32_t)T::from_float(y) << 16;
-}
-
 template <typename T, int HD, bool EXACT>
 __global__ __launch_bounds__(kKvThreads) __attribute__((
     amdgpu_waves_per_eu(HD == 64 ? 4 : HD == 128 ? 3 : 2, 8))) void kv_few_kernel(KvArgs a) {
@@ -390,6 +418,7 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
             for (int r = 0; r < 8; ++r)
                 v[c][r] = s.load_value(s.values_at(p, r >> 2), c, r & 3);
     };
+    const Full full_units(job, job.pa, job.lo_b, a.p.sinks);
     int u = job.u0 + wave;
     Pages now{}, next{};
     if (u < job.u1) {
@@ -400,16 +429,19 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
     }
     for (; u < job.u1; u += 4) {
         const int key0 = first_key(job, u);
-        floatx4 sc[1][2] = {{{0, 0, 0, 0}, {0, 0, 0, 0}}};
+        floatx4 sc[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
 #pragma unroll
         for (int st = 0; st < A::KS; ++st)
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
-                sc[0][tt] = T::mma32(__builtin_bit_cast(V8, k[tt][st]), s.q[0][st], sc[0][tt]);
+                sc[0][0][tt] = T::mma32(__builtin_bit_cast(V8, k[tt][st]), s.q[0][st], sc[0][0][tt]);
         load_keys(next);
-        const bool full = s.all_rows_see(key0);
+        const bool full = full_units.has(u);
+        if (!full)
+            s.mask(sc[0], key0);
+        s.raise(sc);
         V8 hi[1], lw[1];
-        s.weights(sc, key0, full, hi, lw);
+        s.weights(sc[0], hi, lw);
         bool bad = false;
         if (!full)
 #pragma unroll
@@ -485,17 +517,20 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
     }
 }
 
+constexpr int many_waves(int width) { return width == 256 ? 8 : 4; }
+
 template <typename T, int HD, bool EXACT>
-__global__ __launch_bounds__(kKvThreads) __attribute__((
+__global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
     amdgpu_waves_per_eu(2, 8))) void kv_many_kernel(KvArgs a) {
-    constexpr int N = HD == 256 ? 1 : 2, CW = 4;
-    constexpr int SU = HD == 64 ? 4 : HD == 128 ? 2 : 1;  // units of a stage
+    constexpr int NW = many_waves(HD), N = kKvManyRows / (16 * NW), CW = 2;
+    constexpr int U = HD == 64 ? 2 : 1;  // units of a stage
     using A = Attend<T, HD, EXACT, CW, N>;
     using V8 = typename T::vec8;
     // a stage in operand order, 1 KB each: keys [unit][tile][step], values [unit][tile of O^T]
-    constexpr int KW = SU * 2 * A::KS * 512, STAGE = KW + SU * A::NT * 512;
-    __shared__ __attribute__((aligned(16))) uint16_t smem[2][STAGE];
-    __shared__ int marks[3][SU];  // units whose non-finite values were taken out
+    constexpr int KW = U * 2 * A::KS * 512, STAGE = KW + U * A::NT * 512;
+    static_assert(U * 2 * A::KS == 2 * NW && U * A::NC == NW, "a wave's share of a stage");
+    __shared__ __attribute__((aligned(16))) uint16_t smem[3][STAGE];
+    __shared__ int marks[3][NW];  // whether a wave took non-finite values out of the stage
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int index = (int)(blockIdx.x / (unsigned)a.p.kv_heads);
     const int head = (int)(blockIdx.x - (unsigned)index * a.p.kv_heads);
@@ -505,97 +540,170 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
     const int row0 = wave * 16 * N;
     A s(a, job, tid & 63, head, row0);
 
-    // positions of the wave's first and last row (none: it takes no units)
+    // the first and last window, and the first position, of the wave's rows
     int r;
-    const int w_last = min(job.rows, row0 + 16 * N) - 1;
     const int wa = job.ctx + quotient(job.f0 + min(row0, job.rows - 1), a.p.group, a.group_inverse, r);
-    const int wb = w_last < row0 ? -1 : job.ctx + quotient(job.f0 + w_last, a.p.group, a.group_inverse, r);
-    const int lo_wa = wa >= a.p.window ? wa - a.p.window + 1 : 0;
+    const int wb = job.ctx + quotient(job.f0 + min(row0 + 16 * N, job.rows) - 1, a.p.group, a.group_inverse, r);
     const int lo_wb = wb >= a.p.window ? wb - a.p.window + 1 : 0;
 
-    // ---- what the wave stages: a quarter of the stage, all of it of one unit ----
-    const int su = wave * SU / 4;                 // the unit
-    const int o0 = wave * 4 % (2 * A::KS);        // its first of four key operands there
-    const int vc = wave % A::NC;                  // its chunk of the values
-    u32x4 k[4];
-    typename A::Row v[8];
-    auto load = [&](const Pages& p) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int o = o0 + i;
-            k[i] = s.load_key(s.keys_at(p, o / A::KS), o % A::KS);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = s.load_value(s.values_at(p, i >> 2), vc, i & 3);
+    const Full full_wave(job, wa, lo_wb, a.p.sinks), full_block(job, job.pa, job.lo_b, a.p.sinks);
+
+    // ---- what the wave stages: two key operands and 32 columns of the values of one unit ----
+    const int su = wave / A::NC, vc = wave % A::NC, o0 = 2 * wave % (2 * A::KS);
+    // Where a stage's tiles lie (bytes from the head's first page): lane i of these holds the places
+    // of stage (group of 64) + i.
+    long long key_at = 0, value_at0 = 0, value_at1 = 0;
+    auto find_tiles = [&](int st) {
+        const int t = first_key(job, min(job.u0 + (st + s.lane) * U + su, job.u1 - 1)) >> 4;
+        const int tpp = a.p.page_size >> 4, t1 = min(t + 1, job.pb >> 4);
+        int in0, in1;
+        const int32_t* ids = a.page_table + (long long)job.session * a.max_pages;
+        const int id0 = ids[quotient(t, tpp, a.tpp_inverse, in0)];
+        const int id1 = ids[quotient(t1, tpp, a.tpp_inverse, in1)];
+        const long long p0 = s.page_at(id0), p1 = s.page_at(id1);
+        key_at = 2 * (o0 / A::KS ? p1 + (long long)in1 * 16 * s.D : p0 + (long long)in0 * 16 * s.D);
+        value_at0 = 2 * (p0 + (long long)in0 * 16 * s.DV);
+        value_at1 = 2 * (p1 + (long long)in1 * 16 * s.DV);
     };
-    const int stages = (job.u1 - job.u0 + SU - 1) / SU;
-    if (tid < 3 * SU)
-        marks[tid / SU][tid % SU] = 0;
-    __syncthreads();
-    Pages pages = s.find_pages(job.u0 + su);
-    load(pages);
-    for (int st = 0; st < stages; ++st) {
-        uint16_t* const buf = smem[st & 1];
-        const int u0 = job.u0 + st * SU, mine = first_key(job, min(u0 + su, job.u1 - 1));
-        if (!s.all_rows_see(mine)) {
-            const bool bad = s.clean(v, mine);
-            if (__builtin_amdgcn_ballot_w64(bad) && s.lane == 0)
-                marks[st % 3][su] = 1;
-        }
+    auto of_lane = [&](long long x, int i) {
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, i);
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((unsigned long long)x >> 32), i);
+        return (long long)((unsigned long long)hi << 32 | lo);
+    };
+    auto at = [](const uint16_t* p, long long bytes) {
+        return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p) + bytes);
+    };
+    u32x4 k[2];
+    typename A::Row v[8];
+    auto load = [&](int st) {
+        const int i = st & 63;
+        if (i == 0)
+            find_tiles(st);
+        const uint16_t* kt = at(s.keys_of_head, of_lane(key_at, i));
+        const uint16_t* v0 = at(s.values_of_head, of_lane(value_at0, i));
+        const uint16_t* v1 = at(s.values_of_head, of_lane(value_at1, i));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<u32x4*>(buf + (su * 2 * A::KS + o0 + i) * 512 + s.lane * 8) = k[i];
+        for (int i2 = 0; i2 < 2; ++i2)
+            k[i2] = s.load_key(kt, o0 % A::KS + i2);
+#pragma unroll
+        for (int i2 = 0; i2 < 8; ++i2)
+            v[i2] = s.load_value(i2 < 4 ? v0 : v1, vc, i2 & 3);
+    };
+    auto store = [&](int st, int b) {
+        const int u = min(job.u0 + st * U + su, job.u1 - 1);
+        if (!full_block.has(u)) {
+            const bool bad = __builtin_amdgcn_ballot_w64(s.clean(v, first_key(job, u))) != 0;
+            if (s.lane == 0)
+                marks[b][wave] = bad;
+        }
+        uint16_t* const buf = smem[b] + s.lane * 8;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<u32x4*>(buf + (su * 2 * A::KS + o0 + i) * 512) = k[i];
 #pragma unroll
         for (int e = 0; e < CW; ++e)
-            *reinterpret_cast<u32x4*>(buf + KW + (su * A::NT + vc * CW + e) * 512 + s.lane * 8) =
-                A::transposed(v, e);
-        pages = s.find_pages(u0 + SU + su);
-        load(pages);  // (the last one once more, at the end)
-        // The other buffer is free: every wave that passed the barrier before this one has finished
-        // with it.  Likewise the marks: stage st + 2's, last read in stage st - 1, are cleared behind
-        // this barrier and set again behind the next.
-        __syncthreads();
-        if (tid < SU)
-            marks[(st + 2) % 3][tid] = 0;
-#pragma unroll 1
-        for (int x = 0; x < SU; ++x) {
-            if (u0 + x >= job.u1)
-                break;
-            const int key0 = first_key(job, u0 + x);
-            if (key0 > wb || (key0 + kKvTile <= lo_wa && key0 >= a.p.sinks))
-                continue;
-            const uint16_t* const kb = buf + x * 2 * A::KS * 512 + s.lane * 8;
-            const uint16_t* const vb = buf + KW + x * A::NT * 512 + s.lane * 8;
-            floatx4 sc[N][2];
+            *reinterpret_cast<u32x4*>(buf + KW + (su * A::NT + vc * CW + e) * 512) = A::transposed(v, e);
+    };
+    constexpr int NK = U * 2 * A::KS, NV = U * A::NT, AHEAD = 4;
+    auto read = [&](const uint16_t* p, int slot) {
+        return *reinterpret_cast<const V8*>(p + s.lane * 8 + slot * 512);
+    };
+    auto scores = [&](floatx4 (&sc)[U][N][2], const V8 (&ko)[NK]) {
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
 #pragma unroll
             for (int t = 0; t < N; ++t)
-                sc[t][0] = sc[t][1] = floatx4{0, 0, 0, 0};
+                sc[x][t][0] = sc[x][t][1] = floatx4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < A::KS; ++i)
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const V8 y = *reinterpret_cast<const V8*>(kb + (tt * A::KS + i) * 512);
+                for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                     for (int t = 0; t < N; ++t)
-                        sc[t][tt] = T::mma32(y, s.q[t][i], sc[t][tt]);
-                }
-            const bool full = key0 + kKvTile - 1 <= wa &&
-                              (key0 >= lo_wb || key0 + kKvTile - 1 < a.p.sinks);
-            V8 hi[N], lw[N];
-            s.weights(sc, key0, full, hi, lw);
-#pragma unroll
-            for (int i = 0; i < A::NT; ++i) {
-                const V8 y = *reinterpret_cast<const V8*>(vb + i * 512);
-#pragma unroll
-                for (int t = 0; t < N; ++t) {
-                    s.acc[t][i] = T::mma32(y, hi[t], s.acc[t][i]);
-                    s.acc[t][i] = T::mma32(y, lw[t], s.acc[t][i]);
-                }
-            }
-            if (marks[st % 3][x])
-                s.add_nonfinite(s.find_pages(u0 + x), key0, hi, lw);
+                        sc[x][t][tt] = T::mma32(ko[(x * 2 + tt) * A::KS + i], s.q[t][i], sc[x][t][tt]);
         }
+    };
+    const int stages = (job.u1 - job.u0 + U - 1) / U;
+    load(0);
+    store(0, 0);
+    load(1);
+    store(1, 1);
+    load(2);
+    __syncthreads();
+    floatx4 sc[U][N][2];
+    {
+        V8 ko[NK];
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+            ko[i] = read(smem[0], i);
+        scores(sc, ko);
+    }
+    // Stage st: its scores are there, its values in buffer b, stage st + 1 in buffer b1.  Buffer b2,
+    // free since the last barrier, takes stage st + 2.  (Units behind the last are staged as the last
+    // and not used.)
+    int b = 0, b1 = 1, b2 = 2;
+    for (int st = 0; st < stages; ++st) {
+        // the next scores' operands, and the first values', on their way before they are needed
+        V8 ko[NK], ring[AHEAD];
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+            ko[i] = read(smem[b1], i);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            ring[i] = read(smem[b] + KW, i);
+        store(st + 2, b2);
+        load(st + 3);
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const int u = job.u0 + st * U + x;
+            if (!full_wave.has(u) || u >= job.u1)
+                s.mask(sc[x], u < job.u1 ? first_key(job, u) : INT_MAX - 31);
+        }
+        s.raise(sc);
+        floatx4 next[U][N][2];
+        scores(next, ko);
+        V8 hi[U][N], lw[U][N];
+#pragma unroll
+        for (int x = 0; x < U; ++x)
+            s.weights(sc[x], hi[x], lw[x]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const V8 y = ring[i % AHEAD];
+            if (i + AHEAD < NV)
+                ring[i % AHEAD] = read(smem[b] + KW, i + AHEAD);
+            const int x = i / A::NT, tile = i % A::NT;
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+                s.acc[t][tile] = T::mma32(y, hi[x][t], s.acc[t][tile]);
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+                s.acc[t][tile] = T::mma32(y, lw[x][t], s.acc[t][tile]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const int u = job.u0 + st * U + x;
+            if (u < job.u1 && !full_block.has(u)) {
+                bool bad = false;
+#pragma unroll
+                for (int w = 0; w < A::NC; ++w)
+                    bad |= marks[b][x * A::NC + w] != 0;
+                if (__builtin_amdgcn_readfirstlane(bad))
+                    s.add_nonfinite(s.find_pages(u), first_key(job, u), hi[x], lw[x]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < U; ++x)
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+                    sc[x][t][tt] = next[x][t][tt];
+        const int b0 = b;
+        b = b1;
+        b1 = b2;
+        b2 = b0;
     }
 
     // ---- rows, or partials ----
@@ -612,20 +720,24 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
                                  : ((long long)job.part + row) * a.p.kv_heads + head;
         const float inv = 1.0f / l;
 #pragma unroll
-        for (int x = 0; x < A::NT; x += CW)
+        for (int x = 0; x < A::NT; x += 2) {  // eight columns a lane of two tiles
+            const int col = s.column(x, 0);
+            if (!EXACT && col >= s.DV)
+                continue;
+            if (job.part < 0) {
+                u32x4 o;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const int col = s.column(x, y);
-                if (!EXACT && col >= s.DV)
-                    continue;
-                const floatx4 o = {s.acc[t][x][y], s.acc[t][x + 1][y], s.acc[t][x + 2][y],
-                                   s.acc[t][x + 3][y]};
-                if (job.part < 0)
-                    *reinterpret_cast<u32x2*>(a.out + at * s.DV + col) =
-                        u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-                else
-                    *reinterpret_cast<floatx4*>(a.part_o + at * s.DV + col) = o;
+                for (int y = 0; y < 4; ++y)
+                    o[y] = pack2<T>(s.acc[t][x][y] * inv, s.acc[t][x + 1][y] * inv);
+                *reinterpret_cast<u32x4*>(a.out + at * s.DV + col) = o;
+            } else {
+#pragma unroll
+                for (int y = 0; y < 4; y += 2)
+                    *reinterpret_cast<floatx4*>(a.part_o + at * s.DV + col + 2 * y) =
+                        floatx4{s.acc[t][x][y], s.acc[t][x + 1][y], s.acc[t][x][y + 1],
+                                s.acc[t][x + 1][y + 1]};
             }
+        }
         if (s.g == 0) {
             if (job.part < 0) {
                 if (a.lse)
@@ -642,7 +754,7 @@ template <typename T, int HD, bool EXACT>
 hipError_t launch_one(const KvArgs& a, bool many, hipStream_t stream) {
     if (many)
         hipLaunchKernelGGL((kv_many_kernel<T, HD, EXACT>), dim3((unsigned)(a.jobs_m * a.p.kv_heads)),
-                           dim3(kKvThreads), 0, stream, a);
+                           dim3(64 * many_waves(HD)), 0, stream, a);
     else
         hipLaunchKernelGGL((kv_few_kernel<T, HD, EXACT>), dim3((unsigned)(a.jobs_f * a.p.kv_heads)),
                            dim3(kKvThreads), 0, stream, a);

@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
 
     int jobs[2] = {0, 0}, parts = 0;
     for (int list = 0; list < 2; ++list) {
-        const int per = list ? kv_many_rows(p.width) : kKvFewRows;
+        const int per = list ? kKvManyRows : kKvFewRows;
         const int slots = list ? p.slots_m : p.slots_f;
         const int most_jobs = list ? p.max_jobs_m : p.max_jobs_f;
         if (most_jobs == 0)
@@ -252,7 +252,7 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
     const int at_once_m = 512;
     p.slots_f = std::max(1, at_once_f / kv_heads);
     p.slots_m = std::max(1, at_once_m / kv_heads);
-    const int many = kv_many_rows(p.width);
+    const int many = kKvManyRows;
     const bool few = p.group <= kKvFew;
     const long long blocks_f =
         few ? std::min<long long>((long long)B * (kKvFew / kKvFewRows), flat / kKvFewRows + B) : 0;

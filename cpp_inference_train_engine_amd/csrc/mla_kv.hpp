@@ -35,17 +35,17 @@ hipError_t launch_kv_append(const KvAppendArgs& a, int dtype, int row_dtype, hip
 // The query rows of a session that read one kv head, (token, head of the group) one behind the
 // other, are its flat rows.  A job is a block of flat rows over a range of the keys that they see.
 // Sessions of few flat rows go to the list of blocks of 16, whose four waves split the keys; the
-// others to the list of blocks of kv_many_rows, whose four waves split the rows.
+// others to the list of blocks of 128, whose waves split the rows.
 constexpr int kKvThreads = 256;
 constexpr int kKvFewRows = 16;  // rows of a block of the first list
 constexpr int kKvFew = 32;      // sessions of up to so many flat rows are on it
+constexpr int kKvManyRows = 128;  // rows of a block of the other
 constexpr int kKvTile = 32;     // keys of a unit
 // Widths that kernels exist for: both head sizes are padded to the smallest that holds them.
 __host__ __device__ inline int kv_width(int dim, int v_dim) {
     const int w = dim > v_dim ? dim : v_dim;
     return w <= 64 ? 64 : w <= 128 ? 128 : 256;
 }
-__host__ __device__ inline int kv_many_rows(int width) { return width == 256 ? 64 : 128; }
 
 constexpr int kKvJobInts = 8;  // session, its first query row, first flat row, rows, first and last
                                // unit (of those that the block sees) + 1, ctx, first partial row
