@@ -22,8 +22,7 @@
 //   the end.
 // kv_many_kernel -- a job of 128 rows: each of four waves holds 32 (of eight 16 above width 128).
 //   They stage 32 keys (64 at width 64) together in LDS, in operand order, into one of three
-//   buffers: one barrier a stage, and every LDS access is 16 bytes a lane in a row.  The scores of a
-//   stage are computed beside the weights of the one before it.
+//   buffers: one barrier a stage, and every LDS access is 16 bytes a lane in a row.
 //
 // A key past a row's position, or between its sinks and its window, adds nothing to the row,
 // whatever it holds: its score is replaced, and its value is taken as zero where no row of the
@@ -146,12 +145,12 @@ struct Pages {
     __device__ __forceinline__ int in(int tt) const { return tt ? in1 : in0; }
 };
 
-// What both kernels share: T 16-bit type, HD width (head sizes are HD in EXACT instantiations, at
-// most HD in the others), CW consecutive columns of V that a lane transposes (a tile of O^T holds
-// every CW-th), N tiles of 16 rows a wave.
-template <typename T, int HD, bool EXACT, int CW, int N>
+// What both kernels share: T 16-bit type, HK and HV widths of keys and values (the head's sizes in
+// EXACT instantiations, at least those in the others), CW consecutive columns of V that a lane
+// transposes (a tile of O^T holds every CW-th), N tiles of 16 rows a wave.
+template <typename T, int HK, int HV, bool EXACT, int CW, int N>
 struct Attend {
-    static constexpr int KS = HD / 32, NT = HD / 16, NC = NT / CW;
+    static constexpr int KS = HK / 32, NT = HV / 16, NC = NT / CW;
     using V8 = typename T::vec8;
 
     const KvArgs& a;
@@ -166,7 +165,7 @@ struct Attend {
     floatx4 acc[N][NT];
 
     __device__ __forceinline__ Attend(const KvArgs& a_, const Job& j, int lane_, int head_, int row0)
-        : a(a_), job(j), D(EXACT ? HD : a_.p.dim), DV(EXACT ? HD : a_.p.v_dim), lane(lane_),
+        : a(a_), job(j), D(EXACT ? HK : a_.p.dim), DV(EXACT ? HV : a_.p.v_dim), lane(lane_),
           g(lane_ >> 4), n(lane_ & 15), head(head_),
           ptab(table(a_.page_table + (long long)j.session * a_.max_pages)),
           keys_of_head(a_.pages + (long long)head_ * a_.p.page_size * D),
@@ -222,7 +221,7 @@ struct Attend {
     __device__ __forceinline__ u32x4 load_key(const uint16_t* tile, int s) const {
         const int c = 32 * s + 8 * g;
         if constexpr (EXACT)
-            return fetch<u32x4>(tile + 32 * s, (uint32_t)(n * HD + 8 * g) * 2);
+            return fetch<u32x4>(tile + 32 * s, (uint32_t)(n * HK + 8 * g) * 2);
         const u32x4 v = fetch<u32x4>(tile, (uint32_t)(n * D + min(c, D - 8)) * 2);
         return c < D ? v : u32x4{0, 0, 0, 0};
     }
@@ -236,7 +235,7 @@ struct Attend {
         Row r;
         words v;
         if constexpr (EXACT)
-            v = fetch<words>(tile + 16 * CW * c + i * HD, (uint32_t)(4 * g * HD + CW * n) * 2);
+            v = fetch<words>(tile + 16 * CW * c + i * HV, (uint32_t)(4 * g * HV + CW * n) * 2);
         else
             v = fetch<words>(tile + i * DV, (uint32_t)(4 * g * DV + min(col, DV - CW)) * 2);
 #pragma unroll
@@ -387,11 +386,11 @@ struct Attend {
     }
 };
 
-template <typename T, int HD, bool EXACT>
+template <typename T, int HK, int HV, bool EXACT>
 __global__ __launch_bounds__(kKvThreads) __attribute__((
-    amdgpu_waves_per_eu(HD == 64 ? 4 : HD == 128 ? 3 : 2, 8))) void kv_few_kernel(KvArgs a) {
-    constexpr int CW = HD >= 128 ? 8 : 4, PITCH = HD + 4;
-    using A = Attend<T, HD, EXACT, CW, 1>;
+    amdgpu_waves_per_eu(HK == 64 ? 4 : HK == 128 ? 3 : 2, 8))) void kv_few_kernel(KvArgs a) {
+    constexpr int CW = HV >= 128 ? 8 : 4, PITCH = HV + 4;
+    using A = Attend<T, HK, HV, EXACT, CW, 1>;
     using V8 = typename T::vec8;
     __shared__ __attribute__((aligned(16))) float smem[4][16 * PITCH + 32];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -519,16 +518,18 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
 
 constexpr int many_waves(int width) { return width == 256 ? 8 : 4; }
 
-template <typename T, int HD, bool EXACT>
-__global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
+template <typename T, int HK, int HV, bool EXACT>
+__global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
     amdgpu_waves_per_eu(2, 8))) void kv_many_kernel(KvArgs a) {
-    constexpr int NW = many_waves(HD), N = kKvManyRows / (16 * NW), CW = 2;
-    constexpr int U = HD == 64 ? 2 : 1;  // units of a stage
-    using A = Attend<T, HD, EXACT, CW, N>;
+    constexpr int NW = many_waves(HK), N = kKvManyRows / (16 * NW), CW = 2;
+    constexpr int U = HK == 64 ? 2 : 1;  // units of a stage
+    using A = Attend<T, HK, HV, EXACT, CW, N>;
     using V8 = typename T::vec8;
     // a stage in operand order, 1 KB each: keys [unit][tile][step], values [unit][tile of O^T]
     constexpr int KW = U * 2 * A::KS * 512, STAGE = KW + U * A::NT * 512;
-    static_assert(U * 2 * A::KS == 2 * NW && U * A::NC == NW, "a wave's share of a stage");
+    constexpr int KO = U * 2 * A::KS / NW;  // key operands that a wave stages
+    static_assert(KO * NW == U * 2 * A::KS && A::KS % KO == 0 && U * A::NC == NW,
+                  "a wave's share of a stage");
     __shared__ __attribute__((aligned(16))) uint16_t smem[3][STAGE];
     __shared__ int marks[3][NW];  // whether a wave took non-finite values out of the stage
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -548,8 +549,8 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
 
     const Full full_wave(job, wa, lo_wb, a.p.sinks), full_block(job, job.pa, job.lo_b, a.p.sinks);
 
-    // ---- what the wave stages: two key operands and 32 columns of the values of one unit ----
-    const int su = wave / A::NC, vc = wave % A::NC, o0 = 2 * wave % (2 * A::KS);
+    // ---- what the wave stages: key operands of one tile and 32 columns of the values of one unit ----
+    const int su = wave / A::NC, vc = wave % A::NC, o0 = KO * wave % (2 * A::KS);
     // Where a stage's tiles lie (bytes from the head's first page): lane i of these holds the places
     // of stage (group of 64) + i.
     long long key_at = 0, value_at0 = 0, value_at1 = 0;
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
     auto at = [](const uint16_t* p, long long bytes) {
         return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p) + bytes);
     };
-    u32x4 k[2];
+    u32x4 k[KO];
     typename A::Row v[8];
     auto load = [&](int st) {
         const int i = st & 63;
@@ -583,7 +584,7 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
         const uint16_t* v0 = at(s.values_of_head, of_lane(value_at0, i));
         const uint16_t* v1 = at(s.values_of_head, of_lane(value_at1, i));
 #pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2)
+        for (int i2 = 0; i2 < KO; ++i2)
             k[i2] = s.load_key(kt, o0 % A::KS + i2);
 #pragma unroll
         for (int i2 = 0; i2 < 8; ++i2)
@@ -598,7 +599,7 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
         }
         uint16_t* const buf = smem[b] + s.lane * 8;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < KO; ++i)
             *reinterpret_cast<u32x4*>(buf + (su * 2 * A::KS + o0 + i) * 512) = k[i];
 #pragma unroll
         for (int e = 0; e < CW; ++e)
@@ -608,7 +609,24 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
     auto read = [&](const uint16_t* p, int slot) {
         return *reinterpret_cast<const V8*>(p + s.lane * 8 + slot * 512);
     };
-    auto scores = [&](floatx4 (&sc)[U][N][2], const V8 (&ko)[NK]) {
+    const int stages = (job.u1 - job.u0 + U - 1) / U;
+    load(0);
+    store(0, 0);
+    load(1);
+    store(1, 1);
+    load(2);
+    // Stage st lies in buffer b, stage st + 1 in b1; b2, free since the last barrier, takes stage
+    // st + 2.  (Units behind the last are staged as the last and not used.)
+    int b = 0, b1 = 1, b2 = 2;
+    for (int st = 0; st < stages; ++st) {
+        __syncthreads();
+        V8 ko[NK], ring[AHEAD];
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+            ko[i] = read(smem[b], i);
+        store(st + 2, b2);
+        load(st + 3);
+        floatx4 sc[U][N][2];
 #pragma unroll
         for (int x = 0; x < U; ++x) {
 #pragma unroll
@@ -622,37 +640,10 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
                     for (int t = 0; t < N; ++t)
                         sc[x][t][tt] = T::mma32(ko[(x * 2 + tt) * A::KS + i], s.q[t][i], sc[x][t][tt]);
         }
-    };
-    const int stages = (job.u1 - job.u0 + U - 1) / U;
-    load(0);
-    store(0, 0);
-    load(1);
-    store(1, 1);
-    load(2);
-    __syncthreads();
-    floatx4 sc[U][N][2];
-    {
-        V8 ko[NK];
-#pragma unroll
-        for (int i = 0; i < NK; ++i)
-            ko[i] = read(smem[0], i);
-        scores(sc, ko);
-    }
-    // Stage st: its scores are there, its values in buffer b, stage st + 1 in buffer b1.  Buffer b2,
-    // free since the last barrier, takes stage st + 2.  (Units behind the last are staged as the last
-    // and not used.)
-    int b = 0, b1 = 1, b2 = 2;
-    for (int st = 0; st < stages; ++st) {
-        // the next scores' operands, and the first values', on their way before they are needed
-        V8 ko[NK], ring[AHEAD];
-#pragma unroll
-        for (int i = 0; i < NK; ++i)
-            ko[i] = read(smem[b1], i);
+        // the first of the values' operands on their way while the weights are computed
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
             ring[i] = read(smem[b] + KW, i);
-        store(st + 2, b2);
-        load(st + 3);
 #pragma unroll
         for (int x = 0; x < U; ++x) {
             const int u = job.u0 + st * U + x;
@@ -660,24 +651,28 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
                 s.mask(sc[x], u < job.u1 ? first_key(job, u) : INT_MAX - 31);
         }
         s.raise(sc);
-        floatx4 next[U][N][2];
-        scores(next, ko);
         V8 hi[U][N], lw[U][N];
 #pragma unroll
         for (int x = 0; x < U; ++x)
             s.weights(sc[x], hi[x], lw[x]);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const V8 y = ring[i % AHEAD];
-            if (i + AHEAD < NV)
-                ring[i % AHEAD] = read(smem[b] + KW, i + AHEAD);
+        for (int i = 0; i < NV; i += 2) {  // (two tiles at a time: a sum is added to every 4th product)
+            const V8 y[2] = {ring[i % AHEAD], ring[(i + 1) % AHEAD]};
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (i + j + AHEAD < NV)
+                    ring[(i + j) % AHEAD] = read(smem[b] + KW, i + j + AHEAD);
             const int x = i / A::NT, tile = i % A::NT;
 #pragma unroll
-            for (int t = 0; t < N; ++t)
-                s.acc[t][tile] = T::mma32(y, hi[x][t], s.acc[t][tile]);
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int t = 0; t < N; ++t)
-                s.acc[t][tile] = T::mma32(y, lw[x][t], s.acc[t][tile]);
+                for (int t = 0; t < N; ++t)
+                    s.acc[t][tile + j] = T::mma32(y[j], hi[x][t], s.acc[t][tile + j]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int t = 0; t < N; ++t)
+                    s.acc[t][tile + j] = T::mma32(y[j], lw[x][t], s.acc[t][tile + j]);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -692,14 +687,6 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
                     s.add_nonfinite(s.find_pages(u), first_key(job, u), hi[x], lw[x]);
             }
         }
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < U; ++x)
-#pragma unroll
-            for (int t = 0; t < N; ++t)
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-                    sc[x][t][tt] = next[x][t][tt];
         const int b0 = b;
         b = b1;
         b1 = b2;
@@ -750,26 +737,29 @@ __global__ __launch_bounds__(64 * many_waves(HD)) __attribute__((
     }
 }
 
-template <typename T, int HD, bool EXACT>
+template <typename T, int HK, int HV, bool EXACT>
 hipError_t launch_one(const KvArgs& a, bool many, hipStream_t stream) {
+    const dim3 grid((unsigned)((many ? a.jobs_m : a.jobs_f) * a.p.kv_heads));
     if (many)
-        hipLaunchKernelGGL((kv_many_kernel<T, HD, EXACT>), dim3((unsigned)(a.jobs_m * a.p.kv_heads)),
-                           dim3(64 * many_waves(HD)), 0, stream, a);
+        hipLaunchKernelGGL((kv_many_kernel<T, HK, HV, EXACT>), grid, dim3(64 * many_waves(HK)), 0,
+                           stream, a);
     else
-        hipLaunchKernelGGL((kv_few_kernel<T, HD, EXACT>), dim3((unsigned)(a.jobs_f * a.p.kv_heads)),
-                           dim3(kKvThreads), 0, stream, a);
+        hipLaunchKernelGGL((kv_few_kernel<T, HK, HV, EXACT>), grid, dim3(kKvThreads), 0, stream, a);
     return hipGetLastError();
+}
+
+template <typename T, int HK, int HV>
+hipError_t launch_width(const KvArgs& a, bool many, hipStream_t stream) {
+    return a.p.dim == HK && a.p.v_dim == HV ? launch_one<T, HK, HV, true>(a, many, stream)
+                                            : launch_one<T, HK, HV, false>(a, many, stream);
 }
 
 template <typename T>
 hipError_t launch_list(const KvArgs& a, bool many, hipStream_t stream) {
-    const int w = a.p.width;
-    const bool exact = a.p.dim == w && a.p.v_dim == w;
-    if (w == 64)
-        return exact ? launch_one<T, 64, true>(a, many, stream) : launch_one<T, 64, false>(a, many, stream);
-    if (w == 128)
-        return exact ? launch_one<T, 128, true>(a, many, stream) : launch_one<T, 128, false>(a, many, stream);
-    return exact ? launch_one<T, 256, true>(a, many, stream) : launch_one<T, 256, false>(a, many, stream);
+    return a.p.width == 64    ? launch_width<T, 64, 64>(a, many, stream)
+           : a.p.width == 128 ? launch_width<T, 128, 128>(a, many, stream)
+           : a.p.width == 192 ? launch_width<T, 192, 128>(a, many, stream)
+                              : launch_width<T, 256, 256>(a, many, stream);
 }
 
 }  // namespace

@@ -249,7 +249,7 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
     const long long own = std::min(flat, (long long)max_q_len * p.group);
     // Workgroups that 256 compute units hold.
     const int at_once_f = p.width == 64 ? 1536 : p.width == 128 ? 768 : 512;
-    const int at_once_m = 512;
+    const int at_once_m = p.width == 256 ? 256 : 512;
     p.slots_f = std::max(1, at_once_f / kv_heads);
     p.slots_m = std::max(1, at_once_m / kv_heads);
     const int many = kKvManyRows;

@@ -41,10 +41,13 @@ constexpr int kKvFewRows = 16;  // rows of a block of the first list
 constexpr int kKvFew = 32;      // sessions of up to so many flat rows are on it
 constexpr int kKvManyRows = 128;  // rows of a block of the other
 constexpr int kKvTile = 32;     // keys of a unit
-// Widths that kernels exist for: both head sizes are padded to the smallest that holds them.
+// Widths of keys that kernels exist for; their values have the same, beside 192 128.  A shape takes
+// the smallest that holds it.
 __host__ __device__ inline int kv_width(int dim, int v_dim) {
-    const int w = dim > v_dim ? dim : v_dim;
-    return w <= 64 ? 64 : w <= 128 ? 128 : 256;
+    return dim <= 64 && v_dim <= 64     ? 64
+           : dim <= 128 && v_dim <= 128 ? 128
+           : dim <= 192 && v_dim <= 128 ? 192
+                                        : 256;
 }
 
 constexpr int kKvJobInts = 8;  // session, its first query row, first flat row, rows, first and last
