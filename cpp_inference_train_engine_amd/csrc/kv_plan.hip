@@ -4,8 +4,9 @@
 //
 // One workgroup, its tables in LDS (in the plan for large batches).  A session's flat rows
 // (mla_kv.hpp) are cut into blocks, and the units of 32 keys that a block sees into ranges: of a
-// length that gives every slot of the GPU one range where there are fewer blocks than slots, and
-// of twice a slot's share (so that only blocks well above it are cut) where there are more.
+// length that gives every slot of the GPU one range (several where they are long, so that slots
+// with short ones take more of them), or of twice a slot's share (so that only blocks well above it
+// are cut) where there are more blocks than that.
 #include "mla_kv.hpp"
 
 #include <algorithm>
@@ -16,8 +17,9 @@ namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kLdsBlocks = 2800, kLdsSessions = 1400;
-constexpr int kTables = 4, kTries = 24;
+constexpr int kTables = 4, kTries = 24, kEven = 2;
 constexpr int kMinF = 4, kMinM = 16;  // least units of a range
+constexpr int kRounds = 4, kRoundUnits = 24;  // most ranges of a slot, and their least units
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
 
@@ -63,7 +65,7 @@ __device__ __forceinline__ int find(const int32_t* starts, int n, int i) {
 template <bool ON_CHIP>
 __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
     __shared__ int32_t lds[ON_CHIP ? kTables * kLdsBlocks + 2 * kLdsSessions : 1];
-    __shared__ int tmp[kWaves][2], tries[kTries], first_bad;
+    __shared__ int tmp[kWaves][2], tries[kEven + kTries], first_bad;
     __shared__ unsigned long long sum;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const KvShape& p = a.p;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
                 start[s] = blocks + v[0] - mine;
             blocks += total[0];
         }
-        if (tid < kTries)
+        if (tid < kEven + kTries)
             tries[tid] = 0;
         if (tid == 0)
             sum = 0;
@@ -134,13 +136,20 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
             atomicAdd(&sum, mine);
         __syncthreads();
         // ---- the length of a range ----
-        const int share = (int)std::min<unsigned long long>((sum + slots - 1) / slots, 1 << 26);
+        const unsigned long long whole = (sum + slots - 1) / slots;
+        const int rounds =
+            list ? 1 : (int)std::max<unsigned long long>(std::min<unsigned long long>(whole / kRoundUnits, kRounds), 1);
+        const int goal = slots * rounds;
         const int least = list ? kMinM : kMinF;
-        auto length = [&](int c) { return (std::max(share + (int)((long long)share * c / 8), least) + 3) & ~3; };
-        int len = length(8);
-        if (blocks <= slots) {
-            // the shortest candidate, from a slot's share on, whose ranges all run at once
-            if (lane < kTries) {
+        // Candidates: up to an eighth above a slot's share, then from a share of the goal on.
+        auto length = [&](int c) {
+            const int wanted = c < kEven ? slots : goal;
+            const long long share = std::min<long long>((sum + wanted - 1) / wanted, 1 << 26);
+            return (int)(std::max(share + share * (c < kEven ? c : c - kEven) / 8, (long long)least) + 3) & ~3;
+        };
+        int len = length(kEven + 8);
+        if (blocks <= goal) {
+            if (lane < kEven + kTries) {
                 const float inv = 1.0f / (float)length(lane);
                 int n = 0;
                 for (int b = wave; b < blocks; b += kWaves)
@@ -148,9 +157,14 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
                 atomicAdd(&tries[lane], n);
             }
             __syncthreads();
+            // One even range for every slot, if there is such a length; else the shortest of those
+            // that make no more ranges than wanted.
             int c = 0;
-            while (c < kTries - 1 && tries[c] > slots)
+            while (c < kEven && tries[c] > slots)
                 ++c;
+            if (c == kEven)
+                while (c < kEven + kTries - 1 && tries[c] > goal)
+                    ++c;
             len = length(c);
         }
         // ---- jobs and partial rows of each block ----
@@ -258,13 +272,14 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
         few ? std::min<long long>((long long)B * (kKvFew / kKvFewRows), flat / kKvFewRows + B) : 0;
     const long long blocks_m =
         own > kKvFew ? flat / many + std::min<long long>(B, flat / (kKvFew + 1)) : 0;
-    // A range is at least a slot's share long, so that a list's blocks have at most
-    // units / share + blocks <= slots + blocks ranges; those that are cut have fewer than twice
+    // A range is at least a share of the goal long, so that a list's blocks have at most
+    // units / share + blocks <= goal + blocks ranges; those that are cut have fewer than twice
     // units / share, of a block's rows each.
-    p.max_jobs_f = (int)std::min<long long>(blocks_f ? blocks_f + p.slots_f : 0, INT_MAX);
+    const long long goal_f = (long long)kRounds * p.slots_f;
+    p.max_jobs_f = (int)std::min<long long>(blocks_f ? blocks_f + goal_f : 0, INT_MAX);
     p.max_jobs_m = (int)std::min<long long>(blocks_m ? blocks_m + p.slots_m : 0, INT_MAX);
     p.max_blocks = (int)std::min<long long>(std::max(blocks_f, blocks_m), INT_MAX);
-    p.max_parts = (p.max_jobs_f ? 2LL * p.slots_f * kKvFewRows : 0) +
+    p.max_parts = (p.max_jobs_f ? 2 * goal_f * kKvFewRows : 0) +
                   (p.max_jobs_m ? 2LL * p.slots_m * many : 0);
     p.tables_at = kKvHead;
     const bool on_chip = p.max_blocks <= kLdsBlocks && B <= kLdsSessions;
