@@ -19,6 +19,12 @@ constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kLdsBlocks = 2800, kLdsSessions = 1400;
 constexpr int kTables = 4, kTries = 24, kEven = 2;
 constexpr int kMinF = 4, kMinM = 16;  // least units of a range
+// Blocks of the first list are left whole where the longest, taken by its four waves alone, takes no
+// longer than the second launch, which joins what was cut, and a quarter of the time that memory
+// needs for all of them: in ns.  (50 sessions of 900 to 1,100 tokens, 32 heads, kv 8 x 128: 42 us whole,
+// 52 cut in two; 100 of 10 to 5,000: 200 and 183.)
+constexpr int kJoin = 7000, kBytesPerNs = 6500;
+__device__ __forceinline__ int unit_ns(int dim, int v_dim) { return 80 + 15 * (dim + v_dim) / 16; }
 constexpr int kRounds = 4, kRoundUnits = 24;  // most ranges of a slot, and their least units
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
@@ -65,7 +71,7 @@ __device__ __forceinline__ int find(const int32_t* starts, int n, int i) {
 template <bool ON_CHIP>
 __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
     __shared__ int32_t lds[ON_CHIP ? kTables * kLdsBlocks + 2 * kLdsSessions : 1];
-    __shared__ int tmp[kWaves][2], tries[kEven + kTries], first_bad;
+    __shared__ int tmp[kWaves][2], tries[kEven + kTries], longest, first_bad;
     __shared__ unsigned long long sum;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const KvShape& p = a.p;
@@ -117,11 +123,14 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
         }
         if (tid < kEven + kTries)
             tries[tid] = 0;
-        if (tid == 0)
+        if (tid == 0) {
             sum = 0;
+            longest = 0;
+        }
         __syncthreads();
         // ---- the units that each sees ----
         unsigned long long mine = 0;
+        int most = 0;
         for (int b = tid; b < blocks; b += kThreads) {
             const int s = find(start, B, b), f0 = (b - start[s]) * per, n = flat(s);
             const int keys = a.cu_k[s + 1] - a.cu_k[s], ctx = keys - n / G;
@@ -129,11 +138,16 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
             session[b] = s;
             units[b] = kv_units(ctx + f0 / G, ctx + last / G, p.window, p.sinks).count;
             mine += units[b];
+            most = std::max(most, units[b]);
         }
-        for (int d = 32; d > 0; d >>= 1)
+        for (int d = 32; d > 0; d >>= 1) {
             mine += __shfl_xor(mine, d, 64);
-        if (lane == 0 && mine != 0)
+            most = std::max(most, __shfl_xor(most, d, 64));
+        }
+        if (lane == 0 && mine != 0) {
             atomicAdd(&sum, mine);
+            atomicMax(&longest, most);
+        }
         __syncthreads();
         // ---- the length of a range ----
         const unsigned long long whole = (sum + slots - 1) / slots;
@@ -148,7 +162,12 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
             return (int)(std::max(share + share * (c < kEven ? c : c - kEven) / 8, (long long)least) + 3) & ~3;
         };
         int len = length(kEven + 8);
-        if (blocks <= goal) {
+        const unsigned long long memory =
+            sum * p.kv_heads * (kKvTile * 2 * (p.dim + p.v_dim)) / kBytesPerNs;
+        if (list == 0 && (unsigned long long)longest * unit_ns(p.dim, p.v_dim) <=
+                             kJoin + memory / 4) {
+            len = (longest + 3) & ~3;
+        } else if (blocks <= goal) {
             if (lane < kEven + kTries) {
                 const float inv = 1.0f / (float)length(lane);
                 int n = 0;
@@ -166,6 +185,8 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
                 while (c < kEven + kTries - 1 && tries[c] > goal)
                     ++c;
             len = length(c);
+            if (len > longest - longest / 4)  // (would shorten little)
+                len = (longest + 3) & ~3;
         }
         // ---- jobs and partial rows of each block ----
         int at = 0;
