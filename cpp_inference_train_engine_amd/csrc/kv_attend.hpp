@@ -17,9 +17,9 @@
 // P^T enters in two 16-bit parts, e = hi + lo, off by 2^-17 of it (bf16) or 2^-23 (fp16) at most:
 // only the row is rounded to 16 bits.
 //
-// kv_few_kernel -- a job of at most 16 rows: each of four waves holds all of them and takes every
-//   4th unit, straight from memory into the operands' registers; the waves' states meet in LDS at
-//   the end.
+// kv_few_kernel -- a job of at most 16 or 32 rows: each of four waves holds all of them and takes
+//   every 4th unit, straight from memory into the operands' registers; the waves' states meet in LDS
+//   at the end.
 // kv_many_kernel -- a job of 128 rows: each of four waves holds 32 (of eight 16 above width 128).
 //   They stage 32 keys (64 at width 64) together in LDS, in operand order, into one of three
 //   buffers: one barrier a stage, and every LDS access is 16 bytes a lane in a row.
@@ -386,11 +386,11 @@ struct Attend {
     }
 };
 
-template <typename T, int HK, int HV, bool EXACT>
-__global__ __launch_bounds__(kKvThreads) __attribute__((
-    amdgpu_waves_per_eu(HK == 64 ? 4 : HK == 128 ? 3 : 2, 8))) void kv_few_kernel(KvArgs a) {
+template <typename T, int HK, int HV, int N, bool EXACT>
+__global__ __launch_bounds__(kKvThreads) __attribute__((amdgpu_waves_per_eu(
+    HK == 64 ? 5 - N : HK == 128 ? 4 - N : 2, 8))) void kv_few_kernel(KvArgs a) {
     constexpr int CW = HV >= 128 ? 8 : 4, PITCH = HV + 4;
-    using A = Attend<T, HK, HV, EXACT, CW, 1>;
+    using A = Attend<T, HK, HV, EXACT, CW, N>;
     using V8 = typename T::vec8;
     __shared__ __attribute__((aligned(16))) float smem[4][16 * PITCH + 32];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -428,18 +428,23 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
     }
     for (; u < job.u1; u += 4) {
         const int key0 = first_key(job, u);
-        floatx4 sc[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
+        floatx4 sc[1][N][2];
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+            sc[0][t][0] = sc[0][t][1] = floatx4{0, 0, 0, 0};
 #pragma unroll
         for (int st = 0; st < A::KS; ++st)
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
-                sc[0][0][tt] = T::mma32(__builtin_bit_cast(V8, k[tt][st]), s.q[0][st], sc[0][0][tt]);
+#pragma unroll
+                for (int t = 0; t < N; ++t)
+                    sc[0][t][tt] = T::mma32(__builtin_bit_cast(V8, k[tt][st]), s.q[t][st], sc[0][t][tt]);
         load_keys(next);
         const bool full = full_units.has(u);
         if (!full)
             s.mask(sc[0], key0);
         s.raise(sc);
-        V8 hi[1], lw[1];
+        V8 hi[N], lw[N];
         s.weights(sc[0], hi, lw);
         bool bad = false;
         if (!full)
@@ -451,8 +456,12 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
 #pragma unroll
             for (int e = 0; e < CW; ++e) {
                 const V8 x = __builtin_bit_cast(V8, A::transposed(v[c], e));
-                s.acc[0][c * CW + e] = T::mma32(x, hi[0], s.acc[0][c * CW + e]);
-                s.acc[0][c * CW + e] = T::mma32(x, lw[0], s.acc[0][c * CW + e]);
+#pragma unroll
+                for (int t = 0; t < N; ++t)
+                    s.acc[t][c * CW + e] = T::mma32(x, hi[t], s.acc[t][c * CW + e]);
+#pragma unroll
+                for (int t = 0; t < N; ++t)
+                    s.acc[t][c * CW + e] = T::mma32(x, lw[t], s.acc[t][c * CW + e]);
             }
         if (__builtin_amdgcn_ballot_w64(bad))
             s.add_nonfinite(now, key0, hi, lw);
@@ -462,55 +471,62 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
     }
 
     // ---- the waves' states become rows, or partials ----
-    const float l = rows_sum(s.l[0]);
-    float* mine = smem[wave];
-#pragma unroll
-    for (int c = 0; c < A::NC; ++c)
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-#pragma unroll
-            for (int e = 0; e < CW; e += 4) {
-                const int x = c * CW + e;
-                *reinterpret_cast<floatx4*>(mine + s.n * PITCH + s.column(x, y)) =
-                    floatx4{s.acc[0][x][y], s.acc[0][x + 1][y], s.acc[0][x + 2][y], s.acc[0][x + 3][y]};
-            }
-    if (s.g == 0) {
-        mine[16 * PITCH + s.n] = s.m[0];
-        mine[16 * PITCH + 16 + s.n] = l;
-    }
-    __syncthreads();
     const int DV = s.DV, per_row = DV / 4;
-    for (int e = tid; e < job.rows * per_row; e += kKvThreads) {
-        const int r = e / per_row, c = (e - r * per_row) * 4;
-        float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-            M = fmaxf(M, smem[w][16 * PITCH + r]);
-        float L = 0.0f;
-        floatx4 o = {0, 0, 0, 0};
+    for (int t = 0; t < N; ++t) {
+        if (16 * t >= job.rows)
+            break;
+        const float l = rows_sum(s.l[t]);
+        float* mine = smem[wave];
+        if (t > 0)
+            __syncthreads();  // the rows before have been read
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float mv = smem[w][16 * PITCH + r];
-            // A sum of NaN may come with a maximum of -inf (all scores NaN): weight 0 keeps it.
-            const float f = mv == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mv - M);
-            L += smem[w][16 * PITCH + 16 + r] * f;
-            o += *reinterpret_cast<const floatx4*>(&smem[w][r * PITCH + c]) * f;
+        for (int c = 0; c < A::NC; ++c)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int e = 0; e < CW; e += 4) {
+                    const int x = c * CW + e;
+                    *reinterpret_cast<floatx4*>(mine + s.n * PITCH + s.column(x, y)) = floatx4{
+                        s.acc[t][x][y], s.acc[t][x + 1][y], s.acc[t][x + 2][y], s.acc[t][x + 3][y]};
+                }
+        if (s.g == 0) {
+            mine[16 * PITCH + s.n] = s.m[t];
+            mine[16 * PITCH + 16 + s.n] = l;
         }
-        if (job.part < 0) {
-            int in_group;
-            const int i = quotient(job.f0 + r, a.p.group, a.group_inverse, in_group);
-            const long long row = ((long long)job.q0 + i) * a.p.H + head * a.p.group + in_group;
-            const float inv = 1.0f / L;
-            *reinterpret_cast<u32x2*>(a.out + row * DV + c) =
-                u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-            if (a.lse && c == 0)
-                a.lse[row] = (M + __log2f(L)) * kLn2;
-        } else {
-            const long long row = ((long long)job.part + r) * a.p.kv_heads + head;
-            *reinterpret_cast<floatx4*>(a.part_o + row * DV + c) = o;
-            if (c == 0) {
-                a.part_ml[2 * row] = M;
-                a.part_ml[2 * row + 1] = L;
+        __syncthreads();
+        for (int e = tid; e < min(job.rows - 16 * t, 16) * per_row; e += kKvThreads) {
+            const int r = e / per_row, c = (e - r * per_row) * 4;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                M = fmaxf(M, smem[w][16 * PITCH + r]);
+            float L = 0.0f;
+            floatx4 o = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float mv = smem[w][16 * PITCH + r];
+                // A sum of NaN may come with a maximum of -inf (all scores NaN): weight 0 keeps it.
+                const float f = mv == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mv - M);
+                L += smem[w][16 * PITCH + 16 + r] * f;
+                o += *reinterpret_cast<const floatx4*>(&smem[w][r * PITCH + c]) * f;
+            }
+            if (job.part < 0) {
+                int in_group;
+                const int i = quotient(job.f0 + 16 * t + r, a.p.group, a.group_inverse, in_group);
+                const long long row = ((long long)job.q0 + i) * a.p.H + head * a.p.group + in_group;
+                const float inv = 1.0f / L;
+                *reinterpret_cast<u32x2*>(a.out + row * DV + c) =
+                    u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+                if (a.lse && c == 0)
+                    a.lse[row] = (M + __log2f(L)) * kLn2;
+            } else {
+                const long long row = ((long long)job.part + 16 * t + r) * a.p.kv_heads + head;
+                *reinterpret_cast<floatx4*>(a.part_o + row * DV + c) = o;
+                if (c == 0) {
+                    a.part_ml[2 * row] = M;
+                    a.part_ml[2 * row + 1] = L;
+                }
             }
         }
     }
@@ -743,8 +759,11 @@ hipError_t launch_one(const KvArgs& a, bool many, hipStream_t stream) {
     if (many)
         hipLaunchKernelGGL((kv_many_kernel<T, HK, HV, EXACT>), grid, dim3(64 * many_waves(HK)), 0,
                            stream, a);
+    else if (HK == 256 || a.p.few_rows == 16)
+        hipLaunchKernelGGL((kv_few_kernel<T, HK, HV, 1, EXACT>), grid, dim3(kKvThreads), 0, stream, a);
     else
-        hipLaunchKernelGGL((kv_few_kernel<T, HK, HV, EXACT>), grid, dim3(kKvThreads), 0, stream, a);
+        hipLaunchKernelGGL((kv_few_kernel<T, HK, HV, HK == 256 ? 1 : 2, EXACT>), grid, dim3(kKvThreads),
+                           0, stream, a);
     return hipGetLastError();
 }
 

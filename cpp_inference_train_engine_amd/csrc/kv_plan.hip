@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
 
     int jobs[2] = {0, 0}, parts = 0;
     for (int list = 0; list < 2; ++list) {
-        const int per = list ? kKvManyRows : kKvFewRows;
+        const int per = list ? kKvManyRows : p.few_rows;
         const int slots = list ? p.slots_m : p.slots_f;
         const int most_jobs = list ? p.max_jobs_m : p.max_jobs_f;
         if (most_jobs == 0)
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
         for (int s0 = 0; s0 < B; s0 += kThreads) {
             const int s = s0 + tid;
             const int n = s < B ? flat(s) : 0;
-            const int mine = (n <= kKvFew) == (list == 0) ? ceil_div(n, per) : 0;
+            const int mine = (n <= p.few) == (list == 0) ? ceil_div(n, per) : 0;
             int v[2] = {mine, 0}, total[2];
             block_scan2(v, tmp, total);
             if (s < B)
@@ -282,17 +282,22 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
     p.sinks = sinks;
     const long long flat = (long long)rows * p.group;  // of one kv head
     const long long own = std::min(flat, (long long)max_q_len * p.group);
+    // Where no session has more than 16 flat rows, blocks of 16; else of 32 (above width 192, whose
+    // registers hold no more, 16 again), which read the keys half as often.
+    p.few_rows = own <= 16 || p.width == 256 ? 16 : 32;
+    p.few = own <= 16 ? 16 : p.width == 256 ? 32 : 64;
     // Workgroups that 256 compute units hold.
-    const int at_once_f = p.width == 64 ? 1536 : p.width == 128 ? 768 : 512;
+    const int at_once_f = p.width == 64    ? (p.few_rows == 16 ? 1536 : 768)
+                          : p.width == 128 ? (p.few_rows == 16 ? 768 : 512)
+                                           : 512;
     const int at_once_m = p.width == 256 ? 256 : 512;
     p.slots_f = std::max(1, at_once_f / kv_heads);
     p.slots_m = std::max(1, at_once_m / kv_heads);
     const int many = kKvManyRows;
-    const bool few = p.group <= kKvFew;
     const long long blocks_f =
-        few ? std::min<long long>((long long)B * (kKvFew / kKvFewRows), flat / kKvFewRows + B) : 0;
+        p.group <= p.few ? std::min<long long>((long long)B * (p.few / p.few_rows), flat / p.few_rows + B) : 0;
     const long long blocks_m =
-        own > kKvFew ? flat / many + std::min<long long>(B, flat / (kKvFew + 1)) : 0;
+        own > p.few ? flat / many + std::min<long long>(B, flat / (p.few + 1)) : 0;
     // A range is at least a share of the goal long, so that a list's blocks have at most
     // units / share + blocks <= goal + blocks ranges; those that are cut have fewer than twice
     // units / share, of a block's rows each.
@@ -300,7 +305,7 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
     p.max_jobs_f = (int)std::min<long long>(blocks_f ? blocks_f + goal_f : 0, INT_MAX);
     p.max_jobs_m = (int)std::min<long long>(blocks_m ? blocks_m + p.slots_m : 0, INT_MAX);
     p.max_blocks = (int)std::min<long long>(std::max(blocks_f, blocks_m), INT_MAX);
-    p.max_parts = (p.max_jobs_f ? 2 * goal_f * kKvFewRows : 0) +
+    p.max_parts = (p.max_jobs_f ? 2 * goal_f * p.few_rows : 0) +
                   (p.max_jobs_m ? 2LL * p.slots_m * many : 0);
     p.tables_at = kKvHead;
     const bool on_chip = p.max_blocks <= kLdsBlocks && B <= kLdsSessions;

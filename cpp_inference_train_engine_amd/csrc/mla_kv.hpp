@@ -34,12 +34,10 @@ hipError_t launch_kv_append(const KvAppendArgs& a, int dtype, int row_dtype, hip
 // ---- attention ----
 // The query rows of a session that read one kv head, (token, head of the group) one behind the
 // other, are its flat rows.  A job is a block of flat rows over a range of the keys that they see.
-// Sessions of few flat rows go to the list of blocks of 16, whose four waves split the keys; the
-// others to the list of blocks of 128, whose waves split the rows.
+// Sessions of few flat rows go to the list of blocks of 16 or 32 (few_rows), whose four waves split
+// the keys; the others to the list of blocks of 128, whose waves split the rows.
 constexpr int kKvThreads = 256;
-constexpr int kKvFewRows = 16;  // rows of a block of the first list
-constexpr int kKvFew = 32;      // sessions of up to so many flat rows are on it
-constexpr int kKvManyRows = 128;  // rows of a block of the other
+constexpr int kKvManyRows = 128;
 constexpr int kKvTile = 32;     // keys of a unit
 // Widths of keys that kernels exist for; their values have the same, beside 192 128.  A shape takes
 // the smallest that holds it.
@@ -59,6 +57,7 @@ enum { kKvStatus, kKvBad, kKvJobsF, kKvJobsM, kKvParts, kKvRows, kKvTag };
 struct KvShape {
     int B, rows, H, kv_heads, group, dim, v_dim, width, page_size, max_q_len;
     int window, sinks;           // window INT32_MAX: all earlier keys
+    int few_rows, few;           // rows of a block of the first list; most flat rows of its sessions
     int slots_f, slots_m;        // workgroups of a list and kv head that the GPU holds at once
     int max_jobs_f, max_jobs_m;  // of a kv head; 0: no session of these sizes can be on the list
     int max_blocks;
