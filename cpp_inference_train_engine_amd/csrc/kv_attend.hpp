@@ -590,9 +590,11 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
     auto at = [](const uint16_t* p, long long bytes) {
         return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p) + bytes);
     };
-    u32x4 k[KO];
-    typename A::Row v[8];
-    auto load = [&](int st) {
+    struct Loaded {
+        u32x4 k[KO];
+        typename A::Row v[8];
+    };
+    auto load = [&](Loaded& x, int st) {
         const int i = st & 63;
         if (i == 0)
             find_tiles(st);
@@ -601,36 +603,40 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
         const uint16_t* v1 = at(s.values_of_head, of_lane(value_at1, i));
 #pragma unroll
         for (int i2 = 0; i2 < KO; ++i2)
-            k[i2] = s.load_key(kt, o0 % A::KS + i2);
+            x.k[i2] = s.load_key(kt, o0 % A::KS + i2);
 #pragma unroll
         for (int i2 = 0; i2 < 8; ++i2)
-            v[i2] = s.load_value(i2 < 4 ? v0 : v1, vc, i2 & 3);
+            x.v[i2] = s.load_value(i2 < 4 ? v0 : v1, vc, i2 & 3);
     };
-    auto store = [&](int st, int b) {
+    auto store = [&](Loaded& x, int st, int b) {
         const int u = min(job.u0 + st * U + su, job.u1 - 1);
         if (!full_block.has(u)) {
-            const bool bad = __builtin_amdgcn_ballot_w64(s.clean(v, first_key(job, u))) != 0;
+            const bool bad = __builtin_amdgcn_ballot_w64(s.clean(x.v, first_key(job, u))) != 0;
             if (s.lane == 0)
                 marks[b][wave] = bad;
         }
         uint16_t* const buf = smem[b] + s.lane * 8;
 #pragma unroll
         for (int i = 0; i < KO; ++i)
-            *reinterpret_cast<u32x4*>(buf + (su * 2 * A::KS + o0 + i) * 512) = k[i];
+            *reinterpret_cast<u32x4*>(buf + (su * 2 * A::KS + o0 + i) * 512) = x.k[i];
 #pragma unroll
         for (int e = 0; e < CW; ++e)
-            *reinterpret_cast<u32x4*>(buf + KW + (su * A::NT + vc * CW + e) * 512) = A::transposed(v, e);
+            *reinterpret_cast<u32x4*>(buf + KW + (su * A::NT + vc * CW + e) * 512) = A::transposed(x.v, e);
     };
     constexpr int NK = U * 2 * A::KS, NV = U * A::NT, AHEAD = 4;
     auto read = [&](const uint16_t* p, int slot) {
         return *reinterpret_cast<const V8*>(p + s.lane * 8 + slot * 512);
     };
     const int stages = (job.u1 - job.u0 + U - 1) / U;
-    load(0);
-    store(0, 0);
-    load(1);
-    store(1, 1);
-    load(2);
+    Loaded x;
+    {
+        Loaded first;
+        load(first, 0);
+        load(x, 1);
+        store(first, 0, 0);
+        store(x, 1, 1);
+        load(x, 2);
+    }
     // Stage st lies in buffer b, stage st + 1 in b1; b2, free since the last barrier, takes stage
     // st + 2.  (Units behind the last are staged as the last and not used.)
     int b = 0, b1 = 1, b2 = 2;
@@ -640,8 +646,8 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
 #pragma unroll
         for (int i = 0; i < NK; ++i)
             ko[i] = read(smem[b], i);
-        store(st + 2, b2);
-        load(st + 3);
+        store(x, st + 2, b2);
+        load(x, st + 3);
         floatx4 sc[U][N][2];
 #pragma unroll
         for (int x = 0; x < U; ++x) {

@@ -13,7 +13,7 @@ namespace mla {
 namespace {
 
 constexpr int kThreads = 256, kFlight = 4;
-constexpr long long kFewElements = 1 << 20;
+constexpr long long kThreadsAtOnce = 1 << 19;
 constexpr long long kBlocksX = 1 << 20;  // a grid's x: it has fewer than 2^32 threads there
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
@@ -118,10 +118,12 @@ void launch_groups(const KvArgs& a, hipStream_t stream) {
 
 template <typename T>
 hipError_t launch_merge_t(const KvArgs& a, hipStream_t stream) {
-    // few rows: eight groups, so that one round of reads covers 32 partials; many: as many threads
-    // as columns already fill the GPU
-    if ((long long)a.p.rows * a.p.H * a.p.v_dim <= kFewElements)
+    // as many groups as the GPU holds threads for at once (eight: one round of reads covers 32 partials)
+    const long long threads = (long long)a.p.rows * a.p.H * (a.p.v_dim / 4);
+    if (threads * 8 <= kThreadsAtOnce)
         launch_groups<T, 8>(a, stream);
+    else if (threads * 2 <= kThreadsAtOnce)
+        launch_groups<T, 2>(a, stream);
     else
         launch_groups<T, 1>(a, stream);
     return hipGetLastError();
