@@ -596,8 +596,6 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
     };
     auto load = [&](Loaded& x, int st) {
         const int i = st & 63;
-        if (i == 0)
-            find_tiles(st);
         const uint16_t* kt = at(s.keys_of_head, of_lane(key_at, i));
         const uint16_t* v0 = at(s.values_of_head, of_lane(value_at0, i));
         const uint16_t* v1 = at(s.values_of_head, of_lane(value_at1, i));
@@ -608,13 +606,15 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
         for (int i2 = 0; i2 < 8; ++i2)
             x.v[i2] = s.load_value(i2 < 4 ? v0 : v1, vc, i2 & 3);
     };
-    auto store = [&](Loaded& x, int st, int b) {
+    auto clean = [&](Loaded& x, int st, int b) {
         const int u = min(job.u0 + st * U + su, job.u1 - 1);
         if (!full_block.has(u)) {
             const bool bad = __builtin_amdgcn_ballot_w64(s.clean(x.v, first_key(job, u))) != 0;
             if (s.lane == 0)
                 marks[b][wave] = bad;
         }
+    };
+    auto store = [&](const Loaded& x, int b) {
         uint16_t* const buf = smem[b] + s.lane * 8;
 #pragma unroll
         for (int i = 0; i < KO; ++i)
@@ -629,24 +629,36 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
     };
     const int stages = (job.u1 - job.u0 + U - 1) / U;
     Loaded x;
+    find_tiles(0);
     {
         Loaded first;
         load(first, 0);
         load(x, 1);
-        store(first, 0, 0);
-        store(x, 1, 1);
+        clean(first, 0, 0);
+        store(first, 0);
+        clean(x, 1, 1);
+        store(x, 1);
         load(x, 2);
     }
     // Stage st lies in buffer b, stage st + 1 in b1; b2, free since the last barrier, takes stage
     // st + 2.  (Units behind the last are staged as the last and not used.)
     int b = 0, b1 = 1, b2 = 2;
-    for (int st = 0; st < stages; ++st) {
-        __syncthreads();
-        V8 ko[NK], ring[AHEAD];
+    __syncthreads();
+    // The first operands of a stage's scores are read behind the weights of the one before it.
+    constexpr int EARLY = A::KS <= 4 ? NK : 4;
+    V8 ko[NK];
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+    for (int i = 0; i < EARLY; ++i)
+        ko[i] = read(smem[b], i);
+    for (int st = 0; st < stages; ++st) {
+        clean(x, st + 2, b2);
+        if (((st + 3) & 63) == 0)
+            find_tiles(st + 3);
+        // ---- scores; beside them stage st + 2 goes to LDS, and stage st + 3 is sent for ----
+#pragma unroll
+        for (int i = EARLY; i < NK; ++i)
             ko[i] = read(smem[b], i);
-        store(x, st + 2, b2);
+        store(x, b2);
         load(x, st + 3);
         floatx4 sc[U][N][2];
 #pragma unroll
@@ -662,6 +674,7 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
                     for (int t = 0; t < N; ++t)
                         sc[x][t][tt] = T::mma32(ko[(x * 2 + tt) * A::KS + i], s.q[t][i], sc[x][t][tt]);
         }
+        V8 ring[AHEAD];
         // the first of the values' operands on their way while the weights are computed
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
@@ -677,6 +690,9 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
 #pragma unroll
         for (int x = 0; x < U; ++x)
             s.weights(sc[x], hi[x], lw[x]);
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i)
+            ko[i] = read(smem[b1], i);
 #pragma unroll
         for (int i = 0; i < NV; i += 2) {  // (two tiles at a time: a sum is added to every 4th product)
             const V8 y[2] = {ring[i % AHEAD], ring[(i + 1) % AHEAD]};
@@ -709,6 +725,7 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
                     s.add_nonfinite(s.find_pages(u), first_key(job, u), hi[x], lw[x]);
             }
         }
+        __syncthreads();
         const int b0 = b;
         b = b1;
         b1 = b2;
