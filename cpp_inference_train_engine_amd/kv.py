@@ -14,14 +14,15 @@ from __future__ import annotations
 from . import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, PLAN_INFO_INTS, check, lib, ptr, stream_handle)
 from .ops import RaggedBatch, _allocating_on, _check, _check_list, _dtype_of, _gpu, _torch
 
-_row_codes = None
+_row_codes = _int32 = None
 
 
 def _row_code(dtype) -> int | None:
     """MLA_DTYPE_* of appended rows."""
-    global _row_codes
+    global _row_codes, _int32
     if _row_codes is None:
         torch = _torch()
+        _int32 = torch.int32
         _row_codes = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
     return _row_codes.get(dtype)
 
@@ -109,6 +110,18 @@ class Rotation:
 _NO_ROTATION = (None, 0, 0, 1)
 
 
+def _ints(what: str, t, T: int, gpu: int) -> int:
+    """Address of T integers, one for each row."""
+    if t.dtype is not _int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{what}: wanted a contiguous int32 tensor of one dimension, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    if t.shape[0] < T:
+        raise ValueError(f"{what}: {t.shape[0]} for {T} rows")
+    if t.get_device() != gpu:
+        raise ValueError(f"{what}: wanted on the current GPU, is on {t.device}")
+    return t.data_ptr()
+
+
 def _rows(what: str, t, heads: int, dim: int, T: int, dtype, gpu: int):
     """Address and strides of rows [T, heads, dim] whose columns lie one behind the other."""
     if t.dtype is not dtype or t.shape != (T, heads, dim):
@@ -130,31 +143,27 @@ def append_kv(cache: PagedKVCache, layer: int, k, v, slot_mapping, *, rotation: 
     rotated the same way and returned, in ``q_out`` or a new tensor [T, H, head_dim] of the cache's
     type (rows of skipped slots, too).  k, v and q are fp32 or 16-bit rows of one type; slices of
     one projection's rows are taken as they are.  Without ``rotation`` nothing is turned."""
-    torch, gpu, T = _torch(), _gpu(), int(k.shape[0])
+    gpu, T, rows = _gpu(), k.shape[0], k.dtype
     heads, dim, v_dim, page = cache._shape
-    code = _row_code(k.dtype)
+    code = _row_code(rows)
     if code is None:
-        raise ValueError(f"k: wanted float32, float16 or bfloat16 rows, got {k.dtype}")
-    ka = _rows("k", k, heads, dim, T, k.dtype, gpu)
-    va = _rows("v", v, heads, v_dim, T, k.dtype, gpu)
+        raise ValueError(f"k: wanted float32, float16 or bfloat16 rows, got {rows}")
+    ka = _rows("k", k, heads, dim, T, rows, gpu)
+    va = _rows("v", v, heads, v_dim, T, rows, gpu)
     qa, H, out = (None, 0, 0), heads, None
     if q is not None:
-        H = int(q.shape[1])
-        qa = _rows("q", q, H, dim, T, k.dtype, gpu)
+        H = q.shape[1]
+        qa = _rows("q", q, H, dim, T, rows, gpu)
         if q_out is None:
             with _allocating_on(stream):
-                q_out = torch.empty((T, H, dim), dtype=cache._dtype, device=q.device)
+                q_out = _torch().empty((T, H, dim), dtype=cache._dtype, device=q.device)
         out = _check("q_out", q_out, (T, H, dim), cache._dtype, gpu)
-    slots = _check_list("slot_mapping", slot_mapping, gpu)
-    if slot_mapping.numel() < T:
-        raise ValueError(f"slot_mapping: {slot_mapping.numel()} slots for {T} rows")
+    slots = _ints("slot_mapping", slot_mapping, T, gpu)
     at, turn = None, _NO_ROTATION
     if rotation is not None:
         if positions is None:
             raise ValueError("positions: a rotation needs them")
-        at = _check_list("positions", positions, gpu)
-        if positions.numel() < T:
-            raise ValueError(f"positions: {positions.numel()} for {T} rows")
+        at = _ints("positions", positions, T, gpu)
         if rotation._place != gpu:
             raise ValueError(f"rotation: wanted on the current GPU, is on {rotation.frequencies.device}")
         turn = rotation._args
