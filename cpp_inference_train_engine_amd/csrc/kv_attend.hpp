@@ -386,9 +386,19 @@ struct Attend {
     }
 };
 
+// Waves a SIMD: as many as hold a unit, the rows and O^T without spilling.  (64 decode rows, kv 4 x
+// 256: 168 us at one wave, 195 at two, which spill; kv 8 x 96 in the kernel of width 128: 131 at two,
+// 154 at three.)
+constexpr int few_occupancy(int width, int tiles, bool exact) {
+    return width == 64                ? 5 - tiles
+           : width == 128 && exact    ? 4 - tiles
+           : width == 256 && exact    ? 1
+                                      : 2;
+}
+
 template <typename T, int HK, int HV, int N, bool EXACT>
-__global__ __launch_bounds__(kKvThreads) __attribute__((amdgpu_waves_per_eu(
-    HK == 64 ? 5 - N : HK == 128 ? 4 - N : 2, 8))) void kv_few_kernel(KvArgs a) {
+__global__ __launch_bounds__(kKvThreads) __attribute__((
+    amdgpu_waves_per_eu(few_occupancy(HK, N, EXACT), 8))) void kv_few_kernel(KvArgs a) {
     constexpr int CW = HV >= 128 ? 8 : 4, PITCH = HV + 4;
     using A = Attend<T, HK, HV, EXACT, CW, N>;
     using V8 = typename T::vec8;
