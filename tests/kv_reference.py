@@ -95,46 +95,47 @@ class Batch:
         return seen
 
     def expect(self, window=None, sinks=0):
-        """Rows, lse, and what may be off of both.
-
-        A score sums its products in 32 bits, at most 8 steps of 32 (5 levels each): 13 roundings of
-        2^-24 of sum |q k|, and one more each for its scale and its distance from the maximum: within
-        2^-20 of s = scale sum |q k|, twice that between two scores.  Exponentials 2^-22.  The weight's
-        two parts 2^-17.  Sums over n keys: n / 16 additions of 2^-24.  All of it of the mass of
-        absolute values.  Then half a step of the row, and half of fp16's smallest step."""
+        """Rows, lse, and what may be off of both (see attention)."""
         to = lambda x: x.to("cuda" if torch.cuda.is_available() else "cpu")
-        out = to(torch.zeros((self.rows, self.H, self.DV), dtype=torch.float64))
-        lse = to(torch.zeros((self.rows, self.H), dtype=torch.float64))
+        got = [to(torch.zeros((self.rows, self.H, *n), dtype=torch.float64)) for n in ((self.DV,), (), (self.DV,), ())]
         all_k, all_v, all_q = to(self.k), to(self.v), to(self.q)
-        off, off_lse = torch.zeros_like(out), torch.zeros_like(lse)
         r0, G = 0, self.H // self.KH
         for b, (n, q) in enumerate(zip(self.lens, self.q_len)):
             if q == 0:
                 continue
             ids = to(self.ids[self.cu[b]:self.cu[b + 1]])
             seen = to(self.sees(b, window, sinks))
-            rows = slice(r0, r0 + q)
             for h in range(self.H):
-                k = all_k[ids, h // G].reshape(-1, self.D)[:n].double()
-                v = all_v[ids, h // G].reshape(-1, self.DV)[:n].double()
-                x = all_q[rows, h].double()
-                s = torch.where(seen, x @ k.T * self.scale, -torch.inf)
-                lse[rows, h] = torch.logsumexp(s, 1)
-                w = torch.softmax(s, 1)
-                # (a value that a row does not see adds nothing to it, whatever it is)
-                fine = torch.where(torch.isfinite(v), v, 0.0)
-                hit = seen.double() @ (~torch.isfinite(v)).double() > 0
-                out[rows, h] = torch.where(hit, torch.nan, w @ fine)
-                mass = w @ fine.abs()
-                size = torch.where(seen, (x.abs() @ k.abs().T) * self.scale, 0.0)
-                size = torch.nan_to_num(size, nan=0.0, posinf=0.0).amax(1)
-                weights = 2.0 ** -19 * size + 2.0 ** -21 + n / 16 * 2.0 ** -24
-                before = (2 * weights + 2.0 ** -17)[:, None] * mass
-                o = torch.nan_to_num(out[rows, h], nan=0.0, posinf=0.0, neginf=0.0)
-                off[rows, h] = before + HALF_STEP[self.dtype] * (o.abs() + before) + 2.0 ** -25
-                off_lse[rows, h] = weights + 2.0 ** -22 * (1 + torch.nan_to_num(lse[rows, h]).abs())
+                k = all_k[ids, h // G].reshape(-1, self.D)[:n]
+                v = all_v[ids, h // G].reshape(-1, self.DV)[:n]
+                for to_, x in zip(got, attention(all_q[r0:r0 + q, h], k, v, seen, self.scale, self.dtype)):
+                    to_[r0:r0 + q, h] = x
             r0 += q
-        return out.cpu(), lse.cpu(), off.cpu(), off_lse.cpu()
+        return [x.cpu() for x in got]
+
+
+def attention(x, k, v, seen, scale, dtype):
+    """Rows, lse, and what may be off of both, of one head's rows x over keys k and values v.
+
+    A score sums its products in 32 bits, at most 8 steps of 32 (5 levels each): 13 roundings of
+    2^-24 of sum |q k|, and one more each for its scale and its distance from the maximum: within
+    2^-20 of s = scale sum |q k|, twice that between two scores.  Exponentials 2^-22.  The weight's
+    two parts 2^-17.  Sums over n keys: n / 16 additions of 2^-24.  All of it of the mass of
+    absolute values.  Then half a step of the row, and half of fp16's smallest step."""
+    x, k, v, n = x.double(), k.double(), v.double(), len(k)
+    s = torch.where(seen, x @ k.T * scale, -torch.inf)
+    lse, w = torch.logsumexp(s, 1), torch.softmax(s, 1)
+    # (a value that a row does not see adds nothing to it, whatever it is)
+    fine = torch.where(torch.isfinite(v), v, 0.0)
+    hit = seen.double() @ (~torch.isfinite(v)).double() > 0
+    out, mass = torch.where(hit, torch.nan, w @ fine), w @ fine.abs()
+    size = torch.where(seen, (x.abs() @ k.abs().T) * scale, 0.0)
+    size = torch.nan_to_num(size, nan=0.0, posinf=0.0).amax(1)
+    weights = 2.0 ** -19 * size + 2.0 ** -21 + n / 16 * 2.0 ** -24
+    before = (2 * weights + 2.0 ** -17)[:, None] * mass
+    o = torch.nan_to_num(out, nan=0.0, posinf=0.0, neginf=0.0)
+    off = before + HALF_STEP[dtype] * (o.abs() + before) + 2.0 ** -25
+    return out, lse, off, weights + 2.0 ** -22 * (1 + torch.nan_to_num(lse).abs())
 
 
 def near(got, want, off, what):

@@ -57,6 +57,21 @@ def test_drafted_rows_and_chunks(gpu, H, KH, D, DV, page, dtype):
     hold(gpu, Batch(H, KH, D, DV, page, dtype, DRAFTS + CHUNKS, seed=H + D + 1))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (9, 2), (40, 33)])
+@pytest.mark.parametrize("H,KH,D,DV,page", [(8, 8, 64, 64, 64), (4, 2, 128, 128, 16), (2, 2, 192, 128, 64),
+                                            (2, 1, 256, 256, 32), (3, 3, 80, 96, 48)])
+def test_drafted_rows_alone(gpu, H, KH, D, DV, page, window, sinks):
+    """At most 16 rows a session and kv head: blocks of 16, of several positions each, with values
+    that are not finite in the last token's."""
+    say(f"drafts {H} {KH} {D} {DV} {page} {window}")
+    c = Batch(H, KH, D, DV, page, BF16, DRAFTS, seed=H + D + 2)
+    for b, n in enumerate(c.lens):
+        at, slot = c.token(b, n - 1)
+        c.v[at, 0, slot, b % DV] = float("inf")
+    hold(gpu, c, window, sinks)
+
+
 WINDOWS = [(1, 0), (1, 1), (31, 4), (32, 0), (33, 33), (64, 1), (100, 128), (257, 5), (5000, 3)]
 
 
