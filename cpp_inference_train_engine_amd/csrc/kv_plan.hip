@@ -18,7 +18,7 @@ namespace {
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kLdsBlocks = 2800, kLdsSessions = 1400;
 constexpr int kTables = 4, kTries = 24, kEven = 2;
-constexpr int kMinF = 4, kMinM = 16;  // least units of a range
+constexpr int kMinF = 4, kMinM = 8;  // least units of a range
 // Blocks of the first list are left whole where the longest, taken by its four waves alone, takes no
 // longer than the second launch, which joins what was cut, and a quarter of the time that memory
 // needs for all of them: in ns.  (50 sessions of 900 to 1,100 tokens, 32 heads, kv 8 x 128: 42 us whole,
