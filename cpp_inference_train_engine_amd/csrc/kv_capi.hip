@@ -98,6 +98,16 @@ int mla_append_kv(void* stream, int T, int n_heads, int n_kv_heads, int head_dim
     if (misaligned({pages, q ? q_out : nullptr}))
         return invalid(fn, "pages and q_out must lie at multiples of 16 bytes");
     const int size = row_dtype == MLA_DTYPE_F32 ? 4 : 2;
+    if (q) {  // a row's columns are read by several threads: none may be written before
+        const long long far[2] = {(T - 1LL) * q_row, (n_heads - 1LL) * q_head};
+        const char* const from = static_cast<const char*>(q);
+        const char* const first = from + (std::min(far[0], 0LL) + std::min(far[1], 0LL)) * size;
+        const char* const behind =
+            from + (std::max(far[0], 0LL) + std::max(far[1], 0LL) + head_dim) * size;
+        const char* const to = static_cast<const char*>(q_out);
+        if (to < behind && first < to + 2LL * T * n_heads * head_dim)
+            return invalid(fn, "q_out overlaps q");
+    }
     KvAppendArgs a{};
     a.T = T;
     a.heads = n_heads;

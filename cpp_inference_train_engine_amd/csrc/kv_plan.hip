@@ -102,13 +102,14 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
     }
 
     int jobs[2] = {0, 0}, parts = 0;
+    bool cut[2] = {false, false};  // whether the list has partial rows
+    auto flat = [&](int s) { return (a.cu_q[s + 1] - a.cu_q[s]) * G; };
     for (int list = 0; list < 2; ++list) {
         const int per = list ? kKvManyRows : p.few_rows;
         const int slots = list ? p.slots_m : p.slots_f;
         const int most_jobs = list ? p.max_jobs_m : p.max_jobs_f;
         if (most_jobs == 0)
             continue;
-        auto flat = [&](int s) { return (a.cu_q[s + 1] - a.cu_q[s]) * G; };
         // ---- the sessions' blocks ----
         int blocks = 0;
         for (int s0 = 0; s0 < B; s0 += kThreads) {
@@ -190,6 +191,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
         }
         // ---- jobs and partial rows of each block ----
         int at = 0;
+        const int before = parts;
         for (int b0 = 0; b0 < blocks; b0 += kThreads) {
             const int b = b0 + tid;
             int n = 0, splits = 0, range = 0;
@@ -213,6 +215,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
         }
         __syncthreads();
         jobs[list] = at;
+        cut[list] = parts > before;
         if (at > most_jobs || parts > p.max_parts)
             break;  // (the bounds hold for every batch of these sizes: never)
         // ---- the jobs, the last rows' first: a prompt's later blocks see more ----
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
             o[7] = part[b] < 0 ? -1 : part[b] + sp * m;
         }
         // ---- what the merge adds up for each row ----
-        for (int e = tid >> 4; e < blocks; e += kThreads / 16) {
+        for (int e = tid >> 4; cut[list] && e < blocks; e += kThreads / 16) {
             const int s = session[e], f0 = (e - start[s]) * per, n = flat(s), m = std::min(per, n - f0);
             const int splits = part[e] < 0 ? 0 : (e + 1 < blocks ? job[e + 1] : at) - job[e];
             for (int r = tid & 15; r < m; r += 16) {
@@ -246,6 +249,13 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
         }
         __syncthreads();
     }
+    if (parts > 0 && cut[0] != cut[1])  // the rows of the list that has no partial ones
+        for (int s = tid >> 4; s < B; s += kThreads / 16) {
+            const int n = flat(s);
+            if ((n <= p.few) == cut[1])
+                for (int r = tid & 15; r < n; r += 16)
+                    a.plan[p.rows_at + ((long long)a.cu_q[s] * G + r) * kKvRowInts + 1] = 0;
+        }
     const bool fits = jobs[0] <= p.max_jobs_f && jobs[1] <= p.max_jobs_m && parts <= p.max_parts;
     if (tid < kKvHead) {
         int v = 0;
@@ -305,8 +315,8 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
     p.max_jobs_f = (int)std::min<long long>(blocks_f ? blocks_f + goal_f : 0, INT_MAX);
     p.max_jobs_m = (int)std::min<long long>(blocks_m ? blocks_m + p.slots_m : 0, INT_MAX);
     p.max_blocks = (int)std::min<long long>(std::max(blocks_f, blocks_m), INT_MAX);
-    p.max_parts = (p.max_jobs_f ? 2 * goal_f * p.few_rows : 0) +
-                  (p.max_jobs_m ? 2LL * p.slots_m * many : 0);
+    p.max_parts = (p.max_jobs_f ? 2 * goal_f * std::min<long long>(p.few_rows, own) : 0) +
+                  (p.max_jobs_m ? 2LL * p.slots_m * std::min<long long>(many, own) : 0);
     p.tables_at = kKvHead;
     const bool on_chip = p.max_blocks <= kLdsBlocks && B <= kLdsSessions;
     p.rows_at = p.tables_at +

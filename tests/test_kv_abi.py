@@ -36,7 +36,8 @@ def test_append_arguments(L):
                dict(pool=-1), dict(pairs=-1), dict(pairs=33), dict(start=-2), dict(start=1), dict(start=50),
                dict(pairs=2 ** 30, start=2), dict(start=2 ** 31 - 2), dict(k=None), dict(v=None), dict(slots=None),
                dict(pages=None), dict(at=None), dict(f=None), dict(q=a), dict(pages=a + 2),
-               dict(q=a, q_out=a + 8)):
+               dict(q=a, q_out=a + 8), dict(q=a, q_out=a), dict(q=a, q_out=a + 16),
+               dict(q=a + 512, q_out=a)):
         assert call(**kw) == 1, kw
         assert b"mla_append_kv" in L.mla_last_error()
     for kw in (dict(D=40), dict(DV=264), dict(page=8), dict(page=65552)):

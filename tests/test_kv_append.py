@@ -154,6 +154,9 @@ def test_refusals(gpu):
                dict(rotation=gpu.Rotation(torch.ones(4, dtype=torch.float64)))):
         with pytest.raises(ValueError):
             call(**kw)
+    h = torch.zeros((5, 4, 32), dtype=torch.float16, device="cuda")
+    with pytest.raises(gpu.MlaError, match="overlaps"):
+        call(k=k.half(), v=v.half(), q=h, q_out=h)
     for r in (gpu.Rotation.of_theta(17), gpu.Rotation.of_theta(8, start=18), gpu.Rotation.of_theta(4, start=1),
               gpu.Rotation.of_theta(4, start=-2)):
         with pytest.raises(gpu.MlaError):
