@@ -25,6 +25,8 @@ constexpr int kMinF = 4, kMinM = 8;  // least units of a range
 // 52 cut in two; 100 of 10 to 5,000: 200 and 183.)
 constexpr int kJoin = 7000, kBytesPerNs = 6500;
 __device__ __forceinline__ int unit_ns(int dim, int v_dim) { return 80 + 15 * (dim + v_dim) / 16; }
+// Of the second list, blocks of up to so many units (2 x 300 rows: 17 us whole, 21 in ranges of 8).
+constexpr int kWholeM = 16;
 constexpr int kRounds = 4, kRoundUnits = 24;  // most ranges of a slot, and their least units
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
@@ -165,8 +167,8 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
         int len = length(kEven + 8);
         const unsigned long long memory =
             sum * p.kv_heads * (kKvTile * 2 * (p.dim + p.v_dim)) / kBytesPerNs;
-        if (list == 0 && (unsigned long long)longest * unit_ns(p.dim, p.v_dim) <=
-                             kJoin + memory / 4) {
+        if (list == 0 ? (unsigned long long)longest * unit_ns(p.dim, p.v_dim) <= kJoin + memory / 4
+                      : longest <= kWholeM) {
             len = (longest + 3) & ~3;
         } else if (blocks <= goal) {
             if (lane < kEven + kTries) {
