@@ -20,9 +20,30 @@
 // kv_few_kernel -- a job of at most 16 or 32 rows: each of four waves holds all of them and takes
 //   every 4th unit, straight from memory into the operands' registers; the waves' states meet in LDS
 //   at the end.
-// kv_many_kernel -- a job of 128 rows: each of four waves holds 32 (of eight 16 above width 128).
+// kv_many_kernel -- a job of 128 rows: each of four waves holds 32 (of eight 16 above width 192).
 //   They stage 32 keys (64 at width 64) together in LDS, in operand order, into one of three
 //   buffers: one barrier a stage, and every LDS access is 16 bytes a lane in a row.
+//
+// What bounds them, and what was measured (MI355X, on which a 2 GiB copy reaches 4.8 TB/s and an
+// 8,192-cubed bf16 product 1,200 TFLOP/s; operations are the formula's, the second part of P^T not
+// counted):
+//   few rows: memory.  Traced: 64 rows, 32 heads on kv 8 x 128, contexts of 128 .. 14,000 tokens
+//     (1.69 GB) 298 us, 5.7 TB/s; two rows on 100,000 .. 131,072 tokens (0.90 GB) 151 us, 6.0; 64
+//     rows, kv 8 x 64, contexts of 128 .. 4,096 (0.29 GB) 47 us.  One row on 1,040 tokens, kv 8 x 64:
+//     10 us, eight workgroups with 9 units a wave, one behind the other.  There a compute unit's own
+//     rate decides: 600 tokens more of kv x 128 (307 KB) take it 5.4 us, and eight waves in place of
+//     four are no faster (700 tokens 12.5 us against 11.1).
+//   many rows: instruction issue.  A prompt of 8,191 rows, 32 heads on kv 8 x 128 (550 GFLOP) 735 us,
+//     0.75 PFLOP/s (1.1 with the second part); 4,093 rows twice through a window of 1,024 (138 GFLOP)
+//     238 us, 0.58.  The matrix cores are busy 49 % of the time: a stage's 48 MFMAs take 768 cycles of
+//     a SIMD for its two waves, their 150 other vector instructions each most of the rest.  LDS is
+//     busy 25 %, the L2 holds 95 % of what is read.  Then at 742 us: without the staging 680, without
+//     the exponentials 697, the products and LDS reads alone 536, P^T in one part 597.
+//   Measured and not kept for many rows (prompt and window; each against its own time then): four
+//     waves a SIMD of 16 rows 840 and 268 us (730, 240); the 32 x 32 products 780 and 250 (724, 240);
+//     64 keys a stage in two buffers 758 and 247 (740, 239); vector instructions spread among the
+//     MFMAs 758 and 248 (746, 245); raised priority for the products 768 and 249 (747, 245); stages
+//     fetched two ahead 722 and 237 (715, 236).
 //
 // A key past a row's position, or between its sinks and its window, adds nothing to the row,
 // whatever it holds: its score is replaced, and its value is taken as zero where no row of the
