@@ -51,10 +51,11 @@ int plan_scalars(const char* fn, int B, int rows, int n_heads, int n_kv_heads, i
         return invalid(fn, "sinks without a window");
     const KvShape p = kv_shape(B, rows, n_heads, n_kv_heads, head_dim, v_dim, page_size, max_q_len,
                                window ? window : INT_MAX, sinks);
-    // (a launch has fewer than 2^32 threads)
+    // (a launch has fewer than 2^32 threads; kv_many_kernel has twice as many at width 256)
+    const int many_threads = p.width == 256 ? 2 * kKvThreads : kKvThreads;
     if (p.max_parts * n_kv_heads > INT_MAX || p.words > (1LL << 40) ||
         (long long)p.max_jobs_f * n_kv_heads * kKvThreads > 0xffffffffLL ||
-        (long long)p.max_jobs_m * n_kv_heads * kKvThreads > 0xffffffffLL)
+        (long long)p.max_jobs_m * n_kv_heads * many_threads > 0xffffffffLL)
         return invalid(fn, "the batch is too large for one plan");
     return MLA_OK;
 }
@@ -90,6 +91,8 @@ int mla_append_kv(void* stream, int T, int n_heads, int n_kv_heads, int head_dim
         rotary_start > head_dim - 2 * pairs)
         return invalid(fn, "the rotated columns, 2 pairs from an even rotary_start on, must lie "
                            "within head_dim");
+    if (((long long)n_heads + n_kv_heads) * head_dim + (long long)n_kv_heads * v_dim > INT_MAX)
+        return fail(MLA_ERR_UNSUPPORTED, std::string(fn) + ": a token's rows have more than 2^31 columns");
     if (T == 0)
         return MLA_OK;
     if (!k || !v || !slot_mapping || !pages || (q && !q_out) ||

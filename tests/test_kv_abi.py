@@ -78,3 +78,15 @@ def test_plan_and_call_arguments(L):
         assert call(**kw) == 1, kw
     # no session can have a key: nothing to do, nothing launched
     assert call(max_pages=0) == 0 and call(pool=0) == 0
+
+
+def test_largest_sizes(L):
+    """Sizes whose counts would pass 32 bits are refused."""
+    keep, a = buffers()
+    append = lambda heads: L.mla_append_kv(None, 0, heads, 1, 256, 256, 64, 0, 0, a, 512, 64, a, 512, 64, None, 512,
+                                           64, a, a, 8, 0, 1, a, 1, a, None)
+    assert append(2 ** 23 - 4) == 0 and append(2 ** 23) == 3 and append(2 ** 31 - 1) == 3
+    # 2^22 sessions of 256 rows: jobs of 512 threads at width 256, of 256 below it
+    sizes = lambda width: (2 ** 22, 2 ** 30, 1, 1, width, width, 64, 256, 0, 0)
+    assert L.mla_kv_plan_bytes(*sizes(128)) > 0 and L.mla_kv_plan_bytes(*sizes(256)) == 0
+    assert b"too large" in L.mla_last_error()
