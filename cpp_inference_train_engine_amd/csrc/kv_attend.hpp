@@ -14,8 +14,9 @@
 //                         taken as the lanes hold the scores, P^T needs no exchange between lanes.
 //                         V^T: a lane takes some columns of its eight keys' rows and transposes
 //                         them in registers (v_perm_b32).
-// P^T enters in two 16-bit parts, e = hi + lo, off by 2^-17 of it (bf16) or 2^-23 (fp16) at most:
-// only the row is rounded to 16 bits.
+// P^T enters in 16-bit parts: only the row is rounded.  bf16: two, e = hi + lo, off by 2^-17 of it at
+// most.  fp16: two, off by 2^-23 of it or 2^-25, and in units where that is more than 2^-15 of some
+// weight a third, of what they leave, off by 2^-47 (a row's largest weight is 2^11 at least).
 //
 // kv_few_kernel -- a job of at most 16 or 32 rows: each of four waves holds all of them and takes
 //   every 4th unit, straight from memory into the operands' registers; the waves' states meet in LDS
@@ -60,10 +61,25 @@
 namespace mla {
 namespace {
 
-// The reference maximum sits kHead below the row's when it is set, and is raised again when a
-// score passes it by more than kRise: probabilities stay within fp16, and those near the maximum
-// clear of its subnormals.
-constexpr float kHead = 6.0f, kRise = 14.0f;
+// The reference maximum sits HEAD below the row's when it is set, and is raised again when a score
+// passes it by more than RISE: weights stay within fp16.
+// A row can be made of small weights alone, where the values of the tokens far above the others are
+// zero, and a part in fp16 is a multiple of 2^-24.  So where a unit has weights below SMALL, what two
+// parts leave of its weights is multiplied, too, LIFT times as large.  (SMALL is 14.5 nats below the
+// row's largest at least; 2^-15 is about what scores that far apart are off by themselves.)  bf16 has
+// fp32's range.  The check takes 3 % of a prompt's time (4,000 rows, 32 heads on kv 8 x 128: 219 us,
+// 213 without), the third part as much as half of it where every unit needs it (scores spread by
+// 4 nats: 323; by 2: 247); decode rows wait for memory all the same.
+template <typename T>
+struct Weights {
+    static constexpr bool REST = false;
+    static constexpr float HEAD = 6.0f, RISE = 14.0f;
+};
+template <>
+struct Weights<F16> {
+    static constexpr bool REST = true;
+    static constexpr float HEAD = 11.0f, RISE = 15.0f, SMALL = 0x1p-10f, LOG_SMALL = -10.0f, LIFT = 0x1p22f;
+};
 
 // Tables that other kernels wrote are read through the scalar cache.
 typedef const __attribute__((address_space(4))) int32_t* table_ptr;
@@ -261,7 +277,7 @@ struct Attend {
             v = fetch<words>(tile + i * DV, (uint32_t)(4 * g * DV + min(col, DV - CW)) * 2);
 #pragma unroll
         for (int k = 0; k < CW / 2; ++k)
-            r.w[k] = EXACT || col < DV ? v[k] : 0;
+            r.w[k] = v[k];  // (columns past the head's are computed and not stored)
         return r;
     }
     // Operand e of eight rows: their columns e, two keys a word.
@@ -309,8 +325,11 @@ struct Attend {
                 }
     }
     // The rows' reference maxima, and what was summed under lower ones, follow the scores of U units.
+    // Returns whether a weight may be below SMALL (those of scores that were replaced count, too).
     template <int U>
-    __device__ __forceinline__ void raise(const floatx4 (&sc)[U][N][2]) {
+    __device__ __forceinline__ bool raise(const floatx4 (&sc)[U][N][2]) {
+        using W = Weights<T>;
+        bool below = false;
         float mp[N];
         bool above = false;
 #pragma unroll
@@ -324,14 +343,29 @@ struct Attend {
                     for (int i = 0; i < 4; ++i)
                         mp[t] = fmaxf(mp[t], sc[x][t][tt][i]);
             mp[t] *= a.scale_log2;
-            above |= mp[t] > m[t] + kRise;
+            above |= mp[t] > m[t] + W::RISE;
+            if constexpr (W::REST) {
+                float least = INFINITY;
+#pragma unroll
+                for (int x = 0; x < U; ++x)
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            least = fminf(least, sc[x][t][tt][i]);
+                below |= least * a.scale_log2 < m[t] + W::LOG_SMALL;
+            }
         }
-        if (__builtin_amdgcn_ballot_w64(above) == 0)
-            return;
+        if (__builtin_amdgcn_ballot_w64(above || below) == 0)
+            return false;
+        if (W::REST && __builtin_amdgcn_ballot_w64(above) == 0)
+            return true;
 #pragma unroll
         for (int t = 0; t < N; ++t) {
-            const float top = rows_max(mp[t]) - kHead;
-            const float m_new = top > m[t] + (kRise - kHead) ? top : m[t];
+            const float top = rows_max(mp[t]) - W::HEAD;
+            // (with less room above, all rows at once: one raise in place of several, 4,093 rows
+            // twice through a window 250 us in place of 261)
+            const float m_new = top > m[t] + (W::REST ? 0.0f : W::RISE - W::HEAD) ? top : m[t];
             const bool had = m[t] != -INFINITY;  // the row has accumulated state
             if (__builtin_amdgcn_ballot_w64(had && m_new > m[t])) {
                 const float alpha = had ? __builtin_amdgcn_exp2f(m[t] - m_new) : 1.0f;
@@ -342,9 +376,10 @@ struct Attend {
             }
             m[t] = m_new;
         }
+        return W::REST;
     }
-    // Scores become weights, in two parts, and are summed.
-    __device__ __forceinline__ void weights(const floatx4 (&sc)[N][2], V8 (&hi)[N], V8 (&lw)[N]) {
+    // Scores become weights, also in two parts, and are summed.
+    __device__ __forceinline__ void weights(floatx4 (&sc)[N][2], V8 (&hi)[N], V8 (&lw)[N]) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
             const float ref = m[t] == -INFINITY ? 0.0f : m[t];
@@ -358,10 +393,51 @@ struct Attend {
                 sum += e0 + e1;
                 h[x] = pack2<T>(e0, e1);
                 w[x] = pack2<T>(e0 - T::to_float((uint16_t)h[x]), e1 - T::to_float((uint16_t)(h[x] >> 16)));
+                sc[t][x >> 1][2 * (x & 1)] = e0;
+                sc[t][x >> 1][2 * (x & 1) + 1] = e1;
             }
             hi[t] = __builtin_bit_cast(V8, h);
             lw[t] = __builtin_bit_cast(V8, w);
             l[t] += sum;
+        }
+    }
+
+    // Adds what is left of a unit's weights, if some are below SMALL.  `operand`: tile i of its V^T.
+    template <typename F>
+    __device__ __forceinline__ void add_rest(const floatx4 (&e)[N][2], const V8 (&hi)[N], const V8 (&lw)[N],
+                                             F&& operand) {
+        using W = Weights<T>;
+        uint32_t least = ~0u;  // of the weights' bits less one: those of zero are the largest
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = e[t][i >> 2][i & 3];  // (an element itself is not cast right)
+                least = min(least, __builtin_bit_cast(uint32_t, y) - 1);
+            }
+        if (__builtin_amdgcn_ballot_w64(least < __builtin_bit_cast(uint32_t, W::SMALL) - 1) == 0)
+            return;
+        V8 rest[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            u32x4 r;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                float y[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    y[i] = (e[t][x >> 1][2 * (x & 1) + i] - static_cast<float>(hi[t][2 * x + i]) -
+                            static_cast<float>(lw[t][2 * x + i])) * W::LIFT;
+                r[x] = pack2<T>(y[0], y[1]);
+            }
+            rest[t] = __builtin_bit_cast(V8, r);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const V8 x = operand(i);
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+                acc[t][i] += T::mma32(x, rest[t], floatx4{0, 0, 0, 0}) * (1.0f / W::LIFT);
         }
     }
 
@@ -474,7 +550,7 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
         const bool full = full_units.has(u);
         if (!full)
             s.mask(sc[0], key0);
-        s.raise(sc);
+        const bool small = s.raise(sc);
         V8 hi[N], lw[N];
         s.weights(sc[0], hi, lw);
         bool bad = false;
@@ -482,6 +558,11 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
 #pragma unroll
             for (int c = 0; c < A::NC; ++c)
                 bad |= s.clean(v[c], key0);
+        if constexpr (Weights<T>::REST)
+            if (small)
+                s.add_rest(sc[0], hi, lw, [&](int i) {
+                    return __builtin_bit_cast(V8, A::transposed(v[i / CW], i % CW));
+                });
 #pragma unroll
         for (int c = 0; c < A::NC; ++c)
 #pragma unroll
@@ -716,11 +797,16 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
             if (!full_wave.has(u) || u >= job.u1)
                 s.mask(sc[x], u < job.u1 ? first_key(job, u) : INT_MAX - 31);
         }
-        s.raise(sc);
+        const bool small = s.raise(sc);
         V8 hi[U][N], lw[U][N];
 #pragma unroll
         for (int x = 0; x < U; ++x)
             s.weights(sc[x], hi[x], lw[x]);
+        if constexpr (Weights<T>::REST)
+            if (small)
+#pragma unroll
+                for (int x = 0; x < U; ++x)
+                    s.add_rest(sc[x], hi[x], lw[x], [&](int i) { return read(smem[b] + KW, x * A::NT + i); });
 #pragma unroll
         for (int i = 0; i < EARLY; ++i)
             ko[i] = read(smem[b1], i);
