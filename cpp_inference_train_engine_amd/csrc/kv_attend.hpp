@@ -81,12 +81,6 @@ struct Weights<F16> {
     static constexpr float HEAD = 11.0f, RISE = 15.0f, SMALL = 0x1p-10f, LOG_SMALL = -10.0f, LIFT = 0x1p22f;
 };
 
-// Tables that other kernels wrote are read through the scalar cache.
-typedef const __attribute__((address_space(4))) int32_t* table_ptr;
-__device__ __forceinline__ table_ptr table(const int32_t* p) {
-    return (table_ptr)reinterpret_cast<uintptr_t>(p);
-}
-
 // n / d and the rest by a product with floor(2^32 / d) (2^32 - 1 for d = 1): one too small at most
 // for n < 2^32.
 __device__ __forceinline__ int quotient(int n, int d, uint32_t inverse, int& rest) {
@@ -129,8 +123,6 @@ struct Job {
 __device__ __forceinline__ bool take_job(const KvArgs& a, bool many, int index, Job& j) {
     const table_ptr plan = table(a.plan);
     const table_ptr d = plan + (many ? a.p.jobs_m_at : a.p.jobs_f_at) + (long long)index * kKvJobInts;
-    const int jobs_f = plan[kKvJobsF], jobs_m = plan[kKvJobsM], parts = plan[kKvParts],
-              tag = plan[kKvTag];
     j.session = d[0];
     j.q0 = d[1];
     j.f0 = d[2];
@@ -140,7 +132,7 @@ __device__ __forceinline__ bool take_job(const KvArgs& a, bool many, int index, 
     j.ctx = d[6];
     j.part = d[7];
     // no such job; or a plan for other sizes, or a failed one, or not the build that the host knows
-    if (index >= (many ? jobs_m : jobs_f) || !kv_plan_fits(a, tag, jobs_f, jobs_m, parts))
+    if (index >= plan[many ? kKvJobsM : kKvJobsF] || !kv_plan_fits(a, plan))
         return false;
     int r;
     j.pa = j.ctx + quotient(j.f0, a.p.group, a.group_inverse, r);

@@ -23,7 +23,7 @@ template <typename T, int GROUPS>
 __global__ __launch_bounds__(kThreads) void kv_merge_kernel(KvArgs a) {
     constexpr int PER = kThreads / GROUPS;  // threads of a group
     __shared__ float so[GROUPS > 1 ? kThreads * 4 : 4], sml[GROUPS > 1 ? kThreads * 2 : 4];
-    const int32_t* plan = a.plan;
+    const table_ptr plan = table(a.plan);
     const int tid = threadIdx.x, group = tid / PER, me = tid % PER;
     const int DV = a.p.v_dim, per_row = DV / 4, H = a.p.H, G = a.p.group;
     const long long block = blockIdx.y * (long long)gridDim.x + blockIdx.x, e = block * PER + me;
@@ -33,10 +33,9 @@ __global__ __launch_bounds__(kThreads) void kv_merge_kernel(KvArgs a) {
     const int h = (int)(fr - row * H), kh = h / G, in_group = h - kh * G;
     // A row's entry is read with the plan's head, not behind it, and dropped if that does not fit.
     const i32x4 entry = *reinterpret_cast<const i32x4*>(
-        plan + a.p.rows_at + (min(row, (long long)a.p.rows - 1) * G + in_group) * kKvRowInts);
+        a.plan + a.p.rows_at + (min(row, (long long)a.p.rows - 1) * G + in_group) * kKvRowInts);
     const int all = plan[kKvParts], rows = plan[kKvRows];
-    const bool some = kv_plan_fits(a, plan[kKvTag], plan[kKvJobsF], plan[kKvJobsM], all) &&
-                      all > 0 && row < rows;
+    const bool some = kv_plan_fits(a, plan) && all > 0 && row < rows;
     const int parts = some ? entry[1] : 0;  // 0: no such row, or one job wrote it itself
     float M = -INFINITY, L = 0.0f;
     floatx4 o = {0, 0, 0, 0};

@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
     const bool fits = jobs[0] <= p.max_jobs_f && jobs[1] <= p.max_jobs_m && parts <= p.max_parts;
     if (tid < kKvHead) {
         int v = 0;
-        if (fits)
+        if (fits) {
             v = tid == kKvStatus ? jobs[0] + jobs[1]
                 : tid == kKvJobsF ? jobs[0]
                 : tid == kKvJobsM ? jobs[1]
@@ -273,7 +273,10 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(KvPlanArgs a) {
                 : tid == kKvRows  ? total_q
                 : tid == kKvTag   ? (int)p.tag
                                   : 0;
-        else
+#pragma unroll
+            for (int i = 0; i < kKvSizeInts; ++i)
+                v = tid == kKvSizes + i ? p.sizes[i] : v;
+        } else
             v = tid == kKvStatus ? -1 : tid == kKvBad ? -2 : 0;
         head[tid] = v;
     }
@@ -330,10 +333,16 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
     p.jobs_f_at = p.rows_at + flat * kKvRowInts;
     p.jobs_m_at = p.jobs_f_at + (long long)p.max_jobs_f * kKvJobInts;
     p.words = p.jobs_m_at + (long long)p.max_jobs_m * kKvJobInts;
+    // (every bit of a size reaches every bit of the tag; kv_plan_fits compares the sizes themselves)
+    const int sizes[kKvSizeInts] = {B, rows, H, kv_heads, dim, v_dim, page_size, max_q_len, window, sinks};
     uint32_t h = 2166136261u;
-    for (const int v : {B, rows, H, kv_heads, dim, v_dim, page_size, max_q_len, window, sinks})
-        h = (h ^ (uint32_t)v) * 16777619u;
-    p.tag = h | 1u;
+    for (int i = 0; i < kKvSizeInts; ++i) {
+        p.sizes[i] = sizes[i];
+        h = (h ^ (uint32_t)sizes[i]) * 0x9e3779b1u;
+        h = (h ^ (h >> 15)) * 0x85ebca77u;
+        h ^= h >> 13;
+    }
+    p.tag = h ? h : 1;
     return p;
 }
 

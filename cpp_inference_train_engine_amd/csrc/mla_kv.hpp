@@ -52,7 +52,8 @@ constexpr int kKvJobInts = 8;  // session, its first query row, first flat row, 
                                // unit (of those that the block sees) + 1, ctx, first partial row
 constexpr int kKvRowInts = 4;  // partials of a flat row: first, how many (0: none), step
 constexpr int kKvHead = 64;    // words
-enum { kKvStatus, kKvBad, kKvJobsF, kKvJobsM, kKvParts, kKvRows, kKvTag };
+enum { kKvStatus, kKvBad, kKvJobsF, kKvJobsM, kKvParts, kKvRows, kKvTag, kKvSizes = 8 };
+constexpr int kKvSizeInts = 10;  // what a plan's tables and jobs follow from, from kKvSizes on
 
 struct KvShape {
     int B, rows, H, kv_heads, group, dim, v_dim, width, page_size, max_q_len;
@@ -63,7 +64,8 @@ struct KvShape {
     int max_blocks;
     long long max_parts;         // partial rows of a kv head
     long long tables_at, rows_at, jobs_f_at, jobs_m_at, words;  // word offsets
-    uint32_t tag;
+    int sizes[kKvSizeInts];      // B .. sinks as they were given, as a plan's head holds them
+    uint32_t tag;                // of them, for the host's copy of a plan's info
 };
 KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int page_size,
                  int max_q_len, int window, int sinks);
@@ -103,12 +105,21 @@ struct KvArgs {
     uint16_t* out;
     float *lse, *part_o, *part_ml;
 };
-// Whether the call is for this plan (its head): made for the same sizes, and where the host knows
-// its counts, with those.
-__host__ __device__ inline bool kv_plan_fits(const KvArgs& a, int tag, int jobs_f, int jobs_m,
-                                             int parts) {
-    return tag == (int)a.p.tag &&
-           (a.parts < 0 || (jobs_f == a.jobs_f && jobs_m == a.jobs_m && parts == a.parts));
+// Tables that other kernels wrote are read through the scalar cache.
+typedef const __attribute__((address_space(4))) int32_t* table_ptr;
+__device__ __forceinline__ table_ptr table(const int32_t* p) {
+    return (table_ptr)reinterpret_cast<uintptr_t>(p);
+}
+// Whether the call is for the plan of this head: made for the same sizes (a failed one has none), and
+// where the host knows its counts, with those.
+__device__ __forceinline__ bool kv_plan_fits(const KvArgs& a, table_ptr head) {
+    int differ = a.parts < 0 ? 0
+                             : (head[kKvJobsF] ^ a.jobs_f) | (head[kKvJobsM] ^ a.jobs_m) |
+                                   (head[kKvParts] ^ a.parts);
+#pragma unroll
+    for (int i = 0; i < kKvSizeInts; ++i)
+        differ |= head[kKvSizes + i] ^ a.p.sizes[i];
+    return differ == 0;
 }
 hipError_t launch_kv_attention(const KvArgs& a, int dtype, hipStream_t stream);
 // The lists' kernels, one translation unit for each type (kv_attend_*.hip).

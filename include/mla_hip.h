@@ -481,8 +481,8 @@ int mla_read_kv_plan_info(void* stream, const void* plan, int32_t* host_info);
  * mla_read_kv_plan_info returned for this very plan, not built anew since, or NULL: with it the call
  * launches as many workgroups as the plan has jobs, without it as many as a plan of these sizes can
  * have, whose rest returns at once.  A call with the info of another build, whose counts differ,
- * writes nothing; a captured graph that builds the plan takes NULL.  pages, q, plan, out and
- * workspace at multiples of 16 bytes.  The workspace needs no initialisation; calls that share one
+ * or with a plan that was built for other sizes (B .. sinks), writes nothing; a captured graph that
+ * builds the plan takes NULL.  pages, q, plan, out and workspace at multiples of 16 bytes.  The workspace needs no initialisation; calls that share one
  * must be ordered on one stream.  Rows are rounded once, to `dtype`.  A key or value that a row does
  * not see adds nothing to it, whatever it holds.  A value that is not finite makes its column of the
  * rows that see it infinite or NaN, a NaN key those rows. */
