@@ -137,7 +137,7 @@ class PagedLatentCache:
         torch = _torch()
         self.n_layers, self.num_pages, self.page_size = n_layers, num_pages, page_size
         self.kv_rank, self.rope_dim, self.dtype = kv_rank, rope_dim, dtype
-        tdt = torch.float16 if dtype == DTYPE_F16 else torch.bfloat16
+        tdt = _dtype_of(dtype)
         rec = page_size * (kv_rank + rope_dim)
         if storage is None:
             storage = torch.zeros((n_layers, num_pages, rec), dtype=tdt, device=device)
@@ -265,7 +265,10 @@ def prefill_attention(batch: RaggedBatch, pages, q_latent, q_rope, scale: float,
 
 # ------------------------------------------------- 8-bit cache, planned attention ----
 def _dtype_of(code: int):
+    """torch's type of a cache's words."""
     torch = _torch()
+    if code != DTYPE_F16 and code != DTYPE_BF16:
+        raise ValueError(f"dtype: {code!r}, wanted DTYPE_F16 or DTYPE_BF16 (a cache holds 16-bit words)")
     return torch.float16 if code == DTYPE_F16 else torch.bfloat16
 
 
@@ -314,6 +317,7 @@ class QuantizedLatentCache:
         torch = _torch()
         self.n_layers, self.num_pages, self.page_size = n_layers, num_pages, page_size
         self.kv_rank, self.rope_dim, self.dtype = kv_rank, rope_dim, dtype
+        _dtype_of(dtype)
         rec = int(lib().mla_q8_page_bytes(page_size, kv_rank, rope_dim))
         if rec == 0:
             raise ValueError("8-bit latent cache: page_size must be a multiple of 16 up to 65,536, "
