@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
 #include <string>
 
@@ -18,6 +19,12 @@ bool misaligned(std::initializer_list<const void*> ptrs) {
     for (const void* p : ptrs)
         u |= reinterpret_cast<uintptr_t>(p);
     return (u & 15) != 0;
+}
+
+// Whether two stretches of bytes have one in common.
+bool overlap(const void* a, long long a_bytes, const void* b, long long b_bytes) {
+    const char *const x = static_cast<const char*>(a), *const y = static_cast<const char*>(b);
+    return x < y + b_bytes && y < x + a_bytes;
 }
 
 int invalid(const char* fn, const std::string& what) {
@@ -101,15 +108,21 @@ int mla_append_kv(void* stream, int T, int n_heads, int n_kv_heads, int head_dim
     if (misaligned({pages, q ? q_out : nullptr}))
         return invalid(fn, "pages and q_out must lie at multiples of 16 bytes");
     const int size = row_dtype == MLA_DTYPE_F32 ? 4 : 2;
-    if (q) {  // a row's columns are read by several threads: none may be written before
-        const long long far[2] = {(T - 1LL) * q_row, (n_heads - 1LL) * q_head};
-        const char* const from = static_cast<const char*>(q);
-        const char* const first = from + (std::min(far[0], 0LL) + std::min(far[1], 0LL)) * size;
-        const char* const behind =
-            from + (std::max(far[0], 0LL) + std::max(far[1], 0LL) + head_dim) * size;
-        const char* const to = static_cast<const char*>(q_out);
-        if (to < behind && first < to + 2LL * T * n_heads * head_dim)
+    if (q) {  // workgroups write q_out while others still read their rows
+        auto covers = [&](const void* rows, long long row, long long head, int heads, int columns) {
+            const long long far[2] = {(T - 1LL) * row, (heads - 1LL) * head};
+            const char* const from = static_cast<const char*>(rows);
+            return overlap(q_out, 2LL * T * n_heads * head_dim,
+                           from + (std::min(far[0], 0LL) + std::min(far[1], 0LL)) * size,
+                           (std::abs(far[0]) + std::abs(far[1]) + columns) * size);
+        };
+        if (covers(q, q_row, q_head, n_heads, head_dim))
             return invalid(fn, "q_out overlaps q");
+        if (covers(k, k_row, k_head, n_kv_heads, head_dim) || covers(v, v_row, v_head, n_kv_heads, v_dim))
+            return invalid(fn, "q_out overlaps k or v");
+        if (overlap(q_out, 2LL * T * n_heads * head_dim, pages,
+                    2LL * num_pool_pages * kv_record(n_kv_heads, page_size, head_dim, v_dim)))
+            return invalid(fn, "q_out overlaps the pages");
     }
     KvAppendArgs a{};
     a.T = T;

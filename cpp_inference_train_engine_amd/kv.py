@@ -141,8 +141,9 @@ def append_kv(cache: PagedKVCache, layer: int, k, v, slot_mapping, *, rotation: 
     to the cache's type and write row t to flat slot slot_mapping[t] of ``layer``'s pool.  Slots
     outside the pool are skipped; the others are distinct.  With q [T, H, head_dim] its rows are
     rotated the same way and returned, in ``q_out`` or a new tensor [T, H, head_dim] of the cache's
-    type (rows of skipped slots, too).  k, v and q are fp32 or 16-bit rows of one type; slices of
-    one projection's rows are taken as they are.  Without ``rotation`` nothing is turned."""
+    type (rows of skipped slots, too), which shares no memory with q, k, v or the cache.  k, v and
+    q are fp32 or 16-bit rows of one type; slices of one projection's rows are taken as they are.
+    Without ``rotation`` nothing is turned."""
     gpu, T, rows = _gpu(), k.shape[0], k.dtype
     heads, dim, v_dim, page = cache._shape
     code = _row_code(rows)

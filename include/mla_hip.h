@@ -434,8 +434,10 @@ size_t mla_kv_page_words(int n_kv_heads, int head_dim, int v_dim, int page_size)
 /* Row t of k [T x n_kv_heads x head_dim], rotated, and of v [T x n_kv_heads x v_dim] is rounded once
  * to `dtype` and written to flat slot slot_mapping[t]; slots outside the pool are skipped, the others
  * are distinct.  With q [T x n_heads x head_dim] (NULL: none) row t of q is rotated the same way,
- * rounded and written to q_out [T x n_heads x head_dim], which does not overlap q, whatever its
- * slot.  A token's rows have fewer than 2^31 columns in all (MLA_ERR_UNSUPPORTED otherwise).  Rows
+ * rounded and written to q_out [T x n_heads x head_dim], whatever its slot.  q_out lies apart from
+ * the memory between the first and the last element of each of q, k, v and the pages
+ * (MLA_ERR_INVALID_ARGUMENT otherwise); rows of k, v or q within the pages are of slots that the call
+ * does not write.  A token's rows have fewer than 2^31 columns in all (MLA_ERR_UNSUPPORTED otherwise).  Rows
  * are of row_dtype (MLA_DTYPE_*); *_row and *_head are strides in elements (columns lie one behind the other), so
  * that slices of one projection's rows can be given; rows, and strides, at multiples of 16 bytes
  * are read faster.
