@@ -27,6 +27,16 @@ def _row_code(dtype) -> int | None:
     return _row_codes.get(dtype)
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _ints_of_c(**sizes) -> None:
+    """A C int takes the low 32 bits of whatever it is given."""
+    for name, n in sizes.items():
+        if not -_INT_MAX <= n <= _INT_MAX:
+            raise ValueError(f"{name}: {n} does not fit 32 bits")
+
+
 class PagedKVCache:
     """Device page pool of keys and values: 16-bit [layers, pages, record words], a record keys
     [n_kv_heads][page_size][head_dim], then values [n_kv_heads][page_size][v_dim]."""
@@ -37,6 +47,8 @@ class PagedKVCache:
         v_dim = head_dim if v_dim is None else v_dim
         self.n_layers, self.num_pages, self.page_size = n_layers, num_pages, page_size
         self.n_kv_heads, self.head_dim, self.v_dim, self.dtype = n_kv_heads, head_dim, v_dim, dtype
+        _ints_of_c(num_pages=num_pages, page_size=page_size, n_kv_heads=n_kv_heads, head_dim=head_dim,
+                   v_dim=v_dim)
         words = int(lib().mla_kv_page_words(n_kv_heads, head_dim, v_dim, page_size))
         if words == 0:
             raise ValueError("key-value cache: page_size must be a multiple of 16 up to 65,536, "
@@ -97,6 +109,7 @@ class Rotation:
             raise ValueError("rotation: frequencies must be a contiguous float64 tensor of one "
                              "dimension")
         self.frequencies, self.start, self.adjacent = frequencies, int(start), bool(adjacent)
+        _ints_of_c(start=self.start, pairs=frequencies.numel())
         self._place = frequencies.get_device()
         self._args = ptr(frequencies), frequencies.numel(), self.start, int(self.adjacent)
 
@@ -147,6 +160,8 @@ def append_kv(cache: PagedKVCache, layer: int, k, v, slot_mapping, *, rotation: 
     gpu, T, rows = _gpu(), k.shape[0], k.dtype
     heads, dim, v_dim, page = cache._shape
     code = _row_code(rows)
+    if T > _INT_MAX:
+        raise ValueError(f"k: {T} rows do not fit 32 bits")
     if code is None:
         raise ValueError(f"k: wanted float32, float16 or bfloat16 rows, got {rows}")
     ka = _rows("k", k, heads, dim, T, rows, gpu)
@@ -154,6 +169,8 @@ def append_kv(cache: PagedKVCache, layer: int, k, v, slot_mapping, *, rotation: 
     qa, H, out = (None, 0, 0), heads, None
     if q is not None:
         H = q.shape[1]
+        if H > _INT_MAX:
+            raise ValueError(f"q: {H} heads do not fit 32 bits")
         qa = _rows("q", q, H, dim, T, rows, gpu)
         if q_out is None:
             with _allocating_on(stream):
@@ -225,6 +242,7 @@ def plan_kv_attention(batch: RaggedBatch, cache: PagedKVCache, n_heads: int, *,
     torch, gpu = _torch(), _gpu()
     rows = batch.max_rows if rows is None else rows
     max_q_len = max(rows, 1) if max_q_len is None else max_q_len
+    _ints_of_c(n_heads=n_heads, rows=rows, max_q_len=max_q_len, window=window or 0, sinks=sinks)
     if window is not None and window < 1:
         raise ValueError(f"window: {window}, wanted at least 1 (None: no window)")
     if batch.page_size != cache.page_size or batch.num_pool_pages > cache.num_pages:
