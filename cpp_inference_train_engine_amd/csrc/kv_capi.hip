@@ -262,6 +262,28 @@ int mla_kv_attention(void* stream, int B, int rows, int n_heads, int n_kv_heads,
     }
     if (workspace_bytes < workspace_size(a.p))
         return invalid(fn, "workspace needs " + std::to_string(workspace_size(a.p)) + " bytes");
+    // (a row of out may take the place of the row of q that it follows from: its job alone reads that)
+    struct Stretch {
+        const void* at;
+        long long bytes;
+    };
+    const long long words = (long long)rows * n_heads;
+    const long long record = kv_record(n_kv_heads, page_size, head_dim, v_dim);
+    const Stretch own[] = {{out, 2 * words * v_dim},
+                           {lse, lse ? 4 * words : 0},
+                           {workspace, (long long)workspace_size(a.p)}};
+    const Stretch read[] = {{q, 2 * words * head_dim}, {pages, 2 * num_pool_pages * record}};
+    for (const Stretch& x : own) {
+        bool apart = true;
+        for (const Stretch& y : own)
+            apart &= &x == &y || !overlap(x.at, x.bytes, y.at, y.bytes);
+        for (const Stretch& y : read)
+            apart &= (x.at == out && y.at == q && q == out && head_dim == v_dim) ||
+                     !overlap(x.at, x.bytes, y.at, y.bytes);
+        if (!apart)
+            return invalid(fn, "out, lse and workspace must lie apart from each other, q (out may be q "
+                               "itself where head_dim is v_dim) and the pages");
+    }
     a.max_pages = max_pages;
     a.num_pool_pages = num_pool_pages;
     auto inverse = [](int n) { return (uint32_t)std::min<uint64_t>((1ULL << 32) / n, 0xffffffffULL); };

@@ -273,7 +273,8 @@ def kv_attention(plan: KVAttentionPlan, cache: PagedKVCache, layer: int, q, scal
                  lse=None, workspace=None, stream=None):
     """Attention of every query row of the plan's batch over its session's keys and values in
     ``layer`` of ``cache``: q [rows, H, head_dim] in the cache's type; returns out [rows, H, v_dim] in
-    it (and fills lse [rows, H], fp32, if given).  Rows past the batch's are left as they were, and
+    it (and fills lse [rows, H], fp32, if given).  ``out`` may be q itself where v_dim is head_dim, and
+    shares no memory with q or the cache otherwise.  Rows past the batch's are left as they were, and
     over a failed plan (``KVAttentionPlan.read_info`` raises) all of them: zero in a tensor that the
     call makes."""
     torch, gpu = _torch(), _gpu()

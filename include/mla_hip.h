@@ -478,8 +478,9 @@ int mla_plan_kv_attention(void* stream, int B, int rows, int n_heads, int n_kv_h
  * first bad session, ..} with MLA_ERR_INVALID_ARGUMENT and a message. */
 int mla_read_kv_plan_info(void* stream, const void* plan, int32_t* host_info);
 /* The attention.  page_table and max_pages are those of the metadata; q [rows x n_heads x head_dim]
- * and out [rows x n_heads x v_dim] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.  Rows
- * past the batch's are left as they were, and over a failed plan all.  host_info is what
+ * and out [rows x n_heads x v_dim] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.  out
+ * may be q itself where head_dim is v_dim; out, lse and workspace lie apart from each other, q and
+ * the pages otherwise (MLA_ERR_INVALID_ARGUMENT).  Rows past the batch's are left as they were, and over a failed plan all.  host_info is what
  * mla_read_kv_plan_info returned for this very plan, not built anew since, or NULL: with it the call
  * launches as many workgroups as the plan has jobs, without it as many as a plan of these sizes can
  * have, whose rest returns at once.  A call with the info of another build, whose counts differ,

@@ -65,3 +65,50 @@ def test_append_over_its_own_rows(gpu):
         call(*apart, cache.pages.view(-1)[:3 * 128].view(3, 4, 32))
     assert torch.equal(call(*apart, room), apart[2])
     assert torch.equal(cache.keys(0)[0, :, :3].transpose(0, 1), apart[0])
+
+
+SIZES = (2, 4, 8, 4, 64, 64, 64, 3, 0, 0)  # 4 rows of 8 heads of 64: q and out 4,096 bytes, lse 128
+
+
+def test_attention(L):
+    ws_bytes = L.mla_kv_workspace_bytes(*SIZES)
+    pool = 2 * 2 * L.mla_kv_page_words(4, 64, 64, 64)
+    buf = ctypes.create_string_buffer(ws_bytes + pool + (1 << 16))
+    a = ctypes.addressof(buf)
+    a += 256 - a % 256
+    plan, q, out, lse, pages, ws = a, a + 4096, a + 16384, a + 24576, a + 32768, a + 32768 + pool
+
+    def call(q=q, out=out, lse=lse, pages=pages, ws=ws, sizes=SIZES):
+        return L.mla_kv_attention(None, *sizes, 0, 0.1, plan, 4, 2, pages, q, plan, 1 << 40, None, out, lse, ws,
+                                  ws_bytes)
+    assert call() in OK and call(lse=None) in OK and call(out=q + 4096) in OK and call(out=q - 4096) in OK
+    assert call(out=q) in OK  # (out may be q itself)
+    for kw in (dict(out=q + 16), dict(out=q - 4080), dict(lse=q + 4092), dict(lse=q), dict(ws=q), dict(out=pages),
+               dict(out=pages + pool - 16), dict(lse=pages - 124), dict(ws=pages), dict(ws=pages + pool - 256),
+               dict(lse=out), dict(lse=out + 4092), dict(out=ws), dict(lse=ws + 256), dict(out=ws - 4080)):
+        assert call(**kw) == INVALID, kw
+        assert b"apart" in L.mla_last_error()
+    # values of another width than the keys: a row of out lies over another row of q
+    other = (2, 4, 8, 4, 64, 48, 64, 3, 0, 0)
+    assert call(out=q, sizes=other) == INVALID and call(sizes=other) in OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("H,KH,D,page", [(8, 8, 64, 64), (32, 8, 128, 64), (4, 2, 80, 16), (4, 4, 256, 32)])
+def test_attention_in_place_of_its_queries(gpu, H, KH, D, page, dtype):
+    """out=q gives the rows that another tensor gets: decode rows, drafts, chunks, cut or not."""
+    from kv_reference import Batch, say
+    say(f"in place {H} {KH} {D} {dtype}")
+    c = Batch(H, KH, D, D, page, dtype, [(700, 1), (30, 4), (100, 290), (0, 33), (20000, 3), (9000, 1)], seed=3)
+    batch, cache, q = c.device(gpu)
+    for window in (None, 100):
+        plan = gpu.plan_kv_attention(batch, cache, H, rows=c.rows, max_q_len=290, window=window)
+        want = gpu.kv_attention(plan, cache, 0, q, c.scale)
+        x = q.clone()
+        assert gpu.kv_attention(plan, cache, 0, x, c.scale, out=x) is x
+        assert torch.equal(x, want)
+        wide = torch.zeros((c.rows + 1, H, D), dtype=q.dtype, device="cuda")
+        wide[1:] = q
+        with pytest.raises(gpu.MlaError, match="apart"):
+            gpu.kv_attention(plan, cache, 0, wide[1:], c.scale, out=wide[:-1])

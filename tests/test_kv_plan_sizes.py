@@ -33,7 +33,7 @@ def make(gpu, sizes):
 
     def call(s, host):
         st = L.mla_kv_attention(None, *s, 1, c.scale, p(batch.page_table), batch.max_pages,
-                                batch.num_pool_pages, p(cache.pages), p(wide), p(words), n,
+                                batch.num_pool_pages * page // s[6], p(cache.pages), p(wide), p(words), n,
                                 ctypes.addressof(info) if host else None, p(out), None, p(ws), ws.numel())
         torch.cuda.synchronize()
         return st
