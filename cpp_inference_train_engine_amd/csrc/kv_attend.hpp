@@ -67,9 +67,9 @@ namespace {
 // zero, and a part in fp16 is a multiple of 2^-24.  So where a unit has weights below SMALL, what two
 // parts leave of its weights is multiplied, too, LIFT times as large.  (SMALL is 14.5 nats below the
 // row's largest at least; 2^-15 is about what scores that far apart are off by themselves.)  bf16 has
-// fp32's range.  The check takes 3 % of a prompt's time (4,000 rows, 32 heads on kv 8 x 128: 219 us,
-// 213 without), the third part as much as half of it where every unit needs it (scores spread by
-// 4 nats: 323; by 2: 247); decode rows wait for memory all the same.
+// fp32's range.  The check takes 3 % of a prompt's time (4,000 rows, 32 heads on kv 8 x 128: 216 us,
+// 211 without), the third part up to half as much again (216 us with scores spread by 1 nat, 244 by
+// 2, 317 by 4, where every unit needs it); decode rows wait for memory all the same.
 template <typename T>
 struct Weights {
     static constexpr bool REST = false;
@@ -78,7 +78,8 @@ struct Weights {
 template <>
 struct Weights<F16> {
     static constexpr bool REST = true;
-    static constexpr float HEAD = 11.0f, RISE = 15.0f, SMALL = 0x1p-10f, LOG_SMALL = -10.0f, LIFT = 0x1p22f;
+    static constexpr float HEAD = 11.0f, RISE = 15.0f, SMALL = 0x1p-10f, LIFT = 0x1p22f;
+    static constexpr uint16_t SMALL_HALF = 0x1400;  // SMALL in fp16
 };
 
 // n / d and the rest by a product with floor(2^32 / d) (2^32 - 1 for d = 1): one too small at most
@@ -317,11 +318,9 @@ struct Attend {
                 }
     }
     // The rows' reference maxima, and what was summed under lower ones, follow the scores of U units.
-    // Returns whether a weight may be below SMALL (those of scores that were replaced count, too).
     template <int U>
-    __device__ __forceinline__ bool raise(const floatx4 (&sc)[U][N][2]) {
+    __device__ __forceinline__ void raise(const floatx4 (&sc)[U][N][2]) {
         using W = Weights<T>;
-        bool below = false;
         float mp[N];
         bool above = false;
 #pragma unroll
@@ -336,27 +335,14 @@ struct Attend {
                         mp[t] = fmaxf(mp[t], sc[x][t][tt][i]);
             mp[t] *= a.scale_log2;
             above |= mp[t] > m[t] + W::RISE;
-            if constexpr (W::REST) {
-                float least = INFINITY;
-#pragma unroll
-                for (int x = 0; x < U; ++x)
-#pragma unroll
-                    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            least = fminf(least, sc[x][t][tt][i]);
-                below |= least * a.scale_log2 < m[t] + W::LOG_SMALL;
-            }
         }
-        if (__builtin_amdgcn_ballot_w64(above || below) == 0)
-            return false;
-        if (W::REST && __builtin_amdgcn_ballot_w64(above) == 0)
-            return true;
+        if (__builtin_amdgcn_ballot_w64(above) == 0)
+            return;
 #pragma unroll
         for (int t = 0; t < N; ++t) {
             const float top = rows_max(mp[t]) - W::HEAD;
-            // (with less room above, all rows at once: one raise in place of several, 4,093 rows
-            // twice through a window 250 us in place of 261)
+            // (with less room above, all rows at once: one raise in place of several; 4,093 rows
+            // twice through a window then took 250 us in place of 261, and 245 now)
             const float m_new = top > m[t] + (W::REST ? 0.0f : W::RISE - W::HEAD) ? top : m[t];
             const bool had = m[t] != -INFINITY;  // the row has accumulated state
             if (__builtin_amdgcn_ballot_w64(had && m_new > m[t])) {
@@ -368,10 +354,22 @@ struct Attend {
             }
             m[t] = m_new;
         }
-        return W::REST;
     }
+    // The least of some weights' high parts, by their bits: these are ordered as the weights are.
+    struct Least {
+        typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+        u2 x = {0xffff, 0xffff};
+        __device__ __forceinline__ void add(uint32_t word) {
+            x = __builtin_elementwise_min(x, __builtin_bit_cast(u2, word));
+        }
+        // Whether a lane has a weight below SMALL (a zero counts, too).
+        __device__ __forceinline__ bool small() const {
+            const int a = x[0], b = x[1];
+            return __builtin_amdgcn_ballot_w64(min(a, b) < Weights<T>::SMALL_HALF) != 0;
+        }
+    };
     // Scores become weights, also in two parts, and are summed.
-    __device__ __forceinline__ void weights(floatx4 (&sc)[N][2], V8 (&hi)[N], V8 (&lw)[N]) {
+    __device__ __forceinline__ void weights(floatx4 (&sc)[N][2], V8 (&hi)[N], V8 (&lw)[N], Least& least) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
             const float ref = m[t] == -INFINITY ? 0.0f : m[t];
@@ -385,6 +383,7 @@ struct Attend {
                 sum += e0 + e1;
                 h[x] = pack2<T>(e0, e1);
                 w[x] = pack2<T>(e0 - T::to_float((uint16_t)h[x]), e1 - T::to_float((uint16_t)(h[x] >> 16)));
+                least.add(h[x]);
                 sc[t][x >> 1][2 * (x & 1)] = e0;
                 sc[t][x >> 1][2 * (x & 1) + 1] = e1;
             }
@@ -542,16 +541,17 @@ __global__ __launch_bounds__(kKvThreads) __attribute__((
         const bool full = full_units.has(u);
         if (!full)
             s.mask(sc[0], key0);
-        const bool small = s.raise(sc);
+        s.raise(sc);
         V8 hi[N], lw[N];
-        s.weights(sc[0], hi, lw);
+        typename A::Least least;
+        s.weights(sc[0], hi, lw, least);
         bool bad = false;
         if (!full)
 #pragma unroll
             for (int c = 0; c < A::NC; ++c)
                 bad |= s.clean(v[c], key0);
         if constexpr (Weights<T>::REST)
-            if (small)
+            if (least.small())
                 s.add_rest(sc[0], hi, lw, [&](int i) {
                     return __builtin_bit_cast(V8, A::transposed(v[i / CW], i % CW));
                 });
@@ -789,13 +789,14 @@ __global__ __launch_bounds__(64 * many_waves(HK)) __attribute__((
             if (!full_wave.has(u) || u >= job.u1)
                 s.mask(sc[x], u < job.u1 ? first_key(job, u) : INT_MAX - 31);
         }
-        const bool small = s.raise(sc);
+        s.raise(sc);
         V8 hi[U][N], lw[U][N];
+        typename A::Least least;
 #pragma unroll
         for (int x = 0; x < U; ++x)
-            s.weights(sc[x], hi[x], lw[x]);
+            s.weights(sc[x], hi[x], lw[x], least);
         if constexpr (Weights<T>::REST)
-            if (small)
+            if (least.small())
 #pragma unroll
                 for (int x = 0; x < U; ++x)
                     s.add_rest(sc[x], hi[x], lw[x], [&](int i) { return read(smem[b] + KW, x * A::NT + i); });
