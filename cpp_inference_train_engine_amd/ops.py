@@ -446,7 +446,7 @@ class AttentionPlan:
         h = np.zeros(PLAN_INFO_INTS, np.int32)
         check(lib().mla_read_plan_info(stream_handle(stream), self._words[0], h.ctypes.data))
         if not self._captured:
-            self.info = h
+            self.info, self._own_info = h.copy(), h  # (calls read the second)
             self._info = h.ctypes.data
         return h.tolist()
 

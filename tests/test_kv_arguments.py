@@ -56,3 +56,24 @@ def test_sizes_of_calls_past_32_bits(gpu):
     many = torch.zeros((1, 1, 64), device="cuda").expand(1, 2 ** 32 + 1, 64)
     with pytest.raises(ValueError, match="32 bits"):
         gpu.append_kv(cache, 0, k, v, slots, q=many, q_out=torch.zeros(1, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_a_plans_info_is_its_own(gpu):
+    """What a user does with ``plan.info`` changes nothing for the plan's calls."""
+    import gc
+    import torch
+    from kv_reference import Batch
+    c = Batch(8, 4, 64, 64, 64, 0, [(9000, 1), (20, 100)], seed=18)
+    batch, cache, q = c.device(gpu)
+    plan = gpu.plan_kv_attention(batch, cache, 8, rows=c.rows, max_q_len=100)
+    want = gpu.kv_attention(plan, cache, 0, q, 0.1)
+    read = plan.read_info()
+    assert plan.info.tolist() == read
+    for change in ("zero", "none"):
+        if change == "zero":
+            plan.info[:] = 0
+        else:
+            plan.info = None
+            gc.collect()
+        assert torch.equal(gpu.kv_attention(plan, cache, 0, q, 0.1), want), change
