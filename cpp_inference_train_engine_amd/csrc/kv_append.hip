@@ -8,10 +8,11 @@
 //   while the first rows are on their way, then each takes 8 columns of a head at a time.
 //   t is taken in 64 bits, in revolutions, and only the rest of the last one rounded to 32: at
 //   position 131,071 a 32-bit product would be off by up to 2^-8 rad.
-// Every row is read and written once.  Few tokens: a launch and three trips to memory one after the
-// other (position, slot, rows), 3.7 us for 64 tokens of 8 heads, 4.6 for 200 of 48 (with one
-// workgroup a token 6.9).  Many: memory, 8,009 tokens of 48 heads of 128 columns (197 MB) 43 us,
-// 4.6 TB/s where a large copy reaches 4.8.
+// Every row is read and written once (of split halves that are no chunks of 8 columns, or not at
+// multiples of 16 bytes, the turned columns are read twice).  Few tokens: a launch and three trips to
+// memory one after the other (position, slot, rows), 3.5 us for 64 tokens of 8 heads, 4.6 for 200 of
+// 48 (with one workgroup a token 6.9).  Many: memory, 8,009 tokens of 48 heads of 128 columns (197 MB)
+// 43 us, 4.6 TB/s where a large copy reaches 4.8.
 #include "mla_common.hpp"
 #include "mla_kv.hpp"
 

@@ -3,7 +3,7 @@
 //     M = max_i m_i,  L = sum_i l_i 2^(m_i - M),  row = sum_i o_i 2^(m_i - M) / L
 // One thread per 4 columns of a row and each of GROUPS groups, which split the row's partials; each
 // reads kFlight of them at once, and their states meet in LDS.
-// 5-7 us for 1,392 partial rows of 8 groups of heads, 9.5 for 3,557 of 16 heads of 128 columns: two
+// 7.4 us for 1,392 partial rows of 8 groups of heads, 10-11 for 3,557 of 16 heads of 128 columns: two
 // trips to memory one after the other and the launch, then its bytes.
 #include "mla_common.hpp"
 #include "mla_kv.hpp"

@@ -7,7 +7,7 @@
 // length that gives every slot of the GPU one range (several where they are long, so that slots
 // with short ones take more of them), or of twice a slot's share (so that only blocks well above it
 // are cut) where there are more blocks than that.
-// A chain of short phases of one workgroup: 5.5-10 us.  (64 sessions of 128 .. 14,000 tokens, 32
+// A chain of short phases of one workgroup: 6-10 us back to back, up to 14 alone.  (64 sessions of 128 .. 14,000 tokens, 32
 // heads on kv 8 x 128, attend in 302 us with up to four ranges a slot, in 313 with one.  Blocks of
 // many rows keep their order, in which neighbours read the same keys at the same time: 4,000 rows
 // take 204 us, and 212 with the longest blocks first.)
@@ -305,7 +305,9 @@ KvShape kv_shape(int B, int rows, int H, int kv_heads, int dim, int v_dim, int p
     // registers hold no more, 16 again), which read the keys half as often.
     p.few_rows = own <= 16 || p.width == 256 ? 16 : 32;
     p.few = own <= 16 ? 16 : p.width == 256 ? 32 : 64;
-    // Workgroups that 256 compute units hold.
+    // Workgroups of a list at once, which the ranges' lengths follow from.  256 compute units hold
+    // as many, but for blocks of 16 at width 64 (1,024), of smaller heads in fp16 at width 128 (512)
+    // and of width 256 (256): there an even range for each is one and a half or two rounds of them.
     const int at_once_f = p.width == 64    ? (p.few_rows == 16 ? 1536 : 768)
                           : p.width == 128 ? (p.few_rows == 16 ? 768 : 512)
                                            : 512;

@@ -217,7 +217,8 @@ class KVAttentionPlan:
         """Synchronise and return [jobs, 0, jobs of few rows, jobs of many, partial rows, query rows,
         ..]; raises when the batch is invalid.  Calls after it launch no more workgroups than the
         plan has jobs, unless the plan was made in a captured graph: each replay builds that one
-        anew, and its jobs change (before the first one it holds nothing)."""
+        anew, and its jobs change (before the first one it holds nothing:
+        calls with it come behind a replay)."""
         import numpy as np
         h = np.zeros(PLAN_INFO_INTS, np.int32)
         check(lib().mla_read_kv_plan_info(stream_handle(stream), self._words[0], h.ctypes.data))

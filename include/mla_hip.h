@@ -455,8 +455,8 @@ int mla_append_kv(void* stream, int T, int n_heads, int n_kv_heads, int head_dim
  * session, at position p = k_len - q_len + i, sees the keys j <= p, and with window > 0 of these only
  * those with p - j < window or j < sinks:
  *     s_j = (q . k_j) * scale,   out = sum_j softmax(s)_j v_j,   lse = ln sum_j exp(s_j)
- * for decode rows, drafted tokens and prompt chunks alike.  Only pages with keys that some row sees
- * are read.  A plan, built on the GPU once for a batch and one (window, sinks), says which workgroup
+ * for decode rows, drafted tokens and prompt chunks alike.  Only units of 32 keys with one that some
+ * row sees are read.  A plan, built on the GPU once for a batch and one (window, sinks), says which workgroup
  * takes which rows over which keys and serves every such layer's call.  The rows' own keys and
  * values must already be appended. */
 size_t mla_kv_plan_bytes(int B, int rows, int n_heads, int n_kv_heads, int head_dim, int v_dim,
