@@ -31,17 +31,18 @@
 //   few rows: memory.  Traced: 64 rows, 32 heads on kv 8 x 128, contexts of 128 .. 14,000 tokens
 //     (1.69 GB) 298 us, 5.7 TB/s; two rows on 100,000 .. 131,072 tokens (0.90 GB) 154 us, 5.8; 64
 //     rows, kv 8 x 64, contexts of 128 .. 4,096 (0.29 GB) 56 us, 5.1 (46 where the last cache holds
-//     part of them).  One row on 1,040 tokens, kv 8 x 64:
-//     10 us, eight workgroups with 9 units a wave, one behind the other.  There a compute unit's own
-//     rate decides: 600 tokens more of kv x 128 (307 KB) take it 5.4 us, and eight waves in place of
-//     four are no faster (700 tokens 12.5 us against 11.1).
-//   many rows: both pipes of a SIMD, one after the other.  A prompt of 8,191 rows, 32 heads on kv 8 x 128 (550 GFLOP) 735 us,
-//     0.75 PFLOP/s (1.1 with the second part); 4,093 rows twice through a window of 1,024 (138 GFLOP)
-//     238 us, 0.58.  A SIMD takes 1,590 cycles for a wave's stage: 768 are those of its 48 MFMAs (the
-//     matrix cores are busy 49 % of the time), and its 150 other vector instructions, exponentials
-//     among them, take about the rest, so that its two waves hardly ever use both pipes at once.  LDS
-//     is busy 25 %, the L2 holds 95 % of what is read.  Then at 742 us: without the staging 680,
-//     without the exponentials 697, the products and LDS reads alone 536, P^T in one part 597.
+//     part of them).  One row on 1,040 tokens, kv 8 x 64: 10 us, eight workgroups with 9 units a
+//     wave, one behind the other.  There a compute unit's own rate decides: 600 tokens more of
+//     kv x 128 (307 KB) take it 5.4 us, and eight waves in place of four are no faster (700 tokens
+//     12.5 us against 11.1).
+//   many rows: both pipes of a SIMD, one after the other.  A prompt of 8,191 rows, 32 heads on kv
+//     8 x 128 (550 GFLOP) 735 us, 0.75 PFLOP/s (1.1 with the second part); 4,093 rows twice through
+//     a window of 1,024 (138 GFLOP) 238 us, 0.58.  A SIMD takes 1,590 cycles for a wave's stage:
+//     768 are those of its 48 MFMAs (the matrix cores are busy 49 % of the time), and its 150 other
+//     vector instructions, exponentials among them, take about the rest, so that its two waves
+//     hardly ever use both pipes at once.  LDS is busy 25 %, the L2 holds 95 % of what is read.
+//     Then at 742 us: without the staging 680, without the exponentials 697, the products and LDS
+//     reads alone 536, P^T in one part 597.
 //   Measured and not kept for many rows (prompt and window; each against its own time then): four
 //     waves a SIMD of 16 rows 840 and 268 us (730, 240); the 32 x 32 products 780 and 250 (724, 240);
 //     64 keys a stage in two buffers 758 and 247 (740, 239); vector instructions spread among the

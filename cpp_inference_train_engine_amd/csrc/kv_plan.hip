@@ -7,10 +7,10 @@
 // length that gives every slot of the GPU one range (several where they are long, so that slots
 // with short ones take more of them), or of twice a slot's share (so that only blocks well above it
 // are cut) where there are more blocks than that.
-// A chain of short phases of one workgroup: 6-10 us back to back, up to 14 alone.  (64 sessions of 128 .. 14,000 tokens, 32
-// heads on kv 8 x 128, attend in 302 us with up to four ranges a slot, in 313 with one.  Blocks of
-// many rows keep their order, in which neighbours read the same keys at the same time: 4,000 rows
-// take 204 us, and 212 with the longest blocks first.)
+// A chain of short phases of one workgroup: 6-10 us back to back, up to 14 alone.  (64 sessions of
+// 128 .. 14,000 tokens, 32 heads on kv 8 x 128, attend in 302 us with up to four ranges a slot, in
+// 313 with one.  Blocks of many rows keep their order, in which neighbours read the same keys at
+// the same time: 4,000 rows take 204 us, and 212 with the longest blocks first.)
 #include "mla_kv.hpp"
 
 #include <algorithm>

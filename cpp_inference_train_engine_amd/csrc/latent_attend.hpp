@@ -604,9 +604,10 @@ __global__ __launch_bounds__(ROWS ? kThreadsR : kThreadsK) __attribute__((
         }
         const float m_ref = m_run == -INFINITY ? 0.0f : m_run;
         // A weight enters the product as two parts of the 16-bit type, e = hi + lo, off by 2^-17 of
-        // it (bf16), or 2^-23 of it or 2^-25 (fp16; a row's largest is 2^kHead at least, so that a row
-        // made of weights 17 nats below a token with a latent of zero is off by 1 %): as one part it would be off by up to 2^-8 or 2^-11, all
-        // weights of keys of one score the same way, while the mass sums them in 32 bits.
+        // it (bf16), or 2^-23 of it or 2^-25 (fp16; a row's largest is 2^kHead at least, so that a
+        // row made of weights 17 nats below a token with a latent of zero is off by 1 %): as one
+        // part it would be off by up to 2^-8 or 2^-11, all weights of keys of one score the same
+        // way, while the mass sums them in 32 bits.
         float psum = 0.0f;
         V8 pb, pl;
 #pragma unroll

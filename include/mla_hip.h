@@ -432,15 +432,15 @@ int mla_latent_attention(void* stream, int B, int rows, int n_heads, int kv_rank
 /* 16-bit words of a page record; 0 for shapes outside the above. */
 size_t mla_kv_page_words(int n_kv_heads, int head_dim, int v_dim, int page_size);
 /* Row t of k [T x n_kv_heads x head_dim], rotated, and of v [T x n_kv_heads x v_dim] is rounded once
- * to `dtype` and written to flat slot slot_mapping[t]; slots outside the pool are skipped, the others
- * are distinct.  With q [T x n_heads x head_dim] (NULL: none) row t of q is rotated the same way,
- * rounded and written to q_out [T x n_heads x head_dim], whatever its slot.  q_out lies apart from
- * the memory between the first and the last element of each of q, k, v and the pages
- * (MLA_ERR_INVALID_ARGUMENT otherwise); rows of k, v or q within the pages are of slots that the call
- * does not write.  A token's rows have fewer than 2^31 columns in all (MLA_ERR_UNSUPPORTED otherwise).  Rows
- * are of row_dtype (MLA_DTYPE_*); *_row and *_head are strides in elements (columns lie one behind the other), so
- * that slices of one projection's rows can be given; rows, and strides, at multiples of 16 bytes
- * are read faster.
+ * to `dtype` and written to flat slot slot_mapping[t]; slots outside the pool are skipped, the
+ * others are distinct.  With q [T x n_heads x head_dim] (NULL: none) row t of q is rotated the same
+ * way, rounded and written to q_out [T x n_heads x head_dim], whatever its slot.  q_out lies apart
+ * from the memory between the first and the last element of each of q, k, v and the pages
+ * (MLA_ERR_INVALID_ARGUMENT otherwise); rows of k, v or q within the pages are of slots that the
+ * call does not write.  A token's rows have fewer than 2^31 columns in all (MLA_ERR_UNSUPPORTED
+ * otherwise).  Rows are of row_dtype (MLA_DTYPE_*); *_row and *_head are strides in elements
+ * (columns lie one behind the other), so that slices of one projection's rows can be given; rows,
+ * and strides, at multiples of 16 bytes are read faster.
  * The rotation turns pair i of a head at position p = positions[t] by the angle p * frequencies[i]
  * (device fp64, radians; taken in 64 bits): (a, b) -> (a cos - b sin, a sin + b cos).  The pairs'
  * columns are rotary_start + (2i, 2i + 1) with adjacent = 1 (src/model/ops.cpp:88-108), rotary_start
@@ -455,10 +455,10 @@ int mla_append_kv(void* stream, int T, int n_heads, int n_kv_heads, int head_dim
  * session, at position p = k_len - q_len + i, sees the keys j <= p, and with window > 0 of these only
  * those with p - j < window or j < sinks:
  *     s_j = (q . k_j) * scale,   out = sum_j softmax(s)_j v_j,   lse = ln sum_j exp(s_j)
- * for decode rows, drafted tokens and prompt chunks alike.  Only units of 32 keys with one that some
- * row sees are read.  A plan, built on the GPU once for a batch and one (window, sinks), says which workgroup
- * takes which rows over which keys and serves every such layer's call.  The rows' own keys and
- * values must already be appended. */
+ * for decode rows, drafted tokens and prompt chunks alike.  Only units of 32 keys with one that
+ * some row sees are read.  A plan, built on the GPU once for a batch and one (window, sinks), says
+ * which workgroup takes which rows over which keys and serves every such layer's call.  The rows'
+ * own keys and values must already be appended. */
 size_t mla_kv_plan_bytes(int B, int rows, int n_heads, int n_kv_heads, int head_dim, int v_dim,
                          int page_size, int max_q_len, int window, int sinks);
 /* Bytes of the workspace of calls with a plan of these sizes. */
@@ -480,15 +480,16 @@ int mla_read_kv_plan_info(void* stream, const void* plan, int32_t* host_info);
 /* The attention.  page_table and max_pages are those of the metadata; q [rows x n_heads x head_dim]
  * and out [rows x n_heads x v_dim] 16-bit words of `dtype`, lse [rows x n_heads] fp32 or NULL.  out
  * may be q itself where head_dim is v_dim; out, lse and workspace lie apart from each other, q and
- * the pages otherwise (MLA_ERR_INVALID_ARGUMENT).  Rows past the batch's are left as they were, and over a failed plan all.  host_info is what
- * mla_read_kv_plan_info returned for this very plan, not built anew since, or NULL: with it the call
- * launches as many workgroups as the plan has jobs, without it as many as a plan of these sizes can
- * have, whose rest returns at once.  A call with the info of another build, whose counts differ,
- * or with a plan that was built for other sizes (B .. sinks), writes nothing; a captured graph that
- * builds the plan takes NULL.  pages, q, plan, out and workspace at multiples of 16 bytes.  The workspace needs no initialisation; calls that share one
- * must be ordered on one stream.  Rows are rounded once, to `dtype`.  A key or value that a row does
- * not see adds nothing to it, whatever it holds.  A value that is not finite makes its column of the
- * rows that see it infinite or NaN, a NaN key those rows. */
+ * the pages otherwise (MLA_ERR_INVALID_ARGUMENT).  Rows past the batch's are left as they were, and
+ * over a failed plan all.  host_info is what mla_read_kv_plan_info returned for this very plan, not
+ * built anew since, or NULL: with it the call launches as many workgroups as the plan has jobs,
+ * without it as many as a plan of these sizes can have, whose rest returns at once.  A call with
+ * the info of another build, whose counts differ, or with a plan that was built for other sizes (B
+ * .. sinks), writes nothing; a captured graph that builds the plan takes NULL.  pages, q, plan, out
+ * and workspace at multiples of 16 bytes.  The workspace needs no initialisation; calls that share
+ * one must be ordered on one stream.  Rows are rounded once, to `dtype`.  A key or value that a row
+ * does not see adds nothing to it, whatever it holds.  A value that is not finite makes its column
+ * of the rows that see it infinite or NaN, a NaN key those rows. */
 int mla_kv_attention(void* stream, int B, int rows, int n_heads, int n_kv_heads, int head_dim,
                      int v_dim, int page_size, int max_q_len, int window, int sinks, int dtype,
                      float scale, const int32_t* page_table, int max_pages, int num_pool_pages,
