@@ -26,7 +26,7 @@ def at():
 
 def test_append(L, at):
     """3 tokens of 4 heads on kv 2 x 16, values 32 wide, fp32 rows: q_out has 384 bytes, k's rows of 128
-    bytes are 256 apart, v's of 256 are 512 apart, a pool of two pages has 3,072 bytes."""
+    bytes are 256 apart, v's of 256 are 512 apart, a page has 16 tokens of 2 x 48 16-bit words."""
     k, v, q, pages = at + 8192, at + 16384, at + 24576, at + 32768
 
     def call(q_out, k=k, v=v, k_head=16, T=3, fn=L.mla_append_kv):
